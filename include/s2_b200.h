@@ -389,6 +389,87 @@ typedef struct s2_gemm_desc {
 } s2_gemm_desc;
 S2_API s2_status s2_gemm(void *stream, const s2_gemm_desc *desc, int *extra_launches);
 
+/* ---- channels-last operators --------------------------------------------- */
+
+/* For token-major activations: [rows][channels] with the channels contiguous
+ * and any row pitch (in elements), the layout of this header's tensor-core
+ * operands (s2_spatial_attention, s2_gemm). Inference only. Both run on the
+ * current device, which must be the one of `stream` and of every pointer, are
+ * stream-ordered and capturable, allocate nothing and keep nothing between
+ * calls: the caller passes a workspace of at least *_workspace_bytes(desc)
+ * bytes, 16-byte aligned (its contents do not matter; calls that may overlap
+ * need one each). *launches (may be NULL) receives the kernels launched. */
+
+/* Activations: relu max(v, 0); silu v / (1 + e^-v); gelu v (1 + erf(v /
+ * sqrt 2)) / 2; gelu_tanh v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) / 2. */
+typedef enum s2_activation {
+    S2_ACT_NONE = 0,
+    S2_ACT_RELU = 1,
+    S2_ACT_SILU = 2,
+    S2_ACT_GELU = 3,
+    S2_ACT_GELU_TANH = 4
+} s2_activation;
+
+/* Group norm with an activation: x [samples][positions][channels], `groups`
+ * groups of channels / groups consecutive channels. Per sample and group the
+ * mean m and the (biased) variance v over positions and the group's channels,
+ * then y = act((x - m) / sqrt(v + eps) * weight[c] + bias[c]); weight / bias
+ * (device fp32 [channels]) may be NULL (1 / 0). The channels-last counterpart
+ * of s2_vae_group_norm_* (a frame is a sample). x is in_dtype, y out_dtype:
+ * the same, or fp32 in and fp16 / bf16 out. Statistics in fp32 about local
+ * pivots, joined in order (the same call gives the same bits). x_row, y_row
+ * >= channels: elements between positions; x_sample, y_sample: between
+ * samples. y may be x itself (same type, pitch and sample stride), and must
+ * not overlap it otherwise. samples or positions 0: nothing is done. At most
+ * 1024 groups (S2_UNSUPPORTED beyond). err: device int32 error word (may be
+ * NULL), set when a bounded wait inside the kernel gives up. */
+typedef struct s2_group_norm_act_desc {
+    int samples, channels, groups, activation;
+    long long positions;
+    int in_dtype, out_dtype; /* s2_dtype */
+    float eps;
+    const void *x;
+    long long x_row, x_sample;
+    const float *weight, *bias;
+    void *y;
+    long long y_row, y_sample;
+    void *workspace;
+    size_t workspace_bytes;
+    int32_t *err;
+} s2_group_norm_act_desc;
+S2_API size_t s2_group_norm_act_workspace_bytes(const s2_group_norm_act_desc *desc);
+S2_API s2_status s2_group_norm_act(void *stream, const s2_group_norm_act_desc *desc, int *launches);
+
+/* Matrix product with bias, activation and residual: y[m][n] = act(sum_k
+ * x[m][k] w[n][k] + bias[n]) + residual[m][n]. x [M][K] and w [N][K] in dtype
+ * (fp16 or bf16), bias device fp32 [N] or NULL, residual [M][N] (NULL: none)
+ * and y [M][N] in out_dtype: dtype, or fp32. Any M, N, K and pitches (ldx, ldw
+ * >= K, ldr, ldy >= N, in elements); operands whose base and pitch are
+ * multiples of 16 bytes are read in place, others are first copied into the
+ * workspace. Products are summed on the tensor cores in fp32, bias,
+ * activation and residual are applied to the fp32 sum, and y is rounded once.
+ * y may be residual itself (same pitch) and must not overlap any input
+ * otherwise. M 0: nothing is done. err as above. */
+typedef struct s2_linear_act_desc {
+    int N, K, activation;
+    int dtype, out_dtype; /* s2_dtype */
+    long long M;
+    const void *x;
+    long long ldx;
+    const void *w;
+    long long ldw;
+    const float *bias;
+    const void *residual;
+    long long ldr;
+    void *y;
+    long long ldy;
+    void *workspace;
+    size_t workspace_bytes;
+    int32_t *err;
+} s2_linear_act_desc;
+S2_API size_t s2_linear_act_workspace_bytes(const s2_linear_act_desc *desc);
+S2_API s2_status s2_linear_act(void *stream, const s2_linear_act_desc *desc, int *launches);
+
 /* ---- multi-GPU communicator (no counterpart in the reference) ------------ */
 
 /* One rank per GPU; NCCL over NVLink / NVSwitch, loaded on first use

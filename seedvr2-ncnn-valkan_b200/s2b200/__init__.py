@@ -62,6 +62,28 @@ class GemmDesc(ctypes.Structure):
                    ("row_dest", ctypes.c_void_p)])
 
 
+class GroupNormActDesc(ctypes.Structure):
+    """s2_group_norm_act_desc (include/s2_b200.h)."""
+    _fields_ = ([(n, ctypes.c_int) for n in ("samples", "channels", "groups", "activation")]
+                + [("positions", ctypes.c_longlong), ("in_dtype", ctypes.c_int), ("out_dtype", ctypes.c_int),
+                   ("eps", ctypes.c_float), ("x", ctypes.c_void_p), ("x_row", ctypes.c_longlong),
+                   ("x_sample", ctypes.c_longlong), ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p),
+                   ("y", ctypes.c_void_p), ("y_row", ctypes.c_longlong), ("y_sample", ctypes.c_longlong),
+                   ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("err", ctypes.c_void_p)])
+
+
+class LinearActDesc(ctypes.Structure):
+    """s2_linear_act_desc (include/s2_b200.h)."""
+    _fields_ = ([(n, ctypes.c_int) for n in ("N", "K", "activation", "dtype", "out_dtype")]
+                + [("M", ctypes.c_longlong), ("x", ctypes.c_void_p), ("ldx", ctypes.c_longlong),
+                   ("w", ctypes.c_void_p), ("ldw", ctypes.c_longlong), ("bias", ctypes.c_void_p),
+                   ("residual", ctypes.c_void_p), ("ldr", ctypes.c_longlong), ("y", ctypes.c_void_p),
+                   ("ldy", ctypes.c_longlong), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+                   ("err", ctypes.c_void_p)])
+
+
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+
 GEMM_SPLIT_F16, GEMM_GATED_RESID_F32, GEMM_SWIGLU_F16 = 0, 2, 3
 
 
@@ -224,6 +246,10 @@ _SIGS = {
     "s2_vae_conv3d_forward_host": (ctypes.c_int, [_vp, _vp, _vp] + [ctypes.c_int] * 3 + [_vp]),
     "s2_vae_conv3d_last_launches": (ctypes.c_int, [_vp]),
     "s2_vae_conv3d_device_error": (ctypes.c_int, [_vp, _i32p]),
+    "s2_group_norm_act_workspace_bytes": (ctypes.c_size_t, [_vp]),
+    "s2_group_norm_act": (ctypes.c_int, [_vp, _vp, _vp]),
+    "s2_linear_act_workspace_bytes": (ctypes.c_size_t, [_vp]),
+    "s2_linear_act": (ctypes.c_int, [_vp, _vp, _vp]),
     "s2_debug_fail_allocations": (ctypes.c_int, [ctypes.c_int]),
     "s2_debug_attention_fault": (ctypes.c_int, [ctypes.c_int, ctypes.c_ulonglong]),
     "s2_last_error": (ctypes.c_char_p, []),
@@ -929,6 +955,162 @@ def spatial_attention(q, k, v, channels, frames, tokens, out, err, stream=None):
     """Per-frame single-head attention; q/k/v/out fp16 [frames*tokens, padded_channels(channels)]."""
     _check(lib().s2_spatial_attention(_stream_ptr(stream), _ptr(q), _ptr(k), _ptr(v), channels, q.shape[1], frames,
                                       tokens, _ptr(out), _ptr(err)), "s2_spatial_attention")
+
+
+# ---- channels-last operators --------------------------------------------------
+
+def _fail(what: str):
+    raise S2Error(S2_INVALID_ARGUMENT, what)
+
+
+def _activation_code(activation) -> int:
+    code = ACTIVATIONS.get(activation)
+    if code is None:
+        _fail(f"unknown activation {activation!r} (one of {', '.join(ACTIVATIONS)})")
+    return code
+
+
+def _type_of(t, what: str) -> int:
+    try:
+        return _dtype_code(t)
+    except KeyError:
+        _fail(f"{what} must be fp16, bf16 or fp32, not {t.dtype}")
+
+
+def _need_vector(t, n: int, device, what: str):
+    """The address of a contiguous fp32 vector of n values (None: NULL)."""
+    if t is None:
+        return None
+    if t.device != device or t.dtype != _torch().float32 or t.shape != (n,) or not t.is_contiguous():
+        _fail(f"{what} must be a contiguous fp32 tensor of {n} values on {device}")
+    return t.data_ptr()
+
+
+def _need_err(err, device):
+    if err is None:
+        return None
+    if err.device != device or err.dtype != _torch().int32 or err.numel() < 1:
+        _fail(f"err must be an int32 tensor on {device}")
+    return err.data_ptr()
+
+
+def _need_no_grad(torch, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        _fail("inference only: a tensor requires a gradient (call under torch.no_grad())")
+
+
+def _on_own_stream(torch, x, stream, call):
+    """call() with x's device current, and `stream` (default: that device's current one)."""
+    if not x.is_cuda:
+        _fail(f"x is on {x.device}: the operators run on a CUDA device")
+    if stream is not None:
+        if stream.device != x.device:
+            _fail(f"the stream is on {stream.device}, x on {x.device}")
+        with torch.cuda.stream(stream):
+            return call()
+    if x.device.index != torch.cuda.current_device():
+        with torch.cuda.device(x.device):
+            return call()
+    return call()
+
+
+def _run_desc(torch, call, workspace_bytes, desc, device, what: str):
+    ref = ctypes.byref(desc)
+    need = workspace_bytes(ref)
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        desc.workspace, desc.workspace_bytes = ws.data_ptr(), need
+    status = call(_stream_ptr(), ref, None)
+    if status != S2_OK:
+        _check(status, what)
+
+
+def _pitch(t, first: int, what: str):
+    """The dimensions [first, -1) of t as one: (size, pitch in elements). They must be evenly
+    spaced, over contiguous channels."""
+    shape, strides = t.shape, t.stride()
+    if strides[-1] != 1 and shape[-1] > 1:
+        _fail(f"{what}: the last dimension must be contiguous")
+    rows, pitch = 1, None
+    for i in range(len(shape) - 2, first - 1, -1):
+        if shape[i] != 1:
+            if pitch is None:
+                pitch = strides[i]
+            elif strides[i] != pitch * rows:
+                _fail(f"{what}: its rows must be evenly spaced")
+            rows *= shape[i]
+    return rows, (shape[-1] if pitch is None else pitch)
+
+
+def group_norm_act(x, groups: int, weight=None, bias=None, eps: float = 1e-6, activation: str = "none", out=None,
+                   out_dtype=None, err=None, stream=None):
+    """Channels-last group norm with an activation (s2_group_norm_act): x [samples, ..., channels]
+    CUDA tensor (fp16, bf16 or fp32, any even spacing of positions); per sample and group of
+    channels / groups consecutive channels, y = act((x - mean) / sqrt(var + eps) * weight + bias).
+    weight, bias: fp32 [channels] or None. Returns y in out_dtype (x's, or fp16 / bf16 for fp32 x)
+    in x's shape; `out` receives it when given (it may be x). err: device int32 error word."""
+    torch = _torch()
+
+    def call():
+        y = out
+        if x.dim() < 2:
+            _fail("x must be [samples, ..., channels]")
+        _need_no_grad(torch, x, weight, bias)
+        if y is None:
+            y = torch.empty(x.shape, dtype=out_dtype or x.dtype, device=x.device)
+        elif y.shape != x.shape or y.device != x.device or out_dtype not in (None, y.dtype):
+            _fail("out must have x's shape and device, and out_dtype if both are given")
+        positions, x_row = _pitch(x, 1, "x")
+        _, y_row = _pitch(y, 1, "out")
+        samples, channels = x.shape[0], x.shape[-1]
+        many = samples > 1
+        d = GroupNormActDesc(samples, channels, groups, _activation_code(activation), positions, _type_of(x, "x"),
+                             _type_of(y, "out"), eps, x.data_ptr(), x_row, x.stride(0) if many else 0,
+                             _need_vector(weight, channels, x.device, "weight"),
+                             _need_vector(bias, channels, x.device, "bias"), y.data_ptr(), y_row,
+                             y.stride(0) if many else 0, None, 0, _need_err(err, x.device))
+        L = lib()
+        _run_desc(torch, L.s2_group_norm_act, L.s2_group_norm_act_workspace_bytes, d, x.device, "s2_group_norm_act")
+        return y
+
+    return _on_own_stream(torch, x, stream, call)
+
+
+def linear_act(x, w, bias=None, activation: str = "none", residual=None, out=None, out_dtype=None, err=None,
+               stream=None):
+    """y = act(x w^T + bias) + residual (s2_linear_act): x [..., K] and w [N, K] CUDA tensors of one
+    type (fp16 or bf16, rows of any even pitch), bias fp32 [N] or None, residual [..., N] in the
+    output's type or None. Returns y [..., N] in out_dtype (x's, or fp32); `out` receives it when
+    given (it may be the residual). err: device int32 error word."""
+    torch = _torch()
+
+    def call():
+        y = out
+        if x.dim() < 1 or w.dim() != 2 or w.shape[1] != x.shape[-1] or w.dtype != x.dtype or w.device != x.device:
+            _fail("x must be [..., K] and w [N, K], of one type on one device")
+        _need_no_grad(torch, x, w, bias, residual)
+        N, K = w.shape
+        shape = x.shape[:-1] + (N,)
+        if y is None:
+            y = torch.empty(shape, dtype=out_dtype or x.dtype, device=x.device)
+        elif y.shape != shape or y.device != x.device or out_dtype not in (None, y.dtype):
+            _fail(f"out must be {tuple(shape)} on x's device, and of out_dtype if both are given")
+        rows, ldx = _pitch(x, 0, "x")
+        _, ldw = _pitch(w, 0, "w")
+        _, ldy = _pitch(y, 0, "out")
+        res, ldr = None, 0
+        if residual is not None:
+            if residual.shape != shape or residual.dtype != y.dtype or residual.device != x.device:
+                _fail(f"residual must be {tuple(shape)} in the output's type on x's device")
+            res, ldr = residual.data_ptr(), _pitch(residual, 0, "residual")[1]
+        d = LinearActDesc(N, K, _activation_code(activation), _type_of(x, "x"), _type_of(y, "out"), rows, x.data_ptr(),
+                          ldx, w.data_ptr(), ldw, _need_vector(bias, N, x.device, "bias"), res, ldr, y.data_ptr(),
+                          ldy, None, 0, _need_err(err, x.device))
+        L = lib()
+        _run_desc(torch, L.s2_linear_act, L.s2_linear_act_workspace_bytes, d, x.device, "s2_linear_act")
+        return y
+
+    return _on_own_stream(torch, x, stream, call)
 
 
 VAE_WEIGHT_ORDER = ("norm_bias", "norm_weight", "k_bias", "k_weight", "out_bias", "out_weight", "q_bias", "q_weight",

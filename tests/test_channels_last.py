@@ -1,0 +1,111 @@
+"""Refusals of the channels-last operators' calls (no GPU needed: nothing gets as far as a launch)."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+
+import s2b200
+
+torch = pytest.importorskip("torch")
+
+BASE = 1 << 20  # an address that is never read
+
+
+def _norm(**kw):
+    d = dict(samples=2, channels=64, groups=32, activation=2, positions=100, in_dtype=s2b200.S2_F16,
+             out_dtype=s2b200.S2_F16, eps=1e-6, x=BASE, x_row=64, x_sample=6400, weight=None, bias=None, y=2 * BASE,
+             y_row=64, y_sample=6400, workspace=4 * BASE, workspace_bytes=1 << 30, err=None)
+    d.update(kw)
+    return s2b200.GroupNormActDesc(**d)
+
+
+def _linear(**kw):
+    d = dict(N=64, K=128, activation=0, dtype=s2b200.S2_F16, out_dtype=s2b200.S2_F16, M=10, x=BASE, ldx=128,
+             w=2 * BASE, ldw=128, bias=None, residual=None, ldr=0, y=3 * BASE, ldy=64, workspace=4 * BASE,
+             workspace_bytes=1 << 30, err=None)
+    d.update(kw)
+    return s2b200.LinearActDesc(**d)
+
+
+def _call(fn, desc):
+    launches = ctypes.c_int(-1)
+    status = getattr(s2b200.lib(), fn)(None, ctypes.byref(desc), ctypes.byref(launches))
+    return status, launches.value
+
+
+INVALID, UNSUPPORTED = s2b200.S2_INVALID_ARGUMENT, s2b200.S2_UNSUPPORTED
+
+NORM_REFUSALS = [
+    (dict(samples=-1), INVALID), (dict(positions=-1), INVALID), (dict(channels=0), INVALID), (dict(groups=0), INVALID),
+    (dict(groups=33), INVALID), (dict(x=None), INVALID), (dict(y=None), INVALID), (dict(x=BASE + 1), INVALID),
+    (dict(y=2 * BASE + 1), INVALID), (dict(weight=BASE + 2), INVALID), (dict(bias=BASE + 2), INVALID),
+    (dict(x_row=63), INVALID), (dict(y_row=63), INVALID), (dict(x_sample=6399), INVALID), (dict(x_sample=0), INVALID),
+    (dict(y_sample=6399), INVALID), (dict(eps=-1.0), INVALID), (dict(eps=float("nan")), INVALID),
+    (dict(eps=float("inf")), INVALID), (dict(activation=5), UNSUPPORTED), (dict(activation=-1), UNSUPPORTED),
+    (dict(in_dtype=7), UNSUPPORTED), (dict(out_dtype=s2b200.S2_BF16), UNSUPPORTED),
+    (dict(out_dtype=s2b200.S2_F32), UNSUPPORTED), (dict(channels=4096, groups=2048, x_row=4096, y_row=4096), UNSUPPORTED),
+    (dict(samples=1 << 20), UNSUPPORTED), (dict(y=BASE + 64), INVALID), (dict(y=BASE, y_row=72, y_sample=7200), INVALID),
+    (dict(y=BASE, in_dtype=s2b200.S2_F32), INVALID), (dict(x_row=1 << 50, x_sample=1 << 60), INVALID),
+    (dict(x_row=80, y_row=80, x_sample=8000, y_sample=8000, y=BASE + 32), INVALID),
+    (dict(positions=1 << 41), UNSUPPORTED),
+]
+
+
+@pytest.mark.parametrize("kw,status", NORM_REFUSALS, ids=lambda v: str(v))
+def test_norm_refusals(kw, status):
+    assert _call("s2_group_norm_act", _norm(**kw)) == (status, 0)
+    assert "group_norm_act" in s2b200.last_error()
+
+
+@pytest.mark.parametrize("kw", [dict(workspace=None), dict(workspace_bytes=0), dict(workspace=4 * BASE + 4)], ids=str)
+def test_norm_workspace_refusals(kw):
+    big = dict(positions=1 << 22, x_sample=1 << 28, y_sample=1 << 28, y=1 << 40)
+    if s2b200.lib().s2_group_norm_act_workspace_bytes(ctypes.byref(_norm(**big))) == 0:
+        pytest.skip("this size needs no workspace")
+    assert _call("s2_group_norm_act", _norm(**big, **kw)) == (INVALID, 0)
+
+
+@pytest.mark.parametrize("kw", [dict(samples=0), dict(positions=0)], ids=str)
+def test_norm_of_nothing(kw):
+    assert _call("s2_group_norm_act", _norm(x=None, y=None, workspace=None, **kw)) == (0, 0)
+    assert s2b200.lib().s2_group_norm_act_workspace_bytes(ctypes.byref(_norm(**kw))) == 0
+
+
+LINEAR_REFUSALS = [
+    (dict(M=-1), INVALID), (dict(N=0), INVALID), (dict(K=0), INVALID), (dict(x=None), INVALID), (dict(w=None), INVALID),
+    (dict(y=None), INVALID), (dict(x=BASE + 1), INVALID), (dict(w=BASE + 1), INVALID), (dict(y=BASE + 1), INVALID),
+    (dict(bias=BASE + 2), INVALID), (dict(residual=5 * BASE + 1, ldr=64), INVALID), (dict(ldx=127), INVALID),
+    (dict(ldw=127), INVALID), (dict(ldy=63), INVALID), (dict(residual=5 * BASE, ldr=63), INVALID),
+    (dict(activation=5), UNSUPPORTED), (dict(dtype=s2b200.S2_F32, out_dtype=s2b200.S2_F32), UNSUPPORTED),
+    (dict(out_dtype=s2b200.S2_BF16), UNSUPPORTED), (dict(M=1 << 31), UNSUPPORTED), (dict(N=1 << 22, ldy=1 << 22), UNSUPPORTED),
+    (dict(K=1 << 22, ldx=1 << 22, ldw=1 << 22), UNSUPPORTED), (dict(y=BASE), INVALID), (dict(y=2 * BASE + 256), INVALID),
+    (dict(residual=3 * BASE, ldr=72), INVALID), (dict(residual=3 * BASE + 2, ldr=64), INVALID),
+    (dict(bias=3 * BASE + 1024), INVALID), (dict(ldx=1 << 50), INVALID),
+    (dict(out_dtype=s2b200.S2_F32, y=3 * BASE + 2), INVALID),
+]
+
+
+@pytest.mark.parametrize("kw,status", LINEAR_REFUSALS, ids=lambda v: str(v))
+def test_linear_refusals(kw, status):
+    assert _call("s2_linear_act", _linear(**kw)) == (status, 0)
+    assert "linear_act" in s2b200.last_error()
+
+
+def test_linear_of_no_rows():
+    assert _call("s2_linear_act", _linear(M=0, x=None, y=None, workspace=None)) == (0, 0)
+    assert s2b200.lib().s2_linear_act_workspace_bytes(ctypes.byref(_linear(M=0))) == 0
+
+
+def test_null_descriptions():
+    for fn in ("s2_group_norm_act", "s2_linear_act"):
+        assert getattr(s2b200.lib(), fn)(None, None, None) == INVALID
+        assert getattr(s2b200.lib(), fn + "_workspace_bytes")(None) == 0
+
+
+def test_wrappers_refuse_host_tensors():
+    x = torch.zeros(4, 64, dtype=torch.float16)
+    for call in (lambda: s2b200.group_norm_act(x, 8), lambda: s2b200.linear_act(x, x)):
+        with pytest.raises(s2b200.S2Error) as e:
+            call()
+        assert e.value.status == INVALID

@@ -1,0 +1,476 @@
+"""group_norm_act and linear_act on the GPU against plain 64-bit forms (tests/channels_last.py
+has the formulas and says how the bounds are derived)."""
+from __future__ import annotations
+
+import pytest
+
+import s2b200
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+import channels_last as cl  # noqa: E402
+
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+NORM_TYPES = [(F16, F16), (BF16, BF16), (F32, F32), (F32, F16), (F32, BF16)]
+
+
+@pytest.fixture(scope="module", autouse=True)
+def device():
+    assert torch.cuda.is_available(), "GPU tests need a CUDA device"
+    assert s2b200.device_check(0) == 0, s2b200.last_error()
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _normal(shape, gen, dtype=F32):
+    return torch.randn(shape, generator=gen, device="cuda").to(dtype)
+
+
+def _features(shape, gen, dtype, pad=0):
+    C = shape[-1]
+    x = _normal(shape[:-1] + (C + pad,), gen)[..., :C]
+    return (x * torch.exp(0.5 * _normal((C,), gen)) + 2 * _normal((C,), gen)).to(dtype)
+
+
+def _padded(x, pad):
+    """x in rows of `pad` values more, NaN in them."""
+    big = torch.full(x.shape[:-1] + (x.shape[-1] + pad,), float("nan"), dtype=x.dtype, device=x.device)
+    big[..., :x.shape[-1]] = x
+    return big, big[..., :x.shape[-1]]
+
+
+# ---- group norm ------------------------------------------------------------------
+
+# (samples, positions, channels, groups): single values, one channel a group, groups that no vector
+# fits, blocks of columns (more channels than a block's threads hold), few and many rows
+NORM_SHAPES = [(1, 1, 1, 1), (1, 1, 32, 32), (2, 1, 64, 8), (1, 2, 8, 1), (2, 7, 96, 32), (3, 1000, 130, 10),
+               (2, 257, 512, 32), (5, 64, 40, 8), (1, 5003, 24, 8), (1, 17, 4104, 3), (2, 33, 8192, 2),
+               (1, 9, 2056, 257), (1, 40, 1024, 1024), (1, 3001, 128, 1), (17, 130, 48, 16), (1, 70001, 16, 2),
+               (2, 14400, 64, 32)]
+
+
+@pytest.mark.parametrize("types", NORM_TYPES, ids=lambda t: f"{t[0]}-{t[1]}".replace("torch.", ""))
+@pytest.mark.parametrize("shape", NORM_SHAPES, ids=str)
+def test_norm_shapes(shape, types):
+    S, P, C, G = shape
+    gen = _gen(P + C)
+    x = _features((S, P, C), gen, types[0])
+    w, b = 1 + 0.1 * _normal((C,), gen), 0.1 * _normal((C,), gen)
+    act = cl.ACTS[(P + C + G) % 5]
+    y = s2b200.group_norm_act(x, G, w, b, eps=1e-6, activation=act, out_dtype=types[1])
+    assert y.dtype == types[1] and y.shape == x.shape
+    cl.check(y, *cl.norm_exact(x, G, w, b, 1e-6, act), f"{shape} {act}")
+
+
+@pytest.mark.parametrize("act", cl.ACTS)
+@pytest.mark.parametrize("affine", [(False, False), (True, False), (False, True)])
+def test_norm_activations_and_affine(act, affine):
+    gen = _gen(3)
+    x = _features((2, 300, 64), gen, F16)
+    w = _normal((64,), gen) if affine[0] else None
+    b = _normal((64,), gen) if affine[1] else None
+    y = s2b200.group_norm_act(x, 16, w, b, eps=1e-5, activation=act)
+    cl.check(y, *cl.norm_exact(x, 16, w, b, 1e-5, act))
+
+
+@pytest.mark.parametrize("types", NORM_TYPES, ids=lambda t: f"{t[0]}-{t[1]}".replace("torch.", ""))
+@pytest.mark.parametrize("pads", [(8, 8), (0, 8), (8, 0), (1, 0), (0, 3), (2, 2), (4, 4), (5, 16)])
+def test_norm_pitches(types, pads):
+    """Rows of other pitches in and out; what lies between the rows is neither read nor written."""
+    gen = _gen(4)
+    x = _features((3, 211, 96), gen, types[0])
+    _, xp = _padded(x, pads[0])
+    buf, out = _padded(torch.zeros(3, 211, 96, dtype=types[1], device="cuda"), pads[1])
+    w = 1 + 0.1 * _normal((96,), gen)
+    r = s2b200.group_norm_act(xp, 32, w, None, activation="silu", out=out)
+    assert r is out
+    cl.check(out, *cl.norm_exact(x, 32, w, None, 1e-6, "silu"))
+    assert torch.isnan(buf[..., 96:]).all()
+
+
+def test_norm_frames_of_a_video():
+    """[T, H, W, C] with the frames cut out of a longer clip: the sample stride is its own."""
+    gen = _gen(5)
+    clip = _features((6, 9, 11, 64), gen, BF16)
+    x = clip[::2]
+    y = s2b200.group_norm_act(x, 32, activation="silu")
+    assert y.shape == x.shape and y.is_contiguous()
+    cl.check(y, *cl.norm_exact(x, 32, None, None, 1e-6, "silu"))
+
+
+@pytest.mark.parametrize("offset", [0, 1, 2, 4])
+def test_norm_base_alignment(offset):
+    gen = _gen(6)
+    flat = _features((1, 1, 2 * 150 * 64 + 8), gen, F16).flatten()
+    x = flat[offset:offset + 2 * 150 * 64].view(2, 150, 64)
+    y = s2b200.group_norm_act(x, 32, activation="gelu_tanh")
+    cl.check(y, *cl.norm_exact(x, 32, None, None, 1e-6, "gelu_tanh"))
+
+
+@pytest.mark.parametrize("shape", [(2, 301, 64, 32), (1, 9000, 512, 32), (3, 50, 33, 11)])
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_norm_in_place(shape, dtype):
+    S, P, C, G = shape
+    x = _features((S, P, C), _gen(7), dtype)
+    want = s2b200.group_norm_act(x, G, activation="silu")
+    got = x.clone()
+    s2b200.group_norm_act(got, G, activation="silu", out=got)
+    assert torch.equal(got, want)
+
+
+def test_norm_into_the_other_half_of_its_rows():
+    """x and out are column ranges of one buffer."""
+    gen = _gen(8)
+    buf = _features((2, 77, 128), gen, F16)
+    x = buf[..., :64].clone()
+    s2b200.group_norm_act(buf[..., :64], 8, out=buf[..., 64:])
+    assert torch.equal(buf[..., :64], x)
+    cl.check(buf[..., 64:], *cl.norm_exact(x, 8, None, None, 1e-6, "none"))
+
+
+@pytest.mark.parametrize("P", [40, 1000, 30000])
+def test_norm_keeps_a_small_spread_about_a_large_mean(P):
+    gen = _gen(9)
+    x = 1000 + 0.5 * _normal((2, P, 64), gen)
+    y = s2b200.group_norm_act(x, 8)
+    cl.check(y, *cl.norm_exact(x, 8, None, None, 1e-6, "none"))
+
+
+@pytest.mark.parametrize("at", [0, 1, 37, 4999])
+def test_norm_with_an_outlier(at):
+    """One value 10^4 spreads away, at the start of a run too: the other values keep their digits."""
+    gen = _gen(10)
+    x = _normal((1, 5000, 32), gen)
+    x[0, at, 5] = 1e4
+    y = s2b200.group_norm_act(x, 4)
+    cl.check(y, *cl.norm_exact(x, 4, None, None, 1e-6, "none"))
+
+
+def test_norm_of_equal_values():
+    x = torch.full((2, 100, 32), 3.25, device="cuda", dtype=F16)
+    b = torch.linspace(-1, 1, 32, device="cuda")
+    y = s2b200.group_norm_act(x, 4, None, b)
+    assert torch.equal(y, b.half().expand_as(y))
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("at", [0, 500])
+def test_norm_bad_values_stay_in_their_group(bad, at):
+    gen = _gen(11)
+    x = _features((2, 1001, 32), gen, F16)
+    y0 = s2b200.group_norm_act(x, 8, activation="relu")
+    x[1, at, 9] = bad
+    y = s2b200.group_norm_act(x, 8, activation="relu")
+    assert torch.isnan(y[1, :, 8:12]).all()
+    y[1, :, 8:12] = y0[1, :, 8:12]
+    assert torch.equal(y, y0)
+
+
+def test_norm_of_nothing():
+    for shape in ((0, 5, 32), (3, 0, 32)):
+        y = s2b200.group_norm_act(torch.empty(shape, device="cuda", dtype=F16), 8)
+        assert y.shape == shape
+
+
+def test_norm_gives_the_same_bits():
+    x = _features((3, 20000, 96), _gen(12), BF16)
+    first = s2b200.group_norm_act(x, 32, activation="silu")
+    for _ in range(5):
+        assert torch.equal(s2b200.group_norm_act(x, 32, activation="silu"), first)
+
+
+@pytest.mark.parametrize("shape", [(1, 600000, 64, 32), (2, 300000, 128, 32), (1, 120000, 512, 32), (1, 2000000, 16, 4)])
+def test_norm_of_large_samples(shape):
+    """Samples beyond a block's, a cluster's and the chip's memory."""
+    S, P, C, G = shape
+    x = _features((S, P, C), _gen(13), BF16)
+    y = s2b200.group_norm_act(x, G, activation="silu")
+    for s in range(S):
+        cl.check(y[s:s + 1], *cl.norm_exact(x[s:s + 1], G, None, None, 1e-6, "silu"))
+
+
+def test_norm_past_2_31_values():
+    S, P, C, G = 3, 5700000, 128, 32
+    x = torch.empty((S, P, C), dtype=F16, device="cuda")
+    gen = _gen(14)
+    for s in range(S):
+        x[s] = torch.randn((P, C), generator=gen, device="cuda", dtype=F16)
+        x[s] += s
+    y = s2b200.group_norm_act(x, G, activation="none")
+    for s in range(S):
+        var, mean = torch.zeros(G, dtype=torch.float64, device="cuda"), torch.zeros(G, dtype=torch.float64, device="cuda")
+        for part in x[s].split(600000):
+            mean += part.double().view(-1, G, C // G).sum(dim=(0, 2))
+        mean /= P * (C // G)
+        for part in x[s].split(600000):
+            var += ((part.double().view(-1, G, C // G) - mean[:, None]) ** 2).sum(dim=(0, 2))
+        sigma = (var / (P * (C // G)) + 1e-6).sqrt()
+        for r0 in (0, P // 2, P - 1000):
+            d = x[s, r0:r0 + 1000].double().view(-1, G, C // G) - mean[:, None]
+            want = (d / sigma[:, None]).view(-1, C)
+            room = ((d.abs() + mean.abs()[:, None]) / sigma[:, None]).view(-1, C) * 2.0 ** -17
+            cl.check(y[s, r0:r0 + 1000], want, room)
+
+
+# ---- matrix product ----------------------------------------------------------------
+
+LINEAR_SHAPES = [(1, 1, 1), (1, 2560, 2560), (1, 777, 1001), (2, 16, 8), (3, 64, 5120), (7, 130, 65), (16, 128, 64),
+                 (17, 100, 128), (33, 2560, 256), (58, 2560, 5120), (64, 96, 1000), (65, 320, 200), (100, 1, 512),
+                 (128, 256, 1024), (129, 257, 72), (200, 513, 640), (300, 5, 24), (1237, 777, 1001), (1000, 2560, 512),
+                 (4096, 256, 64), (4500, 515, 1032), (8200, 512, 1536), (20000, 24, 48)]
+
+
+def _operands(M, N, K, dtype, seed, res=True, out_dtype=None):
+    gen = _gen(seed)
+    x, w = _normal((M, K), gen, dtype), (0.05 * _normal((N, K), gen)).to(dtype)
+    b = _normal((N,), gen)
+    r = _normal((M, N), gen, out_dtype or dtype) if res else None
+    return x, w, b, r
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=str)
+@pytest.mark.parametrize("shape", LINEAR_SHAPES, ids=str)
+def test_linear_shapes(shape, dtype):
+    M, N, K = shape
+    x, w, b, r = _operands(M, N, K, dtype, M + N + K)
+    act = cl.ACTS[(M + N) % 5]
+    y = s2b200.linear_act(x, w, b, act, r)
+    assert y.dtype == dtype and y.shape == (M, N)
+    cl.check(y, *cl.linear_exact(x, w, b, act, r), f"{shape} {act}")
+
+
+@pytest.mark.parametrize("act", cl.ACTS)
+@pytest.mark.parametrize("parts", [(False, False), (True, False), (False, True), (True, True)])
+@pytest.mark.parametrize("shape", [(1, 200, 96), (40, 264, 192), (700, 264, 192), (4300, 256, 1024)], ids=str)
+def test_linear_epilogues(shape, act, parts):
+    x, w, b, r = _operands(*shape, F16, 21)
+    b, r = b if parts[0] else None, r if parts[1] else None
+    cl.check(s2b200.linear_act(x, w, b, act, r), *cl.linear_exact(x, w, b, act, r))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=str)
+@pytest.mark.parametrize("shape", [(1, 300, 640), (50, 333, 640), (333, 200, 2560), (5000, 512, 1024)], ids=str)
+def test_linear_fp32_out(shape, dtype):
+    x, w, b, r = _operands(*shape, dtype, 22, out_dtype=F32)
+    y = s2b200.linear_act(x, w, b, "silu", r, out_dtype=F32)
+    assert y.dtype == F32
+    cl.check(y, *cl.linear_exact(x, w, b, "silu", r))
+
+
+@pytest.mark.parametrize("shape", [(1, 60, 72), (30, 120, 72), (500, 250, 200), (4200, 260, 1030)], ids=str)
+@pytest.mark.parametrize("pads", [(8, 8, 8, 8), (1, 0, 0, 0), (0, 1, 0, 0), (0, 0, 1, 0), (0, 0, 0, 1), (3, 8, 2, 5)])
+def test_linear_pitches(shape, pads):
+    """x, w, residual and out in rows of other pitches; nothing between the rows counts or changes."""
+    x, w, b, r = _operands(*shape, BF16, 23)
+    xp, wp, rp = _padded(x, pads[0])[1], _padded(w, pads[1])[1], _padded(r, pads[2])[1]
+    buf, out = _padded(torch.zeros_like(r), pads[3])
+    s2b200.linear_act(xp, wp, b, "gelu", rp, out=out)
+    cl.check(out, *cl.linear_exact(x, w, b, "gelu", r))
+    assert torch.isnan(buf[..., shape[1]:]).all()
+
+
+@pytest.mark.parametrize("shape", [(1, 64, 64), (60, 160, 96), (900, 160, 96), (4200, 256, 1024)], ids=str)
+def test_linear_onto_its_residual(shape):
+    x, w, b, r = _operands(*shape, F16, 24)
+    want = s2b200.linear_act(x, w, b, "none", r)
+    got = r.clone()
+    s2b200.linear_act(x, w, b, "none", got, out=got)
+    assert torch.equal(got, want)
+
+
+def test_linear_of_leading_dimensions():
+    x, w, b, _ = _operands(60, 48, 64, F16, 25, res=False)
+    y = s2b200.linear_act(x.view(3, 4, 5, 64), w, b, "relu")
+    assert y.shape == (3, 4, 5, 48) and torch.equal(y.view(60, 48), s2b200.linear_act(x, w, b, "relu"))
+    assert s2b200.linear_act(x[0], w, b, "relu").shape == (48,)
+    assert s2b200.linear_act(x[:0], w, b).shape == (0, 48)
+
+
+@pytest.mark.parametrize("shape", [(20, 130, 200), (1000, 130, 200), (4300, 256, 1024)], ids=str)
+def test_linear_bad_rows_stay_alone(shape):
+    """Infinite and NaN inputs reach their own row (x) or column (w) only."""
+    x, w, b, r = _operands(*shape, F16, 26)
+    y0 = s2b200.linear_act(x, w, b, "relu", r)
+    x, w = x.clone(), w.clone()
+    x[3, 7] = float("inf")
+    w[5, 9] = float("nan")
+    y = s2b200.linear_act(x, w, b, "relu", r)
+    keep = torch.ones_like(y, dtype=torch.bool)
+    keep[3], keep[:, 5] = False, False
+    assert torch.equal(y[keep], y0[keep])
+    assert torch.isnan(y[:, 5]).all()
+    want = cl.linear_exact(x[3:4].float(), w.float(), b, "relu", r[3:4])[0]
+    assert torch.equal(torch.isnan(y[3:4]), torch.isnan(want)) and torch.equal(torch.isinf(y[3:4]), torch.isinf(want))
+
+
+@pytest.mark.parametrize("shape", [(1, 2560, 2560), (58, 2560, 5120), (700, 500, 1024)], ids=str)
+def test_linear_gives_the_same_bits(shape):
+    x, w, b, r = _operands(*shape, F16, 27)
+    first = s2b200.linear_act(x, w, b, "silu", r)
+    for _ in range(5):
+        assert torch.equal(s2b200.linear_act(x, w, b, "silu", r), first)
+
+
+def test_linear_past_2_31_values():
+    """Offsets of x, residual and y pass 2^31 elements."""
+    M, N, K = 4300000, 512, 520
+    gen = _gen(28)
+    x = torch.empty((M, K), dtype=F16, device="cuda").normal_(generator=gen)
+    w = (0.05 * _normal((N, K), gen)).half()
+    r = torch.empty((M, N), dtype=F16, device="cuda").normal_(generator=gen)
+    y = s2b200.linear_act(x, w, None, "none", r)
+    for at in (0, M // 2, M - 500):
+        rows = slice(at, at + 500)
+        cl.check(y[rows], *cl.linear_exact(x[rows], w, None, "none", r[rows]))
+
+
+# ---- streams, graphs, threads --------------------------------------------------------
+
+def _calls(seed):
+    gen = _gen(seed)
+    x = _features((2, 6000, 64), gen, F16)
+    wide = _features((1, 40000, 512), gen, F16)
+    a, w, b, r = _operands(300, 264, 1000, F16, seed)
+    one = a[:1]
+    odd = _padded(a, 3)[1]
+
+    def run(**kw):
+        return [s2b200.group_norm_act(x, 32, activation="silu", **kw), s2b200.group_norm_act(wide, 32, **kw),
+                s2b200.linear_act(a, w, b, "gelu", r, **kw), s2b200.linear_act(one, w, b, **kw),
+                s2b200.linear_act(odd, w, b, "silu", **kw)]
+
+    return (x, wide, a, one, odd, w, b, r), run
+
+
+def test_other_streams():
+    _, run = _calls(31)
+    want = run()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    got = run(stream=side)
+    side.synchronize()
+    assert all(torch.equal(g, w) for g, w in zip(got, want))
+    with torch.cuda.stream(side):
+        got = run()
+    side.synchronize()
+    assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+def test_two_streams_at_once():
+    data = [_calls(32), _calls(33)]
+    want = [run() for _, run in data]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in data]
+    got = [[], []]
+    for _ in range(20):
+        for i, (_, run) in enumerate(data):
+            got[i].append(run(stream=streams[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for outs in got[i]:
+            assert all(torch.equal(g, w) for g, w in zip(outs, want[i]))
+
+
+def test_captured_and_replayed_on_new_inputs():
+    (x, wide, a, one, odd, w, b, r), run = _calls(34)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        run()
+    side.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs = run()
+        graphs.append((g, outs))
+    for seed in (35, 36):
+        gen = _gen(seed)
+        for t in (x, wide, a, odd, r):
+            t.copy_(_normal(t.shape, gen))
+        want = run()
+        for g, outs in graphs:
+            g.replay()
+        for g, outs in graphs:
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(outs, want))
+
+
+def test_threads():
+    import threading
+    data = [_calls(37 + i) for i in range(4)]
+    want = [run() for _, run in data]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        try:
+            s = torch.cuda.Stream()
+            for _ in range(10):
+                got = data[i][1](stream=s)
+                s.synchronize()
+                if not all(torch.equal(g, w) for g, w in zip(got, want[i])):
+                    bad.append(i)
+        except Exception as e:  # noqa: BLE001
+            bad.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad, bad
+
+
+# ---- together ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("C,frames,H,W", [(512, 2, 12, 20), (256, 1, 9, 13)])
+def test_vae_mid_block_attention_channels_last(C, frames, H, W):
+    """Norm -> q, k, v projections -> the spatial attention core -> output projection + residual:
+    the VAE's mid-block attention on token-major fp16, against 64 bits. Roundings to fp16 on the
+    way: the norm, q, k, v, the probabilities, the attention and the result (the last one is
+    check()'s own), 2^-11 relative each; a softmax over scores of size s turns a relative error of
+    q and k into s times as much, s = 4 at most here: the branch is off by 16 * 2^-11 of its size."""
+    gen = _gen(41)
+    tokens = H * W
+    x = _features((frames, tokens, C), gen, F16)
+    gw, gb = 1 + 0.1 * _normal((C,), gen), 0.1 * _normal((C,), gen)
+    ws = [(_normal((C, C), gen) * C ** -0.5).half() for _ in range(4)]
+    bs = [0.1 * _normal((C,), gen) for _ in range(4)]
+    h = s2b200.group_norm_act(x, 32, gw, gb)
+    q, k, v = (s2b200.linear_act(h, w, b).view(-1, C) for w, b in zip(ws[:3], bs))
+    o = torch.empty_like(q)
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    s2b200.spatial_attention(q, k, v, C, frames, tokens, o, err)
+    y = s2b200.linear_act(o.view_as(x), ws[3], bs[3], residual=x, err=err)
+    assert err.item() == 0
+    h64 = cl.norm_exact(x, 32, gw, gb, 1e-6, "none")[0]
+    q64, k64, v64 = (h64 @ w.double().t() + b.double() for w, b in zip(ws[:3], bs))
+    scores = q64 @ k64.transpose(1, 2) * C ** -0.5
+    branch = torch.softmax(scores, dim=-1) @ v64 @ ws[3].double().t() + bs[3].double()
+    size = branch.abs().mean() + branch.abs()
+    cl.check(y, x.double() + branch, 16 * 2.0 ** -11 * size)
+
+
+def test_timestep_mlp():
+    """One row through silu, silu and a wide projection (the timestep embedding's MLP): each layer
+    against 64 bits of its own input."""
+    gen = _gen(42)
+    t = _normal((1, 256), gen, BF16)
+    dims = (256, 2560, 2560, 15360)
+    for i, act in enumerate(("silu", "silu", "none")):
+        w = (_normal((dims[i + 1], dims[i]), gen) * dims[i] ** -0.5).to(BF16)
+        b = 0.1 * _normal((dims[i + 1],), gen)
+        out = s2b200.linear_act(t, w, b, act)
+        cl.check(out, *cl.linear_exact(t, w, b, act, None))
+        t = out
+
+
+def test_err_word_stays_zero():
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    x, w, b, _ = _operands(500, 256, 512, F16, 43, res=False)
+    s2b200.linear_act(x, w, b, err=err)
+    s2b200.group_norm_act(x.view(5, 100, 512), 32, err=err)
+    assert err.item() == 0
