@@ -1,84 +1,652 @@
 // Matrix product with bias, activation and residual (s2_linear_act):
 //   y[m][n] = act(sum_k x[m][k] w[n][k] + bias[n]) + residual[m][n],
 // x, w fp16 or bf16, the sum and everything after it in fp32, one rounding at the end.
+//
+// Two kernels on the tensor cores (tcgen05, accumulators in TMEM, operands staged by TMA in
+// 64-element K slices, 128-byte swizzle, out-of-range rows and K read as zeros):
+//  * linear_tile_kernel, many rows: a pair of CTAs computes 256 x 256 tiles of y, persistent,
+//    two accumulators, so that a tile's epilogue runs beside the next tile's products.
+//  * linear_rows_kernel, few rows: the operands change sides, 128 rows of w against 16 to 128
+//    rows of x, one tile of y^T a CTA, and K split over the CTAs of a cluster, which join their
+//    sums through distributed shared memory in order. The weights stream through at the rate of
+//    the memory however few rows there are, and no workspace or second launch is needed.
+// Operands whose base or pitch is no multiple of 16 bytes (TMA's rule) are first copied into the
+// workspace with such a pitch (pack_rows_kernel).
+// Every wait is bounded: on timeout the CTA records an error code, drains its copies and
+// products, frees its TMEM and ends.
+#include <cuda.h>
 #include <cuda_runtime.h>
+#include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 
 #include "s2_act.cuh"
+#include "s2_gemm.h"
 #include "s2_internal.h"
+#include "s2_launch.h"
 #include "s2_overlap.h"
+#include "s2_sm100.cuh"
 
 namespace {
 
 using namespace s2dev;
 
 struct LinearArgs {
-    const void *x, *w;
     const float *bias;
     const void *residual;
     void *y;
-    long long M, ldx, ldw, ldr, ldy;
+    long long M, ldr, ldy;
     int N, K, act;
+    uint32_t fmt;     // operand format of the products: 0 fp16, 1 bf16
+    int vec;          // residual and y rows start on 16 bytes
+    int ks;           // linear_rows_kernel: CTAs that share a tile's K
+    int32_t *err;
 };
 
-__device__ __forceinline__ float activate_any(float v, int act)
+constexpr int kBK = 64;  // K elements a slice (one 128-byte swizzled row)
+
+// device error codes of these kernels
+enum : int { E_FULL = 80, E_EMPTY = 81, E_ACCF = 82, E_ACCE = 83, E_DRAIN = 84 };
+
+__device__ __forceinline__ bool wait_drain(uint32_t bar, uint32_t parity, int *err)
+{
+    int dummy = 0;
+    return mbar_wait(bar, parity, &dummy, err, E_DRAIN);
+}
+
+// act over N values; the branch is the same for every thread
+template <int N>
+__device__ __forceinline__ void activate_all(float (&v)[N], int act)
 {
     switch (act) {
-    case S2_ACT_RELU: return activate<S2_ACT_RELU>(v);
-    case S2_ACT_SILU: return activate<S2_ACT_SILU>(v);
-    case S2_ACT_GELU: return activate<S2_ACT_GELU>(v);
-    case S2_ACT_GELU_TANH: return activate<S2_ACT_GELU_TANH>(v);
-    default: return v;
+    case S2_ACT_RELU:
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = activate<S2_ACT_RELU>(v[i]);
+        break;
+    case S2_ACT_SILU:
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = activate<S2_ACT_SILU>(v[i]);
+        break;
+    case S2_ACT_GELU:
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = activate<S2_ACT_GELU>(v[i]);
+        break;
+    case S2_ACT_GELU_TANH:
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = activate<S2_ACT_GELU_TANH>(v[i]);
+        break;
+    default: break;
     }
 }
 
-constexpr int kTile = 64, kSlice = 16;
+// ---- few rows ------------------------------------------------------------------
 
-template <typename T, typename TO>
-__global__ void __launch_bounds__(256) linear_kernel(const LinearArgs a)
+constexpr int kRowsThreads = 192;  // warp 0 TMA, warp 1 products, warps 2-5 epilogue
+constexpr int kRowsN = 128;        // rows of w a tile
+
+template <int MB>
+struct Rows {
+    static constexpr uint32_t kWBytes = kRowsN * kBK * 2, kXBytes = MB * kBK * 2;
+    static constexpr uint32_t kStageBytes = kWBytes + kXBytes;
+    // two CTAs an SM: up to 113 KB each
+    static constexpr int kStages = MB <= 32 ? 5 : (MB == 64 ? 4 : 3);
+    static constexpr uint32_t kOffBar = kStages * kStageBytes;
+    static constexpr uint32_t kSmemBytes = kOffBar + 128 + 1024;
+    static constexpr uint32_t kTmemCols = MB < 32 ? 32 : MB;
+    static_assert(kSmemBytes <= 113 * 1024, "two CTAs an SM");
+    static_assert(MB * kRowsN * 4 <= kOffBar, "the partial sums reuse the stages");
+};
+
+template <typename TO>
+__device__ __forceinline__ void finish_value(const LinearArgs &a, float &v, float res, long long m, int n)
 {
-    __shared__ float xs[kSlice][kTile + 4], ws[kSlice][kTile + 4];
-    const long long m0 = 1LL * blockIdx.x * kTile;
-    const int n0 = blockIdx.y * kTile;
-    const int tm = threadIdx.x / 16 * 4, tn = threadIdx.x % 16 * 4;
-    const T *x = static_cast<const T *>(a.x), *w = static_cast<const T *>(a.w);
-    float acc[4][4] = {};
-    for (int k0 = 0; k0 < a.K; k0 += kSlice) {
-        for (int i = threadIdx.x; i < kTile * kSlice; i += 256) {
-            const int r = i / kSlice, k = i % kSlice;
-            xs[k][r] = m0 + r < a.M && k0 + k < a.K ? to_float<T>(x[(m0 + r) * a.ldx + k0 + k]) : 0.f;
-            ws[k][r] = n0 + r < a.N && k0 + k < a.K ? to_float<T>(w[(n0 + r) * a.ldw + k0 + k]) : 0.f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < kSlice; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(xs[k][tm + i], ws[k][tn + j], acc[i][j]);
-        __syncthreads();
-    }
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const long long m = m0 + tm + i;
-            const int n = n0 + tn + j;
-            if (m >= a.M || n >= a.N) continue;
-            float v = activate_any(acc[i][j] + (a.bias ? a.bias[n] : 0.f), a.act);
-            if (a.residual) v += to_float<TO>(static_cast<const TO *>(a.residual)[m * a.ldr + n]);
-            static_cast<TO *>(a.y)[m * a.ldy + n] = from_float<TO>(v);
-        }
+    static_cast<TO *>(a.y)[m * a.ldy + n] = from_float<TO>(v + res);
 }
 
-template <typename T>
-void launch(const LinearArgs &a, bool f32_out, cudaStream_t st)
+template <int MB, typename TO>
+__global__ void __launch_bounds__(kRowsThreads)
+    linear_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+                       const LinearArgs a)
 {
-    const dim3 grid(static_cast<unsigned>((a.M + kTile - 1) / kTile), static_cast<unsigned>((a.N + kTile - 1) / kTile));
-    if (f32_out)
-        linear_kernel<T, float><<<grid, 256, 0, st>>>(a);
-    else
-        linear_kernel<T, T><<<grid, 256, 0, st>>>(a);
+    using R = Rows<MB>;
+    constexpr int kStages = R::kStages;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    uint8_t *gbase = smem_raw + (base - raw);
+    const uint32_t bar_full = base + R::kOffBar, bar_empty = bar_full + 8 * kStages, bar_acc = bar_empty + 8 * kStages;
+    volatile int *abort = reinterpret_cast<volatile int *>(gbase + R::kOffBar + 16 * kStages + 8);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(gbase + R::kOffBar + 16 * kStages + 12);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = static_cast<int>(blockIdx.x) % a.ks;
+    const int n0 = static_cast<int>(blockIdx.x) / a.ks * kRowsN;
+    const long long m0 = static_cast<long long>(blockIdx.y) * MB;
+    const int n_k = (a.K + kBK - 1) / kBK;
+    const int k_lo = static_cast<int>(1LL * n_k * rank / a.ks), k_hi = static_cast<int>(1LL * n_k * (rank + 1) / a.ks);
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2 * kStages + 1; ++i) mbar_init(bar_full + 8 * i, 1);
+        *abort = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(tmem_slot), R::kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t p = 0;
+            for (int kc = k_lo; kc < k_hi; ++kc, ++p) {
+                const uint32_t s = p % kStages, u = p / kStages;
+                if (!mbar_wait(bar_empty + 8 * s, (u & 1u) ^ 1u, abort, a.err, E_EMPTY)) break;
+                const uint32_t sa = base + s * R::kStageBytes;
+                mbar_arrive_expect_tx(bar_full + 8 * s, R::kStageBytes);
+                tma_load_2d(sa, &tmW, bar_full + 8 * s, kc * kBK, n0);
+                tma_load_2d(sa + R::kWBytes, &tmX, bar_full + 8 * s, kc * kBK, static_cast<int>(m0));
+            }
+            // no copy may still be landing when the stages are reused
+            for (uint32_t s = 0; s < kStages; ++s)
+                if (p > s) wait_drain(bar_full + 8 * s, ((p - 1 - s) / kStages) & 1u, a.err);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const uint32_t idesc = idesc_f16(a.fmt, MB, 0);
+            const uint64_t d0 = smem_desc_sw128(base, 16, 1024);
+            uint32_t p = 0;
+            for (int kc = k_lo; kc < k_hi; ++kc, ++p) {
+                const uint32_t s = p % kStages, u = p / kStages;
+                if (!mbar_wait(bar_full + 8 * s, u & 1u, abort, a.err, E_FULL)) break;
+                tc_fence_after();
+                const uint64_t dw = d0 + static_cast<uint64_t>((s * R::kStageBytes) >> 4);
+                const uint64_t dx = dw + static_cast<uint64_t>(R::kWBytes >> 4);
+                mma_chunk_ss_k64(tmem, dw, dx, idesc, kc > k_lo ? 1u : 0u);
+                mma_commit(bar_empty + 8 * s);
+            }
+            mma_commit(bar_acc);
+            wait_drain(bar_acc, 0, a.err);
+        }
+        __syncwarp();
+    } else {
+        bool ok = mbar_wait(bar_acc, 0, abort, a.err, E_ACCF);
+        ok = __all_sync(0xffffffffu, ok);
+        tc_fence_after();
+        const int quad = warp & 3;
+        const uint32_t taddr = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+        const int nl = quad * 32 + lane, n = n0 + nl;
+        const int cols = static_cast<int>(min(static_cast<long long>(MB), a.M - m0));  // rows of x in this tile
+        float *part = reinterpret_cast<float *>(gbase);
+        if (ok && a.ks > 1) {
+            for (int c = 0; c < cols; c += 32) {
+                uint32_t r[32];
+                tmem_ld32(taddr + c, r);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (c + i < cols) part[(c + i) * kRowsN + nl] = __uint_as_float(r[i]);
+            }
+        } else if (ok) {
+            const float bias = a.bias && n < a.N ? __ldg(a.bias + n) : 0.f;
+            const TO *res = static_cast<const TO *>(a.residual);
+            TO *y = static_cast<TO *>(a.y);
+            for (int c = 0; c < cols; c += 32) {
+                uint32_t r[32];
+                tmem_ld32(taddr + c, r);
+                TO rv[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    rv[i] = res && n < a.N && c + i < cols ? res[(m0 + c + i) * a.ldr + n] : from_float<TO>(0.f);
+                tmem_wait_ld();
+                float v[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]) + bias;
+                activate_all<32>(v, a.act);
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (n < a.N && c + i < cols)
+                        y[(m0 + c + i) * a.ldy + n] = from_float<TO>(v[i] + to_float<TO>(rv[i]));
+            }
+        }
+    }
+    if (a.ks > 1) {
+        // every CTA's sums of its part of K lie in its shared memory: rank r adds those of rows
+        // [MB r / ks, MB (r + 1) / ks) of x, in the order of the parts, and finishes them
+        __syncwarp();
+        cluster_sync();
+        if (warp >= 2) {
+            const int nl = (warp & 3) * 32 + lane, n = n0 + nl;
+            const int cols = static_cast<int>(min(static_cast<long long>(MB), a.M - m0));
+            const int c0 = MB * rank / a.ks, c1 = min(cols, MB * (rank + 1) / a.ks);
+            const float bias = a.bias && n < a.N ? __ldg(a.bias + n) : 0.f;
+            const TO *res = static_cast<const TO *>(a.residual);
+            for (int c = c0; c < c1; ++c) {
+                const uint32_t at = base + static_cast<uint32_t>(c * kRowsN + nl) * 4;
+                const float rv = res && n < a.N ? to_float<TO>(res[(m0 + c) * a.ldr + n]) : 0.f;
+                float q[8];
+#pragma unroll
+                for (int t = 0; t < 8; ++t) q[t] = t < a.ks ? ld_cluster_f32(cluster_map(at, t)) : 0.f;
+                float v[1] = {q[0]};
+#pragma unroll
+                for (int t = 1; t < 8; ++t)
+                    if (t < a.ks) v[0] += q[t];
+                v[0] += bias;
+                activate_all<1>(v, a.act);
+                if (n < a.N) static_cast<TO *>(a.y)[(m0 + c) * a.ldy + n] = from_float<TO>(v[0] + rv);
+            }
+        }
+        __syncwarp();
+        cluster_sync();  // no CTA leaves while others read its sums
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, R::kTmemCols);
+    }
+}
+
+// ---- many rows -------------------------------------------------------------------
+
+constexpr int kTileThreads = 320;  // warp 0 TMA, warp 1 products, warps 2-9 epilogue
+constexpr int kTileN = 256, kTileHalf = 128;
+
+struct Tile {
+    static constexpr uint32_t kABytes = kTileHalf * kBK * 2, kBBytes = kTileHalf * kBK * 2;
+    static constexpr uint32_t kStageBytes = kABytes + kBBytes;  // of each CTA of the pair
+    static constexpr int kStages = 6;
+    static constexpr uint32_t kSlabBytes = 32 * 128;  // an epilogue warp's 32 rows x 128 bytes
+    static constexpr uint32_t kOffSlab = kStages * kStageBytes;
+    static constexpr uint32_t kOffBar = kOffSlab + 8 * kSlabBytes;
+    static constexpr uint32_t kSmemBytes = kOffBar + 256 + 1024;
+    static_assert(kSmemBytes <= 232448, "shared memory budget");
+};
+enum TileBar {
+    T_FULL = 0,
+    T_EMPTY = T_FULL + Tile::kStages,
+    T_ACCF = T_EMPTY + Tile::kStages,
+    T_ACCE = T_ACCF + 2,
+    T_DRAIN = T_ACCE + 2,
+    T_COUNT
+};
+static_assert(8 * T_COUNT + 8 <= 256, "barrier area");
+
+// Tiles in bands of kBand row blocks, column by column in a band: the CTA pairs that run at one
+// time share few blocks of x and of w.
+constexpr int kBand = 8;
+__device__ __forceinline__ void tile_of(int t, int m_blocks, int n_blocks, int &mb, int &nb)
+{
+    const int per = kBand * n_blocks, band = t / per, in = t - band * per;
+    const int rows = min(kBand, m_blocks - band * kBand);
+    nb = in / rows;
+    mb = band * kBand + in - nb * rows;
+}
+
+template <typename TO>
+__global__ void __launch_bounds__(kTileThreads, 1)
+    linear_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
+                       const LinearArgs a)
+{
+    constexpr int kStages = Tile::kStages;
+    constexpr int kE = 16 / sizeof(TO);   // values of 16 bytes
+    constexpr int kSlab = 8 * kE;         // columns of a slab
+    const uint32_t rank = cluster_rank();
+    const int unit = static_cast<int>(blockIdx.x >> 1), n_units = static_cast<int>(gridDim.x >> 1);
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    uint8_t *gbase = smem_raw + (base - raw);
+    const uint32_t bar0 = base + Tile::kOffBar;
+    volatile int *abort = reinterpret_cast<volatile int *>(gbase + Tile::kOffBar + 8 * T_COUNT);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(gbase + Tile::kOffBar + 8 * T_COUNT + 4);
+    auto bar = [&](int i) { return bar0 + 8u * static_cast<uint32_t>(i); };
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int n_blocks = (a.N + kTileN - 1) / kTileN, m_blocks = static_cast<int>((a.M + 255) / 256);
+    const int n_tiles = m_blocks * n_blocks;
+    const int n_k = (a.K + kBK - 1) / kBK;
+
+    if (threadIdx.x == 0) {
+        // the accumulator-empty barriers (rank 0's) count both CTAs' epilogue threads
+        for (int i = 0; i < T_COUNT; ++i) mbar_init(bar(i), i >= T_ACCE && i < T_ACCE + 2 ? 512u : 1u);
+        *abort = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(smem_u32(tmem_slot), 2 * kTileN);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();  // both CTAs' barriers exist before any signal between them
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            tma_prefetch_desc(&tmX);
+            tma_prefetch_desc(&tmW);
+            uint32_t p = 0;
+            bool ok = true;
+            for (int t = unit; ok && t < n_tiles; t += n_units) {
+                int mb, nb;
+                tile_of(t, m_blocks, n_blocks, mb, nb);
+                const int m0 = mb * 256 + static_cast<int>(rank) * kTileHalf;
+                const int n0 = nb * kTileN + static_cast<int>(rank) * kTileHalf;
+                for (int kc = 0; kc < n_k; ++kc, ++p) {
+                    const uint32_t s = p % kStages, u = p / kStages;
+                    if (!(ok = mbar_wait(bar(T_EMPTY + s), (u & 1u) ^ 1u, abort, a.err, E_EMPTY))) break;
+                    const uint32_t sa = base + s * Tile::kStageBytes;
+                    // both CTAs' slices are counted on rank 0's barrier
+                    if (rank == 0) mbar_arrive_expect_tx(bar(T_FULL + s), 2 * Tile::kStageBytes);
+                    const uint32_t fb = cluster_map(bar(T_FULL + s), 0);
+                    tma_load_2d_pair(sa, &tmX, fb, kc * kBK, m0);
+                    tma_load_2d_pair(sa + Tile::kABytes, &tmW, fb, kc * kBK, n0);
+                }
+            }
+            // No copy may still be landing when the CTA exits: rank 0 drains the full barriers, rank 1
+            // waits for its last stages to be released by the products that read them.
+            for (uint32_t s = 0; s < kStages; ++s)
+                if (p > s) wait_drain(bar((rank == 0 ? T_FULL : T_EMPTY) + s), ((p - 1 - s) / kStages) & 1u, a.err);
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            const uint32_t idesc = idesc_f16(a.fmt, kTileN, 0, 256u);
+            const uint64_t d0 = smem_desc_sw128(base, 16, 1024);
+            auto commit = [&](uint32_t b) {  // arrives in both CTAs
+                mma_commit_pair(cluster_map(b, 0));
+                mma_commit_pair(cluster_map(b, 1));
+            };
+            uint32_t p = 0, lt = 0;
+            bool ok = true;
+            for (int t = unit; ok && t < n_tiles; t += n_units, ++lt) {
+                const uint32_t b = lt & 1u;
+                if (!(ok = mbar_wait(bar(T_ACCE + b), ((lt >> 1) & 1u) ^ 1u, abort, a.err, E_ACCE))) break;
+                tc_fence_after();
+                for (int kc = 0; kc < n_k; ++kc, ++p) {
+                    const uint32_t s = p % kStages, u = p / kStages;
+                    if (!(ok = mbar_wait(bar(T_FULL + s), u & 1u, abort, a.err, E_FULL))) break;
+                    tc_fence_after();
+                    const uint64_t da = d0 + static_cast<uint64_t>((s * Tile::kStageBytes) >> 4);
+                    const uint64_t db = da + static_cast<uint64_t>(Tile::kABytes >> 4);
+                    mma_chunk_pair_k64(tmem + b * kTileN, da, db, idesc, kc > 0 ? 1u : 0u);
+                    commit(bar(T_EMPTY + s));
+                }
+                if (!ok) break;
+                commit(bar(T_ACCF + b));
+            }
+            mma_commit_pair(cluster_map(bar(T_DRAIN), 0));
+            wait_drain(bar(T_DRAIN), 0, a.err);
+        }
+    } else {
+        // Warp w holds TMEM lanes 32 (w % 4) .. +31, rows of the tile, and one half of its columns.
+        // A slab is 32 rows x 128 bytes of y: the residual comes in by whole row pieces (each load
+        // instruction four rows x 128 bytes) through shared memory to the thread of its row, the
+        // values of y go back the same way. 16-byte piece k of row r lies at k ^ (r % 8).
+        const int quad = warp & 3, half = (warp - 2) >> 2;
+        const uint32_t lane_off = static_cast<uint32_t>(quad * 32) << 16;
+        uint8_t *slab = gbase + Tile::kOffSlab + (warp - 2) * Tile::kSlabBytes;
+        uint4 *slab4 = reinterpret_cast<uint4 *>(slab);
+        const TO *res = static_cast<const TO *>(a.residual);
+        TO *y = static_cast<TO *>(a.y);
+        const bool bias4 = (reinterpret_cast<uintptr_t>(a.bias) & 15) == 0;
+        const int lrow = lane >> 3, lch = lane & 7;
+
+        uint4 ahead[8];  // the next slab's residual pieces
+        auto fetch = [&](long long m, int n) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const long long row = m + 4 * i + lrow;
+                const int col = n + lch * kE;
+                if (row < a.M && col + kE <= a.N) ahead[i] = __ldcs(reinterpret_cast<const uint4 *>(res + row * a.ldr + col));
+            }
+        };
+        uint32_t lt = 0;
+        bool ok = true;
+        for (int t = unit; ok && t < n_tiles; t += n_units, ++lt) {
+            int mb, nb;
+            tile_of(t, m_blocks, n_blocks, mb, nb);
+            const long long m0 = mb * 256LL + rank * kTileHalf + quad * 32;
+            const int n_lo = nb * kTileN + half * kTileHalf, n_hi = min(a.N, n_lo + kTileHalf);
+            const uint32_t b = lt & 1u;
+            const bool direct = res && a.vec && a.N % kE == 0;
+            if (direct && n_lo < n_hi) fetch(m0, n_lo);
+            ok = mbar_wait(bar(T_ACCF + b), (lt >> 1) & 1u, abort, a.err, E_ACCF);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            for (int n = n_lo; n < n_hi; n += kSlab) {
+                if (direct) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int r = 4 * i + lrow;
+                        slab4[r * 8 + (lch ^ (r & 7))] = ahead[i];
+                    }
+                    if (n + kSlab < n_hi) fetch(m0, n + kSlab);
+                } else if (res) {
+                    for (int r = 0; r < 32; ++r)
+                        for (int c = lane; c < kSlab; c += 32)
+                            if (m0 + r < a.M && n + c < n_hi)
+                                reinterpret_cast<TO *>(slab)[(r * 8 + ((c / kE) ^ (r & 7))) * kE + c % kE] =
+                                    res[(m0 + r) * a.ldr + n + c];
+                }
+                __syncwarp();
+#pragma unroll
+                for (int h = 0; h < kSlab / 32; ++h) {
+                    uint32_t r32[32];
+                    tmem_ld32(tmem + lane_off + b * kTileN + static_cast<uint32_t>(n - nb * kTileN + 32 * h), r32);
+                    tmem_wait_ld();
+                    float v[32];
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) {
+                        const int col = n + 32 * h + 4 * q;
+                        float4 bv = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (a.bias && bias4 && col + 4 <= a.N) {
+                            bv = __ldg(reinterpret_cast<const float4 *>(a.bias + col));
+                        } else if (a.bias) {
+                            if (col < a.N) bv.x = __ldg(a.bias + col);
+                            if (col + 1 < a.N) bv.y = __ldg(a.bias + col + 1);
+                            if (col + 2 < a.N) bv.z = __ldg(a.bias + col + 2);
+                            if (col + 3 < a.N) bv.w = __ldg(a.bias + col + 3);
+                        }
+                        v[4 * q] = __uint_as_float(r32[4 * q]) + bv.x;
+                        v[4 * q + 1] = __uint_as_float(r32[4 * q + 1]) + bv.y;
+                        v[4 * q + 2] = __uint_as_float(r32[4 * q + 2]) + bv.z;
+                        v[4 * q + 3] = __uint_as_float(r32[4 * q + 3]) + bv.w;
+                    }
+                    activate_all<32>(v, a.act);
+#pragma unroll
+                    for (int k = 0; k < 32 / kE; ++k) {
+                        uint4 &cell = slab4[lane * 8 + ((h * (32 / kE) + k) ^ (lane & 7))];
+                        float *f = v + k * kE;
+                        if constexpr (sizeof(TO) == 4) {
+                            if (res) {
+                                const float4 q = *reinterpret_cast<const float4 *>(&cell);
+                                f[0] += q.x;
+                                f[1] += q.y;
+                                f[2] += q.z;
+                                f[3] += q.w;
+                            }
+                            *reinterpret_cast<float4 *>(&cell) = make_float4(f[0], f[1], f[2], f[3]);
+                        } else {
+                            if (res) {
+                                const uint4 q = cell;
+                                const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    const float2 g = unpack2<TO>(u[j]);
+                                    f[2 * j] += g.x;
+                                    f[2 * j + 1] += g.y;
+                                }
+                            }
+                            cell = make_uint4(pack2<TO>(f[0], f[1]), pack2<TO>(f[2], f[3]), pack2<TO>(f[4], f[5]),
+                                              pack2<TO>(f[6], f[7]));
+                        }
+                    }
+                }
+                if (n + kSlab >= n_hi) {
+                    // the accumulator is read: the products of the tile after the next may overwrite it
+                    tc_fence_before();
+                    if (rank == 0)
+                        mbar_arrive(bar(T_ACCE + b));
+                    else
+                        mbar_arrive_remote_relaxed(cluster_map(bar(T_ACCE + b), 0));
+                }
+                __syncwarp();
+                if (a.vec) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int r = 4 * i + lrow, col = n + lch * kE;
+                        if (m0 + r < a.M) {
+                            const uint4 q = slab4[r * 8 + (lch ^ (r & 7))];
+                            TO *dst = y + (m0 + r) * a.ldy + col;
+                            if (col + kE <= a.N) {
+                                __stcs(reinterpret_cast<uint4 *>(dst), q);
+                            } else {
+                                const TO *e = reinterpret_cast<const TO *>(&slab4[r * 8 + (lch ^ (r & 7))]);
+                                for (int j = 0; j < kE; ++j)
+                                    if (col + j < a.N) dst[j] = e[j];
+                            }
+                        }
+                    }
+                } else {
+                    for (int r = 0; r < 32; ++r)
+                        for (int c = lane; c < kSlab; c += 32)
+                            if (m0 + r < a.M && n + c < n_hi)
+                                y[(m0 + r) * a.ldy + n + c] =
+                                    reinterpret_cast<const TO *>(slab)[(r * 8 + ((c / kE) ^ (r & 7))) * kE + c % kE];
+                }
+                __syncwarp();
+            }
+            if (n_lo >= n_hi) {  // no columns of this half inside y
+                tc_fence_before();
+                if (rank == 0)
+                    mbar_arrive(bar(T_ACCE + b));
+                else
+                    mbar_arrive_remote_relaxed(cluster_map(bar(T_ACCE + b), 0));
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();  // no CTA leaves while its partner may still signal it
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem, 2 * kTileN);
+    }
+}
+
+// ---- operands TMA cannot read -----------------------------------------------------
+
+// Rows of K 16-bit values at any pitch -> rows at `ldd`, a multiple of 8 values. A block a row
+// piece; what lies between K and ldd is not written (the tensor map ends at K).
+__global__ void __launch_bounds__(256) pack_rows_kernel(const uint16_t *__restrict__ src, long long lds, long long rows,
+                                                        int K, uint16_t *__restrict__ dst, long long ldd)
+{
+    for (long long r = blockIdx.x; r < rows; r += gridDim.x)
+        for (int k = threadIdx.x; k < K; k += 256) dst[r * ldd + k] = src[r * lds + k];
+}
+
+long long round_up8(long long v) { return (v + 7) / 8 * 8; }
+
+bool tma_ready(const void *p, long long ld, long long rows)
+{
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows == 1 || ld % 8 == 0);
+}
+
+template <int MB, typename TO>
+s2_status launch_rows(LinearArgs a, int ks, const void *x, long long ldx, const void *w, long long ldw, cudaStream_t st)
+{
+    using R = Rows<MB>;
+    CUtensorMap mw, mx;
+    if (!s2::make_map_2d(&mw, w, a.K, a.N, ldw * 2, kBK, kRowsN) || !s2::make_map_2d(&mx, x, a.K, a.M, ldx * 2, kBK, MB))
+        return s2::set_error(S2_INFERENCE_FAILED, "s2_linear_act: cuTensorMapEncodeTiled failed");
+    static std::atomic<uint64_t> configured{0};
+    const s2_status cs = s2::once_per_device(configured, [] {
+        const cudaError_t e = cudaFuncSetAttribute(linear_rows_kernel<MB, TO>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   R::kSmemBytes);
+        return e == cudaSuccess ? S2_OK : s2::set_error(S2_INFERENCE_FAILED, "s2_linear_act: %s", cudaGetErrorString(e));
+    });
+    if (cs != S2_OK) return cs;
+    a.ks = ks;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(ks);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>((a.N + kRowsN - 1) / kRowsN * ks), static_cast<unsigned>((a.M + MB - 1) / MB));
+    cfg.blockDim = dim3(kRowsThreads);
+    cfg.dynamicSmemBytes = R::kSmemBytes;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, linear_rows_kernel<MB, TO>, mw, mx, a);
+    return e == cudaSuccess ? S2_OK : s2::set_error(S2_INFERENCE_FAILED, "s2_linear_act: launch failed: %s", cudaGetErrorString(e));
+}
+
+template <typename TO>
+s2_status launch_tile(const LinearArgs &a, int sms, const void *x, long long ldx, const void *w, long long ldw,
+                      cudaStream_t st)
+{
+    CUtensorMap mx, mw;
+    if (!s2::make_map_2d(&mx, x, a.K, a.M, ldx * 2, kBK, kTileHalf) ||
+        !s2::make_map_2d(&mw, w, a.K, a.N, ldw * 2, kBK, kTileHalf))
+        return s2::set_error(S2_INFERENCE_FAILED, "s2_linear_act: cuTensorMapEncodeTiled failed");
+    static std::atomic<uint64_t> configured{0};
+    const s2_status cs = s2::once_per_device(configured, [] {
+        const cudaError_t e = cudaFuncSetAttribute(linear_tile_kernel<TO>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   Tile::kSmemBytes);
+        return e == cudaSuccess ? S2_OK : s2::set_error(S2_INFERENCE_FAILED, "s2_linear_act: %s", cudaGetErrorString(e));
+    });
+    if (cs != S2_OK) return cs;
+    const long long tiles = (a.M + 255) / 256 * ((a.N + kTileN - 1) / kTileN);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(2 * std::min<long long>(tiles, sms / 2)));
+    cfg.blockDim = dim3(kTileThreads);
+    cfg.dynamicSmemBytes = Tile::kSmemBytes;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, linear_tile_kernel<TO>, mx, mw, a);
+    return e == cudaSuccess ? S2_OK : s2::set_error(S2_INFERENCE_FAILED, "s2_linear_act: launch failed: %s", cudaGetErrorString(e));
+}
+
+template <typename TO>
+s2_status launch_linear(const LinearArgs &a, const void *x, long long ldx, const void *w, long long ldw, cudaStream_t st)
+{
+    int dev = 0, sms = 148;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    const long long tiles = (a.M + 255) / 256 * ((a.N + kTileN - 1) / kTileN);
+    if (tiles * 2 > sms && a.M > 128) {
+        if (tiles > (1LL << 30)) return s2::set_error(S2_UNSUPPORTED, "s2_linear_act: too many tiles");
+        return launch_tile<TO>(a, sms, x, ldx, w, ldw, st);
+    }
+    const int mb = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;
+    const long long ctas = (a.N + kRowsN - 1LL) / kRowsN * ((a.M + mb - 1) / mb);
+    const int n_k = (a.K + kBK - 1) / kBK;
+    int ks = 8;
+    while (ks > 1 && (ctas * ks > 2LL * sms || n_k < 2 * ks)) ks /= 2;
+    switch (mb) {
+    case 16: return launch_rows<16, TO>(a, ks, x, ldx, w, ldw, st);
+    case 32: return launch_rows<32, TO>(a, ks, x, ldx, w, ldw, st);
+    case 64: return launch_rows<64, TO>(a, ks, x, ldx, w, ldw, st);
+    default: return launch_rows<128, TO>(a, ks, x, ldx, w, ldw, st);
+    }
 }
 
 s2_status check(const s2_linear_act_desc *d)
@@ -123,8 +691,11 @@ s2_status check_operands(const s2_linear_act_desc &d)
 extern "C" size_t s2_linear_act_workspace_bytes(const s2_linear_act_desc *d)
 {
     s2::clear_error();
-    check(d);
-    return 0;
+    if (check(d) != S2_OK || d->M == 0) return 0;
+    size_t need = 0;
+    if (!tma_ready(d->x, d->ldx, d->M)) need += static_cast<size_t>(d->M) * round_up8(d->K) * 2;
+    if (!tma_ready(d->w, d->ldw, d->N)) need += static_cast<size_t>(d->N) * round_up8(d->K) * 2;
+    return need;
 }
 
 extern "C" s2_status s2_linear_act(void *stream, const s2_linear_act_desc *d, int *launches)
@@ -135,26 +706,49 @@ extern "C" s2_status s2_linear_act(void *stream, const s2_linear_act_desc *d, in
     if (s != S2_OK) return s;
     if (d->M == 0) return S2_OK;
     if ((s = check_operands(*d)) != S2_OK) return s;
+    const size_t need = s2_linear_act_workspace_bytes(d);
+    if (need > 0 && (!d->workspace || d->workspace_bytes < need || reinterpret_cast<uintptr_t>(d->workspace) % 16))
+        return s2::set_error(S2_INVALID_ARGUMENT, "s2_linear_act: workspace of %zu bytes, 16-byte aligned, needed", need);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    int count = 0;
+    uint16_t *ws = static_cast<uint16_t *>(d->workspace);
+    // an operand as TMA reads it: in place, or packed
+    auto operand = [&](const void *p, long long ld, long long rows, const void **out, long long *ldo) {
+        *out = p;
+        *ldo = rows == 1 ? round_up8(d->K) : ld;
+        if (tma_ready(p, ld, rows)) return;
+        *ldo = round_up8(d->K);
+        pack_rows_kernel<<<static_cast<unsigned>(std::min<long long>(rows, 65536)), 256, 0, st>>>(
+            static_cast<const uint16_t *>(p), ld, rows, d->K, ws, *ldo);
+        *out = ws;
+        ws += rows * *ldo;
+        ++count;
+    };
+    const void *x, *w;
+    long long ldx, ldw;
+    operand(d->x, d->ldx, d->M, &x, &ldx);
+    operand(d->w, d->ldw, d->N, &w, &ldw);
+
     LinearArgs a;
-    a.x = d->x;
-    a.w = d->w;
     a.bias = d->bias;
     a.residual = d->residual;
     a.y = d->y;
     a.M = d->M;
-    a.ldx = d->ldx;
-    a.ldw = d->ldw;
     a.ldr = d->ldr;
     a.ldy = d->ldy;
     a.N = d->N;
     a.K = d->K;
     a.act = d->activation;
-    if (d->dtype == S2_F16)
-        launch<__half>(a, d->out_dtype == S2_F32, static_cast<cudaStream_t>(stream));
-    else
-        launch<__nv_bfloat16>(a, d->out_dtype == S2_F32, static_cast<cudaStream_t>(stream));
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return s2::set_error(S2_INFERENCE_FAILED, "s2_linear_act: launch failed: %s", cudaGetErrorString(e));
-    if (launches) *launches = 1;
+    a.fmt = d->dtype == S2_BF16 ? 1u : 0u;
+    const uintptr_t oe = d->out_dtype == S2_F32 ? 4 : 2;
+    a.vec = (reinterpret_cast<uintptr_t>(d->y) | d->ldy * oe | reinterpret_cast<uintptr_t>(d->residual) |
+             (d->residual ? d->ldr * oe : 0)) % 16 == 0;
+    a.ks = 1;
+    a.err = d->err;
+    s = d->out_dtype == S2_F32   ? launch_linear<float>(a, x, ldx, w, ldw, st)
+        : d->out_dtype == S2_F16 ? launch_linear<__half>(a, x, ldx, w, ldw, st)
+                                 : launch_linear<__nv_bfloat16>(a, x, ldx, w, ldw, st);
+    if (s != S2_OK) return s;
+    if (launches) *launches = count + 1;
     return S2_OK;
 }

@@ -186,6 +186,14 @@ __device__ __forceinline__ uint32_t cluster_map(uint32_t saddr, uint32_t rank)
     return r;
 }
 
+// 32-bit value of another CTA's shared memory (a cluster_map address)
+__device__ __forceinline__ float ld_cluster_f32(uint32_t caddr)
+{
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(caddr) : "memory");
+    return v;
+}
+
 __device__ __forceinline__ void cluster_sync()
 {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
