@@ -21,6 +21,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cstdint>
+#include <type_traits>
 
 #include "s2_act.cuh"
 #include "s2_gemm.h"
@@ -48,7 +49,7 @@ struct LinearArgs {
 constexpr int kBK = 64;  // K elements a slice (one 128-byte swizzled row)
 
 // device error codes of these kernels
-enum : int { E_FULL = 80, E_EMPTY = 81, E_ACCF = 82, E_ACCE = 83, E_DRAIN = 84 };
+enum : int { E_FULL = 80, E_EMPTY = 81, E_ACCF = 82, E_ACCE = 83, E_DRAIN = 84, E_RES = 85 };
 
 __device__ __forceinline__ bool wait_drain(uint32_t bar, uint32_t parity, int *err)
 {
@@ -96,17 +97,11 @@ struct Rows {
     static constexpr uint32_t kSmemBytes = kOffBar + 128 + 1024;
     static constexpr uint32_t kTmemCols = MB < 32 ? 32 : MB;
     static_assert(kSmemBytes <= 113 * 1024, "two CTAs an SM");
-    static_assert(MB * kRowsN * 4 <= kOffBar, "the partial sums reuse the stages");
+    static_assert(MB * kRowsN * 4 <= kOffBar, "the joined sums reuse the stages");
 };
 
-template <typename TO>
-__device__ __forceinline__ void finish_value(const LinearArgs &a, float &v, float res, long long m, int n)
-{
-    static_cast<TO *>(a.y)[m * a.ldy + n] = from_float<TO>(v + res);
-}
-
 template <int MB, typename TO>
-__global__ void __launch_bounds__(kRowsThreads)
+__global__ void __launch_bounds__(kRowsThreads, 2)
     linear_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                        const LinearArgs a)
 {
@@ -176,80 +171,194 @@ __global__ void __launch_bounds__(kRowsThreads)
         }
         __syncwarp();
     } else {
-        bool ok = mbar_wait(bar_acc, 0, abort, a.err, E_ACCF);
-        ok = __all_sync(0xffffffffu, ok);
+        const bool ok = mbar_wait(bar_acc, 0, abort, a.err, E_ACCF);
+        __all_sync(0xffffffffu, ok);
         tc_fence_after();
-        const int quad = warp & 3;
-        const uint32_t taddr = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-        const int nl = quad * 32 + lane, n = n0 + nl;
-        const int cols = static_cast<int>(min(static_cast<long long>(MB), a.M - m0));  // rows of x in this tile
-        float *part = reinterpret_cast<float *>(gbase);
-        if (ok && a.ks > 1) {
-            for (int c = 0; c < cols; c += 32) {
-                uint32_t r[32];
-                tmem_ld32(taddr + c, r);
-                tmem_wait_ld();
+    }
+    // CTA r joins and finishes rows [MB r / ks, MB (r + 1) / ks) of x: once no CTA reads its stages any
+    // more, every CTA sends it its sums, [part][row][128] in place of the stages, and they are added in
+    // the order of the parts. (Sent, not fetched: fetches would cost a round trip a row.)
+    __syncwarp();
+    if (a.ks > 1) cluster_sync();
+    const int cols = static_cast<int>(min(static_cast<long long>(MB), a.M - m0));
+    const int share = MB / a.ks, shift = 31 - __clz(share);
+    const int quad = warp & 3, nl = quad * 32 + lane, n = n0 + nl;
+    if (warp >= 2) {
+        for (int c = 0; c < cols; c += 16) {
+            uint32_t r[16];
+            tmem_ld16(tmem + (static_cast<uint32_t>(quad * 32) << 16) + c, r);
+            tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (c + i < cols) part[(c + i) * kRowsN + nl] = __uint_as_float(r[i]);
-            }
-        } else if (ok) {
-            const float bias = a.bias && n < a.N ? __ldg(a.bias + n) : 0.f;
-            const TO *res = static_cast<const TO *>(a.residual);
-            TO *y = static_cast<TO *>(a.y);
-            for (int c = 0; c < cols; c += 32) {
-                uint32_t r[32];
-                tmem_ld32(taddr + c, r);
-                TO rv[32];
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    rv[i] = res && n < a.N && c + i < cols ? res[(m0 + c + i) * a.ldr + n] : from_float<TO>(0.f);
-                tmem_wait_ld();
-                float v[32];
-#pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]) + bias;
-                activate_all<32>(v, a.act);
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (n < a.N && c + i < cols)
-                        y[(m0 + c + i) * a.ldy + n] = from_float<TO>(v[i] + to_float<TO>(rv[i]));
+            for (int i = 0; i < 16; ++i) {
+                const uint32_t to = static_cast<uint32_t>(c + i) >> shift, row = (c + i) & (share - 1);
+                const uint32_t at = base + static_cast<uint32_t>((rank * share + row) * kRowsN + nl) * 4;
+                if (c + i < cols) st_cluster_b32(cluster_map(at, to), r[i]);
             }
         }
     }
-    if (a.ks > 1) {
-        // every CTA's sums of its part of K lie in its shared memory: rank r adds those of rows
-        // [MB r / ks, MB (r + 1) / ks) of x, in the order of the parts, and finishes them
-        __syncwarp();
+    __syncwarp();
+    if (a.ks > 1)
         cluster_sync();
-        if (warp >= 2) {
-            const int nl = (warp & 3) * 32 + lane, n = n0 + nl;
-            const int cols = static_cast<int>(min(static_cast<long long>(MB), a.M - m0));
-            const int c0 = MB * rank / a.ks, c1 = min(cols, MB * (rank + 1) / a.ks);
-            const float bias = a.bias && n < a.N ? __ldg(a.bias + n) : 0.f;
-            const TO *res = static_cast<const TO *>(a.residual);
-            for (int c = c0; c < c1; ++c) {
-                const uint32_t at = base + static_cast<uint32_t>(c * kRowsN + nl) * 4;
-                const float rv = res && n < a.N ? to_float<TO>(res[(m0 + c) * a.ldr + n]) : 0.f;
-                float q[8];
+    else
+        __syncthreads();
+    if (warp >= 2 && n < a.N) {
+        const float *part = reinterpret_cast<const float *>(gbase) + nl;
+        const float bias = a.bias ? __ldg(a.bias + n) : 0.f;
+        const int c0 = rank * share, c1 = min(cols, c0 + share);
+        const TO *res = static_cast<const TO *>(a.residual) + (m0 + c0) * a.ldr + n;
+        TO *y = static_cast<TO *>(a.y) + (m0 + c0) * a.ldy + n;
+        constexpr int kRun = 8;  // rows at a time: their residuals are all asked for first
+        for (int i = 0; c0 + i < c1; i += kRun) {
+            float rv[kRun], v[kRun];
 #pragma unroll
-                for (int t = 0; t < 8; ++t) q[t] = t < a.ks ? ld_cluster_f32(cluster_map(at, t)) : 0.f;
-                float v[1] = {q[0]};
+            for (int k = 0; k < kRun; ++k)
+                rv[k] = a.residual && c0 + i + k < c1 ? to_float<TO>(res[(i + k) * a.ldr]) : 0.f;
 #pragma unroll
-                for (int t = 1; t < 8; ++t)
-                    if (t < a.ks) v[0] += q[t];
-                v[0] += bias;
-                activate_all<1>(v, a.act);
-                if (n < a.N) static_cast<TO *>(a.y)[(m0 + c) * a.ldy + n] = from_float<TO>(v[0] + rv);
-            }
+            for (int k = 0; k < kRun; ++k) v[k] = part[min(i + k, share - 1) * kRowsN];
+            for (int t = 1; t < a.ks; ++t)
+#pragma unroll
+                for (int k = 0; k < kRun; ++k) v[k] += part[(t * share + min(i + k, share - 1)) * kRowsN];
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) v[k] += bias;
+            activate_all<kRun>(v, a.act);
+#pragma unroll
+            for (int k = 0; k < kRun; ++k)
+                if (c0 + i + k < c1) y[(i + k) * a.ldy] = from_float<TO>(v[k] + rv[k]);
         }
-        __syncwarp();
-        cluster_sync();  // no CTA leaves while others read its sums
     }
     tc_fence_before();
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem, R::kTmemCols);
+    }
+}
+
+// ---- up to four rows ---------------------------------------------------------------
+
+constexpr int kVecThreads = 256, kVecWarps = kVecThreads / 32;
+
+// VEC 16-bit values as they are loaded
+template <int VEC>
+struct Raw;
+template <>
+struct Raw<8> {
+    using type = uint4;
+    static __device__ __forceinline__ uint4 zero() { return make_uint4(0, 0, 0, 0); }
+    static __device__ __forceinline__ uint4 load(const void *p) { return __ldg(static_cast<const uint4 *>(p)); }
+    // weights, read once: past L1
+    static __device__ __forceinline__ uint4 stream(const void *p)
+    {
+        uint4 v;
+        asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                     : "l"(p));
+        return v;
+    }
+    template <typename T>
+    static __device__ __forceinline__ void floats(const uint4 &v, float (&f)[8])
+    {
+        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 q = unpack2<T>(u[i]);
+            f[2 * i] = q.x;
+            f[2 * i + 1] = q.y;
+        }
+    }
+};
+template <>
+struct Raw<1> {
+    using type = uint16_t;
+    static __device__ __forceinline__ uint16_t zero() { return 0; }
+    static __device__ __forceinline__ uint16_t load(const void *p) { return __ldg(static_cast<const uint16_t *>(p)); }
+    static __device__ __forceinline__ uint16_t stream(const void *p) { return load(p); }
+    template <typename T>
+    static __device__ __forceinline__ void floats(uint16_t v, float (&f)[1])
+    {
+        f[0] = to_float<T>(*reinterpret_cast<const T *>(&v));
+    }
+};
+
+// One to four rows of x: every warp streams two rows of w, a.ks warps (1, 2, 4 or 8) share their K
+// by pieces of 32 vectors. VEC = 8: w and x rows start on 16 bytes; else values one by one.
+template <typename T, typename TO, int MR, int VEC>
+__global__ void __launch_bounds__(kVecThreads)
+    linear_vec_kernel(const T *__restrict__ x, long long ldx, const T *__restrict__ w, long long ldw, const LinearArgs a)
+{
+    constexpr int kPiece = 32 * VEC, kAhead = VEC == 8 ? 4 : 8;
+    __shared__ float sums[kVecWarps][2 * MR];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int group = (static_cast<int>(blockIdx.x) * kVecWarps + warp) / a.ks, part = warp % a.ks;
+    const int n = 2 * group;
+    float acc[2][MR] = {};
+    if (n < a.N) {
+        const T *w0 = w + n * ldw + lane * VEC;
+        const T *w1 = w + min(n + 1, a.N - 1) * ldw + lane * VEC;
+        const T *xl = x + lane * VEC;
+        const int step = kPiece * a.ks, whole = a.K / VEC * VEC - (lane + 1) * VEC;
+        for (int k = part * kPiece; k < a.K; k += kAhead * step) {
+            typename Raw<VEC>::type q[2][kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const bool in = k + u * step <= whole;
+                q[0][u] = in ? Raw<VEC>::stream(w0 + k + u * step) : Raw<VEC>::zero();
+                q[1][u] = in ? Raw<VEC>::stream(w1 + k + u * step) : Raw<VEC>::zero();
+            }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+                if (k + u * step <= whole) {
+                    float f0[VEC], f1[VEC];
+                    Raw<VEC>::template floats<T>(q[0][u], f0);
+                    Raw<VEC>::template floats<T>(q[1][u], f1);
+#pragma unroll
+                    for (int m = 0; m < MR; ++m) {
+                        float f[VEC];
+                        Raw<VEC>::template floats<T>(Raw<VEC>::load(xl + min(static_cast<long long>(m), a.M - 1) * ldx + k + u * step), f);
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) {
+                            acc[0][m] = fmaf(f0[e], f[e], acc[0][m]);
+                            acc[1][m] = fmaf(f1[e], f[e], acc[1][m]);
+                        }
+                    }
+                }
+        }
+        // the values past the last whole vector, one a lane
+        const int tail = a.K / VEC * VEC + lane;
+        if (VEC > 1 && part == 0 && tail < a.K) {
+#pragma unroll
+            for (int m = 0; m < MR; ++m) {
+                const float f = to_float<T>(x[min(static_cast<long long>(m), a.M - 1) * ldx + tail]);
+                acc[0][m] = fmaf(to_float<T>(w[n * ldw + tail]), f, acc[0][m]);
+                acc[1][m] = fmaf(to_float<T>(w[min(n + 1, a.N - 1) * ldw + tail]), f, acc[1][m]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int m = 0; m < MR; ++m)
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) acc[i][m] += __shfl_xor_sync(0xffffffffu, acc[i][m], o);
+    }
+    if (lane == 0)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int m = 0; m < MR; ++m) sums[warp][i * MR + m] = acc[i][m];
+    __syncthreads();
+    // thread (group of the block, i, m): the parts' sums in order, then the epilogue
+    const int groups = kVecWarps / a.ks;
+    if (threadIdx.x < groups * 2 * MR) {
+        const int g = threadIdx.x / (2 * MR), im = threadIdx.x % (2 * MR), m = im % MR;
+        const int col = 2 * (static_cast<int>(blockIdx.x) * groups + g) + im / MR;
+        if (col < a.N && m < a.M) {
+            float v[1] = {sums[g * a.ks][im]};
+            for (int t = 1; t < a.ks; ++t) v[0] += sums[g * a.ks + t][im];
+            if (a.bias) v[0] += __ldg(a.bias + col);
+            activate_all<1>(v, a.act);
+            if (a.residual) v[0] += to_float<TO>(static_cast<const TO *>(a.residual)[m * a.ldr + col]);
+            static_cast<TO *>(a.y)[m * a.ldy + col] = from_float<TO>(v[0]);
+        }
     }
 }
 
@@ -261,11 +370,12 @@ constexpr int kTileN = 256, kTileHalf = 128;
 struct Tile {
     static constexpr uint32_t kABytes = kTileHalf * kBK * 2, kBBytes = kTileHalf * kBK * 2;
     static constexpr uint32_t kStageBytes = kABytes + kBBytes;  // of each CTA of the pair
-    static constexpr int kStages = 6;
-    static constexpr uint32_t kSlabBytes = 32 * 128;  // an epilogue warp's 32 rows x 128 bytes
+    static constexpr int kStages = 5;
+    static constexpr uint32_t kSlabBytes = 32 * 128;  // 32 rows x 128 bytes of y; each epilogue warp has two
     static constexpr uint32_t kOffSlab = kStages * kStageBytes;
-    static constexpr uint32_t kOffBar = kOffSlab + 8 * kSlabBytes;
-    static constexpr uint32_t kSmemBytes = kOffBar + 256 + 1024;
+    static constexpr uint32_t kOffBias = kOffSlab + 16 * kSlabBytes;
+    static constexpr uint32_t kOffBar = kOffBias + kTileN * 4;
+    static constexpr uint32_t kSmemBytes = kOffBar + 384 + 1024;
     static_assert(kSmemBytes <= 232448, "shared memory budget");
 };
 enum TileBar {
@@ -274,9 +384,10 @@ enum TileBar {
     T_ACCF = T_EMPTY + Tile::kStages,
     T_ACCE = T_ACCF + 2,
     T_DRAIN = T_ACCE + 2,
-    T_COUNT
+    T_RES = T_DRAIN + 1,  // [8 epilogue warps][2] a residual slab has landed
+    T_COUNT = T_RES + 16
 };
-static_assert(8 * T_COUNT + 8 <= 256, "barrier area");
+static_assert(8 * T_COUNT + 8 <= 384, "barrier area");
 
 // Tiles in bands of kBand row blocks, column by column in a band: the CTA pairs that run at one
 // time share few blocks of x and of w.
@@ -292,6 +403,7 @@ __device__ __forceinline__ void tile_of(int t, int m_blocks, int n_blocks, int &
 template <typename TO>
 __global__ void __launch_bounds__(kTileThreads, 1)
     linear_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
+                       const __grid_constant__ CUtensorMap tmR, const __grid_constant__ CUtensorMap tmY,
                        const LinearArgs a)
 {
     constexpr int kStages = Tile::kStages;
@@ -387,111 +499,133 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
     } else {
         // Warp w holds TMEM lanes 32 (w % 4) .. +31, rows of the tile, and one half of its columns.
-        // A slab is 32 rows x 128 bytes of y: the residual comes in by whole row pieces (each load
-        // instruction four rows x 128 bytes) through shared memory to the thread of its row, the
-        // values of y go back the same way. 16-byte piece k of row r lies at k ^ (r % 8).
-        const int quad = warp & 3, half = (warp - 2) >> 2;
+        // A slab is 32 rows x 128 bytes of y. With aligned rows (a.vec) its residual is brought in and
+        // its values are stored by TMA, one slab ahead and one behind; 16-byte piece k of row r lies at
+        // k ^ (r % 8), TMA's 128-byte swizzle, so that a thread's row is read without conflicts.
+        // Otherwise the warp moves slabs value by value, whole rows at a time.
+        const int quad = warp & 3, half = (warp - 2) >> 2, hw = warp - 2;
         const uint32_t lane_off = static_cast<uint32_t>(quad * 32) << 16;
-        uint8_t *slab = gbase + Tile::kOffSlab + (warp - 2) * Tile::kSlabBytes;
-        uint4 *slab4 = reinterpret_cast<uint4 *>(slab);
+        const uint32_t slab_s = base + Tile::kOffSlab + hw * 2 * Tile::kSlabBytes;
+        uint8_t *slab_g = gbase + Tile::kOffSlab + hw * 2 * Tile::kSlabBytes;
+        float *bias_g = reinterpret_cast<float *>(gbase + Tile::kOffBias) + hw * 32;  // of the warp's 32 columns
         const TO *res = static_cast<const TO *>(a.residual);
         TO *y = static_cast<TO *>(a.y);
-        const bool bias4 = (reinterpret_cast<uintptr_t>(a.bias) & 15) == 0;
-        const int lrow = lane >> 3, lch = lane & 7;
+        const bool ahead = res && a.vec;
 
-        uint4 ahead[8];  // the next slab's residual pieces
-        auto fetch = [&](long long m, int n) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const long long row = m + 4 * i + lrow;
-                const int col = n + lch * kE;
-                if (row < a.M && col + kE <= a.N) ahead[i] = __ldcs(reinterpret_cast<const uint4 *>(res + row * a.ldr + col));
+        // asks for the residual of slab `js` (counted over the warp's tiles) at column n of row m
+        auto ask = [&](uint32_t js, int n, int m) {
+            if (lane == 0) {
+                const uint32_t rb = bar(T_RES + 2 * hw + (js & 1u));
+                mbar_arrive_expect_tx(rb, Tile::kSlabBytes);
+                tma_load_2d(slab_s + (js & 1u) * Tile::kSlabBytes, &tmR, rb, n, m);
             }
         };
-        uint32_t lt = 0;
+        auto ask_tile = [&](uint32_t js, int t) {
+            int mb, nb;
+            tile_of(t, m_blocks, n_blocks, mb, nb);
+            ask(js, nb * kTileN + half * kTileHalf, mb * 256 + static_cast<int>(rank) * kTileHalf + quad * 32);
+        };
+        uint32_t lt = 0, js = 0, asked = 0;  // slabs begun, residual slabs asked for
         bool ok = true;
+        if (ahead && unit < n_tiles) {
+            ask_tile(0, unit);
+            asked = 1;
+        }
         for (int t = unit; ok && t < n_tiles; t += n_units, ++lt) {
             int mb, nb;
             tile_of(t, m_blocks, n_blocks, mb, nb);
-            const long long m0 = mb * 256LL + rank * kTileHalf + quad * 32;
-            const int n_lo = nb * kTileN + half * kTileHalf, n_hi = min(a.N, n_lo + kTileHalf);
+            const int m0 = mb * 256 + static_cast<int>(rank) * kTileHalf + quad * 32;
+            const int n_lo = nb * kTileN + half * kTileHalf;
             const uint32_t b = lt & 1u;
-            const bool direct = res && a.vec && a.N % kE == 0;
-            if (direct && n_lo < n_hi) fetch(m0, n_lo);
             ok = mbar_wait(bar(T_ACCF + b), (lt >> 1) & 1u, abort, a.err, E_ACCF);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
-            for (int n = n_lo; n < n_hi; n += kSlab) {
-                if (direct) {
+#pragma unroll 1
+            for (int s = 0; ok && s < kTileHalf / kSlab; ++s, ++js) {
+                const int n = n_lo + s * kSlab;
+                float bias[kSlab / 32];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int r = 4 * i + lrow;
-                        slab4[r * 8 + (lch ^ (r & 7))] = ahead[i];
+                for (int h = 0; h < kSlab / 32; ++h)
+                    bias[h] = a.bias && n + 32 * h + lane < a.N ? __ldg(a.bias + n + 32 * h + lane) : 0.f;
+                const uint32_t buf = js & 1u;
+                uint4 *slab4 = reinterpret_cast<uint4 *>(slab_g + buf * Tile::kSlabBytes);
+                TO *slab = reinterpret_cast<TO *>(slab4);
+                if (ahead) {
+                    // the other slab is free once its store has read it
+                    const bool more = s + 1 < kTileHalf / kSlab;
+                    if (more || t + n_units < n_tiles) {
+                        if (lane == 0) bulk_wait_group_read<0>();
+                        if (more)
+                            ask(js + 1, n + kSlab, m0);
+                        else
+                            ask_tile(js + 1, t + n_units);
+                        ++asked;
                     }
-                    if (n + kSlab < n_hi) fetch(m0, n + kSlab);
-                } else if (res) {
-                    for (int r = 0; r < 32; ++r)
-                        for (int c = lane; c < kSlab; c += 32)
-                            if (m0 + r < a.M && n + c < n_hi)
-                                reinterpret_cast<TO *>(slab)[(r * 8 + ((c / kE) ^ (r & 7))) * kE + c % kE] =
-                                    res[(m0 + r) * a.ldr + n + c];
+                    ok = mbar_wait(bar(T_RES + 2 * hw + buf), (js >> 1) & 1u, abort, a.err, E_RES);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                } else {
+                    if (lane == 0) bulk_wait_group_read<1>();
+                    __syncwarp();
+                    if (res)
+                        for (int r = 0; r < 32; ++r)
+                            for (int c = lane; c < kSlab; c += 32)
+                                if (m0 + r < a.M && n + c < a.N)
+                                    slab[(r * 8 + ((c / kE) ^ (r & 7))) * kE + c % kE] = res[(m0 + r) * a.ldr + n + c];
                 }
                 __syncwarp();
 #pragma unroll
                 for (int h = 0; h < kSlab / 32; ++h) {
+                    __syncwarp();
+                    bias_g[lane] = bias[h];
+                    __syncwarp();
                     uint32_t r32[32];
-                    tmem_ld32(tmem + lane_off + b * kTileN + static_cast<uint32_t>(n - nb * kTileN + 32 * h), r32);
+                    tmem_ld32(tmem + lane_off + b * kTileN + static_cast<uint32_t>(half * kTileHalf + s * kSlab + 32 * h), r32);
                     tmem_wait_ld();
                     float v[32];
 #pragma unroll
                     for (int q = 0; q < 8; ++q) {
-                        const int col = n + 32 * h + 4 * q;
-                        float4 bv = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (a.bias && bias4 && col + 4 <= a.N) {
-                            bv = __ldg(reinterpret_cast<const float4 *>(a.bias + col));
-                        } else if (a.bias) {
-                            if (col < a.N) bv.x = __ldg(a.bias + col);
-                            if (col + 1 < a.N) bv.y = __ldg(a.bias + col + 1);
-                            if (col + 2 < a.N) bv.z = __ldg(a.bias + col + 2);
-                            if (col + 3 < a.N) bv.w = __ldg(a.bias + col + 3);
-                        }
+                        const float4 bv = *reinterpret_cast<const float4 *>(bias_g + 4 * q);
                         v[4 * q] = __uint_as_float(r32[4 * q]) + bv.x;
                         v[4 * q + 1] = __uint_as_float(r32[4 * q + 1]) + bv.y;
                         v[4 * q + 2] = __uint_as_float(r32[4 * q + 2]) + bv.z;
                         v[4 * q + 3] = __uint_as_float(r32[4 * q + 3]) + bv.w;
                     }
                     activate_all<32>(v, a.act);
+                    uint4 *cell[32 / kE];
 #pragma unroll
-                    for (int k = 0; k < 32 / kE; ++k) {
-                        uint4 &cell = slab4[lane * 8 + ((h * (32 / kE) + k) ^ (lane & 7))];
-                        float *f = v + k * kE;
-                        if constexpr (sizeof(TO) == 4) {
-                            if (res) {
-                                const float4 q = *reinterpret_cast<const float4 *>(&cell);
-                                f[0] += q.x;
-                                f[1] += q.y;
-                                f[2] += q.z;
-                                f[3] += q.w;
-                            }
-                            *reinterpret_cast<float4 *>(&cell) = make_float4(f[0], f[1], f[2], f[3]);
-                        } else {
-                            if (res) {
-                                const uint4 q = cell;
-                                const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+                    for (int k = 0; k < 32 / kE; ++k) cell[k] = slab4 + lane * 8 + ((h * (32 / kE) + k) ^ (lane & 7));
+                    if (res) {
 #pragma unroll
-                                for (int j = 0; j < 4; ++j) {
+                        for (int k = 0; k < 32 / kE; ++k) {
+                            const uint4 q = *cell[k];
+                            const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+                            float *f = v + k * kE;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                if constexpr (sizeof(TO) == 4) {
+                                    f[j] += __uint_as_float(u[j]);
+                                } else {
                                     const float2 g = unpack2<TO>(u[j]);
                                     f[2 * j] += g.x;
                                     f[2 * j + 1] += g.y;
                                 }
                             }
-                            cell = make_uint4(pack2<TO>(f[0], f[1]), pack2<TO>(f[2], f[3]), pack2<TO>(f[4], f[5]),
-                                              pack2<TO>(f[6], f[7]));
                         }
                     }
+#pragma unroll
+                    for (int k = 0; k < 32 / kE; ++k) {
+                        const float *f = v + k * kE;
+                        if constexpr (sizeof(TO) == 4)
+                            *cell[k] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
+                                                  __float_as_uint(f[3]));
+                        else
+                            *cell[k] = make_uint4(pack2<TO>(f[0], f[1]), pack2<TO>(f[2], f[3]), pack2<TO>(f[4], f[5]),
+                                                  pack2<TO>(f[6], f[7]));
+                    }
                 }
-                if (n + kSlab >= n_hi) {
+                if (s + 1 == kTileHalf / kSlab) {
                     // the accumulator is read: the products of the tile after the next may overwrite it
                     tc_fence_before();
                     if (rank == 0)
@@ -499,40 +633,26 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     else
                         mbar_arrive_remote_relaxed(cluster_map(bar(T_ACCE + b), 0));
                 }
-                __syncwarp();
                 if (a.vec) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int r = 4 * i + lrow, col = n + lch * kE;
-                        if (m0 + r < a.M) {
-                            const uint4 q = slab4[r * 8 + (lch ^ (r & 7))];
-                            TO *dst = y + (m0 + r) * a.ldy + col;
-                            if (col + kE <= a.N) {
-                                __stcs(reinterpret_cast<uint4 *>(dst), q);
-                            } else {
-                                const TO *e = reinterpret_cast<const TO *>(&slab4[r * 8 + (lch ^ (r & 7))]);
-                                for (int j = 0; j < kE; ++j)
-                                    if (col + j < a.N) dst[j] = e[j];
-                            }
-                        }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (m0 < a.M && n < a.N) tma_store_2d(&tmY, slab_s + buf * Tile::kSlabBytes, n, m0);
+                        bulk_commit_group();
                     }
                 } else {
+                    __syncwarp();
                     for (int r = 0; r < 32; ++r)
                         for (int c = lane; c < kSlab; c += 32)
-                            if (m0 + r < a.M && n + c < n_hi)
-                                y[(m0 + r) * a.ldy + n + c] =
-                                    reinterpret_cast<const TO *>(slab)[(r * 8 + ((c / kE) ^ (r & 7))) * kE + c % kE];
+                            if (m0 + r < a.M && n + c < a.N)
+                                y[(m0 + r) * a.ldy + n + c] = slab[(r * 8 + ((c / kE) ^ (r & 7))) * kE + c % kE];
+                    __syncwarp();
                 }
-                __syncwarp();
-            }
-            if (n_lo >= n_hi) {  // no columns of this half inside y
-                tc_fence_before();
-                if (rank == 0)
-                    mbar_arrive(bar(T_ACCE + b));
-                else
-                    mbar_arrive_remote_relaxed(cluster_map(bar(T_ACCE + b), 0));
             }
         }
+        // no copy of this warp's may still be under way when the CTA exits
+        if (lane == 0) bulk_wait_group_all();
+        for (; js < asked; ++js) wait_drain(bar(T_RES + 2 * hw + (js & 1u)), (js >> 1) & 1u, a.err);
     }
     __syncwarp();
     tc_fence_before();
@@ -560,6 +680,36 @@ long long round_up8(long long v) { return (v + 7) / 8 * 8; }
 bool tma_ready(const void *p, long long ld, long long rows)
 {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows == 1 || ld % 8 == 0);
+}
+
+constexpr int kVecRows = 4;
+
+template <typename T, typename TO>
+s2_status launch_vec(LinearArgs a, int sms, const s2_linear_act_desc &d, cudaStream_t st)
+{
+    const T *x = static_cast<const T *>(d.x), *w = static_cast<const T *>(d.w);
+    const bool wide = (reinterpret_cast<uintptr_t>(d.x) | reinterpret_cast<uintptr_t>(d.w) |
+                       (d.M > 1 ? d.ldx * 2 : 0) | (d.N > 1 ? d.ldw * 2 : 0)) % 16 == 0;
+    // warps that share a row's K: as many as fill the GPU (32 warps an SM) and have a piece each
+    const int pieces = std::max(1, a.K / (wide ? 256 : 32)), pairs = (a.N + 1) / 2;
+    a.ks = 1;
+    while (a.ks < kVecWarps && a.ks * 2 <= pieces && 1LL * pairs * a.ks < 32LL * sms) a.ks *= 2;
+    const unsigned grid = static_cast<unsigned>((1LL * pairs * a.ks + kVecWarps - 1) / kVecWarps);
+    auto go = [&](auto rows) {
+        constexpr int MR = decltype(rows)::value;
+        if (wide)
+            linear_vec_kernel<T, TO, MR, 8><<<grid, kVecThreads, 0, st>>>(x, d.ldx, w, d.ldw, a);
+        else
+            linear_vec_kernel<T, TO, MR, 1><<<grid, kVecThreads, 0, st>>>(x, d.ldx, w, d.ldw, a);
+    };
+    if (a.M == 1)
+        go(std::integral_constant<int, 1>());
+    else if (a.M == 2)
+        go(std::integral_constant<int, 2>());
+    else
+        go(std::integral_constant<int, 4>());
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? S2_OK : s2::set_error(S2_INFERENCE_FAILED, "s2_linear_act: launch failed: %s", cudaGetErrorString(e));
 }
 
 template <int MB, typename TO>
@@ -601,6 +751,14 @@ s2_status launch_tile(const LinearArgs &a, int sms, const void *x, long long ldx
     if (!s2::make_map_2d(&mx, x, a.K, a.M, ldx * 2, kBK, kTileHalf) ||
         !s2::make_map_2d(&mw, w, a.K, a.N, ldw * 2, kBK, kTileHalf))
         return s2::set_error(S2_INFERENCE_FAILED, "s2_linear_act: cuTensorMapEncodeTiled failed");
+    // slabs of y and of the residual: 32 rows x 128 bytes, swizzled (16-bit maps move any 16-bit type)
+    auto slab_map = [&](CUtensorMap *map, const void *ptr, long long ld) {
+        return sizeof(TO) == 4 ? s2::make_map_2d_plain_f32(map, ptr, a.N, a.M, ld * 4, 32, 32)
+                               : s2::make_map_2d(map, ptr, a.N, a.M, ld * 2, 64, 32);
+    };
+    CUtensorMap my = mx, mr = mx;  // unused ones repeat a valid map
+    if (a.vec && (!slab_map(&my, a.y, a.ldy) || (a.residual && !slab_map(&mr, a.residual, a.ldr))))
+        return s2::set_error(S2_INFERENCE_FAILED, "s2_linear_act: cuTensorMapEncodeTiled failed");
     static std::atomic<uint64_t> configured{0};
     const s2_status cs = s2::once_per_device(configured, [] {
         const cudaError_t e = cudaFuncSetAttribute(linear_tile_kernel<TO>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -621,16 +779,14 @@ s2_status launch_tile(const LinearArgs &a, int sms, const void *x, long long ldx
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, linear_tile_kernel<TO>, mx, mw, a);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, linear_tile_kernel<TO>, mx, mw, mr, my, a);
     return e == cudaSuccess ? S2_OK : s2::set_error(S2_INFERENCE_FAILED, "s2_linear_act: launch failed: %s", cudaGetErrorString(e));
 }
 
 template <typename TO>
-s2_status launch_linear(const LinearArgs &a, const void *x, long long ldx, const void *w, long long ldw, cudaStream_t st)
+s2_status launch_linear(const LinearArgs &a, int sms, const void *x, long long ldx, const void *w, long long ldw,
+                        cudaStream_t st)
 {
-    int dev = 0, sms = 148;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     const long long tiles = (a.M + 255) / 256 * ((a.N + kTileN - 1) / kTileN);
     if (tiles * 2 > sms && a.M > 128) {
         if (tiles > (1LL << 30)) return s2::set_error(S2_UNSUPPORTED, "s2_linear_act: too many tiles");
@@ -691,7 +847,7 @@ s2_status check_operands(const s2_linear_act_desc &d)
 extern "C" size_t s2_linear_act_workspace_bytes(const s2_linear_act_desc *d)
 {
     s2::clear_error();
-    if (check(d) != S2_OK || d->M == 0) return 0;
+    if (check(d) != S2_OK || d->M <= kVecRows) return 0;
     size_t need = 0;
     if (!tma_ready(d->x, d->ldx, d->M)) need += static_cast<size_t>(d->M) * round_up8(d->K) * 2;
     if (!tma_ready(d->w, d->ldw, d->N)) need += static_cast<size_t>(d->N) * round_up8(d->K) * 2;
@@ -710,25 +866,6 @@ extern "C" s2_status s2_linear_act(void *stream, const s2_linear_act_desc *d, in
     if (need > 0 && (!d->workspace || d->workspace_bytes < need || reinterpret_cast<uintptr_t>(d->workspace) % 16))
         return s2::set_error(S2_INVALID_ARGUMENT, "s2_linear_act: workspace of %zu bytes, 16-byte aligned, needed", need);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    int count = 0;
-    uint16_t *ws = static_cast<uint16_t *>(d->workspace);
-    // an operand as TMA reads it: in place, or packed
-    auto operand = [&](const void *p, long long ld, long long rows, const void **out, long long *ldo) {
-        *out = p;
-        *ldo = rows == 1 ? round_up8(d->K) : ld;
-        if (tma_ready(p, ld, rows)) return;
-        *ldo = round_up8(d->K);
-        pack_rows_kernel<<<static_cast<unsigned>(std::min<long long>(rows, 65536)), 256, 0, st>>>(
-            static_cast<const uint16_t *>(p), ld, rows, d->K, ws, *ldo);
-        *out = ws;
-        ws += rows * *ldo;
-        ++count;
-    };
-    const void *x, *w;
-    long long ldx, ldw;
-    operand(d->x, d->ldx, d->M, &x, &ldx);
-    operand(d->w, d->ldw, d->N, &w, &ldw);
-
     LinearArgs a;
     a.bias = d->bias;
     a.residual = d->residual;
@@ -745,9 +882,39 @@ extern "C" s2_status s2_linear_act(void *stream, const s2_linear_act_desc *d, in
              (d->residual ? d->ldr * oe : 0)) % 16 == 0;
     a.ks = 1;
     a.err = d->err;
-    s = d->out_dtype == S2_F32   ? launch_linear<float>(a, x, ldx, w, ldw, st)
-        : d->out_dtype == S2_F16 ? launch_linear<__half>(a, x, ldx, w, ldw, st)
-                                 : launch_linear<__nv_bfloat16>(a, x, ldx, w, ldw, st);
+    int dev = 0, sms = 148;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    int count = 0;
+    if (d->M <= kVecRows) {
+        const bool f32 = d->out_dtype == S2_F32;
+        if (d->dtype == S2_F16)
+            s = f32 ? launch_vec<__half, float>(a, sms, *d, st) : launch_vec<__half, __half>(a, sms, *d, st);
+        else
+            s = f32 ? launch_vec<__nv_bfloat16, float>(a, sms, *d, st)
+                    : launch_vec<__nv_bfloat16, __nv_bfloat16>(a, sms, *d, st);
+    } else {
+        uint16_t *ws = static_cast<uint16_t *>(d->workspace);
+        // an operand as TMA reads it: in place, or packed
+        auto operand = [&](const void *p, long long ld, long long rows, const void **out, long long *ldo) {
+            *out = p;
+            *ldo = rows == 1 ? round_up8(d->K) : ld;
+            if (tma_ready(p, ld, rows)) return;
+            *ldo = round_up8(d->K);
+            pack_rows_kernel<<<static_cast<unsigned>(std::min<long long>(rows, 65536)), 256, 0, st>>>(
+                static_cast<const uint16_t *>(p), ld, rows, d->K, ws, *ldo);
+            *out = ws;
+            ws += rows * *ldo;
+            ++count;
+        };
+        const void *x, *w;
+        long long ldx, ldw;
+        operand(d->x, d->ldx, d->M, &x, &ldx);
+        operand(d->w, d->ldw, d->N, &w, &ldw);
+        s = d->out_dtype == S2_F32   ? launch_linear<float>(a, sms, x, ldx, w, ldw, st)
+            : d->out_dtype == S2_F16 ? launch_linear<__half>(a, sms, x, ldx, w, ldw, st)
+                                     : launch_linear<__nv_bfloat16>(a, sms, x, ldx, w, ldw, st);
+    }
     if (s != S2_OK) return s;
     if (launches) *launches = count + 1;
     return S2_OK;

@@ -963,83 +963,90 @@ def _fail(what: str):
     raise S2Error(S2_INVALID_ARGUMENT, what)
 
 
-def _activation_code(activation) -> int:
-    code = ACTIVATIONS.get(activation)
-    if code is None:
-        _fail(f"unknown activation {activation!r} (one of {', '.join(ACTIVATIONS)})")
-    return code
+_DTYPES = {}
 
 
 def _type_of(t, what: str) -> int:
-    try:
-        return _dtype_code(t)
-    except KeyError:
+    if not _DTYPES:
+        torch = _torch()
+        _DTYPES.update({torch.float32: S2_F32, torch.float16: S2_F16, torch.bfloat16: S2_BF16})
+    code = _DTYPES.get(t.dtype)
+    if code is None:
         _fail(f"{what} must be fp16, bf16 or fp32, not {t.dtype}")
+    return code
 
 
 def _need_vector(t, n: int, device, what: str):
-    """The address of a contiguous fp32 vector of n values (None: NULL)."""
-    if t is None:
-        return None
+    """The address of a contiguous fp32 vector of n values."""
     if t.device != device or t.dtype != _torch().float32 or t.shape != (n,) or not t.is_contiguous():
         _fail(f"{what} must be a contiguous fp32 tensor of {n} values on {device}")
+    if t.requires_grad:
+        _need_no_grad()
     return t.data_ptr()
 
 
 def _need_err(err, device):
-    if err is None:
-        return None
     if err.device != device or err.dtype != _torch().int32 or err.numel() < 1:
         _fail(f"err must be an int32 tensor on {device}")
     return err.data_ptr()
 
 
-def _need_no_grad(torch, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+def _need_no_grad():
+    if _torch().is_grad_enabled():
         _fail("inference only: a tensor requires a gradient (call under torch.no_grad())")
-
-
-def _on_own_stream(torch, x, stream, call):
-    """call() with x's device current, and `stream` (default: that device's current one)."""
-    if not x.is_cuda:
-        _fail(f"x is on {x.device}: the operators run on a CUDA device")
-    if stream is not None:
-        if stream.device != x.device:
-            _fail(f"the stream is on {stream.device}, x on {x.device}")
-        with torch.cuda.stream(stream):
-            return call()
-    if x.device.index != torch.cuda.current_device():
-        with torch.cuda.device(x.device):
-            return call()
-    return call()
-
-
-def _run_desc(torch, call, workspace_bytes, desc, device, what: str):
-    ref = ctypes.byref(desc)
-    need = workspace_bytes(ref)
-    if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=device)
-        desc.workspace, desc.workspace_bytes = ws.data_ptr(), need
-    status = call(_stream_ptr(), ref, None)
-    if status != S2_OK:
-        _check(status, what)
 
 
 def _pitch(t, first: int, what: str):
     """The dimensions [first, -1) of t as one: (size, pitch in elements). They must be evenly
     spaced, over contiguous channels."""
     shape, strides = t.shape, t.stride()
-    if strides[-1] != 1 and shape[-1] > 1:
+    last = shape[-1]
+    if strides[-1] != 1 and last > 1:
         _fail(f"{what}: the last dimension must be contiguous")
     rows, pitch = 1, None
     for i in range(len(shape) - 2, first - 1, -1):
-        if shape[i] != 1:
+        size = shape[i]
+        if size != 1:
             if pitch is None:
                 pitch = strides[i]
             elif strides[i] != pitch * rows:
                 _fail(f"{what}: its rows must be evenly spaced")
-            rows *= shape[i]
-    return rows, (shape[-1] if pitch is None else pitch)
+            rows *= size
+    return rows, (last if pitch is None else pitch)
+
+
+def _elsewhere(fn, x, stream, *args):
+    """fn(x, *args, stream=None) with x's device, or `stream`, made current."""
+    torch = _torch()
+    if not x.is_cuda:
+        _fail(f"x is on {x.device}: the operators run on a CUDA device")
+    if stream is None:
+        with torch.cuda.device(x.device):
+            return fn(x, *args)
+    if stream.device != x.device:
+        _fail(f"the stream is on {stream.device}, x on {x.device}")
+    with torch.cuda.stream(stream):
+        return fn(x, *args)
+
+
+def _run_desc(call, workspace_bytes, desc, x, index: int, what: str):
+    """Calls with a workspace of the current stream's, on the current stream of the current device."""
+    ref = ctypes.byref(desc)
+    need = workspace_bytes(ref)
+    if need:
+        torch = _torch()
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+        desc.workspace, desc.workspace_bytes = ws.data_ptr(), need
+    status = call(_raw_stream(index), ref, None)
+    if status != S2_OK:
+        _check(status, what)
+
+
+def _raw_stream(index: int) -> int:
+    """The current stream of a device, without the cost of a torch.cuda.Stream object."""
+    torch = _torch()
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(index) if raw is not None else torch.cuda.current_stream(index).cuda_stream
 
 
 def group_norm_act(x, groups: int, weight=None, bias=None, eps: float = 1e-6, activation: str = "none", out=None,
@@ -1050,30 +1057,34 @@ def group_norm_act(x, groups: int, weight=None, bias=None, eps: float = 1e-6, ac
     weight, bias: fp32 [channels] or None. Returns y in out_dtype (x's, or fp16 / bf16 for fp32 x)
     in x's shape; `out` receives it when given (it may be x). err: device int32 error word."""
     torch = _torch()
-
-    def call():
-        y = out
-        if x.dim() < 2:
-            _fail("x must be [samples, ..., channels]")
-        _need_no_grad(torch, x, weight, bias)
-        if y is None:
-            y = torch.empty(x.shape, dtype=out_dtype or x.dtype, device=x.device)
-        elif y.shape != x.shape or y.device != x.device or out_dtype not in (None, y.dtype):
-            _fail("out must have x's shape and device, and out_dtype if both are given")
-        positions, x_row = _pitch(x, 1, "x")
-        _, y_row = _pitch(y, 1, "out")
-        samples, channels = x.shape[0], x.shape[-1]
-        many = samples > 1
-        d = GroupNormActDesc(samples, channels, groups, _activation_code(activation), positions, _type_of(x, "x"),
-                             _type_of(y, "out"), eps, x.data_ptr(), x_row, x.stride(0) if many else 0,
-                             _need_vector(weight, channels, x.device, "weight"),
-                             _need_vector(bias, channels, x.device, "bias"), y.data_ptr(), y_row,
-                             y.stride(0) if many else 0, None, 0, _need_err(err, x.device))
-        L = lib()
-        _run_desc(torch, L.s2_group_norm_act, L.s2_group_norm_act_workspace_bytes, d, x.device, "s2_group_norm_act")
-        return y
-
-    return _on_own_stream(torch, x, stream, call)
+    device = x.device
+    index = device.index
+    if stream is not None or not x.is_cuda or index != torch.cuda.current_device():
+        return _elsewhere(group_norm_act, x, stream, groups, weight, bias, eps, activation, out, out_dtype, err)
+    if x.dim() < 2:
+        _fail("x must be [samples, ..., channels]")
+    code = ACTIVATIONS.get(activation)
+    if code is None:
+        _fail(f"unknown activation {activation!r} (one of {', '.join(ACTIVATIONS)})")
+    if x.requires_grad:
+        _need_no_grad()
+    shape = x.shape
+    if out is None:
+        out = torch.empty(shape, dtype=out_dtype or x.dtype, device=device)
+    elif out.shape != shape or out.device != device or out_dtype not in (None, out.dtype):
+        _fail("out must have x's shape and device, and out_dtype if both are given")
+    samples, channels = shape[0], shape[-1]
+    positions, x_row = _pitch(x, 1, "x")
+    _, y_row = _pitch(out, 1, "out")
+    x_sample, y_sample = (x.stride(0), out.stride(0)) if samples > 1 else (0, 0)
+    d = GroupNormActDesc(samples, channels, groups, code, positions, _type_of(x, "x"), _type_of(out, "out"), eps,
+                         x.data_ptr(), x_row, x_sample,
+                         None if weight is None else _need_vector(weight, channels, device, "weight"),
+                         None if bias is None else _need_vector(bias, channels, device, "bias"), out.data_ptr(), y_row,
+                         y_sample, None, 0, None if err is None else _need_err(err, device))
+    L = lib()
+    _run_desc(L.s2_group_norm_act, L.s2_group_norm_act_workspace_bytes, d, x, index, "s2_group_norm_act")
+    return out
 
 
 def linear_act(x, w, bias=None, activation: str = "none", residual=None, out=None, out_dtype=None, err=None,
@@ -1083,34 +1094,39 @@ def linear_act(x, w, bias=None, activation: str = "none", residual=None, out=Non
     output's type or None. Returns y [..., N] in out_dtype (x's, or fp32); `out` receives it when
     given (it may be the residual). err: device int32 error word."""
     torch = _torch()
-
-    def call():
-        y = out
-        if x.dim() < 1 or w.dim() != 2 or w.shape[1] != x.shape[-1] or w.dtype != x.dtype or w.device != x.device:
-            _fail("x must be [..., K] and w [N, K], of one type on one device")
-        _need_no_grad(torch, x, w, bias, residual)
-        N, K = w.shape
-        shape = x.shape[:-1] + (N,)
-        if y is None:
-            y = torch.empty(shape, dtype=out_dtype or x.dtype, device=x.device)
-        elif y.shape != shape or y.device != x.device or out_dtype not in (None, y.dtype):
-            _fail(f"out must be {tuple(shape)} on x's device, and of out_dtype if both are given")
-        rows, ldx = _pitch(x, 0, "x")
-        _, ldw = _pitch(w, 0, "w")
-        _, ldy = _pitch(y, 0, "out")
-        res, ldr = None, 0
-        if residual is not None:
-            if residual.shape != shape or residual.dtype != y.dtype or residual.device != x.device:
-                _fail(f"residual must be {tuple(shape)} in the output's type on x's device")
-            res, ldr = residual.data_ptr(), _pitch(residual, 0, "residual")[1]
-        d = LinearActDesc(N, K, _activation_code(activation), _type_of(x, "x"), _type_of(y, "out"), rows, x.data_ptr(),
-                          ldx, w.data_ptr(), ldw, _need_vector(bias, N, x.device, "bias"), res, ldr, y.data_ptr(),
-                          ldy, None, 0, _need_err(err, x.device))
-        L = lib()
-        _run_desc(torch, L.s2_linear_act, L.s2_linear_act_workspace_bytes, d, x.device, "s2_linear_act")
-        return y
-
-    return _on_own_stream(torch, x, stream, call)
+    device = x.device
+    index = device.index
+    if stream is not None or not x.is_cuda or index != torch.cuda.current_device():
+        return _elsewhere(linear_act, x, stream, w, bias, activation, residual, out, out_dtype, err)
+    if x.dim() < 1 or w.dim() != 2 or w.shape[1] != x.shape[-1] or w.dtype != x.dtype or w.device != device:
+        _fail("x must be [..., K] and w [N, K], of one type on one device")
+    code = ACTIVATIONS.get(activation)
+    if code is None:
+        _fail(f"unknown activation {activation!r} (one of {', '.join(ACTIVATIONS)})")
+    if x.requires_grad or w.requires_grad:
+        _need_no_grad()
+    N, K = w.shape
+    shape = x.shape[:-1] + (N,)
+    if out is None:
+        out = torch.empty(shape, dtype=out_dtype or x.dtype, device=device)
+    elif out.shape != shape or out.device != device or out_dtype not in (None, out.dtype):
+        _fail(f"out must be {tuple(shape)} on x's device, and of out_dtype if both are given")
+    rows, ldx = _pitch(x, 0, "x")
+    _, ldw = _pitch(w, 0, "w")
+    _, ldy = _pitch(out, 0, "out")
+    res, ldr = None, 0
+    if residual is not None:
+        if residual.shape != shape or residual.dtype != out.dtype or residual.device != device:
+            _fail(f"residual must be {tuple(shape)} in the output's type on x's device")
+        if residual.requires_grad:
+            _need_no_grad()
+        res, ldr = residual.data_ptr(), _pitch(residual, 0, "residual")[1]
+    d = LinearActDesc(N, K, code, _type_of(x, "x"), _type_of(out, "out"), rows, x.data_ptr(), ldx, w.data_ptr(), ldw,
+                      None if bias is None else _need_vector(bias, N, device, "bias"), res, ldr, out.data_ptr(), ldy,
+                      None, 0, None if err is None else _need_err(err, device))
+    L = lib()
+    _run_desc(L.s2_linear_act, L.s2_linear_act_workspace_bytes, d, x, index, "s2_linear_act")
+    return out
 
 
 VAE_WEIGHT_ORDER = ("norm_bias", "norm_weight", "k_bias", "k_weight", "out_bias", "out_weight", "q_bias", "q_weight",
