@@ -84,7 +84,20 @@ __device__ __forceinline__ float activate(float v)
 {
     if constexpr (kAct == S2_ACT_RELU) return v < 0.f ? 0.f : v;
     if constexpr (kAct == S2_ACT_SILU) return __fdividef(v, 1.f + __expf(-v));
-    if constexpr (kAct == S2_ACT_GELU) return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
+    if constexpr (kAct == S2_ACT_GELU) {
+        // erfc(u) = t (a1 + t (a2 + ... + t a5)) e^-u^2, t = 1 / (1 + 0.3275911 u), u >= 0, within
+        // 1.5e-7 (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26); here u = |v| /
+        // sqrt 2, and 1 + erf(v / sqrt 2) is erfc(u) below 0 and 2 - erfc(u) above: nothing cancels.
+        // A third of erff's instructions, one branch-free run: the product at 21600 x 10240 x 2560
+        // spends 4500 of a tile's 20500 cycles on its activation with erff.
+        const float t = __fdividef(1.f, fmaf(0.3275911f * 0.70710678118654752f, fabsf(v), 1.f));
+        float p = fmaf(t, 1.061405429f, -1.453152027f);
+        p = fmaf(t, p, 1.421413741f);
+        p = fmaf(t, p, -0.284496736f);
+        p = fmaf(t, p, 0.254829592f);
+        const float c = p * t * __expf(-0.5f * v * v);
+        return 0.5f * v * (v >= 0.f ? 2.f - c : c);
+    }
     if constexpr (kAct == S2_ACT_GELU_TANH) {
         // 0.5 v (1 + tanh u) = v / (1 + e^-2u), u = sqrt(2 / pi) (v + 0.044715 v^3)
         const float u2 = 1.5957691216057308f * v * (1.f + 0.044715f * v * v);

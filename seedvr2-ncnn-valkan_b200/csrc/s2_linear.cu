@@ -153,22 +153,26 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t idesc = idesc_f16(a.fmt, MB, 0);
-            const uint64_t d0 = smem_desc_sw128(base, 16, 1024);
-            uint32_t p = 0;
-            for (int kc = k_lo; kc < k_hi; ++kc, ++p) {
-                const uint32_t s = p % kStages, u = p / kStages;
-                if (!mbar_wait(bar_full + 8 * s, u & 1u, abort, a.err, E_FULL)) break;
-                tc_fence_after();
-                const uint64_t dw = d0 + static_cast<uint64_t>((s * R::kStageBytes) >> 4);
-                const uint64_t dx = dw + static_cast<uint64_t>(R::kWBytes >> 4);
-                mma_chunk_ss_k64(tmem, dw, dx, idesc, kc > k_lo ? 1u : 0u);
+        const bool leader = elect_one();
+        const uint32_t idesc = idesc_f16(a.fmt, MB, 0);
+        const uint64_t d0 = smem_desc_sw128(base, 16, 1024);
+        uint32_t s = 0, phase = 0;
+        for (int kc = k_lo; kc < k_hi; ++kc) {
+            if (!__all_sync(0xffffffffu, mbar_wait(bar_full + 8 * s, phase, abort, a.err, E_FULL))) break;
+            tc_fence_after();
+            const uint64_t dw = d0 + static_cast<uint64_t>((s * R::kStageBytes) >> 4);
+            if (leader) {
+                mma_chunk_ss_k64(tmem, dw, dw + (R::kWBytes >> 4), idesc, kc > k_lo ? 1u : 0u);
                 mma_commit(bar_empty + 8 * s);
             }
-            mma_commit(bar_acc);
-            wait_drain(bar_acc, 0, a.err);
+            __syncwarp();
+            if (++s == kStages) {
+                s = 0;
+                phase ^= 1u;
+            }
         }
+        if (leader) mma_commit(bar_acc);
+        wait_drain(bar_acc, 0, a.err);
         __syncwarp();
     } else {
         const bool ok = mbar_wait(bar_acc, 0, abort, a.err, E_ACCF);
@@ -469,32 +473,40 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 if (p > s) wait_drain(bar((rank == 0 ? T_FULL : T_EMPTY) + s), ((p - 1 - s) / kStages) & 1u, a.err);
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        // The warp stays together and one lane issues: descriptors and barriers stay in uniform
+        // registers, and the issue keeps ahead of the products (with a lone thread's loop they took
+        // 570 to 650 cycles a slice where the tensor cores need 512).
+        if (rank == 0) {
+            const bool leader = elect_one();
             const uint32_t idesc = idesc_f16(a.fmt, kTileN, 0, 256u);
             const uint64_t d0 = smem_desc_sw128(base, 16, 1024);
-            auto commit = [&](uint32_t b) {  // arrives in both CTAs
-                mma_commit_pair(cluster_map(b, 0));
-                mma_commit_pair(cluster_map(b, 1));
-            };
-            uint32_t p = 0, lt = 0;
+            uint32_t lt = 0, s = 0, phase = 0;
             bool ok = true;
             for (int t = unit; ok && t < n_tiles; t += n_units, ++lt) {
                 const uint32_t b = lt & 1u;
-                if (!(ok = mbar_wait(bar(T_ACCE + b), ((lt >> 1) & 1u) ^ 1u, abort, a.err, E_ACCE))) break;
+                ok = __all_sync(0xffffffffu, mbar_wait(bar(T_ACCE + b), ((lt >> 1) & 1u) ^ 1u, abort, a.err, E_ACCE));
+                if (!ok) break;
                 tc_fence_after();
-                for (int kc = 0; kc < n_k; ++kc, ++p) {
-                    const uint32_t s = p % kStages, u = p / kStages;
-                    if (!(ok = mbar_wait(bar(T_FULL + s), u & 1u, abort, a.err, E_FULL))) break;
+                for (int kc = 0; kc < n_k; ++kc) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(bar(T_FULL + s), phase, abort, a.err, E_FULL));
+                    if (!ok) break;
                     tc_fence_after();
                     const uint64_t da = d0 + static_cast<uint64_t>((s * Tile::kStageBytes) >> 4);
-                    const uint64_t db = da + static_cast<uint64_t>(Tile::kABytes >> 4);
-                    mma_chunk_pair_k64(tmem + b * kTileN, da, db, idesc, kc > 0 ? 1u : 0u);
-                    commit(bar(T_EMPTY + s));
+                    if (leader) {
+                        mma_chunk_pair_k64(tmem + b * kTileN, da, da + (Tile::kABytes >> 4), idesc, kc > 0 ? 1u : 0u);
+                        mma_commit_both(bar(T_EMPTY + s));
+                    }
+                    __syncwarp();
+                    if (++s == kStages) {
+                        s = 0;
+                        phase ^= 1u;
+                    }
                 }
                 if (!ok) break;
-                commit(bar(T_ACCF + b));
+                if (leader) mma_commit_both(bar(T_ACCF + b));
+                __syncwarp();
             }
-            mma_commit_pair(cluster_map(bar(T_DRAIN), 0));
+            if (leader) mma_commit_pair(cluster_map(bar(T_DRAIN), 0));
             wait_drain(bar(T_DRAIN), 0, a.err);
         }
     } else {

@@ -246,6 +246,23 @@ __device__ __forceinline__ void mma_commit_pair(uint32_t cluster_bar)
                  : "memory");
 }
 
+// the same to the barrier at this offset in both CTAs of the pair
+__device__ __forceinline__ void mma_commit_both(uint32_t bar)
+{
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
+}
+
+// true in one lane of a converged warp
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 // One K=64 slice of a pair tile D[256][N] (+)= A[256][64] B[N][64]^T: four K=16
 // MMAs; A rows 0-127 / 128-255 and B rows 0-N/2-1 / N/2-N-1 live at the same
 // shared-memory offsets of CTA rank 0 / 1.
