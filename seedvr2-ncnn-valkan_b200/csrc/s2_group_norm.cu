@@ -15,28 +15,45 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
+#include <cstdlib>
 
 #include "s2_act.cuh"
 #include "s2_internal.h"
+#include "s2_launch.h"
 #include "s2_overlap.h"
+#include "s2_sm100.cuh"
 
 namespace {
 
 using namespace s2dev;
 
 constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
 constexpr int kMaxGroups = 1024;
-constexpr int kUnroll = 8;  // rows a thread has in flight
+constexpr int kSliceGroups = 64;   // groups of one unit
+constexpr int kMaxCluster = 8;
+constexpr int kAhead = 8;          // vectors a thread has in flight while it reads
 
+// How the members of a unit exchange their groups' moments.
+enum Join : int {
+    kAlone = 0,    // one block
+    kCluster = 1,  // the blocks of a cluster, through distributed shared memory
+    kGrid = 2,     // blocks of a cooperative grid, through the workspace
+};
+
+// A unit is the slice of `slice_groups` groups of one sample; `members` blocks share its positions:
+// the first `more_rows` of them rows + 1 each, the others `rows`.
 struct GnArgs {
     const void *x;
     void *y;
     const float *weight, *bias;
-    float2 *part;  // [sample][member][group] (mean, M2)
-    long long P, x_row, x_sample, y_row, y_sample;
-    int C, G, cpg, members, act;
+    float2 *part;       // kGrid: [unit][member][group of the slice] (mean, M2)
+    uint32_t *arrived;  // kGrid: [unit] members whose moments are written (zero before)
+    int32_t *err;
+    long long rows, x_row, x_sample, y_row, y_sample;
+    int more_rows, C, G, cpg, slices, slice_groups, units, members, teams, join, hold, act;
+    int group_lanes;    // threads that join one group's moments: a power of two up to 32
     float eps;
 };
 
@@ -44,52 +61,94 @@ struct Moments {
     float n = 0.f, mean = 0.f, m2 = 0.f;
 };
 
+// Both may be empty; the moments of one alone come through unchanged. The reciprocal is the hardware's
+// (1 ulp): it weighs a difference of means, which is 0 for equal ones.
 __device__ __forceinline__ Moments join(const Moments &a, const Moments &b)
 {
-    if (b.n == 0.f) return a;
     Moments r;
     r.n = a.n + b.n;
-    const float d = b.mean - a.mean, w = __fdiv_rn(b.n, r.n);
-    r.mean = fmaf(d, w, a.mean);
-    r.m2 = a.m2 + b.m2 + d * d * a.n * w;
+    const float w = __fdividef(b.n, r.n), d = b.mean - a.mean;
+    const bool both = a.n > 0.f && b.n > 0.f;
+    r.mean = both ? fmaf(d, w, a.mean) : (b.n > 0.f ? b.mean : a.mean);
+    r.m2 = both ? fmaf(d * d, a.n * w, a.m2 + b.m2) : a.m2 + b.m2;
     return r;
 }
 
-// VEC elements of T, 16 bytes or one element
+// `lanes` neighbouring threads' moments in the first of them.
+__device__ __forceinline__ Moments join_lanes(Moments m, int lanes)
+{
+    for (int o = lanes >> 1; o > 0; o >>= 1) {
+        Moments t;
+        t.n = __shfl_down_sync(0xffffffffu, m.n, o);
+        t.mean = __shfl_down_sync(0xffffffffu, m.mean, o);
+        t.m2 = __shfl_down_sync(0xffffffffu, m.m2, o);
+        m = join(m, t);
+    }
+    return m;
+}
+
+// Two floats in one 64-bit register: one instruction works on both.
+__device__ __forceinline__ uint64_t pair(float a, float b)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 floats_of(uint64_t p)
+{
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+// VEC elements of T as they are loaded: 16 bytes or one element
 template <typename T, int VEC>
-struct Vec;
-template <typename T>
-struct Vec<T, 1> {
-    T v;
-    __device__ __forceinline__ void load(const T *p) { v = *p; }
-    __device__ __forceinline__ void floats(float (&f)[1]) const { f[0] = to_float<T>(v); }
-};
-template <typename T>
-struct Vec<T, 8> {
-    uint4 v;
-    __device__ __forceinline__ void load(const T *p) { v = *reinterpret_cast<const uint4 *>(p); }
-    __device__ __forceinline__ void floats(float (&f)[8]) const
+struct Raw {
+    using type = uint4;
+    static __device__ __forceinline__ uint4 load(const T *p)
+    {
+        uint4 v;
+        asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                     : "l"(p)
+                     : "memory");
+        return v;
+    }
+    static __device__ __forceinline__ void floats(const uint4 &v, float (&f)[VEC])
     {
         const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+        if constexpr (sizeof(T) == 4) {
+            static_assert(VEC == 4, "");
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 t = unpack2<T>(u[i]);
-            f[2 * i] = t.x;
-            f[2 * i + 1] = t.y;
+            for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(u[i]);
+        } else {
+            static_assert(VEC == 8, "");
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 t = unpack2<T>(u[i]);
+                f[2 * i] = t.x;
+                f[2 * i + 1] = t.y;
+            }
         }
     }
 };
-template <>
-struct Vec<float, 4> {
-    float4 v;
-    __device__ __forceinline__ void load(const float *p) { v = *reinterpret_cast<const float4 *>(p); }
-    __device__ __forceinline__ void floats(float (&f)[4]) const
-    {
-        f[0] = v.x;
-        f[1] = v.y;
-        f[2] = v.z;
-        f[3] = v.w;
-    }
+template <typename T>
+struct Raw<T, 1> {
+    using type = T;
+    static __device__ __forceinline__ T load(const T *p) { return *p; }
+    static __device__ __forceinline__ void floats(T v, float (&f)[1]) { f[0] = to_float<T>(v); }
 };
 
 template <typename T, int VEC>
@@ -98,7 +157,6 @@ __device__ __forceinline__ void store_vec(T *p, const float (&f)[VEC])
     if constexpr (VEC == 1) {
         *p = from_float<T>(f[0]);
     } else if constexpr (sizeof(T) == 4) {
-        static_assert(VEC == 4, "");
         *reinterpret_cast<float4 *>(p) = make_float4(f[0], f[1], f[2], f[3]);
     } else if constexpr (VEC == 8) {
         *reinterpret_cast<uint4 *>(p) =
@@ -108,181 +166,470 @@ __device__ __forceinline__ void store_vec(T *p, const float (&f)[VEC])
     }
 }
 
-// Part one: (mean, M2) of every group over the rows of one member of the sample.
-template <typename TI, int VEC>
-__global__ void __launch_bounds__(kThreads) gn_stats_kernel(const GnArgs a)
+// A run: up to kAhead vectors of one column, read, held in shared memory when they come before `hold`,
+// and their moments joined to mo: N = 1 those of all values together, N = VEC of each of a vector's
+// channels. The pivot is the run's first vector.
+template <typename TI, int VEC, int N, bool kFull>
+__device__ __forceinline__ void read_run(const TI *px, long long step, int n, int i, int hold,
+                                         typename Raw<TI, VEC>::type *held, Moments (&mo)[N])
 {
-    __shared__ Moments entry[VEC][kThreads];
-    __shared__ Moments group[kMaxGroups];
-    const int s = blockIdx.y, member = blockIdx.x;
-    const long long r0 = a.P * member / a.members, r1 = a.P * (member + 1) / a.members;
-    const TI *x = static_cast<const TI *>(a.x) + s * a.x_sample;
-    for (int g = threadIdx.x; g < a.G; g += kThreads) group[g] = Moments();
-    const int ncols = a.C / VEC;
-    for (int cb = 0; cb < ncols; cb += kThreads) {
-        // columns [cb, cb + nb) of vectors, `lanes` rows at a time
-        const int nb = min(kThreads, ncols - cb), lanes = kThreads / nb;
-        const int col = threadIdx.x % nb, rl = threadIdx.x / nb;
-        Moments mo[VEC];
-        if (rl < lanes) {
-            const TI *px = x + static_cast<long long>(cb + col) * VEC;
-            for (long long r = r0 + rl; r < r1; r += 1LL * kUnroll * lanes) {
-                Vec<TI, VEC> v[kUnroll];
-                const int n = static_cast<int>(min(1LL * kUnroll, (r1 - r + lanes - 1) / lanes));
+    using R = Raw<TI, VEC>;
+    constexpr int kPairs = VEC > 1 ? VEC / 2 : 1, kSums = N == 1 ? (VEC > 2 ? 2 : 1) : kPairs, kPer = VEC / N;
+    if (kFull) n = kAhead;
+    typename R::type v[kAhead];
 #pragma unroll
-                for (int u = 0; u < kUnroll; ++u)
-                    if (u < n) v[u].load(px + (r + 1LL * u * lanes) * a.x_row);
-                float p[VEC], sum[VEC], sq[VEC];
-                v[0].floats(p);
+    for (int u = 0; u < kAhead; ++u) {
+        if (kFull || u < n) v[u] = R::load(px);
+        px += step;
+    }
+    if (i + kAhead <= hold) {
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) sum[e] = sq[e] = 0.f;
+        for (int u = 0; u < kAhead; ++u)
+            if (kFull || u < n) held[(i + u) * kThreads] = v[u];
+    } else if (i < hold) {
 #pragma unroll
-                for (int u = 1; u < kUnroll; ++u)
-                    if (u < n) {
-                        float f[VEC];
-                        v[u].floats(f);
+        for (int u = 0; u < kAhead; ++u)
+            if (u < n && i + u < hold) held[(i + u) * kThreads] = v[u];
+    }
+    float f[VEC], p[N], sum[N], sq[N];
+    R::floats(v[0], f);
 #pragma unroll
-                        for (int e = 0; e < VEC; ++e) {
-                            const float d = f[e] - p[e];
-                            sum[e] += d;
-                            sq[e] = fmaf(d, d, sq[e]);
-                        }
-                    }
-                const float inv = __fdiv_rn(1.f, static_cast<float>(n));
+    for (int e = 0; e < N; ++e) p[e] = f[e * kPer];
+    if constexpr (VEC == 1) {
+        sum[0] = sq[0] = 0.f;
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    Moments run;
-                    run.n = static_cast<float>(n);
-                    run.mean = fmaf(sum[e], inv, p[e]);
-                    // not below 0 by rounding; 0 * sq keeps the NaN of a value that is not finite
-                    run.m2 = fmaxf(sq[e] - sum[e] * sum[e] * inv, 0.f * sq[e]);
-                    mo[e] = join(mo[e], run);
+        for (int u = 1; u < kAhead; ++u)
+            if (kFull || u < n) {
+                R::floats(v[u], f);
+                const float d = f[0] - p[0];
+                sum[0] += d;
+                sq[0] = fmaf(d, d, sq[0]);
+            }
+    } else {
+        uint64_t minus[N == 1 ? 1 : kPairs], s2[kSums], q2[kSums];
+#pragma unroll
+        for (int k = 0; k < (N == 1 ? 1 : kPairs); ++k)
+            minus[k] = N == 1 ? pair(-p[0], -p[0]) : pair(-p[2 * k < N ? 2 * k : 0], -p[2 * k + 1 < N ? 2 * k + 1 : 0]);
+#pragma unroll
+        for (int k = 0; k < kSums; ++k) s2[k] = q2[k] = 0;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (kFull || u < n) {
+                R::floats(v[u], f);
+#pragma unroll
+                for (int k = 0; k < kPairs; ++k) {
+                    const uint64_t d = add2(pair(f[2 * k], f[2 * k + 1]), minus[N == 1 ? 0 : k]);
+                    s2[k % kSums] = add2(s2[k % kSums], d);
+                    q2[k % kSums] = fma2(d, d, q2[k % kSums]);
                 }
             }
-        }
-        __syncthreads();
+        if constexpr (N == 1) {
+            const float2 a = floats_of(kSums == 2 ? add2(s2[0], s2[kSums - 1]) : s2[0]);
+            const float2 b = floats_of(kSums == 2 ? add2(q2[0], q2[kSums - 1]) : q2[0]);
+            sum[0] = a.x + a.y;
+            sq[0] = b.x + b.y;
+        } else {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) entry[e][threadIdx.x] = mo[e];
-        __syncthreads();
-        // a warp per group that has channels in [cb, cb + nb) * VEC
-        const int c0 = cb * VEC, c1 = (cb + nb) * VEC;
-        for (int g = c0 / a.cpg + (threadIdx.x >> 5); g * a.cpg < c1; g += kWarps) {
-            const int lo = max(c0, g * a.cpg), w = min(c1, (g + 1) * a.cpg) - lo;
+            for (int k = 0; k < kPairs; ++k) {
+                const float2 a = floats_of(s2[k]), b = floats_of(q2[k]);
+                sum[2 * k] = a.x;
+                sum[2 * k + 1] = a.y;
+                sq[2 * k] = b.x;
+                sq[2 * k + 1] = b.y;
+            }
+        }
+    }
+    const float cnt = static_cast<float>(n * kPer), inv = __fdividef(1.f, cnt);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        Moments run;
+        run.n = cnt;
+        run.mean = fmaf(sum[e], inv, p[e]);
+        // not below 0 by rounding; 0 * sq keeps the NaN of a value that is not finite
+        run.m2 = fmaxf(fmaf(-sum[e] * inv, sum[e], sq[e]), 0.f * sq[e]);
+        mo[e] = join(mo[e], run);
+    }
+}
+
+template <typename TI, int VEC, int N>
+__device__ __forceinline__ void read_rows(const TI *px, long long step, int count, int hold,
+                                          typename Raw<TI, VEC>::type *held, Moments (&mo)[N])
+{
+    int i = 0;
+#pragma unroll 1
+    for (; i + kAhead <= count; i += kAhead, px += kAhead * step) read_run<TI, VEC, N, true>(px, step, kAhead, i, hold, held, mo);
+    if (i < count) read_run<TI, VEC, N, false>(px, step, count - i, i, hold, held, mo);
+}
+
+// y = act((x - mean) scale + shift) of one vector; `minus` is -mean, one (kOne) or a pair of channels each.
+// The subtraction comes first, as in the formula: values that all equal the mean give the shift itself.
+template <typename TI, typename TO, int VEC, int N, int kAct>
+__device__ __forceinline__ void finish(const typename Raw<TI, VEC>::type &v, TO *py, const float (&minus)[N],
+                                       const float (&scale)[VEC], const float (&shift)[VEC])
+{
+    float f[VEC];
+    Raw<TI, VEC>::floats(v, f);
+    if constexpr (VEC == 1) {
+        f[0] = fmaf(f[0] + minus[0], scale[0], shift[0]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < VEC / 2; ++k) {
+            const uint64_t d = add2(pair(f[2 * k], f[2 * k + 1]), pair(minus[2 * k % N], minus[(2 * k + 1) % N]));
+            const float2 r = floats_of(fma2(d, pair(scale[2 * k], scale[2 * k + 1]), pair(shift[2 * k], shift[2 * k + 1])));
+            f[2 * k] = r.x;
+            f[2 * k + 1] = r.y;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) f[e] = activate<kAct>(f[e]);
+    store_vec<TO, VEC>(py, f);
+}
+
+// y of the thread's vectors: those that are not held once more from global memory, the latest read
+// first (they are in L2 the longest), then the held ones.
+template <typename TI, typename TO, int VEC, int N, int kAct>
+__device__ __forceinline__ void write_rows(const TI *px, long long x_step, TO *py, long long y_step, int count, int hold,
+                                           const typename Raw<TI, VEC>::type *held, const float (&minus)[N],
+                                           const float (&scale)[VEC], const float (&shift)[VEC])
+{
+    using R = Raw<TI, VEC>;
+    constexpr int kRun = 4;
+    int i = count;
+    if (i > hold) {
+        const TI *qx = px + (count - 1) * x_step;
+        TO *qy = py + (count - 1) * y_step;
+#pragma unroll 1
+        for (; i - kRun >= hold; i -= kRun) {
+            typename R::type v[kRun];
+#pragma unroll
+            for (int u = 0; u < kRun; ++u, qx -= x_step) v[u] = R::load(qx);
+#pragma unroll
+            for (int u = 0; u < kRun; ++u, qy -= y_step) finish<TI, TO, VEC, N, kAct>(v[u], qy, minus, scale, shift);
+        }
+#pragma unroll 1
+        for (; i > hold; --i, qx -= x_step, qy -= y_step) finish<TI, TO, VEC, N, kAct>(R::load(qx), qy, minus, scale, shift);
+    }
+#pragma unroll 2
+    for (int k = 0; k < i; ++k) {
+        finish<TI, TO, VEC, N, kAct>(held[k * kThreads], py, minus, scale, shift);
+        py += y_step;
+    }
+}
+
+__device__ __forceinline__ uint32_t ld_acquire(const uint32_t *p)
+{
+    uint32_t v;
+    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
+
+enum : int { E_JOIN = 96 };  // device error code: the wait for the other members ran out
+
+// kOne: the VEC channels of a vector always belong to one group.
+template <typename TI, typename TO, int VEC, bool kOne>
+__global__ void __launch_bounds__(kThreads, 2) group_norm_kernel(const GnArgs a)
+{
+    using R = Raw<TI, VEC>;
+    constexpr int N = kOne ? 1 : VEC;
+    extern __shared__ uint4 held_raw[];
+    __shared__ float2 entry[N][kThreads];  // (mean, M2) a thread and channel, and of how many values
+    __shared__ float entry_n[kThreads];
+    __shared__ Moments group[kSliceGroups];
+    __shared__ float2 received[kMaxCluster][kSliceGroups];
+    __shared__ float2 norm[kSliceGroups];  // mean, 1 / sqrt(v + eps)
+    __shared__ int gave_up;
+    typename R::type *held = reinterpret_cast<typename R::type *>(held_raw) + threadIdx.x;
+    const int member = static_cast<int>(blockIdx.x) % a.members;
+    const long long r0 = member * a.rows + min(member, a.more_rows), rows = a.rows + (member < a.more_rows);
+    // for the joins of groups: group_lanes threads a group
+    const int sub = static_cast<int>(threadIdx.x) / a.group_lanes, sub_lane = threadIdx.x % a.group_lanes;
+    if (threadIdx.x == 0) gave_up = 0;
+    if (a.join == kCluster) cluster_arrive();  // waited for below: no block writes to one that has not begun
+
+    for (int unit = static_cast<int>(blockIdx.x) / a.members; unit < a.units; unit += a.teams) {
+        const int s = unit / a.slices, g0 = (unit - s * a.slices) * a.slice_groups;
+        const int gs = min(a.slice_groups, a.G - g0), c0 = g0 * a.cpg;
+        const int ncols = gs * a.cpg / VEC;
+        const int hold = ncols <= kThreads ? a.hold : 0;
+        const TI *x = static_cast<const TI *>(a.x) + s * a.x_sample + r0 * a.x_row + c0;
+        if (sub_lane == 0 && sub < gs) group[sub] = Moments();
+
+        // Columns of vectors, kThreads of them at a time (all, unless a single group is wider than that):
+        // a thread keeps one column and takes every lanes-th row.
+        int nb = 0, lanes = 0, col = 0, rl = 0, count = 0;
+        auto place = [&](int cb) {
+            nb = min(kThreads, ncols - cb);
+            lanes = kThreads / nb;
+            rl = static_cast<int>(threadIdx.x) / nb;
+            col = cb + static_cast<int>(threadIdx.x) - rl * nb;
+            count = rl < lanes && rl < rows ? static_cast<int>((rows - rl + lanes - 1) / lanes) : 0;
+        };
+        for (int cb = 0; cb < ncols; cb += kThreads) {
+            place(cb);
+            Moments mo[N];
+            read_rows<TI, VEC, N>(x + rl * a.x_row + static_cast<long long>(col) * VEC, lanes * a.x_row, count, hold, held, mo);
+            // down the rows: halves of the row lanes joined until one is left
+            if (cb > 0) __syncthreads();
+#pragma unroll
+            for (int e = 0; e < N; ++e) entry[e][threadIdx.x] = make_float2(mo[e].mean, mo[e].m2);
+            entry_n[threadIdx.x] = mo[0].n;
+            __syncthreads();
+            for (int left = lanes; left > 1;) {
+                const int half = (left + 1) / 2;
+                if (rl + half < left) {
+                    const int other = threadIdx.x + half * nb;
+                    const float n = entry_n[other];
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        const float2 q = entry[e][other];
+                        Moments t;
+                        t.n = n;
+                        t.mean = q.x;
+                        t.m2 = q.y;
+                        mo[e] = join(mo[e], t);
+                        entry[e][threadIdx.x] = make_float2(mo[e].mean, mo[e].m2);
+                    }
+                    entry_n[threadIdx.x] = mo[0].n;
+                }
+                left = half;
+                __syncthreads();
+            }
+            // across the columns of each group (N = 1), or its channels
             Moments m;
-            for (int i = threadIdx.x & 31; i < lanes * w; i += 32) {
-                const int c = lo - c0 + i % w;
-                m = join(m, entry[c % VEC][(i / w) * nb + c / VEC]);
+            if (sub < gs) {
+                constexpr int kUnit = N == 1 ? VEC : 1;
+                const int lo = max(sub * a.cpg / kUnit, cb * (VEC / kUnit)) - cb * (VEC / kUnit);
+                const int end = min((sub + 1) * a.cpg / kUnit, (cb + nb) * (VEC / kUnit)) - cb * (VEC / kUnit);
+                for (int k = lo + sub_lane; k < end; k += a.group_lanes) {
+                    const float2 q = N == 1 ? entry[0][k] : entry[k % N][k / N];
+                    Moments t;
+                    t.n = entry_n[0];
+                    t.mean = q.x;
+                    t.m2 = q.y;
+                    m = join(m, t);
+                }
             }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                Moments t;
-                t.n = __shfl_down_sync(0xffffffffu, m.n, o);
-                t.mean = __shfl_down_sync(0xffffffffu, m.mean, o);
-                t.m2 = __shfl_down_sync(0xffffffffu, m.m2, o);
-                m = join(m, t);
+            m = join_lanes(m, a.group_lanes);
+            if (sub_lane == 0 && sub < gs) group[sub] = join(group[sub], m);
+        }
+        __syncthreads();
+
+        // hand the moments to the other members and take theirs
+        const float2 *part = &received[0][0];
+        int pitch = kSliceGroups;
+        if (a.join == kAlone) {
+            if (threadIdx.x < gs) received[0][threadIdx.x] = make_float2(group[threadIdx.x].mean, group[threadIdx.x].m2);
+            __syncthreads();
+        } else if (a.join == kCluster) {
+            cluster_wait();
+            for (int i = threadIdx.x; i < kSliceGroups * a.members; i += kThreads) {
+                const int to = i / kSliceGroups, g = i % kSliceGroups;
+                if (g < gs) {
+                    const uint32_t at = cluster_map(smem_u32(&received[member][g]), static_cast<uint32_t>(to));
+                    st_cluster_b32(at, __float_as_uint(group[g].mean));
+                    st_cluster_b32(at + 4, __float_as_uint(group[g].m2));
+                }
             }
-            if ((threadIdx.x & 31) == 0) group[g] = join(group[g], m);
+            __syncwarp();
+            cluster_sync();
+        } else {
+            float2 *mine = a.part + (static_cast<long long>(unit) * a.members + member) * a.slice_groups;
+            if (threadIdx.x < gs) mine[threadIdx.x] = make_float2(group[threadIdx.x].mean, group[threadIdx.x].m2);
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                __threadfence();
+                atomicAdd(a.arrived + unit, 1u);
+                if (ld_acquire(a.arrived + unit) < static_cast<uint32_t>(a.members)) {
+                    const uint64_t t0 = global_timer_ns();
+                    while (ld_acquire(a.arrived + unit) < static_cast<uint32_t>(a.members))
+                        if (global_timer_ns() - t0 > kWaitTimeoutNs) {
+                            if (a.err) atomicCAS(a.err, 0, E_JOIN);
+                            gave_up = 1;
+                            break;
+                        }
+                }
+            }
+            __syncthreads();
+            if (gave_up) return;
+            part = a.part + static_cast<long long>(unit) * a.members * a.slice_groups;
+            pitch = a.slice_groups;
         }
-    }
-    __syncthreads();
-    for (int g = threadIdx.x; g < a.G; g += kThreads)
-        a.part[(static_cast<long long>(s) * a.members + member) * a.G + g] = make_float2(group[g].mean, group[g].m2);
-}
+        Moments m;
+        if (sub < gs)
+#pragma unroll 4
+            for (int t = sub_lane; t < a.members; t += a.group_lanes) {
+                const float2 q = a.join == kGrid ? __ldcg(part + t * pitch + sub) : part[t * pitch + sub];
+                Moments o;
+                o.n = static_cast<float>((a.rows + (t < a.more_rows)) * a.cpg);
+                o.mean = q.x;
+                o.m2 = q.y;
+                m = join(m, o);
+            }
+        m = join_lanes(m, a.group_lanes);
+        if (sub_lane == 0 && sub < gs) norm[sub] = make_float2(m.mean, __frsqrt_rn(__fdiv_rn(m.m2, m.n) + a.eps));
+        __syncthreads();
 
-template <int VEC>
-__device__ __forceinline__ void activate_vec(float (&f)[VEC], int act)
-{
+        TO *y = static_cast<TO *>(a.y) + s * a.y_sample + r0 * a.y_row + c0;
+        for (int cb = 0; cb < ncols; cb += kThreads) {
+            if (ncols > kThreads) place(cb);
+            if (count == 0) continue;
+            float minus[N], scale[VEC], shift[VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-        if (act == S2_ACT_RELU) f[e] = activate<S2_ACT_RELU>(f[e]);
-        if (act == S2_ACT_SILU) f[e] = activate<S2_ACT_SILU>(f[e]);
-        if (act == S2_ACT_GELU) f[e] = activate<S2_ACT_GELU>(f[e]);
-        if (act == S2_ACT_GELU_TANH) f[e] = activate<S2_ACT_GELU_TANH>(f[e]);
+            for (int e = 0; e < VEC; ++e) {
+                const int c = col * VEC + e;
+                const float2 mr = norm[(kOne ? col * VEC : c) / a.cpg];
+                minus[e % N] = -mr.x;
+                scale[e] = a.weight ? mr.y * __ldg(a.weight + c0 + c) : mr.y;
+                shift[e] = a.bias ? __ldg(a.bias + c0 + c) : 0.f;
+            }
+            const TI *px = x + rl * a.x_row + static_cast<long long>(col) * VEC;
+            TO *py = y + rl * a.y_row + static_cast<long long>(col) * VEC;
+            const long long xs = lanes * a.x_row, ys = lanes * a.y_row;
+            switch (a.act) {
+            case S2_ACT_RELU: write_rows<TI, TO, VEC, N, S2_ACT_RELU>(px, xs, py, ys, count, hold, held, minus, scale, shift); break;
+            case S2_ACT_SILU: write_rows<TI, TO, VEC, N, S2_ACT_SILU>(px, xs, py, ys, count, hold, held, minus, scale, shift); break;
+            case S2_ACT_GELU: write_rows<TI, TO, VEC, N, S2_ACT_GELU>(px, xs, py, ys, count, hold, held, minus, scale, shift); break;
+            case S2_ACT_GELU_TANH:
+                write_rows<TI, TO, VEC, N, S2_ACT_GELU_TANH>(px, xs, py, ys, count, hold, held, minus, scale, shift);
+                break;
+            default: write_rows<TI, TO, VEC, N, S2_ACT_NONE>(px, xs, py, ys, count, hold, held, minus, scale, shift);
+            }
+        }
+        __syncthreads();  // the next unit reuses the moments
     }
 }
 
-// Part two: the members' moments joined, then the rows of one member.
-template <typename TI, typename TO, int VEC>
-__global__ void __launch_bounds__(kThreads) gn_apply_kernel(const GnArgs a)
+// The units, members and shared memory of a call.
+struct Plan {
+    int slices, slice_groups, units, members, teams, join, hold;
+    size_t smem;
+};
+
+size_t elem(int dtype) { return dtype == S2_F32 ? 4 : 2; }
+
+// Vectors of 16 bytes of x (their y 8 or 16 bytes) need every row to start on one.
+bool is_wide(const s2_group_norm_act_desc &d)
 {
-    // mean = hi + lo, 1 / sqrt(v + eps)
-    __shared__ float hi[kMaxGroups], lo[kMaxGroups], rstd[kMaxGroups];
-    const int s = blockIdx.y, member = blockIdx.x;
-    const long long r0 = a.P * member / a.members, r1 = a.P * (member + 1) / a.members;
-    for (int g = threadIdx.x; g < a.G; g += kThreads) {
-        double n = 0.0, mean = 0.0, m2 = 0.0;
-        for (int t = 0; t < a.members; ++t) {
-            const double nb = static_cast<double>(a.P * (t + 1) / a.members - a.P * t / a.members) * a.cpg;
-            if (nb == 0.0) continue;
-            const float2 q = a.part[(static_cast<long long>(s) * a.members + t) * a.G + g];
-            const double d = q.x - mean, w = nb / (n + nb);
-            mean += d * w;
-            m2 += q.y + d * d * n * w;
-            n += nb;
-        }
-        hi[g] = static_cast<float>(mean);
-        lo[g] = static_cast<float>(mean - hi[g]);
-        rstd[g] = static_cast<float>(1.0 / sqrt(m2 / n + a.eps));
-    }
-    __syncthreads();
-    const TI *x = static_cast<const TI *>(a.x) + s * a.x_sample;
-    TO *y = static_cast<TO *>(a.y) + s * a.y_sample;
-    const int ncols = a.C / VEC;
-    for (int cb = 0; cb < ncols; cb += kThreads) {
-        const int nb = min(kThreads, ncols - cb), lanes = kThreads / nb;
-        const int col = cb + threadIdx.x % nb, rl = threadIdx.x / nb;
-        if (rl >= lanes) continue;
-        // y = (x - hi) scale + shift: the subtraction first, as the formula has it
-        float mean[VEC], scale[VEC], shift[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const int c = col * VEC + e, g = c / a.cpg;
-            mean[e] = hi[g];
-            scale[e] = rstd[g] * (a.weight ? __ldg(a.weight + c) : 1.f);
-            shift[e] = (a.bias ? __ldg(a.bias + c) : 0.f) - lo[g] * scale[e];
-        }
-        for (long long r = r0 + rl; r < r1; r += lanes) {
-            Vec<TI, VEC> v;
-            v.load(x + r * a.x_row + static_cast<long long>(col) * VEC);
-            float f[VEC];
-            v.floats(f);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) f[e] = fmaf(f[e] - mean[e], scale[e], shift[e]);
-            activate_vec<VEC>(f, a.act);
-            store_vec<TO, VEC>(y + r * a.y_row + static_cast<long long>(col) * VEC, f);
-        }
-    }
+    const size_t ie = elem(d.in_dtype), oe = elem(d.out_dtype), vec = 16 / ie;
+    const uintptr_t xb = reinterpret_cast<uintptr_t>(d.x) | d.x_row * ie | (d.samples > 1 ? d.x_sample * ie : 0);
+    const uintptr_t yb = reinterpret_cast<uintptr_t>(d.y) | d.y_row * oe | (d.samples > 1 ? d.y_sample * oe : 0);
+    // slices begin at whole groups, so these have to fall on whole vectors too
+    return d.channels % vec == 0 && xb % 16 == 0 && yb % (vec * oe) == 0;
 }
 
-int members_of(const s2_group_norm_act_desc &d)
+constexpr size_t kPiece = kThreads * 16;    // shared memory of one vector a thread
+constexpr size_t kHoldTwo = 22 * kPiece;    // held by each of two blocks an SM
+constexpr size_t kMaxHold = 50 * kPiece;    // by a block alone
+
+Plan plan_of(const s2_group_norm_act_desc &d, int sms)
 {
-    const long long want = std::max<long long>(1, 1184 / std::max(1, d.samples));
-    return static_cast<int>(std::max<long long>(1, std::min<long long>(want, d.positions / 16)));
+    const bool wide = is_wide(d);
+    const long long size = static_cast<long long>(elem(d.in_dtype)), cpg = d.channels / d.groups;
+    const int vec = wide ? static_cast<int>(16 / size) : 1;
+    // slices are whole vectors
+    int step = 1;
+    while (step * cpg % vec != 0) ++step;
+    auto slices_of = [&](int sg) { return (d.groups + sg - 1) / sg; };
+    auto bytes_of = [&](int sg) { return d.positions * sg * cpg * size; };  // of a unit
+    auto fit = [&](int sg, int members, size_t hold) { return (bytes_of(sg) + members - 1) / members <= static_cast<long long>(hold * 15 / 16); };
+    Plan p;
+    p.slice_groups = std::max(step, std::min(d.groups, kSliceGroups / step * step));
+    auto halve = [&](int sg) { return std::max(step, sg / 2 / step * step); };
+    auto width = [&](int sg) { return sg * cpg * size; };
+    p.smem = kHoldTwo;
+    p.join = kGrid;
+    for (int sg = p.slice_groups;; sg = halve(sg)) {
+        if (fit(sg, kMaxCluster, kHoldTwo)) {
+            p.slice_groups = sg;
+            p.join = kCluster;
+            break;
+        }
+        if (halve(sg) == sg || width(halve(sg)) < 128) break;
+    }
+    if (p.join == kCluster) {
+        p.members = 1;
+        while (!fit(p.slice_groups, p.members, kHoldTwo)) p.members *= 2;
+        auto few = [&] { return 1LL * d.samples * slices_of(p.slice_groups) * p.members < sms; };
+        while (few() && p.members < kMaxCluster && d.positions >= 32 * p.members) p.members *= 2;
+        while (few() && halve(p.slice_groups) < p.slice_groups && width(halve(p.slice_groups)) >= 128) p.slice_groups = halve(p.slice_groups);
+    } else {
+        while (!fit(p.slice_groups, sms, kHoldTwo) && halve(p.slice_groups) < p.slice_groups && width(halve(p.slice_groups)) >= 64)
+            p.slice_groups = halve(p.slice_groups);
+        const long long want = (bytes_of(p.slice_groups) + kHoldTwo - 1) / kHoldTwo;
+        p.members = static_cast<int>(std::min<long long>(sms, want));
+    }
+    if (const char *e = getenv("GN_SG")) p.slice_groups = atoi(e);
+    if (const char *e = getenv("GN_JOIN")) p.join = atoi(e);
+    if (const char *e = getenv("GN_T")) p.members = atoi(e);
+    if (const char *e = getenv("GN_HOLD")) p.smem = atoi(e) * kPiece;
+    p.slices = slices_of(p.slice_groups);
+    p.units = d.samples * p.slices;
+    p.teams = p.units;
+    if (p.join == kGrid)
+        p.teams = std::max(1, std::min(p.units, (p.smem <= kHoldTwo ? 2 : 1) * sms / p.members));
+    if (const char *e = getenv("GN_TEAMS")) p.teams = atoi(e);
+    if (p.join == kCluster && p.members == 1) p.join = kAlone;
+    // no more shared memory than the rows need
+    const long long rows = (d.positions + p.members - 1) / p.members, ncols = p.slice_groups * cpg / vec;
+    const long long lanes = std::max<long long>(1, kThreads / ncols), pieces = (rows + lanes - 1) / lanes;
+    p.smem = std::min<size_t>(p.smem, static_cast<size_t>(pieces) * kThreads * (wide ? 16 : size));
+    return p;
 }
 
-template <typename TI, typename TO, int VEC>
-void launch(const GnArgs &a, int samples, cudaStream_t st)
+size_t workspace_of(const Plan &p)
 {
-    const dim3 grid(static_cast<unsigned>(a.members), static_cast<unsigned>(samples));
-    gn_stats_kernel<TI, VEC><<<grid, kThreads, 0, st>>>(a);
-    gn_apply_kernel<TI, TO, VEC><<<grid, kThreads, 0, st>>>(a);
+    if (p.join != kGrid) return 0;
+    return (static_cast<size_t>(p.units) * 4 + 15) / 16 * 16 +
+           static_cast<size_t>(p.units) * p.members * p.slice_groups * sizeof(float2);
+}
+
+int sm_count()
+{
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        cudaGetLastError();
+    return sms > 0 ? sms : 148;
+}
+
+template <typename TI, typename TO, int VEC, bool kOne>
+s2_status launch(GnArgs &a, const Plan &p, cudaStream_t st)
+{
+    auto kernel = group_norm_kernel<TI, TO, VEC, kOne>;
+    static std::atomic<uint64_t> configured{0};
+    const s2_status cs = s2::once_per_device(configured, [&] {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxHold);
+        return e == cudaSuccess ? S2_OK : s2::set_error(S2_INFERENCE_FAILED, "s2_group_norm_act: %s", cudaGetErrorString(e));
+    });
+    if (cs != S2_OK) return cs;
+    a.hold = static_cast<int>(p.smem / (kThreads * sizeof(typename Raw<TI, VEC>::type)));
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    if (p.join == kGrid) {
+        attr[0].id = cudaLaunchAttributeCooperative;
+        attr[0].val.cooperative = 1;
+    } else {
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = static_cast<unsigned>(p.members);
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+    }
+    cfg.gridDim = dim3(static_cast<unsigned>(p.teams) * p.members);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = p.smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+    return e == cudaSuccess ? S2_OK : s2::set_error(S2_INFERENCE_FAILED, "s2_group_norm_act: launch failed: %s", cudaGetErrorString(e));
 }
 
 template <typename TI, typename TO>
-void launch_types(const GnArgs &a, int samples, cudaStream_t st)
+s2_status launch_types(GnArgs &a, const Plan &p, bool wide, cudaStream_t st)
 {
     constexpr int kWide = 16 / sizeof(TI);
-    const uintptr_t out_bytes = kWide * sizeof(TO);
-    const bool wide = a.C % kWide == 0 && (reinterpret_cast<uintptr_t>(a.x) | a.x_row * sizeof(TI) |
-                                           a.x_sample * sizeof(TI)) % 16 == 0 &&
-                      (reinterpret_cast<uintptr_t>(a.y) | a.y_row * sizeof(TO) | a.y_sample * sizeof(TO)) % out_bytes == 0;
-    if (wide)
-        launch<TI, TO, kWide>(a, samples, st);
-    else
-        launch<TI, TO, 1>(a, samples, st);
+    if (!wide) return launch<TI, TO, 1, true>(a, p, st);
+    return a.cpg % kWide == 0 ? launch<TI, TO, kWide, true>(a, p, st) : launch<TI, TO, kWide, false>(a, p, st);
 }
-
-size_t elem(int dtype) { return dtype == S2_F32 ? 4 : 2; }
 
 s2_status check(const s2_group_norm_act_desc *d)
 {
@@ -290,8 +637,8 @@ s2_status check(const s2_group_norm_act_desc *d)
     if (d->samples < 0 || d->positions < 0 || d->channels <= 0 || d->groups <= 0 || d->channels % d->groups != 0)
         return s2::set_error(S2_INVALID_ARGUMENT, "s2_group_norm_act: bad shape (samples %d, positions %lld, channels %d, groups %d)",
                              d->samples, d->positions, d->channels, d->groups);
-    if (d->groups > kMaxGroups || d->samples > 65535 || d->positions > (1LL << 40))
-        return s2::set_error(S2_UNSUPPORTED, "s2_group_norm_act: at most %d groups, 65535 samples and 2^40 positions", kMaxGroups);
+    if (d->groups > kMaxGroups || d->samples > 65535 || d->positions > (1LL << 31))
+        return s2::set_error(S2_UNSUPPORTED, "s2_group_norm_act: at most %d groups, 65535 samples and 2^31 positions", kMaxGroups);
     const bool types = (d->in_dtype == S2_F32 && (d->out_dtype == S2_F32 || d->out_dtype == S2_F16 || d->out_dtype == S2_BF16)) ||
                        ((d->in_dtype == S2_F16 || d->in_dtype == S2_BF16) && d->out_dtype == d->in_dtype);
     if (!types)
@@ -325,7 +672,7 @@ extern "C" size_t s2_group_norm_act_workspace_bytes(const s2_group_norm_act_desc
 {
     s2::clear_error();
     if (check(d) != S2_OK || d->samples == 0 || d->positions == 0) return 0;
-    return static_cast<size_t>(d->samples) * members_of(*d) * d->groups * sizeof(float2);
+    return workspace_of(plan_of(*d, sm_count()));
 }
 
 extern "C" s2_status s2_group_norm_act(void *stream, const s2_group_norm_act_desc *d, int *launches)
@@ -347,16 +694,26 @@ extern "C" s2_status s2_group_norm_act(void *stream, const s2_group_norm_act_des
     if (!in_place(*d) && s2::may_overlap(span(d->x, *d, d->x_row, d->x_sample, static_cast<long long>(ie)),
                                          span(d->y, *d, d->y_row, d->y_sample, static_cast<long long>(oe))))
         return s2::set_error(S2_INVALID_ARGUMENT, "s2_group_norm_act: y overlaps x");
-    const size_t need = s2_group_norm_act_workspace_bytes(d);
+    const Plan p = plan_of(*d, sm_count());
+    const size_t need = workspace_of(p);
     if (need > 0 && (!d->workspace || d->workspace_bytes < need || reinterpret_cast<uintptr_t>(d->workspace) % 16))
         return s2::set_error(S2_INVALID_ARGUMENT, "s2_group_norm_act: workspace of %zu bytes, 16-byte aligned, needed", need);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
     GnArgs a;
     a.x = d->x;
     a.y = d->y;
     a.weight = d->weight;
     a.bias = d->bias;
-    a.part = static_cast<float2 *>(d->workspace);
-    a.P = d->positions;
+    a.arrived = static_cast<uint32_t *>(d->workspace);
+    a.part = nullptr;
+    if (p.join == kGrid) {
+        a.part = reinterpret_cast<float2 *>(static_cast<char *>(d->workspace) + (static_cast<size_t>(p.units) * 4 + 15) / 16 * 16);
+        const cudaError_t e = cudaMemsetAsync(a.arrived, 0, static_cast<size_t>(p.units) * 4, st);
+        if (e != cudaSuccess) return s2::set_error(S2_INFERENCE_FAILED, "s2_group_norm_act: %s", cudaGetErrorString(e));
+    }
+    a.err = d->err;
+    a.rows = d->positions / p.members;
+    a.more_rows = static_cast<int>(d->positions % p.members);
     a.x_row = d->x_row;
     a.x_sample = d->samples > 1 ? d->x_sample : 0;
     a.y_row = d->y_row;
@@ -364,22 +721,28 @@ extern "C" s2_status s2_group_norm_act(void *stream, const s2_group_norm_act_des
     a.C = d->channels;
     a.G = d->groups;
     a.cpg = d->channels / d->groups;
-    a.members = members_of(*d);
+    a.slices = p.slices;
+    a.slice_groups = p.slice_groups;
+    a.units = p.units;
+    a.members = p.members;
+    a.teams = p.teams;
+    a.join = p.join;
+    a.group_lanes = 32;
+    while (a.group_lanes * p.slice_groups > kThreads) a.group_lanes /= 2;
     a.act = d->activation;
     a.eps = d->eps;
-    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool wide = is_wide(*d);
+    s2_status s;
     if (d->in_dtype == S2_F16)
-        launch_types<__half, __half>(a, d->samples, st);
+        s = launch_types<__half, __half>(a, p, wide, st);
     else if (d->in_dtype == S2_BF16)
-        launch_types<__nv_bfloat16, __nv_bfloat16>(a, d->samples, st);
+        s = launch_types<__nv_bfloat16, __nv_bfloat16>(a, p, wide, st);
     else if (d->out_dtype == S2_F32)
-        launch_types<float, float>(a, d->samples, st);
+        s = launch_types<float, float>(a, p, wide, st);
     else if (d->out_dtype == S2_F16)
-        launch_types<float, __half>(a, d->samples, st);
+        s = launch_types<float, __half>(a, p, wide, st);
     else
-        launch_types<float, __nv_bfloat16>(a, d->samples, st);
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return s2::set_error(S2_INFERENCE_FAILED, "s2_group_norm_act: launch failed: %s", cudaGetErrorString(e));
-    if (launches) *launches = 2;
-    return S2_OK;
+        s = launch_types<float, __nv_bfloat16>(a, p, wide, st);
+    if (s == S2_OK && launches) *launches = 1;
+    return s;
 }

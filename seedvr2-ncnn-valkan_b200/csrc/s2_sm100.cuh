@@ -186,6 +186,10 @@ __device__ __forceinline__ uint32_t cluster_map(uint32_t saddr, uint32_t rank)
     return r;
 }
 
+// the two halves of cluster_sync
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 // store to another CTA's shared memory (a cluster_map address)
 __device__ __forceinline__ void st_cluster_b32(uint32_t caddr, uint32_t v)
 {
