@@ -75,35 +75,95 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b)
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// The activations in fp32. silu and gelu_tanh divide by 1 + e^-z, with the hardware's
-// exponential and division (a few 2^-23 relative each, far below an output's rounding to
-// 16 bits); a negative argument whose e^-z overflows gives -0, as the formula does.
-// A NaN stays a NaN, under relu too.
-template <int kAct>
-__device__ __forceinline__ float activate(float v)
+// Two floats in one 64-bit register: one instruction works on both.
+__device__ __forceinline__ uint64_t pair(float a, float b)
 {
-    if constexpr (kAct == S2_ACT_RELU) return v < 0.f ? 0.f : v;
-    if constexpr (kAct == S2_ACT_SILU) return __fdividef(v, 1.f + __expf(-v));
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 floats_of(uint64_t p)
+{
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t both(float a) { return pair(a, a); }
+
+// 2^x and 1 / x as the hardware gives them (2^-22 relative). The .ftz forms: without it each takes four
+// more instructions for denormals, which change nothing here (2^x of a denormal is 1).
+__device__ __forceinline__ uint64_t ex2_2(uint64_t x)
+{
+    float2 f = floats_of(x);
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(f.x));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(f.y));
+    return pair(f.x, f.y);
+}
+__device__ __forceinline__ uint64_t rcp_2(uint64_t x)
+{
+    float2 f = floats_of(x);
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(f.x));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(f.y));
+    return pair(f.x, f.y);
+}
+
+// The activations of two values in fp32, a few 2^-23 relative each, far below an output's rounding to 16
+// bits. Where e^-z overflows, silu and gelu_tanh give -0, as their formulas do; a NaN stays a NaN, under
+// relu too.
+template <int kAct>
+__device__ __forceinline__ uint64_t activate2(uint64_t v)
+{
+    constexpr float kLog2e = 1.4426950408889634f;
+    if constexpr (kAct == S2_ACT_RELU) {
+        const float2 f = floats_of(v);
+        return pair(f.x < 0.f ? 0.f : f.x, f.y < 0.f ? 0.f : f.y);
+    }
+    if constexpr (kAct == S2_ACT_SILU)  // v / (1 + e^-v)
+        return mul2(v, rcp_2(add2(ex2_2(mul2(v, both(-kLog2e))), both(1.f))));
+    if constexpr (kAct == S2_ACT_GELU_TANH) {
+        // 0.5 v (1 + tanh u) = v / (1 + e^-2u), u = sqrt(2 / pi) (v + 0.044715 v^3)
+        const uint64_t u = mul2(v, fma2(mul2(v, v), both(-2.f * 0.7978845608028654f * 0.044715f * kLog2e),
+                                        both(-2.f * 0.7978845608028654f * kLog2e)));
+        return mul2(v, rcp_2(add2(ex2_2(u), both(1.f))));
+    }
     if constexpr (kAct == S2_ACT_GELU) {
         // erfc(u) = t (a1 + t (a2 + ... + t a5)) e^-u^2, t = 1 / (1 + 0.3275911 u), u >= 0, within
         // 1.5e-7 (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26); here u = |v| /
         // sqrt 2, and 1 + erf(v / sqrt 2) is erfc(u) below 0 and 2 - erfc(u) above: nothing cancels.
-        // A third of erff's instructions, one branch-free run: the product at 21600 x 10240 x 2560
-        // spends 4500 of a tile's 20500 cycles on its activation with erff.
-        const float t = __fdividef(1.f, fmaf(0.3275911f * 0.70710678118654752f, fabsf(v), 1.f));
-        float p = fmaf(t, 1.061405429f, -1.453152027f);
-        p = fmaf(t, p, 1.421413741f);
-        p = fmaf(t, p, -0.284496736f);
-        p = fmaf(t, p, 0.254829592f);
-        const float c = p * t * __expf(-0.5f * v * v);
-        return 0.5f * v * (v >= 0.f ? 2.f - c : c);
-    }
-    if constexpr (kAct == S2_ACT_GELU_TANH) {
-        // 0.5 v (1 + tanh u) = v / (1 + e^-2u), u = sqrt(2 / pi) (v + 0.044715 v^3)
-        const float u2 = 1.5957691216057308f * v * (1.f + 0.044715f * v * v);
-        return __fdividef(v, 1.f + __expf(-u2));
+        const float2 f = floats_of(v);
+        const uint64_t t = rcp_2(fma2(pair(fabsf(f.x), fabsf(f.y)), both(0.3275911f * 0.70710678118654752f), both(1.f)));
+        uint64_t p = fma2(t, both(1.061405429f), both(-1.453152027f));
+        p = fma2(t, p, both(1.421413741f));
+        p = fma2(t, p, both(-0.284496736f));
+        p = fma2(t, p, both(0.254829592f));
+        const uint64_t c = mul2(mul2(p, t), ex2_2(mul2(mul2(v, v), both(-0.5f * kLog2e))));
+        const float2 lo = floats_of(c), hi = floats_of(fma2(c, both(-1.f), both(2.f)));
+        return mul2(mul2(v, both(0.5f)), pair(f.x >= 0.f ? hi.x : lo.x, f.y >= 0.f ? hi.y : lo.y));
     }
     return v;
+}
+template <int kAct>
+__device__ __forceinline__ float activate(float v)
+{
+    return floats_of(activate2<kAct>(pair(v, v))).x;
 }
 
 }  // namespace s2dev

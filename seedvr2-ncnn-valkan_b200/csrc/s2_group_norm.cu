@@ -40,6 +40,7 @@ enum Join : int {
     kAlone = 0,    // one block
     kCluster = 1,  // the blocks of a cluster, through distributed shared memory
     kGrid = 2,     // blocks of a cooperative grid, through the workspace
+    kRing = 3,     // the same, one block an SM that streams its rows through a ring (group_norm_ring_kernel)
 };
 
 // A unit is the slice of `slice_groups` groups of one sample; `members` blocks share its positions:
@@ -53,6 +54,7 @@ struct GnArgs {
     int32_t *err;
     long long rows, x_row, x_sample, y_row, y_sample;
     int more_rows, C, G, cpg, slices, slice_groups, units, members, teams, join, hold, act;
+    int ahead;          // the ring holds two units: the next one's statistics come before this one's output
     int group_lanes;    // threads that join one group's moments: a power of two up to 32
     float eps;
 };
@@ -85,32 +87,6 @@ __device__ __forceinline__ Moments join_lanes(Moments m, int lanes)
         m = join(m, t);
     }
     return m;
-}
-
-// Two floats in one 64-bit register: one instruction works on both.
-__device__ __forceinline__ uint64_t pair(float a, float b)
-{
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float2 floats_of(uint64_t p)
-{
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
-{
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
-{
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
 }
 
 // VEC elements of T as they are loaded: 16 bytes or one element
@@ -270,18 +246,17 @@ __device__ __forceinline__ void finish(const typename Raw<TI, VEC>::type &v, TO 
     float f[VEC];
     Raw<TI, VEC>::floats(v, f);
     if constexpr (VEC == 1) {
-        f[0] = fmaf(f[0] + minus[0], scale[0], shift[0]);
+        f[0] = activate<kAct>(fmaf(f[0] + minus[0], scale[0], shift[0]));
     } else {
 #pragma unroll
         for (int k = 0; k < VEC / 2; ++k) {
-            const uint64_t d = add2(pair(f[2 * k], f[2 * k + 1]), pair(minus[2 * k % N], minus[(2 * k + 1) % N]));
-            const float2 r = floats_of(fma2(d, pair(scale[2 * k], scale[2 * k + 1]), pair(shift[2 * k], shift[2 * k + 1])));
+            const uint64_t d = add2(pair(f[2 * k], f[2 * k + 1]), pair(minus[2 * k / (VEC / N)], minus[(2 * k + 1) / (VEC / N)]));
+            const float2 r = floats_of(activate2<kAct>(
+                fma2(d, pair(scale[2 * k], scale[2 * k + 1]), pair(shift[2 * k], shift[2 * k + 1]))));
             f[2 * k] = r.x;
             f[2 * k + 1] = r.y;
         }
     }
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) f[e] = activate<kAct>(f[e]);
     store_vec<TO, VEC>(py, f);
 }
 
@@ -323,7 +298,8 @@ __device__ __forceinline__ uint32_t ld_acquire(const uint32_t *p)
     return v;
 }
 
-enum : int { E_JOIN = 96 };  // device error code: the wait for the other members ran out
+// device error codes: the wait for the other members, for the ring's loads
+enum : int { E_JOIN = 96, E_RING = 97 };
 
 // kOne: the VEC channels of a vector always belong to one group.
 template <typename TI, typename TO, int VEC, bool kOne>
@@ -499,6 +475,397 @@ __global__ void __launch_bounds__(kThreads, 2) group_norm_kernel(const GnArgs a)
     }
 }
 
+// ---- large units -----------------------------------------------------------------
+
+constexpr int kRingThreads = 256;             // and a warp that only loads; two blocks an SM
+constexpr int kSlotPasses = 2;                // passes of a slot
+constexpr int kRunSlots = 4;                  // slots summed about one pivot
+constexpr uint32_t kSlotBytes = kSlotPasses * kRingThreads * 16;
+
+// Slots of the ring: what is left beside the joins' shared memory.
+template <int N>
+__host__ __device__ constexpr int ring_slots()
+{
+    return N == 1 ? 13 : 12;
+}
+
+// A member's slots over one unit: slot i holds kSlotPasses times `lanes` of its rows.
+struct Slots {
+    int lanes, rows;  // of a pass, of a slot
+    int total, held;  // held: the last ones stay in the ring from the statistics to the output
+};
+
+template <int N>
+__device__ __forceinline__ Slots slots_of(long long rows, int ncols)
+{
+    Slots p;
+    p.lanes = kRingThreads / ncols;
+    p.rows = kSlotPasses * p.lanes;
+    p.total = static_cast<int>((rows + p.rows - 1) / p.rows);
+    p.held = min(p.total, ring_slots<N>());
+    return p;
+}
+
+// One thread's view of the ring: a place in the sequence of loads, and its own 16 bytes of a slot.
+template <int kSlots>
+struct Cursor {
+    const uint4 *mine;
+    uint32_t full0, empty0;
+    volatile int *abort;
+    int *err;
+    uint32_t slot, phase;
+    __device__ __forceinline__ void go(uint32_t q)
+    {
+        slot = q % kSlots;
+        phase = q / kSlots & 1u;
+    }
+    // A wait that ran out raises `abort`, which ends all later ones at once: the block runs on to its end
+    // (every thread meets the same barriers) with the error recorded.
+    __device__ __forceinline__ void wait() const { mbar_wait(full0 + 8 * slot, phase, abort, err, E_RING); }
+    // the thread's vector of pass k of the slot
+    __device__ __forceinline__ uint4 get(int k, int stride) const
+    {
+        return mine[slot * (kSlotPasses * kRingThreads) + k * stride];
+    }
+    __device__ __forceinline__ void release() const
+    {
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(empty0 + 8 * slot);
+    }
+    __device__ __forceinline__ void next()
+    {
+        if (++slot == kSlots) {
+            slot = 0;
+            phase ^= 1u;
+        }
+    }
+};
+
+// The unit's rows of one thread, in the order in which the ring holds them. `count`: its rows, `stride`:
+// vectors of a pass.
+template <typename TI, typename TO, int N, int kAct, int kSlots>
+__device__ __forceinline__ void write_slots(Cursor<kSlots> c, const Slots &p, int count, int stride, TO *y, long long step,
+                                            const float (&minus)[N], const float (&scale)[16 / sizeof(TI)],
+                                            const float (&shift)[16 / sizeof(TI)])
+{
+    constexpr int VEC = 16 / sizeof(TI);
+    const int first = p.total - p.held;
+    for (int q = 0; q < p.total; ++q) {
+        const int i = q < p.held ? first + q : p.total - 1 - q;
+        if (q >= p.held) c.wait();
+        TO *py = y + i * (kSlotPasses * step);
+        uint4 v[kSlotPasses];
+#pragma unroll
+        for (int k = 0; k < kSlotPasses; ++k) v[k] = c.get(k, stride);
+        c.release();
+#pragma unroll
+        for (int k = 0; k < kSlotPasses; ++k)
+            if (kSlotPasses * i + k < count) finish<TI, TO, VEC, N, kAct>(v[k], py + k * step, minus, scale, shift);
+        c.next();
+    }
+}
+
+// Group norm of units that are shared by the blocks of a cooperative grid. A loading warp streams the
+// member's rows through a ring of slots with bulk copies, far ahead of the threads that sum and write,
+// so that the memory is never waited for; what the ring can hold is read once. Rows beyond it come a
+// second time, the latest first (from L2, as far as it holds them). With a.ahead the ring holds two
+// units: the next one's statistics come before this one's output, and the members' join is hidden.
+// N: moments a vector, 16 / sizeof(TI) / N channels each, which always belong to one group.
+template <typename TI, typename TO, int N>
+__global__ void __launch_bounds__(kRingThreads + 32, 2) group_norm_ring_kernel(const GnArgs a)
+{
+    constexpr int VEC = 16 / sizeof(TI), kPer = VEC / N, kPairs = VEC / 2, kSlots = ring_slots<N>();
+    constexpr int kRound = N < 4 ? N : 4;  // moments joined at a time
+    using R = Raw<TI, VEC>;
+    extern __shared__ uint4 ring[];
+    __shared__ float2 entry[kRound][kRingThreads];
+    __shared__ float entry_n[kRingThreads];
+    __shared__ Moments group[kSliceGroups];
+    __shared__ float2 norm[kSliceGroups];
+    __shared__ uint64_t bars[2 * kSlots];
+    __shared__ int abort_flag;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int member = static_cast<int>(blockIdx.x) % a.members, team = static_cast<int>(blockIdx.x) / a.members;
+    const long long r0 = member * a.rows + min(member, a.more_rows), rows = a.rows + (member < a.more_rows);
+    const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * kSlots;
+    volatile int *abort = &abort_flag;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kSlots; ++i) {
+            mbar_init(full0 + 8 * i, 1);
+            mbar_init(empty0 + 8 * i, kRingThreads / 32);
+        }
+        abort_flag = 0;
+        fence_mbar_init();
+    }
+    __syncthreads();
+
+    if (warp == kRingThreads / 32) {
+        uint32_t slot = 0, phase = 0, issued = 0;
+        bool ok = true;
+        for (int unit = team; ok && unit < a.units; unit += a.teams) {
+            const int s = unit / a.slices, g0 = (unit - s * a.slices) * a.slice_groups;
+            const int ncols = min(a.slice_groups, a.G - g0) * a.cpg / VEC;
+            const Slots p = slots_of<N>(rows, ncols);
+            const TI *x = static_cast<const TI *>(a.x) + s * a.x_sample + r0 * a.x_row + g0 * a.cpg;
+            const uint32_t row_bytes = ncols * 16;
+            const bool dense = a.x_row * sizeof(TI) == row_bytes;
+            const int loads = 2 * p.total - p.held;
+            for (int q = 0; q < loads; ++q, ++issued) {
+                const int i = q < p.total ? q : p.total - p.held - 1 - (q - p.total);
+                const long long first = static_cast<long long>(i) * p.rows;
+                const int n = static_cast<int>(min(static_cast<long long>(p.rows), rows - first));
+                ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * slot, phase ^ 1u, abort, a.err, E_RING));
+                if (!ok) break;
+                const uint32_t dst = smem_u32(ring) + slot * kSlotBytes, bar = full0 + 8 * slot;
+                if (lane == 0) mbar_arrive_expect_tx(bar, n * row_bytes);
+                __syncwarp();
+                const TI *src = x + first * a.x_row;
+                if (dense) {
+                    if (lane == 0) bulk_load(dst, src, n * row_bytes, bar);
+                } else {
+                    for (int r = lane; r < n; r += 32) bulk_load(dst + r * row_bytes, src + r * a.x_row, row_bytes, bar);
+                }
+                if (++slot == kSlots) {
+                    slot = 0;
+                    phase ^= 1u;
+                }
+            }
+        }
+        if (!ok) {
+            // no copy may still be landing when the block ends: wait for the slots' last loads
+            int dummy = 0;
+            for (uint32_t k = 0; k < kSlots && k < issued; ++k) {
+                const uint32_t q = issued - 1 - k;
+                mbar_wait(full0 + 8 * (q % kSlots), (q / kSlots) & 1u, &dummy, a.err, E_RING);
+            }
+        }
+        return;
+    }
+
+    const int sub = static_cast<int>(threadIdx.x) / a.group_lanes, sub_lane = threadIdx.x % a.group_lanes;
+    Cursor<kSlots> cur{ring + threadIdx.x, full0, empty0, abort, a.err, 0, 0};
+    auto sync = [] { named_barrier_sync(1, kRingThreads); };
+    // where the next unit's loads begin in the ring's sequence
+    uint32_t begin = 0;
+
+    struct Unit {
+        int s, g0, gs, ncols, rl, col, count;
+        uint32_t begin;
+        Slots p;
+    };
+    auto describe = [&](int unit) {
+        Unit u;
+        u.s = unit / a.slices;
+        u.g0 = (unit - u.s * a.slices) * a.slice_groups;
+        u.gs = min(a.slice_groups, a.G - u.g0);
+        u.ncols = u.gs * a.cpg / VEC;
+        u.p = slots_of<N>(rows, u.ncols);
+        u.rl = static_cast<int>(threadIdx.x) / u.ncols;
+        u.col = static_cast<int>(threadIdx.x) - u.rl * u.ncols;
+        u.count = u.rl < u.p.lanes && u.rl < rows ? static_cast<int>((rows - u.rl + u.p.lanes - 1) / u.p.lanes) : 0;
+        u.begin = begin;
+        begin += 2 * u.p.total - u.p.held;
+        return u;
+    };
+    // the unit's moments, handed to its members
+    auto statistics = [&](int unit, const Unit &u) {
+        Moments mo[N];
+        cur.go(u.begin);
+        const int stride = u.p.lanes * u.ncols;
+        for (int i = 0; i < u.p.total; i += kRunSlots) {
+            constexpr int kSums = N == 1 ? 2 : kPairs;
+            float p[N];
+            uint64_t minus[N == 1 ? 1 : kPairs], s2[kSums], q2[kSums];
+#pragma unroll
+            for (int k = 0; k < kSums; ++k) s2[k] = q2[k] = 0;
+            const int n = min(kRunSlots, u.p.total - i), valid = min(n * kSlotPasses, u.count - i * kSlotPasses);
+#pragma unroll
+            for (int v = 0; v < kRunSlots; ++v) {
+                if (v >= n) break;
+                cur.wait();
+                uint4 raw[kSlotPasses];
+#pragma unroll
+                for (int w = 0; w < kSlotPasses; ++w) raw[w] = cur.get(w, stride);
+                if (i + v < u.p.total - u.p.held) cur.release();
+                cur.next();
+#pragma unroll
+                for (int w = 0; w < kSlotPasses; ++w) {
+                    if (v * kSlotPasses + w < valid) {
+                        float f[VEC];
+                        R::floats(raw[w], f);
+                        if (v + w == 0) {
+#pragma unroll
+                            for (int e = 0; e < N; ++e) p[e] = f[e * kPer];
+#pragma unroll
+                            for (int k = 0; k < (N == 1 ? 1 : kPairs); ++k)
+                                minus[k] = pair(-p[N == 1 ? 0 : 2 * k / kPer], -p[N == 1 ? 0 : (2 * k + 1) / kPer]);
+                        }
+#pragma unroll
+                        for (int k = 0; k < kPairs; ++k) {
+                            const uint64_t d = add2(pair(f[2 * k], f[2 * k + 1]), minus[N == 1 ? 0 : k]);
+                            s2[k % kSums] = add2(s2[k % kSums], d);
+                            q2[k % kSums] = fma2(d, d, q2[k % kSums]);
+                        }
+                    }
+                }
+            }
+            if (valid > 0) {
+                float sum[N], sq[N];
+#pragma unroll
+                for (int e = 0; e < N; ++e) sum[e] = sq[e] = 0.f;
+#pragma unroll
+                for (int k = 0; k < kSums; ++k) {
+                    const float2 b = floats_of(s2[k]), c = floats_of(q2[k]);
+                    const int e0 = N == 1 ? 0 : 2 * k / kPer, e1 = N == 1 ? 0 : (2 * k + 1) / kPer;
+                    sum[e0] += b.x;
+                    sum[e1] += b.y;
+                    sq[e0] += c.x;
+                    sq[e1] += c.y;
+                }
+                const float cnt = static_cast<float>(valid * kPer), inv = __fdividef(1.f, cnt);
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    Moments run;
+                    run.n = cnt;
+                    run.mean = fmaf(sum[e], inv, p[e]);
+                    run.m2 = fmaxf(fmaf(-sum[e] * inv, sum[e], sq[e]), 0.f * sq[e]);
+                    mo[e] = join(mo[e], run);
+                }
+            }
+        }
+        if (sub_lane == 0 && sub < u.gs) group[sub] = Moments();
+#pragma unroll
+        for (int first = 0; first < N; first += kRound) {
+            sync();
+#pragma unroll
+            for (int e = 0; e < kRound; ++e) entry[e][threadIdx.x] = make_float2(mo[first + e].mean, mo[first + e].m2);
+            float n = mo[0].n;
+            entry_n[threadIdx.x] = n;
+            sync();
+            for (int left = u.p.lanes; left > 1;) {
+                const int half = (left + 1) / 2;
+                if (u.rl + half < left) {
+                    const int other = threadIdx.x + half * u.ncols;
+                    const float on = entry_n[other];
+#pragma unroll
+                    for (int e = 0; e < kRound; ++e) {
+                        const float2 o = entry[e][other], m = entry[e][threadIdx.x];
+                        Moments b, c;
+                        b.n = n;
+                        b.mean = m.x;
+                        b.m2 = m.y;
+                        c.n = on;
+                        c.mean = o.x;
+                        c.m2 = o.y;
+                        b = join(b, c);
+                        entry[e][threadIdx.x] = make_float2(b.mean, b.m2);
+                    }
+                    n += on;
+                    entry_n[threadIdx.x] = n;
+                }
+                left = half;
+                sync();
+            }
+            // group `sub`: the moments [sub cpg / kPer, (sub + 1) cpg / kPer) along a row of vectors, those
+            // of this round
+            Moments m;
+            if (sub < u.gs)
+                for (int k = sub * a.cpg / kPer + sub_lane; k < (sub + 1) * a.cpg / kPer; k += a.group_lanes) {
+                    const int e = k % N - first;
+                    if (e >= 0 && e < kRound) {
+                        const float2 o = entry[e][k / N];
+                        Moments c;
+                        c.n = entry_n[0];
+                        c.mean = o.x;
+                        c.m2 = o.y;
+                        m = join(m, c);
+                    }
+                }
+            m = join_lanes(m, a.group_lanes);
+            if (sub_lane == 0 && sub < u.gs) group[sub] = join(group[sub], m);
+        }
+        sync();
+        float2 *part = a.part + (static_cast<long long>(unit) * a.members + member) * a.slice_groups;
+        if (threadIdx.x < u.gs) part[threadIdx.x] = make_float2(group[threadIdx.x].mean, group[threadIdx.x].m2);
+        sync();
+        if (threadIdx.x == 0) {
+            __threadfence();
+            atomicAdd(a.arrived + unit, 1u);
+        }
+    };
+
+    auto output = [&](int unit, const Unit &u) {
+        if (threadIdx.x == 0) {
+            const uint64_t t0 = global_timer_ns();
+            while (ld_acquire(a.arrived + unit) < static_cast<uint32_t>(a.members))
+                if (*abort || global_timer_ns() - t0 > kWaitTimeoutNs) {
+                    if (a.err) atomicCAS(a.err, 0, E_JOIN);
+                    *abort = 1;
+                    break;
+                }
+        }
+        sync();
+        Moments m;
+        const float2 *part = a.part + static_cast<long long>(unit) * a.members * a.slice_groups;
+        if (sub < u.gs)
+#pragma unroll 4
+            for (int t = sub_lane; t < a.members; t += a.group_lanes) {
+                const float2 q = __ldcg(part + t * a.slice_groups + sub);
+                Moments o;
+                o.n = static_cast<float>((a.rows + (t < a.more_rows)) * a.cpg);
+                o.mean = q.x;
+                o.m2 = q.y;
+                m = join(m, o);
+            }
+        m = join_lanes(m, a.group_lanes);
+        if (sub_lane == 0 && sub < u.gs) norm[sub] = make_float2(m.mean, __frsqrt_rn(__fdiv_rn(m.m2, m.n) + a.eps));
+        sync();
+        float minus[N], scale[VEC], shift[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const int c = u.col * VEC + e;
+            const float2 mr = norm[min((u.col * VEC + e / kPer * kPer) / a.cpg, u.gs - 1)];
+            const int ch = min(u.g0 * a.cpg + c, a.C - 1);
+            minus[e / kPer] = -mr.x;
+            scale[e] = a.weight ? mr.y * __ldg(a.weight + ch) : mr.y;
+            shift[e] = a.bias ? __ldg(a.bias + ch) : 0.f;
+        }
+        TO *y = static_cast<TO *>(a.y) + u.s * a.y_sample + (r0 + u.rl) * a.y_row + u.g0 * a.cpg + u.col * VEC;
+        const long long y_step = u.p.lanes * a.y_row;
+        const int stride = u.p.lanes * u.ncols;
+        cur.go(u.begin + u.p.total - u.p.held);
+        switch (a.act) {
+        case S2_ACT_RELU: write_slots<TI, TO, N, S2_ACT_RELU>(cur, u.p, u.count, stride, y, y_step, minus, scale, shift); break;
+        case S2_ACT_SILU: write_slots<TI, TO, N, S2_ACT_SILU>(cur, u.p, u.count, stride, y, y_step, minus, scale, shift); break;
+        case S2_ACT_GELU: write_slots<TI, TO, N, S2_ACT_GELU>(cur, u.p, u.count, stride, y, y_step, minus, scale, shift); break;
+        case S2_ACT_GELU_TANH:
+            write_slots<TI, TO, N, S2_ACT_GELU_TANH>(cur, u.p, u.count, stride, y, y_step, minus, scale, shift);
+            break;
+        default: write_slots<TI, TO, N, S2_ACT_NONE>(cur, u.p, u.count, stride, y, y_step, minus, scale, shift);
+        }
+    };
+
+    if (a.ahead) {
+        Unit now = describe(team);
+        if (team < a.units) statistics(team, now);
+        for (int unit = team; unit < a.units; unit += a.teams) {
+            Unit then = now;
+            if (unit + a.teams < a.units) {
+                then = describe(unit + a.teams);
+                statistics(unit + a.teams, then);
+            }
+            output(unit, now);
+            now = then;
+        }
+    } else {
+        for (int unit = team; unit < a.units; unit += a.teams) {
+            const Unit u = describe(unit);
+            statistics(unit, u);
+            output(unit, u);
+        }
+    }
+}
+
 // The units, members and shared memory of a call.
 struct Plan {
     int slices, slice_groups, units, members, teams, join, hold;
@@ -567,6 +934,7 @@ Plan plan_of(const s2_group_norm_act_desc &d, int sms)
     p.teams = p.units;
     if (p.join == kGrid)
         p.teams = std::max(1, std::min(p.units, (p.smem <= kHoldTwo ? 2 : 1) * sms / p.members));
+    if (p.join == kRing) p.teams = std::max(1, std::min(p.units, 2 * sms / p.members));
     if (const char *e = getenv("GN_TEAMS")) p.teams = atoi(e);
     if (p.join == kCluster && p.members == 1) p.join = kAlone;
     // no more shared memory than the rows need
@@ -578,7 +946,7 @@ Plan plan_of(const s2_group_norm_act_desc &d, int sms)
 
 size_t workspace_of(const Plan &p)
 {
-    if (p.join != kGrid) return 0;
+    if (p.join != kGrid && p.join != kRing) return 0;
     return (static_cast<size_t>(p.units) * 4 + 15) / 16 * 16 +
            static_cast<size_t>(p.units) * p.members * p.slice_groups * sizeof(float2);
 }
@@ -623,10 +991,42 @@ s2_status launch(GnArgs &a, const Plan &p, cudaStream_t st)
     return e == cudaSuccess ? S2_OK : s2::set_error(S2_INFERENCE_FAILED, "s2_group_norm_act: launch failed: %s", cudaGetErrorString(e));
 }
 
+template <typename TI, typename TO, int N>
+s2_status launch_ring(const GnArgs &a, const Plan &p, cudaStream_t st)
+{
+    auto kernel = group_norm_ring_kernel<TI, TO, N>;
+    constexpr int kBytes = static_cast<int>(ring_slots<N>() * kSlotBytes);
+    static std::atomic<uint64_t> configured{0};
+    const s2_status cs = s2::once_per_device(configured, [&] {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+        return e == cudaSuccess ? S2_OK : s2::set_error(S2_INFERENCE_FAILED, "s2_group_norm_act: %s", cudaGetErrorString(e));
+    });
+    if (cs != S2_OK) return cs;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeCooperative;
+    attr[0].val.cooperative = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(p.teams) * p.members);
+    cfg.blockDim = dim3(kRingThreads + 32);
+    cfg.dynamicSmemBytes = kBytes;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+    return e == cudaSuccess ? S2_OK : s2::set_error(S2_INFERENCE_FAILED, "s2_group_norm_act: launch failed: %s", cudaGetErrorString(e));
+}
+
 template <typename TI, typename TO>
 s2_status launch_types(GnArgs &a, const Plan &p, bool wide, cudaStream_t st)
 {
     constexpr int kWide = 16 / sizeof(TI);
+    if (p.join == kRing) {
+        if (a.cpg % kWide == 0) return launch_ring<TI, TO, 1>(a, p, st);
+        if (a.cpg % (kWide / 2) == 0) return launch_ring<TI, TO, 2>(a, p, st);
+        if constexpr (kWide == 8)
+            if (a.cpg % 2 == 0) return launch_ring<TI, TO, 4>(a, p, st);
+        return launch_ring<TI, TO, kWide>(a, p, st);
+    }
     if (!wide) return launch<TI, TO, 1, true>(a, p, st);
     return a.cpg % kWide == 0 ? launch<TI, TO, kWide, true>(a, p, st) : launch<TI, TO, kWide, false>(a, p, st);
 }
@@ -706,7 +1106,7 @@ extern "C" s2_status s2_group_norm_act(void *stream, const s2_group_norm_act_des
     a.bias = d->bias;
     a.arrived = static_cast<uint32_t *>(d->workspace);
     a.part = nullptr;
-    if (p.join == kGrid) {
+    if (p.join == kGrid || p.join == kRing) {
         a.part = reinterpret_cast<float2 *>(static_cast<char *>(d->workspace) + (static_cast<size_t>(p.units) * 4 + 15) / 16 * 16);
         const cudaError_t e = cudaMemsetAsync(a.arrived, 0, static_cast<size_t>(p.units) * 4, st);
         if (e != cudaSuccess) return s2::set_error(S2_INFERENCE_FAILED, "s2_group_norm_act: %s", cudaGetErrorString(e));
@@ -728,7 +1128,9 @@ extern "C" s2_status s2_group_norm_act(void *stream, const s2_group_norm_act_des
     a.teams = p.teams;
     a.join = p.join;
     a.group_lanes = 32;
-    while (a.group_lanes * p.slice_groups > kThreads) a.group_lanes /= 2;
+    while (a.group_lanes * p.slice_groups > (p.join == kRing ? kRingThreads : kThreads)) a.group_lanes /= 2;
+    const long long lanes = kRingThreads / (1LL * p.slice_groups * a.cpg * elem(d->in_dtype) / 16 + 1);  // at least
+    a.ahead = p.join == kRing && lanes > 0 && getenv("GN_AHEAD") && atoi(getenv("GN_AHEAD"));
     a.act = d->activation;
     a.eps = d->eps;
     const bool wide = is_wide(*d);

@@ -57,27 +57,30 @@ __device__ __forceinline__ bool wait_drain(uint32_t bar, uint32_t parity, int *e
     return mbar_wait(bar, parity, &dummy, err, E_DRAIN);
 }
 
+template <int N, int kAct>
+__device__ __forceinline__ void activate_each(float (&v)[N])
+{
+    if constexpr (N == 1) {
+        v[0] = activate<kAct>(v[0]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const float2 f = floats_of(activate2<kAct>(pair(v[i], v[i + 1])));
+            v[i] = f.x;
+            v[i + 1] = f.y;
+        }
+    }
+}
+
 // act over N values; the branch is the same for every thread
 template <int N>
 __device__ __forceinline__ void activate_all(float (&v)[N], int act)
 {
     switch (act) {
-    case S2_ACT_RELU:
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = activate<S2_ACT_RELU>(v[i]);
-        break;
-    case S2_ACT_SILU:
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = activate<S2_ACT_SILU>(v[i]);
-        break;
-    case S2_ACT_GELU:
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = activate<S2_ACT_GELU>(v[i]);
-        break;
-    case S2_ACT_GELU_TANH:
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = activate<S2_ACT_GELU_TANH>(v[i]);
-        break;
+    case S2_ACT_RELU: activate_each<N, S2_ACT_RELU>(v); break;
+    case S2_ACT_SILU: activate_each<N, S2_ACT_SILU>(v); break;
+    case S2_ACT_GELU: activate_each<N, S2_ACT_GELU>(v); break;
+    case S2_ACT_GELU_TANH: activate_each<N, S2_ACT_GELU_TANH>(v); break;
     default: break;
     }
 }
