@@ -49,12 +49,13 @@ struct GnArgs {
     const void *x;
     void *y;
     const float *weight, *bias;
-    float2 *part;       // kGrid: [unit][member][group of the slice] (mean, M2)
-    uint32_t *arrived;  // kGrid: [unit] members whose moments are written (zero before)
+    // members of a grid: [unit][member][group of the slice] (mean, M2), [unit][group] (mean, 1 / sigma),
+    // and per unit the members whose moments are written and, once set, that the unit's are (zero before)
+    float2 *part, *joined;
+    uint32_t *arrived, *ready;
     int32_t *err;
     long long rows, x_row, x_sample, y_row, y_sample;
     int more_rows, C, G, cpg, slices, slice_groups, units, members, teams, join, hold, act;
-    int ahead;          // the ring holds two units: the next one's statistics come before this one's output
     int group_lanes;    // threads that join one group's moments: a power of two up to 32
     float eps;
 };
@@ -127,18 +128,19 @@ struct Raw<T, 1> {
     static __device__ __forceinline__ void floats(T v, float (&f)[1]) { f[0] = to_float<T>(v); }
 };
 
+// y is not read again here: its lines leave L2 first
 template <typename T, int VEC>
 __device__ __forceinline__ void store_vec(T *p, const float (&f)[VEC])
 {
     if constexpr (VEC == 1) {
         *p = from_float<T>(f[0]);
     } else if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<float4 *>(p) = make_float4(f[0], f[1], f[2], f[3]);
+        __stcs(reinterpret_cast<float4 *>(p), make_float4(f[0], f[1], f[2], f[3]));
     } else if constexpr (VEC == 8) {
-        *reinterpret_cast<uint4 *>(p) =
-            make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+        __stcs(reinterpret_cast<uint4 *>(p),
+               make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7])));
     } else {
-        *reinterpret_cast<uint2 *>(p) = make_uint2(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]));
+        __stcs(reinterpret_cast<uint2 *>(p), make_uint2(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3])));
     }
 }
 
@@ -237,6 +239,26 @@ __device__ __forceinline__ void read_rows(const TI *px, long long step, int coun
     if (i < count) read_run<TI, VEC, N, false>(px, step, count - i, i, hold, held, mo);
 }
 
+// silu and gelu_tanh of two values with one reciprocal for both: 1 / a = b / (a b). e^-z is cut off at 2^60
+// (a value below -41 gives -41 * 2^-60 and the like instead of 0), so that a b stays finite. Exponentials
+// and reciprocals share a unit of 16 a clock on an SM; at two each a value the output of 16-bit vectors took
+// 32 clocks a warp's vector there, at three for two 24, where the memory needs 22.
+template <int kAct>
+__device__ __forceinline__ uint64_t activate_pair(uint64_t v)
+{
+    if constexpr (kAct == S2_ACT_SILU || kAct == S2_ACT_GELU_TANH) {
+        constexpr float kLog2e = 1.4426950408889634f, kTanh = -2.f * 0.7978845608028654f * kLog2e;
+        const uint64_t z = kAct == S2_ACT_SILU ? mul2(v, both(-kLog2e))
+                                               : mul2(v, fma2(mul2(v, v), both(kTanh * 0.044715f), both(kTanh)));
+        const float2 zf = floats_of(z);
+        const float2 d = floats_of(add2(ex2_2(pair(fminf(zf.x, 60.f), fminf(zf.y, 60.f))), both(1.f)));
+        float r = d.x * d.y;
+        asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(r));
+        return mul2(v, mul2(both(r), pair(d.y, d.x)));
+    }
+    return activate2<kAct>(v);
+}
+
 // y = act((x - mean) scale + shift) of one vector; `minus` is -mean, one (kOne) or a pair of channels each.
 // The subtraction comes first, as in the formula: values that all equal the mean give the shift itself.
 template <typename TI, typename TO, int VEC, int N, int kAct>
@@ -251,7 +273,7 @@ __device__ __forceinline__ void finish(const typename Raw<TI, VEC>::type &v, TO 
 #pragma unroll
         for (int k = 0; k < VEC / 2; ++k) {
             const uint64_t d = add2(pair(f[2 * k], f[2 * k + 1]), pair(minus[2 * k / (VEC / N)], minus[(2 * k + 1) / (VEC / N)]));
-            const float2 r = floats_of(activate2<kAct>(
+            const float2 r = floats_of(activate_pair<kAct>(
                 fma2(d, pair(scale[2 * k], scale[2 * k + 1]), pair(shift[2 * k], shift[2 * k + 1]))));
             f[2 * k] = r.x;
             f[2 * k + 1] = r.y;
@@ -301,6 +323,88 @@ __device__ __forceinline__ uint32_t ld_acquire(const uint32_t *p)
 // device error codes: the wait for the other members, for the ring's loads
 enum : int { E_JOIN = 96, E_RING = 97 };
 
+// The members' moments of group `sub` of the slice, by group_lanes threads a group (sub_lane of them): in the
+// first of these. Eight are asked for at a time and joined in four chains; which thread joins what depends on
+// the shape alone.
+template <bool kGlobal>
+__device__ __noinline__ Moments join_members(const GnArgs &a, const float2 *part, int pitch, int sub, int sub_lane, int gs)
+{
+    Moments chain[4];
+    if (sub < gs)
+        for (int t0 = sub_lane; t0 < a.members; t0 += 8 * a.group_lanes) {
+            float2 q[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int t = t0 + k * a.group_lanes;
+                if (t < a.members) q[k] = kGlobal ? __ldcg(part + t * pitch + sub) : part[t * pitch + sub];
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int t = t0 + k * a.group_lanes;
+                if (t < a.members) {
+                    Moments o;
+                    o.n = static_cast<float>((a.rows + (t < a.more_rows)) * a.cpg);
+                    o.mean = q[k].x;
+                    o.m2 = q[k].y;
+                    chain[k & 3] = join(chain[k & 3], o);
+                }
+            }
+        }
+    return join_lanes(join(join(chain[0], chain[1]), join(chain[2], chain[3])), a.group_lanes);
+}
+
+// mean and 1 / sigma of a group
+__device__ __forceinline__ float2 norm_of(const Moments &m, float eps)
+{
+    return make_float2(m.mean, __frsqrt_rn(__fdiv_rn(m.m2, m.n) + eps));
+}
+
+// The members of a grid join a unit's moments (group[], gs of them): each writes its own, the last to arrive
+// joins all of them and publishes the unit's, the others wait for these. (Every member joining all for itself
+// read 296 x 32 moments 296 times from the same lines of L2: 8 us a unit.) `sync` is the barrier of the
+// threads that call this; *stop ends the wait, which is bounded. On return norm[] holds the unit's.
+template <typename Sync>
+__device__ __forceinline__ void join_grid(const GnArgs &a, int unit, int member, const Moments *group, int gs, int sub,
+                                          int sub_lane, float2 *norm, volatile int *last, volatile int *stop, Sync sync)
+{
+    const long long at = static_cast<long long>(unit) * a.members;
+    if (threadIdx.x < gs)
+        __stcg(a.part + (at + member) * a.slice_groups + threadIdx.x, make_float2(group[threadIdx.x].mean, group[threadIdx.x].m2));
+    sync();
+    if (threadIdx.x == 0) {
+        __threadfence();
+        *last = atomicAdd(a.arrived + unit, 1u) == static_cast<uint32_t>(a.members) - 1;
+        __threadfence();
+    }
+    sync();
+    float2 *joined = a.joined + static_cast<long long>(unit) * a.slice_groups;
+    if (*last) {
+        const Moments m = join_members<true>(a, a.part + at * a.slice_groups, a.slice_groups, sub, sub_lane, gs);
+        if (sub_lane == 0 && sub < gs) {
+            norm[sub] = norm_of(m, a.eps);
+            __stcg(joined + sub, norm[sub]);
+        }
+        sync();
+        if (threadIdx.x == 0) {
+            __threadfence();
+            atomicExch(a.ready + unit, 1u);
+        }
+    } else {
+        if (threadIdx.x == 0 && ld_acquire(a.ready + unit) == 0) {
+            const uint64_t t0 = global_timer_ns();
+            while (ld_acquire(a.ready + unit) == 0)
+                if (*stop || global_timer_ns() - t0 > kWaitTimeoutNs) {
+                    if (a.err) atomicCAS(a.err, 0, E_JOIN);
+                    *stop = 1;
+                    break;
+                }
+        }
+        sync();
+        if (threadIdx.x < gs) norm[threadIdx.x] = __ldcg(joined + threadIdx.x);
+        sync();
+    }
+}
+
 // kOne: the VEC channels of a vector always belong to one group.
 template <typename TI, typename TO, int VEC, bool kOne>
 __global__ void __launch_bounds__(kThreads, 2) group_norm_kernel(const GnArgs a)
@@ -313,13 +417,13 @@ __global__ void __launch_bounds__(kThreads, 2) group_norm_kernel(const GnArgs a)
     __shared__ Moments group[kSliceGroups];
     __shared__ float2 received[kMaxCluster][kSliceGroups];
     __shared__ float2 norm[kSliceGroups];  // mean, 1 / sqrt(v + eps)
-    __shared__ int gave_up;
+    __shared__ int last, stop;
     typename R::type *held = reinterpret_cast<typename R::type *>(held_raw) + threadIdx.x;
     const int member = static_cast<int>(blockIdx.x) % a.members;
     const long long r0 = member * a.rows + min(member, a.more_rows), rows = a.rows + (member < a.more_rows);
     // for the joins of groups: group_lanes threads a group
     const int sub = static_cast<int>(threadIdx.x) / a.group_lanes, sub_lane = threadIdx.x % a.group_lanes;
-    if (threadIdx.x == 0) gave_up = 0;
+    if (threadIdx.x == 0) stop = 0;
     if (a.join == kCluster) cluster_arrive();  // waited for below: no block writes to one that has not begun
 
     for (int unit = static_cast<int>(blockIdx.x) / a.members; unit < a.units; unit += a.teams) {
@@ -391,8 +495,6 @@ __global__ void __launch_bounds__(kThreads, 2) group_norm_kernel(const GnArgs a)
         __syncthreads();
 
         // hand the moments to the other members and take theirs
-        const float2 *part = &received[0][0];
-        int pitch = kSliceGroups;
         if (a.join == kAlone) {
             if (threadIdx.x < gs) received[0][threadIdx.x] = make_float2(group[threadIdx.x].mean, group[threadIdx.x].m2);
             __syncthreads();
@@ -409,41 +511,14 @@ __global__ void __launch_bounds__(kThreads, 2) group_norm_kernel(const GnArgs a)
             __syncwarp();
             cluster_sync();
         } else {
-            float2 *mine = a.part + (static_cast<long long>(unit) * a.members + member) * a.slice_groups;
-            if (threadIdx.x < gs) mine[threadIdx.x] = make_float2(group[threadIdx.x].mean, group[threadIdx.x].m2);
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                __threadfence();
-                atomicAdd(a.arrived + unit, 1u);
-                if (ld_acquire(a.arrived + unit) < static_cast<uint32_t>(a.members)) {
-                    const uint64_t t0 = global_timer_ns();
-                    while (ld_acquire(a.arrived + unit) < static_cast<uint32_t>(a.members))
-                        if (global_timer_ns() - t0 > kWaitTimeoutNs) {
-                            if (a.err) atomicCAS(a.err, 0, E_JOIN);
-                            gave_up = 1;
-                            break;
-                        }
-                }
-            }
-            __syncthreads();
-            if (gave_up) return;
-            part = a.part + static_cast<long long>(unit) * a.members * a.slice_groups;
-            pitch = a.slice_groups;
+            join_grid(a, unit, member, group, gs, sub, sub_lane, norm, &last, &stop, [] { __syncthreads(); });
+            if (stop) return;
         }
-        Moments m;
-        if (sub < gs)
-#pragma unroll 4
-            for (int t = sub_lane; t < a.members; t += a.group_lanes) {
-                const float2 q = a.join == kGrid ? __ldcg(part + t * pitch + sub) : part[t * pitch + sub];
-                Moments o;
-                o.n = static_cast<float>((a.rows + (t < a.more_rows)) * a.cpg);
-                o.mean = q.x;
-                o.m2 = q.y;
-                m = join(m, o);
-            }
-        m = join_lanes(m, a.group_lanes);
-        if (sub_lane == 0 && sub < gs) norm[sub] = make_float2(m.mean, __frsqrt_rn(__fdiv_rn(m.m2, m.n) + a.eps));
-        __syncthreads();
+        if (a.join != kGrid) {
+            const Moments m = join_members<false>(a, &received[0][0], kSliceGroups, sub, sub_lane, gs);
+            if (sub_lane == 0 && sub < gs) norm[sub] = norm_of(m, a.eps);
+            __syncthreads();
+        }
 
         TO *y = static_cast<TO *>(a.y) + s * a.y_sample + r0 * a.y_row + c0;
         for (int cb = 0; cb < ncols; cb += kThreads) {
@@ -478,15 +553,15 @@ __global__ void __launch_bounds__(kThreads, 2) group_norm_kernel(const GnArgs a)
 // ---- large units -----------------------------------------------------------------
 
 constexpr int kRingThreads = 256;             // and a warp that only loads; two blocks an SM
-constexpr int kSlotPasses = 2;                // passes of a slot
-constexpr int kRunSlots = 4;                  // slots summed about one pivot
+constexpr int kSlotPasses = 4;                // passes of a slot
+constexpr int kRunSlots = 2;                  // slots summed about one pivot
 constexpr uint32_t kSlotBytes = kSlotPasses * kRingThreads * 16;
 
 // Slots of the ring: what is left beside the joins' shared memory.
 template <int N>
 __host__ __device__ constexpr int ring_slots()
 {
-    return N == 1 ? 13 : 12;
+    return 6;
 }
 
 // A member's slots over one unit: slot i holds kSlotPasses times `lanes` of its rows.
@@ -509,7 +584,7 @@ __device__ __forceinline__ Slots slots_of(long long rows, int ncols)
 // One thread's view of the ring: a place in the sequence of loads, and its own 16 bytes of a slot.
 template <int kSlots>
 struct Cursor {
-    const uint4 *mine;
+    uint32_t mine;  // shared address of the thread's vector of slot 0
     uint32_t full0, empty0;
     volatile int *abort;
     int *err;
@@ -522,10 +597,16 @@ struct Cursor {
     // A wait that ran out raises `abort`, which ends all later ones at once: the block runs on to its end
     // (every thread meets the same barriers) with the error recorded.
     __device__ __forceinline__ void wait() const { mbar_wait(full0 + 8 * slot, phase, abort, err, E_RING); }
-    // the thread's vector of pass k of the slot
-    __device__ __forceinline__ uint4 get(int k, int stride) const
+    // the thread's vector of pass k of the slot, `stride` bytes a pass (the ring is only written by copies
+    // the compiler does not see, so its loads are spelled out)
+    __device__ __forceinline__ uint4 get(int k, uint32_t stride) const
     {
-        return mine[slot * (kSlotPasses * kRingThreads) + k * stride];
+        uint4 v;
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                     : "r"(mine + slot * kSlotBytes + k * stride)
+                     : "memory");
+        return v;
     }
     __device__ __forceinline__ void release() const
     {
@@ -544,24 +625,36 @@ struct Cursor {
 // The unit's rows of one thread, in the order in which the ring holds them. `count`: its rows, `stride`:
 // vectors of a pass.
 template <typename TI, typename TO, int N, int kAct, int kSlots>
-__device__ __forceinline__ void write_slots(Cursor<kSlots> c, const Slots &p, int count, int stride, TO *y, long long step,
+__device__ __forceinline__ void write_slots(Cursor<kSlots> c, const Slots &p, int count, uint32_t stride, TO *y, long long step,
                                             const float (&minus)[N], const float (&scale)[16 / sizeof(TI)],
                                             const float (&shift)[16 / sizeof(TI)])
 {
     constexpr int VEC = 16 / sizeof(TI);
-    const int first = p.total - p.held;
-    for (int q = 0; q < p.total; ++q) {
-        const int i = q < p.held ? first + q : p.total - 1 - q;
-        if (q >= p.held) c.wait();
-        TO *py = y + i * (kSlotPasses * step);
+    auto slot = [&](int i, TO *py) __attribute__((always_inline)) {
         uint4 v[kSlotPasses];
 #pragma unroll
         for (int k = 0; k < kSlotPasses; ++k) v[k] = c.get(k, stride);
         c.release();
-#pragma unroll
-        for (int k = 0; k < kSlotPasses; ++k)
-            if (kSlotPasses * i + k < count) finish<TI, TO, VEC, N, kAct>(v[k], py + k * step, minus, scale, shift);
         c.next();
+        if ((i + 1) * kSlotPasses <= count) {
+#pragma unroll
+            for (int k = 0; k < kSlotPasses; ++k, py += step) finish<TI, TO, VEC, N, kAct>(v[k], py, minus, scale, shift);
+        } else {
+#pragma unroll
+            for (int k = 0; k < kSlotPasses; ++k, py += step)
+                if (i * kSlotPasses + k < count) finish<TI, TO, VEC, N, kAct>(v[k], py, minus, scale, shift);
+        }
+    };
+    const long long slot_step = kSlotPasses * step;
+    const int first = p.total - p.held;
+    TO *py = y + first * slot_step;
+#pragma unroll 1
+    for (int i = first; i < p.total; ++i, py += slot_step) slot(i, py);
+    py = y + (first - 1) * slot_step;
+#pragma unroll 1
+    for (int i = first - 1; i >= 0; --i, py -= slot_step) {
+        c.wait();
+        slot(i, py);
     }
 }
 
@@ -583,7 +676,7 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2) group_norm_ring_kernel(c
     __shared__ Moments group[kSliceGroups];
     __shared__ float2 norm[kSliceGroups];
     __shared__ uint64_t bars[2 * kSlots];
-    __shared__ int abort_flag;
+    __shared__ int abort_flag, last;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int member = static_cast<int>(blockIdx.x) % a.members, team = static_cast<int>(blockIdx.x) / a.members;
     const long long r0 = member * a.rows + min(member, a.more_rows), rows = a.rows + (member < a.more_rows);
@@ -602,6 +695,7 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2) group_norm_ring_kernel(c
     if (warp == kRingThreads / 32) {
         uint32_t slot = 0, phase = 0, issued = 0;
         bool ok = true;
+        const uint64_t once = l2_evict_first(), again = l2_evict_last();
         for (int unit = team; ok && unit < a.units; unit += a.teams) {
             const int s = unit / a.slices, g0 = (unit - s * a.slices) * a.slice_groups;
             const int ncols = min(a.slice_groups, a.G - g0) * a.cpg / VEC;
@@ -620,10 +714,11 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2) group_norm_ring_kernel(c
                 if (lane == 0) mbar_arrive_expect_tx(bar, n * row_bytes);
                 __syncwarp();
                 const TI *src = x + first * a.x_row;
+                const uint64_t policy = q < p.total - p.held ? again : once;
                 if (dense) {
-                    if (lane == 0) bulk_load(dst, src, n * row_bytes, bar);
+                    if (lane == 0) bulk_load(dst, src, n * row_bytes, bar, policy);
                 } else {
-                    for (int r = lane; r < n; r += 32) bulk_load(dst + r * row_bytes, src + r * a.x_row, row_bytes, bar);
+                    for (int r = lane; r < n; r += 32) bulk_load(dst + r * row_bytes, src + r * a.x_row, row_bytes, bar, policy);
                 }
                 if (++slot == kSlots) {
                     slot = 0;
@@ -643,7 +738,7 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2) group_norm_ring_kernel(c
     }
 
     const int sub = static_cast<int>(threadIdx.x) / a.group_lanes, sub_lane = threadIdx.x % a.group_lanes;
-    Cursor<kSlots> cur{ring + threadIdx.x, full0, empty0, abort, a.err, 0, 0};
+    Cursor<kSlots> cur{smem_u32(ring) + threadIdx.x * 16, full0, empty0, abort, a.err, 0, 0};
     auto sync = [] { named_barrier_sync(1, kRingThreads); };
     // where the next unit's loads begin in the ring's sequence
     uint32_t begin = 0;
@@ -671,7 +766,7 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2) group_norm_ring_kernel(c
     auto statistics = [&](int unit, const Unit &u) {
         Moments mo[N];
         cur.go(u.begin);
-        const int stride = u.p.lanes * u.ncols;
+        const uint32_t stride = u.p.lanes * u.ncols * 16;
         for (int i = 0; i < u.p.total; i += kRunSlots) {
             constexpr int kSums = N == 1 ? 2 : kPairs;
             float p[N];
@@ -679,34 +774,41 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2) group_norm_ring_kernel(c
 #pragma unroll
             for (int k = 0; k < kSums; ++k) s2[k] = q2[k] = 0;
             const int n = min(kRunSlots, u.p.total - i), valid = min(n * kSlotPasses, u.count - i * kSlotPasses);
+            auto add = [&](const uint4 &raw) __attribute__((always_inline)) {
+                float f[VEC];
+                R::floats(raw, f);
 #pragma unroll
-            for (int v = 0; v < kRunSlots; ++v) {
-                if (v >= n) break;
-                cur.wait();
+                for (int k = 0; k < kPairs; ++k) {
+                    const uint64_t d = add2(pair(f[2 * k], f[2 * k + 1]), minus[N == 1 ? 0 : k]);
+                    s2[k % kSums] = add2(s2[k % kSums], d);
+                    q2[k % kSums] = fma2(d, d, q2[k % kSums]);
+                }
+            };
+            cur.wait();
+            {
+                float f[VEC];
+                R::floats(cur.get(0, stride), f);
+#pragma unroll
+                for (int e = 0; e < N; ++e) p[e] = f[e * kPer];
+#pragma unroll
+                for (int k = 0; k < (N == 1 ? 1 : kPairs); ++k)
+                    minus[k] = pair(-p[N == 1 ? 0 : 2 * k / kPer], -p[N == 1 ? 0 : (2 * k + 1) / kPer]);
+            }
+#pragma unroll 1
+            for (int v = 0; v < n; ++v) {
+                if (v > 0) cur.wait();
                 uint4 raw[kSlotPasses];
 #pragma unroll
                 for (int w = 0; w < kSlotPasses; ++w) raw[w] = cur.get(w, stride);
                 if (i + v < u.p.total - u.p.held) cur.release();
                 cur.next();
+                if ((v + 1) * kSlotPasses <= valid) {
 #pragma unroll
-                for (int w = 0; w < kSlotPasses; ++w) {
-                    if (v * kSlotPasses + w < valid) {
-                        float f[VEC];
-                        R::floats(raw[w], f);
-                        if (v + w == 0) {
+                    for (int w = 0; w < kSlotPasses; ++w) add(raw[w]);
+                } else {
 #pragma unroll
-                            for (int e = 0; e < N; ++e) p[e] = f[e * kPer];
-#pragma unroll
-                            for (int k = 0; k < (N == 1 ? 1 : kPairs); ++k)
-                                minus[k] = pair(-p[N == 1 ? 0 : 2 * k / kPer], -p[N == 1 ? 0 : (2 * k + 1) / kPer]);
-                        }
-#pragma unroll
-                        for (int k = 0; k < kPairs; ++k) {
-                            const uint64_t d = add2(pair(f[2 * k], f[2 * k + 1]), minus[N == 1 ? 0 : k]);
-                            s2[k % kSums] = add2(s2[k % kSums], d);
-                            q2[k % kSums] = fma2(d, d, q2[k % kSums]);
-                        }
-                    }
+                    for (int w = 0; w < kSlotPasses; ++w)
+                        if (v * kSlotPasses + w < valid) add(raw[w]);
                 }
             }
             if (valid > 0) {
@@ -785,41 +887,10 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2) group_norm_ring_kernel(c
             if (sub_lane == 0 && sub < u.gs) group[sub] = join(group[sub], m);
         }
         sync();
-        float2 *part = a.part + (static_cast<long long>(unit) * a.members + member) * a.slice_groups;
-        if (threadIdx.x < u.gs) part[threadIdx.x] = make_float2(group[threadIdx.x].mean, group[threadIdx.x].m2);
-        sync();
-        if (threadIdx.x == 0) {
-            __threadfence();
-            atomicAdd(a.arrived + unit, 1u);
-        }
+        join_grid(a, unit, member, group, u.gs, sub, sub_lane, norm, &last, abort, sync);
     };
 
-    auto output = [&](int unit, const Unit &u) {
-        if (threadIdx.x == 0) {
-            const uint64_t t0 = global_timer_ns();
-            while (ld_acquire(a.arrived + unit) < static_cast<uint32_t>(a.members))
-                if (*abort || global_timer_ns() - t0 > kWaitTimeoutNs) {
-                    if (a.err) atomicCAS(a.err, 0, E_JOIN);
-                    *abort = 1;
-                    break;
-                }
-        }
-        sync();
-        Moments m;
-        const float2 *part = a.part + static_cast<long long>(unit) * a.members * a.slice_groups;
-        if (sub < u.gs)
-#pragma unroll 4
-            for (int t = sub_lane; t < a.members; t += a.group_lanes) {
-                const float2 q = __ldcg(part + t * a.slice_groups + sub);
-                Moments o;
-                o.n = static_cast<float>((a.rows + (t < a.more_rows)) * a.cpg);
-                o.mean = q.x;
-                o.m2 = q.y;
-                m = join(m, o);
-            }
-        m = join_lanes(m, a.group_lanes);
-        if (sub_lane == 0 && sub < u.gs) norm[sub] = make_float2(m.mean, __frsqrt_rn(__fdiv_rn(m.m2, m.n) + a.eps));
-        sync();
+    auto output = [&](const Unit &u) {
         float minus[N], scale[VEC], shift[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
@@ -832,7 +903,7 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2) group_norm_ring_kernel(c
         }
         TO *y = static_cast<TO *>(a.y) + u.s * a.y_sample + (r0 + u.rl) * a.y_row + u.g0 * a.cpg + u.col * VEC;
         const long long y_step = u.p.lanes * a.y_row;
-        const int stride = u.p.lanes * u.ncols;
+        const uint32_t stride = u.p.lanes * u.ncols * 16;
         cur.go(u.begin + u.p.total - u.p.held);
         switch (a.act) {
         case S2_ACT_RELU: write_slots<TI, TO, N, S2_ACT_RELU>(cur, u.p, u.count, stride, y, y_step, minus, scale, shift); break;
@@ -845,24 +916,10 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2) group_norm_ring_kernel(c
         }
     };
 
-    if (a.ahead) {
-        Unit now = describe(team);
-        if (team < a.units) statistics(team, now);
-        for (int unit = team; unit < a.units; unit += a.teams) {
-            Unit then = now;
-            if (unit + a.teams < a.units) {
-                then = describe(unit + a.teams);
-                statistics(unit + a.teams, then);
-            }
-            output(unit, now);
-            now = then;
-        }
-    } else {
-        for (int unit = team; unit < a.units; unit += a.teams) {
-            const Unit u = describe(unit);
-            statistics(unit, u);
-            output(unit, u);
-        }
+    for (int unit = team; unit < a.units; unit += a.teams) {
+        const Unit u = describe(unit);
+        statistics(unit, u);
+        output(u);
     }
 }
 
@@ -944,11 +1001,13 @@ Plan plan_of(const s2_group_norm_act_desc &d, int sms)
     return p;
 }
 
+size_t round_up16(size_t v) { return (v + 15) / 16 * 16; }
+
 size_t workspace_of(const Plan &p)
 {
     if (p.join != kGrid && p.join != kRing) return 0;
-    return (static_cast<size_t>(p.units) * 4 + 15) / 16 * 16 +
-           static_cast<size_t>(p.units) * p.members * p.slice_groups * sizeof(float2);
+    return round_up16(static_cast<size_t>(p.units) * 8) +
+           static_cast<size_t>(p.units) * (p.members + 1) * p.slice_groups * sizeof(float2);
 }
 
 int sm_count()
@@ -1104,11 +1163,14 @@ extern "C" s2_status s2_group_norm_act(void *stream, const s2_group_norm_act_des
     a.y = d->y;
     a.weight = d->weight;
     a.bias = d->bias;
-    a.arrived = static_cast<uint32_t *>(d->workspace);
-    a.part = nullptr;
+    a.part = a.joined = nullptr;
+    a.arrived = a.ready = nullptr;
     if (p.join == kGrid || p.join == kRing) {
-        a.part = reinterpret_cast<float2 *>(static_cast<char *>(d->workspace) + (static_cast<size_t>(p.units) * 4 + 15) / 16 * 16);
-        const cudaError_t e = cudaMemsetAsync(a.arrived, 0, static_cast<size_t>(p.units) * 4, st);
+        a.arrived = static_cast<uint32_t *>(d->workspace);
+        a.ready = a.arrived + p.units;
+        a.joined = reinterpret_cast<float2 *>(static_cast<char *>(d->workspace) + round_up16(static_cast<size_t>(p.units) * 8));
+        a.part = a.joined + static_cast<size_t>(p.units) * p.slice_groups;
+        const cudaError_t e = cudaMemsetAsync(a.arrived, 0, static_cast<size_t>(p.units) * 8, st);
         if (e != cudaSuccess) return s2::set_error(S2_INFERENCE_FAILED, "s2_group_norm_act: %s", cudaGetErrorString(e));
     }
     a.err = d->err;
@@ -1129,8 +1191,6 @@ extern "C" s2_status s2_group_norm_act(void *stream, const s2_group_norm_act_des
     a.join = p.join;
     a.group_lanes = 32;
     while (a.group_lanes * p.slice_groups > (p.join == kRing ? kRingThreads : kThreads)) a.group_lanes /= 2;
-    const long long lanes = kRingThreads / (1LL * p.slice_groups * a.cpg * elem(d->in_dtype) / 16 + 1);  // at least
-    a.ahead = p.join == kRing && lanes > 0 && getenv("GN_AHEAD") && atoi(getenv("GN_AHEAD"));
     a.act = d->activation;
     a.eps = d->eps;
     const bool wide = is_wide(*d);

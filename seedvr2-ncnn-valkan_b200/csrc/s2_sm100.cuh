@@ -121,13 +121,29 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const void *tmap, uint
         : "memory");
 }
 
-// Untiled bulk copy global -> shared of `bytes` (a multiple of 16; both addresses 16-byte aligned),
-// completion counted on an mbarrier of this CTA. No multicast.
-__device__ __forceinline__ void bulk_load(uint32_t sdst, const void *gsrc, uint32_t bytes, uint32_t bar)
+// L2 policies for loads and stores that are told how long their lines matter.
+__device__ __forceinline__ uint64_t l2_evict_first()
 {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(sdst),
-                 "l"(reinterpret_cast<uint64_t>(gsrc)), "r"(bytes), "r"(bar)
-                 : "memory");
+    uint64_t p;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+__device__ __forceinline__ uint64_t l2_evict_last()
+{
+    uint64_t p;
+    asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+
+// Untiled bulk copy global -> shared of `bytes` (a multiple of 16; both addresses 16-byte aligned) under
+// an L2 policy, completion counted on an mbarrier of this CTA. No multicast.
+__device__ __forceinline__ void bulk_load(uint32_t sdst, const void *gsrc, uint32_t bytes, uint32_t bar, uint64_t policy)
+{
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(
+            sdst),
+        "l"(reinterpret_cast<uint64_t>(gsrc)), "r"(bytes), "r"(bar), "l"(policy)
+        : "memory");
 }
 
 // barrier `id` (1-15) over `threads` threads of the CTA (whole warps)
