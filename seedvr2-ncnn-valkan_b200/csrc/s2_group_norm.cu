@@ -5,19 +5,27 @@
 //   m = sum x / n,  v = sum (x - m)^2 / n,  y = act((x - m) / sqrt(v + eps) * w[c] + b[c]).
 //
 // Statistics: a thread keeps one vector of channels and walks down the rows. It sums d = x - p
-// and d^2 about a pivot p of its own (the first value of each short run of rows) in fp32 and
-// turns every run into (count, mean, M2 = sum of squares about the mean); runs, threads and
-// blocks are joined by
+// and d^2 about a pivot p of its own (the first value of each run of 8 rows) in fp32 and turns
+// every run into (count, mean, M2 = sum of squares about the mean); runs, threads and blocks are
+// joined by
 //   m = ma + (mb - ma) nb / n,   M2 = M2a + M2b + (mb - ma)^2 na nb / n,
 // which loses nothing when the mean is far larger than the spread, and an outlier only reaches
-// the run that holds it. Blocks are joined in double, in order: the result does not depend on
-// timing.
+// the run that holds it. What is joined with what depends on the shape alone, never on timing.
+//
+// A unit (a slice of the groups of one sample) is shared by a team of blocks. Two kernels:
+//  * group_norm_held_kernel: the blocks read their rows into shared memory while they sum them, and
+//    write the output from there. Small units are held whole by the blocks of a cluster, which
+//    exchange their moments through distributed shared memory: one read, no workspace. Larger ones
+//    whose rows do not start on 16 bytes take the blocks of a cooperative grid, and rows that are
+//    not held are read twice.
+//  * group_norm_ring_kernel, large units with aligned rows: a loading warp streams the rows through a
+//    ring of slots with bulk copies, so that the memory never waits for the threads that sum and
+//    write; what the ring holds at the end of the statistics is read once.
 #include <cuda_runtime.h>
 
 #include <algorithm>
 #include <atomic>
 #include <cstdint>
-#include <cstdlib>
 
 #include "s2_act.cuh"
 #include "s2_internal.h"
@@ -31,37 +39,37 @@ using namespace s2dev;
 
 constexpr int kThreads = 256;
 constexpr int kMaxGroups = 1024;
-constexpr int kSliceGroups = 64;   // groups of one unit
+constexpr int kSliceGroups = 64;  // groups of one unit
 constexpr int kMaxCluster = 8;
-constexpr int kAhead = 8;          // vectors a thread has in flight while it reads
+constexpr int kAhead = 8;         // vectors a thread has in flight while it sums, and the rows of a run
+constexpr int kBatch = 4;         // ... while it writes
 
-// How the members of a unit exchange their groups' moments.
+// How the parts of a unit exchange their moments.
 enum Join : int {
     kAlone = 0,    // one block
     kCluster = 1,  // the blocks of a cluster, through distributed shared memory
     kGrid = 2,     // blocks of a cooperative grid, through the workspace
-    kRing = 3,     // the same, one block an SM that streams its rows through a ring (group_norm_ring_kernel)
 };
 
-// A unit is the slice of `slice_groups` groups of one sample; `members` blocks share its positions:
-// the first `more_rows` of them rows + 1 each, the others `rows`.
+// `parts` blocks share a unit, `part_rows` rows each (the last ones fewer); `teams` of them take the units
+// in turn.
 struct GnArgs {
     const void *x;
     void *y;
     const float *weight, *bias;
-    // members of a grid: [unit][member][group of the slice] (mean, M2), [unit][group] (mean, 1 / sigma),
-    // and per unit the members whose moments are written and, once set, that the unit's are (zero before)
-    float2 *part, *joined;
-    uint32_t *arrived, *ready;
     int32_t *err;
-    long long rows, x_row, x_sample, y_row, y_sample;
-    int more_rows, C, G, cpg, slices, slice_groups, units, members, teams, join, hold, act;
-    int group_lanes;    // threads that join one group's moments: a power of two up to 32
+    long long P, part_rows, x_row, x_sample, y_row, y_sample;
+    int C, G, cpg, slices, slice_groups, units, parts, teams, join, hold, act;
+    int group_lanes;  // threads that join one group's moments: a power of two up to 32
     float eps;
+    // a grid's: (mean, M2) per [unit][part][group], (mean, 1 / sigma) per [unit][group]; counters, zero
+    // before: parts whose moments are written, units whose norm is
+    float2 *part, *norm;
+    uint32_t *arrived, *ready;
 };
 
 struct Moments {
-    float n = 0.f, mean = 0.f, m2 = 0.f;
+    float n, mean, m2;
 };
 
 // Both may be empty; the moments of one alone come through unchanged. The reciprocal is the hardware's
@@ -90,16 +98,52 @@ __device__ __forceinline__ Moments join_lanes(Moments m, int lanes)
     return m;
 }
 
+// Moments of group `sub` of a slice over `parts` parts of `rows` rows each (`total` in all), by group_lanes
+// threads a group (sub_lane of them): in the first of these. Eight are asked for at a time, in four chains.
+template <bool kGlobal>
+__device__ __noinline__ Moments join_parts(const float2 *part, int pitch, int parts, long long rows, long long total,
+                                           int cpg, int group_lanes, int sub, int sub_lane, int gs)
+{
+    Moments chain[4] = {};
+    if (sub < gs)
+        for (int t0 = sub_lane; t0 < parts; t0 += 8 * group_lanes) {
+            float2 q[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int t = t0 + k * group_lanes;
+                if (t < parts) q[k] = kGlobal ? __ldcg(part + t * pitch + sub) : part[t * pitch + sub];
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int t = t0 + k * group_lanes;
+                if (t < parts) {
+                    Moments o;
+                    o.n = static_cast<float>(max(0LL, min(rows, total - t * rows)) * cpg);
+                    o.mean = q[k].x;
+                    o.m2 = q[k].y;
+                    chain[k & 3] = join(chain[k & 3], o);
+                }
+            }
+        }
+    return join_lanes(join(join(chain[0], chain[1]), join(chain[2], chain[3])), group_lanes);
+}
+
+// mean and 1 / sigma of a group
+__device__ __forceinline__ float2 norm_of(const Moments &m, float eps)
+{
+    return make_float2(m.mean, __frsqrt_rn(__fdiv_rn(m.m2, m.n) + eps));
+}
+
 // VEC elements of T as they are loaded: 16 bytes or one element
 template <typename T, int VEC>
 struct Raw {
     using type = uint4;
-    static __device__ __forceinline__ uint4 load(const T *p)
+    static __device__ __forceinline__ uint4 load(const T *p, uint64_t policy)
     {
         uint4 v;
-        asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+        asm volatile("ld.global.L1::no_allocate.L2::cache_hint.v4.u32 {%0, %1, %2, %3}, [%4], %5;"
                      : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                     : "l"(p)
+                     : "l"(p), "l"(policy)
                      : "memory");
         return v;
     }
@@ -124,7 +168,7 @@ struct Raw {
 template <typename T>
 struct Raw<T, 1> {
     using type = T;
-    static __device__ __forceinline__ T load(const T *p) { return *p; }
+    static __device__ __forceinline__ T load(const T *p, uint64_t) { return *p; }
     static __device__ __forceinline__ void floats(T v, float (&f)[1]) { f[0] = to_float<T>(v); }
 };
 
@@ -144,123 +188,198 @@ __device__ __forceinline__ void store_vec(T *p, const float (&f)[VEC])
     }
 }
 
-// A run: up to kAhead vectors of one column, read, held in shared memory when they come before `hold`,
-// and their moments joined to mo: N = 1 those of all values together, N = VEC of each of a vector's
-// channels. The pivot is the run's first vector.
-template <typename TI, int VEC, int N, bool kFull>
-__device__ __forceinline__ void read_run(const TI *px, long long step, int n, int i, int hold,
-                                         typename Raw<TI, VEC>::type *held, Moments (&mo)[N])
+// A run of vectors of one column, summed about its first: N moments a vector, of VEC / N channels each that
+// belong to one group.
+template <typename TI, int VEC, int N>
+struct Run {
+    using R = Raw<TI, VEC>;
+    static constexpr int kPer = VEC / N, kPairs = VEC / 2, kSums = N == 1 ? (VEC > 2 ? 2 : 1) : kPairs;
+    float p[N];
+    uint64_t minus[N == 1 ? 1 : kPairs], s2[kSums], q2[kSums];
+    __device__ __forceinline__ Run(const typename R::type &first)
+    {
+        float f[VEC];
+        R::floats(first, f);
+#pragma unroll
+        for (int e = 0; e < N; ++e) p[e] = f[e * kPer];
+#pragma unroll
+        for (int k = 0; k < (N == 1 ? 1 : kPairs); ++k)
+            minus[k] = pair(-p[N == 1 ? 0 : 2 * k / kPer], -p[N == 1 ? 0 : (2 * k + 1) / kPer]);
+#pragma unroll
+        for (int k = 0; k < kSums; ++k) s2[k] = q2[k] = 0;
+    }
+    __device__ __forceinline__ void add(const typename R::type &v)
+    {
+        float f[VEC];
+        R::floats(v, f);
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) {
+            const uint64_t d = add2(pair(f[2 * k], f[2 * k + 1]), minus[N == 1 ? 0 : k]);
+            s2[k % kSums] = add2(s2[k % kSums], d);
+            q2[k % kSums] = fma2(d, d, q2[k % kSums]);
+        }
+    }
+    // joins the run's `n` vectors to mo
+    __device__ __forceinline__ void end(int n, Moments (&mo)[N]) const
+    {
+        float sum[N], sq[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum[e] = sq[e] = 0.f;
+#pragma unroll
+        for (int k = 0; k < kSums; ++k) {
+            const float2 b = floats_of(s2[k]), c = floats_of(q2[k]);
+            const int e0 = N == 1 ? 0 : 2 * k / kPer, e1 = N == 1 ? 0 : (2 * k + 1) / kPer;
+            sum[e0] += b.x;
+            sum[e1] += b.y;
+            sq[e0] += c.x;
+            sq[e1] += c.y;
+        }
+        const float cnt = static_cast<float>(n * kPer), inv = __fdividef(1.f, cnt);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            Moments run;
+            run.n = cnt;
+            run.mean = fmaf(sum[e], inv, p[e]);
+            // not below 0 by rounding; 0 * sq keeps the NaN of a value that is not finite
+            run.m2 = fmaxf(fmaf(-sum[e] * inv, sum[e], sq[e]), 0.f * sq[e]);
+            mo[e] = join(mo[e], run);
+        }
+    }
+};
+template <typename TI>
+struct Run<TI, 1, 1> {
+    float p, sum = 0.f, sq = 0.f;
+    __device__ __forceinline__ Run(const TI &first) { p = to_float<TI>(first); }
+    __device__ __forceinline__ void add(const TI &v)
+    {
+        const float d = to_float<TI>(v) - p;
+        sum += d;
+        sq = fmaf(d, d, sq);
+    }
+    __device__ __forceinline__ void end(int n, Moments (&mo)[1]) const
+    {
+        const float cnt = static_cast<float>(n), inv = __fdividef(1.f, cnt);
+        mo[0] = join(mo[0], Moments{cnt, fmaf(sum, inv, p), fmaxf(fmaf(-sum * inv, sum, sq), 0.f * sq)});
+    }
+};
+
+// The moments of a thread's `count` vectors, `step` elements apart; the first `hold` stay in shared memory.
+template <typename TI, int VEC, int N>
+__device__ __forceinline__ void read_rows(const TI *px, long long step, int count, uint64_t policy, int hold,
+                                          typename Raw<TI, VEC>::type *held, Moments (&mo)[N])
 {
     using R = Raw<TI, VEC>;
-    constexpr int kPairs = VEC > 1 ? VEC / 2 : 1, kSums = N == 1 ? (VEC > 2 ? 2 : 1) : kPairs, kPer = VEC / N;
-    if (kFull) n = kAhead;
     typename R::type v[kAhead];
+    int i = 0;
+#pragma unroll 1
+    for (; i + kAhead <= count; i += kAhead) {
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-        if (kFull || u < n) v[u] = R::load(px);
-        px += step;
+        for (int u = 0; u < kAhead; ++u, px += step) v[u] = R::load(px, policy);
+        if (i + kAhead <= hold) {
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) held[(i + u) * kThreads] = v[u];
+        } else if (i < hold) {
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+                if (i + u < hold) held[(i + u) * kThreads] = v[u];
+        }
+        Run<TI, VEC, N> run(v[0]);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) run.add(v[u]);
+        run.end(kAhead, mo);
     }
-    if (i + kAhead <= hold) {
+    if (i < count) {
+        const int n = count - i;
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u)
-            if (kFull || u < n) held[(i + u) * kThreads] = v[u];
-    } else if (i < hold) {
+        for (int u = 0; u < kAhead; ++u, px += step)
+            if (u < n) v[u] = R::load(px, policy);
 #pragma unroll
         for (int u = 0; u < kAhead; ++u)
             if (u < n && i + u < hold) held[(i + u) * kThreads] = v[u];
-    }
-    float f[VEC], p[N], sum[N], sq[N];
-    R::floats(v[0], f);
-#pragma unroll
-    for (int e = 0; e < N; ++e) p[e] = f[e * kPer];
-    if constexpr (VEC == 1) {
-        sum[0] = sq[0] = 0.f;
-#pragma unroll
-        for (int u = 1; u < kAhead; ++u)
-            if (kFull || u < n) {
-                R::floats(v[u], f);
-                const float d = f[0] - p[0];
-                sum[0] += d;
-                sq[0] = fmaf(d, d, sq[0]);
-            }
-    } else {
-        uint64_t minus[N == 1 ? 1 : kPairs], s2[kSums], q2[kSums];
-#pragma unroll
-        for (int k = 0; k < (N == 1 ? 1 : kPairs); ++k)
-            minus[k] = N == 1 ? pair(-p[0], -p[0]) : pair(-p[2 * k < N ? 2 * k : 0], -p[2 * k + 1 < N ? 2 * k + 1 : 0]);
-#pragma unroll
-        for (int k = 0; k < kSums; ++k) s2[k] = q2[k] = 0;
+        Run<TI, VEC, N> run(v[0]);
 #pragma unroll
         for (int u = 0; u < kAhead; ++u)
-            if (kFull || u < n) {
-                R::floats(v[u], f);
+            if (u < n) run.add(v[u]);
+        run.end(n, mo);
+    }
+}
+
+// Columns of vectors of a unit that a block works on at a time (all, unless a single group is wider than
+// the block), and a thread's place: one column, every lanes-th row.
+struct Place {
+    int nb, lanes, col, rl, count;
+};
+__device__ __forceinline__ Place place_of(int cb, int ncols, long long rows)
+{
+    Place p;
+    p.nb = min(kThreads, ncols - cb);
+    p.lanes = kThreads / p.nb;
+    p.rl = static_cast<int>(threadIdx.x) / p.nb;
+    p.col = cb + static_cast<int>(threadIdx.x) - p.rl * p.nb;
+    p.count = p.rl < p.lanes && p.rl < rows ? static_cast<int>((rows - p.rl + p.lanes - 1) / p.lanes) : 0;
+    return p;
+}
+
+// The block's moments of a unit's groups, from its threads'.
+template <int N>
+struct BlockMoments {
+    float2 entry[N][kThreads];  // (mean, M2) a thread and moment, and of how many values
+    float n[kThreads];
+    Moments group[kSliceGroups];
+};
+
+// Joins the threads' moments of the columns at cb to s.group[]. Ends without a barrier.
+// `sync` is the barrier of the kThreads threads.
+template <int VEC, int N, typename Sync>
+__device__ __forceinline__ void join_block(BlockMoments<N> &s, Moments (&mo)[N], const Place &p, int cb, int cpg, int gs,
+                                           int group_lanes, int sub, int sub_lane, Sync sync)
+{
+    sync();
 #pragma unroll
-                for (int k = 0; k < kPairs; ++k) {
-                    const uint64_t d = add2(pair(f[2 * k], f[2 * k + 1]), minus[N == 1 ? 0 : k]);
-                    s2[k % kSums] = add2(s2[k % kSums], d);
-                    q2[k % kSums] = fma2(d, d, q2[k % kSums]);
-                }
-            }
-        if constexpr (N == 1) {
-            const float2 a = floats_of(kSums == 2 ? add2(s2[0], s2[kSums - 1]) : s2[0]);
-            const float2 b = floats_of(kSums == 2 ? add2(q2[0], q2[kSums - 1]) : q2[0]);
-            sum[0] = a.x + a.y;
-            sq[0] = b.x + b.y;
-        } else {
+    for (int e = 0; e < N; ++e) s.entry[e][threadIdx.x] = make_float2(mo[e].mean, mo[e].m2);
+    s.n[threadIdx.x] = mo[0].n;
+    sync();
+    // down the rows: halves of the row lanes joined until one is left
+    for (int left = p.lanes; left > 1;) {
+        const int half = (left + 1) / 2;
+        if (p.rl + half < left) {
+            const int other = threadIdx.x + half * p.nb;
+            const float n = s.n[other];
 #pragma unroll
-            for (int k = 0; k < kPairs; ++k) {
-                const float2 a = floats_of(s2[k]), b = floats_of(q2[k]);
-                sum[2 * k] = a.x;
-                sum[2 * k + 1] = a.y;
-                sq[2 * k] = b.x;
-                sq[2 * k + 1] = b.y;
+            for (int e = 0; e < N; ++e) {
+                const float2 q = s.entry[e][other];
+                Moments t;
+                t.n = n;
+                t.mean = q.x;
+                t.m2 = q.y;
+                mo[e] = join(mo[e], t);
+                s.entry[e][threadIdx.x] = make_float2(mo[e].mean, mo[e].m2);
             }
+            s.n[threadIdx.x] = mo[0].n;
+        }
+        left = half;
+        sync();
+    }
+    // across each group's moments along a row
+    constexpr int kPer = VEC / N;
+    Moments m = {0.f, 0.f, 0.f};
+    if (sub < gs) {
+        const int lo = max(sub * cpg / kPer, cb * N), end = min((sub + 1) * cpg / kPer, (cb + p.nb) * N);
+        for (int k = lo + sub_lane; k < end; k += group_lanes) {
+            const float2 q = s.entry[k % N][k / N - cb];
+            Moments t;
+            t.n = s.n[0];
+            t.mean = q.x;
+            t.m2 = q.y;
+            m = join(m, t);
         }
     }
-    const float cnt = static_cast<float>(n * kPer), inv = __fdividef(1.f, cnt);
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-        Moments run;
-        run.n = cnt;
-        run.mean = fmaf(sum[e], inv, p[e]);
-        // not below 0 by rounding; 0 * sq keeps the NaN of a value that is not finite
-        run.m2 = fmaxf(fmaf(-sum[e] * inv, sum[e], sq[e]), 0.f * sq[e]);
-        mo[e] = join(mo[e], run);
-    }
+    m = join_lanes(m, group_lanes);
+    if (sub_lane == 0 && sub < gs) s.group[sub] = join(s.group[sub], m);
 }
 
-template <typename TI, int VEC, int N>
-__device__ __forceinline__ void read_rows(const TI *px, long long step, int count, int hold,
-                                          typename Raw<TI, VEC>::type *held, Moments (&mo)[N])
-{
-    int i = 0;
-#pragma unroll 1
-    for (; i + kAhead <= count; i += kAhead, px += kAhead * step) read_run<TI, VEC, N, true>(px, step, kAhead, i, hold, held, mo);
-    if (i < count) read_run<TI, VEC, N, false>(px, step, count - i, i, hold, held, mo);
-}
-
-// silu and gelu_tanh of two values with one reciprocal for both: 1 / a = b / (a b). e^-z is cut off at 2^60
-// (a value below -41 gives -41 * 2^-60 and the like instead of 0), so that a b stays finite. Exponentials
-// and reciprocals share a unit of 16 a clock on an SM; at two each a value the output of 16-bit vectors took
-// 32 clocks a warp's vector there, at three for two 24, where the memory needs 22.
-template <int kAct>
-__device__ __forceinline__ uint64_t activate_pair(uint64_t v)
-{
-    if constexpr (kAct == S2_ACT_SILU || kAct == S2_ACT_GELU_TANH) {
-        constexpr float kLog2e = 1.4426950408889634f, kTanh = -2.f * 0.7978845608028654f * kLog2e;
-        const uint64_t z = kAct == S2_ACT_SILU ? mul2(v, both(-kLog2e))
-                                               : mul2(v, fma2(mul2(v, v), both(kTanh * 0.044715f), both(kTanh)));
-        const float2 zf = floats_of(z);
-        const float2 d = floats_of(add2(ex2_2(pair(fminf(zf.x, 60.f), fminf(zf.y, 60.f))), both(1.f)));
-        float r = d.x * d.y;
-        asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(r));
-        return mul2(v, mul2(both(r), pair(d.y, d.x)));
-    }
-    return activate2<kAct>(v);
-}
-
-// y = act((x - mean) scale + shift) of one vector; `minus` is -mean, one (kOne) or a pair of channels each.
-// The subtraction comes first, as in the formula: values that all equal the mean give the shift itself.
+// y = act((x - mean) scale + shift) of one vector; `minus` is -mean, one for VEC / N channels each. The
+// subtraction comes first, as in the formula: values that all equal the mean give the shift itself.
 template <typename TI, typename TO, int VEC, int N, int kAct>
 __device__ __forceinline__ void finish(const typename Raw<TI, VEC>::type &v, TO *py, const float (&minus)[N],
                                        const float (&scale)[VEC], const float (&shift)[VEC])
@@ -273,7 +392,7 @@ __device__ __forceinline__ void finish(const typename Raw<TI, VEC>::type &v, TO 
 #pragma unroll
         for (int k = 0; k < VEC / 2; ++k) {
             const uint64_t d = add2(pair(f[2 * k], f[2 * k + 1]), pair(minus[2 * k / (VEC / N)], minus[(2 * k + 1) / (VEC / N)]));
-            const float2 r = floats_of(activate_pair<kAct>(
+            const float2 r = floats_of(activate2<kAct>(
                 fma2(d, pair(scale[2 * k], scale[2 * k + 1]), pair(shift[2 * k], shift[2 * k + 1]))));
             f[2 * k] = r.x;
             f[2 * k + 1] = r.y;
@@ -282,34 +401,72 @@ __device__ __forceinline__ void finish(const typename Raw<TI, VEC>::type &v, TO 
     store_vec<TO, VEC>(py, f);
 }
 
-// y of the thread's vectors: those that are not held once more from global memory, the latest read
-// first (they are in L2 the longest), then the held ones.
+// y of a thread's `count` vectors, the first `hold` of them from shared memory.
 template <typename TI, typename TO, int VEC, int N, int kAct>
-__device__ __forceinline__ void write_rows(const TI *px, long long x_step, TO *py, long long y_step, int count, int hold,
-                                           const typename Raw<TI, VEC>::type *held, const float (&minus)[N],
-                                           const float (&scale)[VEC], const float (&shift)[VEC])
+__device__ __forceinline__ void write_rows(const TI *px, long long x_step, TO *py, long long y_step, int count,
+                                           uint64_t policy, int hold, const typename Raw<TI, VEC>::type *held,
+                                           const float (&minus)[N], const float (&scale)[VEC], const float (&shift)[VEC])
 {
     using R = Raw<TI, VEC>;
-    constexpr int kRun = 4;
-    int i = count;
-    if (i > hold) {
-        const TI *qx = px + (count - 1) * x_step;
-        TO *qy = py + (count - 1) * y_step;
-#pragma unroll 1
-        for (; i - kRun >= hold; i -= kRun) {
-            typename R::type v[kRun];
-#pragma unroll
-            for (int u = 0; u < kRun; ++u, qx -= x_step) v[u] = R::load(qx);
-#pragma unroll
-            for (int u = 0; u < kRun; ++u, qy -= y_step) finish<TI, TO, VEC, N, kAct>(v[u], qy, minus, scale, shift);
-        }
-#pragma unroll 1
-        for (; i > hold; --i, qx -= x_step, qy -= y_step) finish<TI, TO, VEC, N, kAct>(R::load(qx), qy, minus, scale, shift);
-    }
+    const int kept = min(count, hold);
 #pragma unroll 2
-    for (int k = 0; k < i; ++k) {
-        finish<TI, TO, VEC, N, kAct>(held[k * kThreads], py, minus, scale, shift);
-        py += y_step;
+    for (int k = 0; k < kept; ++k, py += y_step) finish<TI, TO, VEC, N, kAct>(held[k * kThreads], py, minus, scale, shift);
+    px += kept * x_step;
+    int i = kept;
+#pragma unroll 1
+    for (; i + kBatch <= count; i += kBatch) {
+        typename R::type v[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u, px += x_step) v[u] = R::load(px, policy);
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u, py += y_step) finish<TI, TO, VEC, N, kAct>(v[u], py, minus, scale, shift);
+    }
+#pragma unroll 1
+    for (; i < count; ++i, px += x_step, py += y_step)
+        finish<TI, TO, VEC, N, kAct>(R::load(px, policy), py, minus, scale, shift);
+}
+
+// What the output does to the channels of a unit's column `col`; the unit's channels begin at c0, norm[g]:
+// mean and 1 / sigma.
+template <int VEC, int N>
+__device__ __forceinline__ void affine_of(const GnArgs &a, int col, int c0, const float2 *norm, float (&minus)[N],
+                                          float (&scale)[VEC], float (&shift)[VEC])
+{
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        const float2 mr = norm[(col * VEC + e * (VEC / N)) / a.cpg];
+        minus[e] = -mr.x;
+#pragma unroll
+        for (int k = 0; k < VEC / N; ++k) {
+            const int i = e * (VEC / N) + k, c = c0 + col * VEC + i;
+            scale[i] = a.weight ? mr.y * __ldg(a.weight + c) : mr.y;
+            shift[i] = a.bias ? __ldg(a.bias + c) : 0.f;
+        }
+    }
+}
+
+// Output of a thread's column of a unit.
+template <typename TI, typename TO, int VEC, int N>
+__device__ __forceinline__ void write_column(const GnArgs &a, const Place &p, int c0, const float2 *norm, const TI *px,
+                                             TO *py, uint64_t policy, int hold, const typename Raw<TI, VEC>::type *held)
+{
+    float minus[N], scale[VEC], shift[VEC];
+    affine_of<VEC, N>(a, p.col, c0, norm, minus, scale, shift);
+    const long long xs = p.lanes * a.x_row, ys = p.lanes * a.y_row;
+    switch (a.act) {
+    case S2_ACT_RELU:
+        write_rows<TI, TO, VEC, N, S2_ACT_RELU>(px, xs, py, ys, p.count, policy, hold, held, minus, scale, shift);
+        break;
+    case S2_ACT_SILU:
+        write_rows<TI, TO, VEC, N, S2_ACT_SILU>(px, xs, py, ys, p.count, policy, hold, held, minus, scale, shift);
+        break;
+    case S2_ACT_GELU:
+        write_rows<TI, TO, VEC, N, S2_ACT_GELU>(px, xs, py, ys, p.count, policy, hold, held, minus, scale, shift);
+        break;
+    case S2_ACT_GELU_TANH:
+        write_rows<TI, TO, VEC, N, S2_ACT_GELU_TANH>(px, xs, py, ys, p.count, policy, hold, held, minus, scale, shift);
+        break;
+    default: write_rows<TI, TO, VEC, N, S2_ACT_NONE>(px, xs, py, ys, p.count, policy, hold, held, minus, scale, shift);
     }
 }
 
@@ -320,66 +477,31 @@ __device__ __forceinline__ uint32_t ld_acquire(const uint32_t *p)
     return v;
 }
 
-// device error codes: the wait for the other members, for the ring's loads
+// device error codes: the wait for the other parts of a unit, for the ring's loads
 enum : int { E_JOIN = 96, E_RING = 97 };
 
-// The members' moments of group `sub` of the slice, by group_lanes threads a group (sub_lane of them): in the
-// first of these. Eight are asked for at a time and joined in four chains; which thread joins what depends on
-// the shape alone.
-template <bool kGlobal>
-__device__ __noinline__ Moments join_members(const GnArgs &a, const float2 *part, int pitch, int sub, int sub_lane, int gs)
-{
-    Moments chain[4];
-    if (sub < gs)
-        for (int t0 = sub_lane; t0 < a.members; t0 += 8 * a.group_lanes) {
-            float2 q[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int t = t0 + k * a.group_lanes;
-                if (t < a.members) q[k] = kGlobal ? __ldcg(part + t * pitch + sub) : part[t * pitch + sub];
-            }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int t = t0 + k * a.group_lanes;
-                if (t < a.members) {
-                    Moments o;
-                    o.n = static_cast<float>((a.rows + (t < a.more_rows)) * a.cpg);
-                    o.mean = q[k].x;
-                    o.m2 = q[k].y;
-                    chain[k & 3] = join(chain[k & 3], o);
-                }
-            }
-        }
-    return join_lanes(join(join(chain[0], chain[1]), join(chain[2], chain[3])), a.group_lanes);
-}
-
-// mean and 1 / sigma of a group
-__device__ __forceinline__ float2 norm_of(const Moments &m, float eps)
-{
-    return make_float2(m.mean, __frsqrt_rn(__fdiv_rn(m.m2, m.n) + eps));
-}
-
-// The members of a grid join a unit's moments (group[], gs of them): each writes its own, the last to arrive
-// joins all of them and publishes the unit's, the others wait for these. (Every member joining all for itself
-// read 296 x 32 moments 296 times from the same lines of L2: 8 us a unit.) `sync` is the barrier of the
-// threads that call this; *stop ends the wait, which is bounded. On return norm[] holds the unit's.
+// The parts of a unit on a grid join their moments (group[], gs of them): each writes its own, the last to
+// arrive joins all of them and publishes the unit's mean and 1 / sigma, the others wait for these. `sync` is
+// the barrier of the threads that call this; *stop ends the wait, which is bounded. On return norm[] holds
+// the unit's.
 template <typename Sync>
 __device__ __forceinline__ void join_grid(const GnArgs &a, int unit, int member, const Moments *group, int gs, int sub,
                                           int sub_lane, float2 *norm, volatile int *last, volatile int *stop, Sync sync)
 {
-    const long long at = static_cast<long long>(unit) * a.members;
+    const long long at = static_cast<long long>(unit) * a.parts;
     if (threadIdx.x < gs)
         __stcg(a.part + (at + member) * a.slice_groups + threadIdx.x, make_float2(group[threadIdx.x].mean, group[threadIdx.x].m2));
     sync();
     if (threadIdx.x == 0) {
         __threadfence();
-        *last = atomicAdd(a.arrived + unit, 1u) == static_cast<uint32_t>(a.members) - 1;
+        *last = atomicAdd(a.arrived + unit, 1u) == static_cast<uint32_t>(a.parts) - 1;
         __threadfence();
     }
     sync();
-    float2 *joined = a.joined + static_cast<long long>(unit) * a.slice_groups;
+    float2 *joined = a.norm + static_cast<long long>(unit) * a.slice_groups;
     if (*last) {
-        const Moments m = join_members<true>(a, a.part + at * a.slice_groups, a.slice_groups, sub, sub_lane, gs);
+        const Moments m = join_parts<true>(a.part + at * a.slice_groups, a.slice_groups, a.parts, a.part_rows, a.P, a.cpg,
+                                           a.group_lanes, sub, sub_lane, gs);
         if (sub_lane == 0 && sub < gs) {
             norm[sub] = norm_of(m, a.eps);
             __stcg(joined + sub, norm[sub]);
@@ -405,183 +527,100 @@ __device__ __forceinline__ void join_grid(const GnArgs &a, int unit, int member,
     }
 }
 
-// kOne: the VEC channels of a vector always belong to one group.
-template <typename TI, typename TO, int VEC, bool kOne>
-__global__ void __launch_bounds__(kThreads, 2) group_norm_kernel(const GnArgs a)
+// ---- rows held by the blocks ---------------------------------------------------------
+
+template <typename TI, typename TO, int VEC, int N>
+__global__ void __launch_bounds__(kThreads, 2) group_norm_held_kernel(const GnArgs a)
 {
-    using R = Raw<TI, VEC>;
-    constexpr int N = kOne ? 1 : VEC;
     extern __shared__ uint4 held_raw[];
-    __shared__ float2 entry[N][kThreads];  // (mean, M2) a thread and channel, and of how many values
-    __shared__ float entry_n[kThreads];
-    __shared__ Moments group[kSliceGroups];
-    __shared__ float2 received[kMaxCluster][kSliceGroups];
-    __shared__ float2 norm[kSliceGroups];  // mean, 1 / sqrt(v + eps)
+    __shared__ BlockMoments<N> s;
+    __shared__ float2 received[kMaxCluster][kSliceGroups], norm[kSliceGroups];
     __shared__ int last, stop;
-    typename R::type *held = reinterpret_cast<typename R::type *>(held_raw) + threadIdx.x;
-    const int member = static_cast<int>(blockIdx.x) % a.members;
-    const long long r0 = member * a.rows + min(member, a.more_rows), rows = a.rows + (member < a.more_rows);
-    // for the joins of groups: group_lanes threads a group
+    auto *held = reinterpret_cast<typename Raw<TI, VEC>::type *>(held_raw) + threadIdx.x;
+    const int team = static_cast<int>(blockIdx.x) / a.parts, member = static_cast<int>(blockIdx.x) - team * a.parts;
     const int sub = static_cast<int>(threadIdx.x) / a.group_lanes, sub_lane = threadIdx.x % a.group_lanes;
     if (threadIdx.x == 0) stop = 0;
     if (a.join == kCluster) cluster_arrive();  // waited for below: no block writes to one that has not begun
-
-    for (int unit = static_cast<int>(blockIdx.x) / a.members; unit < a.units; unit += a.teams) {
-        const int s = unit / a.slices, g0 = (unit - s * a.slices) * a.slice_groups;
-        const int gs = min(a.slice_groups, a.G - g0), c0 = g0 * a.cpg;
-        const int ncols = gs * a.cpg / VEC;
+    const long long r0 = member * a.part_rows, rows = max(0LL, min(a.part_rows, a.P - r0));
+    const uint64_t policy = l2_evict_first();
+    for (int unit = team; unit < a.units; unit += a.teams) {  // a cluster has one unit
+        const int smp = unit / a.slices, g0 = (unit - smp * a.slices) * a.slice_groups;
+        const int gs = min(a.slice_groups, a.G - g0), c0 = g0 * a.cpg, ncols = gs * a.cpg / VEC;
+        const TI *x = static_cast<const TI *>(a.x) + smp * a.x_sample + r0 * a.x_row + c0;
+        TO *y = static_cast<TO *>(a.y) + smp * a.y_sample + r0 * a.y_row + c0;
         const int hold = ncols <= kThreads ? a.hold : 0;
-        const TI *x = static_cast<const TI *>(a.x) + s * a.x_sample + r0 * a.x_row + c0;
-        if (sub_lane == 0 && sub < gs) group[sub] = Moments();
-
-        // Columns of vectors, kThreads of them at a time (all, unless a single group is wider than that):
-        // a thread keeps one column and takes every lanes-th row.
-        int nb = 0, lanes = 0, col = 0, rl = 0, count = 0;
-        auto place = [&](int cb) {
-            nb = min(kThreads, ncols - cb);
-            lanes = kThreads / nb;
-            rl = static_cast<int>(threadIdx.x) / nb;
-            col = cb + static_cast<int>(threadIdx.x) - rl * nb;
-            count = rl < lanes && rl < rows ? static_cast<int>((rows - rl + lanes - 1) / lanes) : 0;
-        };
+        if (threadIdx.x < gs) s.group[threadIdx.x] = Moments{0.f, 0.f, 0.f};
+        Place p;
         for (int cb = 0; cb < ncols; cb += kThreads) {
-            place(cb);
-            Moments mo[N];
-            read_rows<TI, VEC, N>(x + rl * a.x_row + static_cast<long long>(col) * VEC, lanes * a.x_row, count, hold, held, mo);
-            // down the rows: halves of the row lanes joined until one is left
-            if (cb > 0) __syncthreads();
-#pragma unroll
-            for (int e = 0; e < N; ++e) entry[e][threadIdx.x] = make_float2(mo[e].mean, mo[e].m2);
-            entry_n[threadIdx.x] = mo[0].n;
-            __syncthreads();
-            for (int left = lanes; left > 1;) {
-                const int half = (left + 1) / 2;
-                if (rl + half < left) {
-                    const int other = threadIdx.x + half * nb;
-                    const float n = entry_n[other];
-#pragma unroll
-                    for (int e = 0; e < N; ++e) {
-                        const float2 q = entry[e][other];
-                        Moments t;
-                        t.n = n;
-                        t.mean = q.x;
-                        t.m2 = q.y;
-                        mo[e] = join(mo[e], t);
-                        entry[e][threadIdx.x] = make_float2(mo[e].mean, mo[e].m2);
-                    }
-                    entry_n[threadIdx.x] = mo[0].n;
-                }
-                left = half;
-                __syncthreads();
-            }
-            // across the columns of each group (N = 1), or its channels
-            Moments m;
-            if (sub < gs) {
-                constexpr int kUnit = N == 1 ? VEC : 1;
-                const int lo = max(sub * a.cpg / kUnit, cb * (VEC / kUnit)) - cb * (VEC / kUnit);
-                const int end = min((sub + 1) * a.cpg / kUnit, (cb + nb) * (VEC / kUnit)) - cb * (VEC / kUnit);
-                for (int k = lo + sub_lane; k < end; k += a.group_lanes) {
-                    const float2 q = N == 1 ? entry[0][k] : entry[k % N][k / N];
-                    Moments t;
-                    t.n = entry_n[0];
-                    t.mean = q.x;
-                    t.m2 = q.y;
-                    m = join(m, t);
-                }
-            }
-            m = join_lanes(m, a.group_lanes);
-            if (sub_lane == 0 && sub < gs) group[sub] = join(group[sub], m);
+            p = place_of(cb, ncols, rows);
+            Moments mo[N] = {};
+            read_rows<TI, VEC, N>(x + p.rl * a.x_row + static_cast<long long>(p.col) * VEC, p.lanes * a.x_row, p.count, policy,
+                                  hold, held, mo);
+            join_block<VEC, N>(s, mo, p, cb, a.cpg, gs, a.group_lanes, sub, sub_lane, [] { __syncthreads(); });
         }
         __syncthreads();
-
-        // hand the moments to the other members and take theirs
-        if (a.join == kAlone) {
-            if (threadIdx.x < gs) received[0][threadIdx.x] = make_float2(group[threadIdx.x].mean, group[threadIdx.x].m2);
-            __syncthreads();
+        if (a.join == kGrid) {
+            join_grid(a, unit, member, s.group, gs, sub, sub_lane, norm, &last, &stop, [] { __syncthreads(); });
+            if (stop) return;
         } else if (a.join == kCluster) {
             cluster_wait();
-            for (int i = threadIdx.x; i < kSliceGroups * a.members; i += kThreads) {
+            for (int i = threadIdx.x; i < kSliceGroups * a.parts; i += kThreads) {
                 const int to = i / kSliceGroups, g = i % kSliceGroups;
                 if (g < gs) {
                     const uint32_t at = cluster_map(smem_u32(&received[member][g]), static_cast<uint32_t>(to));
-                    st_cluster_b32(at, __float_as_uint(group[g].mean));
-                    st_cluster_b32(at + 4, __float_as_uint(group[g].m2));
+                    st_cluster_b32(at, __float_as_uint(s.group[g].mean));
+                    st_cluster_b32(at + 4, __float_as_uint(s.group[g].m2));
                 }
             }
             __syncwarp();
             cluster_sync();
-        } else {
-            join_grid(a, unit, member, group, gs, sub, sub_lane, norm, &last, &stop, [] { __syncthreads(); });
-            if (stop) return;
-        }
-        if (a.join != kGrid) {
-            const Moments m = join_members<false>(a, &received[0][0], kSliceGroups, sub, sub_lane, gs);
+            const Moments m = join_parts<false>(&received[0][0], kSliceGroups, a.parts, a.part_rows, a.P, a.cpg,
+                                                a.group_lanes, sub, sub_lane, gs);
             if (sub_lane == 0 && sub < gs) norm[sub] = norm_of(m, a.eps);
-            __syncthreads();
+        } else if (threadIdx.x < gs) {
+            norm[threadIdx.x] = norm_of(s.group[threadIdx.x], a.eps);
         }
-
-        TO *y = static_cast<TO *>(a.y) + s * a.y_sample + r0 * a.y_row + c0;
+        __syncthreads();
         for (int cb = 0; cb < ncols; cb += kThreads) {
-            if (ncols > kThreads) place(cb);
-            if (count == 0) continue;
-            float minus[N], scale[VEC], shift[VEC];
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const int c = col * VEC + e;
-                const float2 mr = norm[(kOne ? col * VEC : c) / a.cpg];
-                minus[e % N] = -mr.x;
-                scale[e] = a.weight ? mr.y * __ldg(a.weight + c0 + c) : mr.y;
-                shift[e] = a.bias ? __ldg(a.bias + c0 + c) : 0.f;
-            }
-            const TI *px = x + rl * a.x_row + static_cast<long long>(col) * VEC;
-            TO *py = y + rl * a.y_row + static_cast<long long>(col) * VEC;
-            const long long xs = lanes * a.x_row, ys = lanes * a.y_row;
-            switch (a.act) {
-            case S2_ACT_RELU: write_rows<TI, TO, VEC, N, S2_ACT_RELU>(px, xs, py, ys, count, hold, held, minus, scale, shift); break;
-            case S2_ACT_SILU: write_rows<TI, TO, VEC, N, S2_ACT_SILU>(px, xs, py, ys, count, hold, held, minus, scale, shift); break;
-            case S2_ACT_GELU: write_rows<TI, TO, VEC, N, S2_ACT_GELU>(px, xs, py, ys, count, hold, held, minus, scale, shift); break;
-            case S2_ACT_GELU_TANH:
-                write_rows<TI, TO, VEC, N, S2_ACT_GELU_TANH>(px, xs, py, ys, count, hold, held, minus, scale, shift);
-                break;
-            default: write_rows<TI, TO, VEC, N, S2_ACT_NONE>(px, xs, py, ys, count, hold, held, minus, scale, shift);
-            }
+            if (ncols > kThreads) p = place_of(cb, ncols, rows);
+            if (p.count > 0)
+                write_column<TI, TO, VEC, N>(a, p, c0, norm, x + p.rl * a.x_row + static_cast<long long>(p.col) * VEC,
+                                             y + p.rl * a.y_row + static_cast<long long>(p.col) * VEC, policy, hold, held);
         }
         __syncthreads();  // the next unit reuses the moments
     }
 }
 
-// ---- large units -----------------------------------------------------------------
+// ---- rows through a ring ---------------------------------------------------------------
 
-constexpr int kRingThreads = 256;             // and a warp that only loads; two blocks an SM
-constexpr int kSlotPasses = 4;                // passes of a slot
-constexpr int kRunSlots = 2;                  // slots summed about one pivot
-constexpr uint32_t kSlotBytes = kSlotPasses * kRingThreads * 16;
-
-// Slots of the ring: what is left beside the joins' shared memory.
+constexpr int kSlotPasses = 4;  // rows a thread has in a slot
+constexpr int kRunSlots = kAhead / kSlotPasses;
+constexpr uint32_t kSlotBytes = kSlotPasses * kThreads * 16;
+// Slots beside the moments, of two blocks an SM.
 template <int N>
 __host__ __device__ constexpr int ring_slots()
 {
-    return 6;
+    return N == 8 ? 5 : 6;
 }
 
-// A member's slots over one unit: slot i holds kSlotPasses times `lanes` of its rows.
+// A part's slots over one unit: slot i holds the unit's rows [i * rows, (i + 1) * rows) of the part.
 struct Slots {
-    int lanes, rows;  // of a pass, of a slot
+    int lanes, rows;  // rows of a pass, of a slot
     int total, held;  // held: the last ones stay in the ring from the statistics to the output
 };
 
-template <int N>
+template <int kSlots>
 __device__ __forceinline__ Slots slots_of(long long rows, int ncols)
 {
     Slots p;
-    p.lanes = kRingThreads / ncols;
+    p.lanes = kThreads / ncols;
     p.rows = kSlotPasses * p.lanes;
     p.total = static_cast<int>((rows + p.rows - 1) / p.rows);
-    p.held = min(p.total, ring_slots<N>());
+    p.held = min(p.total, kSlots);
     return p;
 }
 
-// One thread's view of the ring: a place in the sequence of loads, and its own 16 bytes of a slot.
+// One thread's view of the ring: a place in the sequence of loads, and its own vectors of that slot.
 template <int kSlots>
 struct Cursor {
     uint32_t mine;  // shared address of the thread's vector of slot 0
@@ -594,11 +633,11 @@ struct Cursor {
         slot = q % kSlots;
         phase = q / kSlots & 1u;
     }
-    // A wait that ran out raises `abort`, which ends all later ones at once: the block runs on to its end
+    // A wait that runs out raises `abort`, which ends all later ones at once: the block runs on to its end
     // (every thread meets the same barriers) with the error recorded.
     __device__ __forceinline__ void wait() const { mbar_wait(full0 + 8 * slot, phase, abort, err, E_RING); }
-    // the thread's vector of pass k of the slot, `stride` bytes a pass (the ring is only written by copies
-    // the compiler does not see, so its loads are spelled out)
+    // the thread's vector of pass k of the slot, `stride` bytes a pass (the ring is written by copies that the
+    // compiler does not see, so its loads are spelled out)
     __device__ __forceinline__ uint4 get(int k, uint32_t stride) const
     {
         uint4 v;
@@ -622,8 +661,8 @@ struct Cursor {
     }
 };
 
-// The unit's rows of one thread, in the order in which the ring holds them. `count`: its rows, `stride`:
-// vectors of a pass.
+// The unit's rows of one thread, in the order in which the ring holds them: the held slots, then the others
+// again, the latest first. `count`: its rows, `stride`: bytes of a pass.
 template <typename TI, typename TO, int N, int kAct, int kSlots>
 __device__ __forceinline__ void write_slots(Cursor<kSlots> c, const Slots &p, int count, uint32_t stride, TO *y, long long step,
                                             const float (&minus)[N], const float (&scale)[16 / sizeof(TI)],
@@ -658,49 +697,41 @@ __device__ __forceinline__ void write_slots(Cursor<kSlots> c, const Slots &p, in
     }
 }
 
-// Group norm of units that are shared by the blocks of a cooperative grid. A loading warp streams the
-// member's rows through a ring of slots with bulk copies, far ahead of the threads that sum and write,
-// so that the memory is never waited for; what the ring can hold is read once. Rows beyond it come a
-// second time, the latest first (from L2, as far as it holds them). With a.ahead the ring holds two
-// units: the next one's statistics come before this one's output, and the members' join is hidden.
 // N: moments a vector, 16 / sizeof(TI) / N channels each, which always belong to one group.
 template <typename TI, typename TO, int N>
-__global__ void __launch_bounds__(kRingThreads + 32, 2) group_norm_ring_kernel(const GnArgs a)
+__global__ void __launch_bounds__(kThreads + 32, 2) group_norm_ring_kernel(const GnArgs a)
 {
-    constexpr int VEC = 16 / sizeof(TI), kPer = VEC / N, kPairs = VEC / 2, kSlots = ring_slots<N>();
-    constexpr int kRound = N < 4 ? N : 4;  // moments joined at a time
-    using R = Raw<TI, VEC>;
+    constexpr int VEC = 16 / sizeof(TI), kSlots = ring_slots<N>();
     extern __shared__ uint4 ring[];
-    __shared__ float2 entry[kRound][kRingThreads];
-    __shared__ float entry_n[kRingThreads];
-    __shared__ Moments group[kSliceGroups];
+    __shared__ BlockMoments<N> s;
     __shared__ float2 norm[kSliceGroups];
     __shared__ uint64_t bars[2 * kSlots];
     __shared__ int abort_flag, last;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int member = static_cast<int>(blockIdx.x) % a.members, team = static_cast<int>(blockIdx.x) / a.members;
-    const long long r0 = member * a.rows + min(member, a.more_rows), rows = a.rows + (member < a.more_rows);
+    const int team = static_cast<int>(blockIdx.x) / a.parts, member = static_cast<int>(blockIdx.x) - team * a.parts;
+    const long long r0 = member * a.part_rows, rows = max(0LL, min(a.part_rows, a.P - r0));
     const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * kSlots;
     volatile int *abort = &abort_flag;
     if (threadIdx.x == 0) {
         for (int i = 0; i < kSlots; ++i) {
             mbar_init(full0 + 8 * i, 1);
-            mbar_init(empty0 + 8 * i, kRingThreads / 32);
+            mbar_init(empty0 + 8 * i, kThreads / 32);
         }
         abort_flag = 0;
         fence_mbar_init();
     }
     __syncthreads();
 
-    if (warp == kRingThreads / 32) {
+    if (warp == kThreads / 32) {
+        // the loads of all units, as far ahead as slots are free
+        const uint64_t once = l2_evict_first(), again = l2_evict_last();
         uint32_t slot = 0, phase = 0, issued = 0;
         bool ok = true;
-        const uint64_t once = l2_evict_first(), again = l2_evict_last();
         for (int unit = team; ok && unit < a.units; unit += a.teams) {
-            const int s = unit / a.slices, g0 = (unit - s * a.slices) * a.slice_groups;
+            const int smp = unit / a.slices, g0 = (unit - smp * a.slices) * a.slice_groups;
             const int ncols = min(a.slice_groups, a.G - g0) * a.cpg / VEC;
-            const Slots p = slots_of<N>(rows, ncols);
-            const TI *x = static_cast<const TI *>(a.x) + s * a.x_sample + r0 * a.x_row + g0 * a.cpg;
+            const Slots p = slots_of<kSlots>(rows, ncols);
+            const TI *x = static_cast<const TI *>(a.x) + smp * a.x_sample + r0 * a.x_row + g0 * a.cpg;
             const uint32_t row_bytes = ncols * 16;
             const bool dense = a.x_row * sizeof(TI) == row_bytes;
             const int loads = 2 * p.total - p.held;
@@ -738,194 +769,72 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2) group_norm_ring_kernel(c
     }
 
     const int sub = static_cast<int>(threadIdx.x) / a.group_lanes, sub_lane = threadIdx.x % a.group_lanes;
+    auto sync = [] { named_barrier_sync(1, kThreads); };
     Cursor<kSlots> cur{smem_u32(ring) + threadIdx.x * 16, full0, empty0, abort, a.err, 0, 0};
-    auto sync = [] { named_barrier_sync(1, kRingThreads); };
-    // where the next unit's loads begin in the ring's sequence
-    uint32_t begin = 0;
-
-    struct Unit {
-        int s, g0, gs, ncols, rl, col, count;
-        uint32_t begin;
-        Slots p;
-    };
-    auto describe = [&](int unit) {
-        Unit u;
-        u.s = unit / a.slices;
-        u.g0 = (unit - u.s * a.slices) * a.slice_groups;
-        u.gs = min(a.slice_groups, a.G - u.g0);
-        u.ncols = u.gs * a.cpg / VEC;
-        u.p = slots_of<N>(rows, u.ncols);
-        u.rl = static_cast<int>(threadIdx.x) / u.ncols;
-        u.col = static_cast<int>(threadIdx.x) - u.rl * u.ncols;
-        u.count = u.rl < u.p.lanes && u.rl < rows ? static_cast<int>((rows - u.rl + u.p.lanes - 1) / u.p.lanes) : 0;
-        u.begin = begin;
-        begin += 2 * u.p.total - u.p.held;
-        return u;
-    };
-    // the unit's moments, handed to its members
-    auto statistics = [&](int unit, const Unit &u) {
-        Moments mo[N];
-        cur.go(u.begin);
-        const uint32_t stride = u.p.lanes * u.ncols * 16;
-        for (int i = 0; i < u.p.total; i += kRunSlots) {
-            constexpr int kSums = N == 1 ? 2 : kPairs;
-            float p[N];
-            uint64_t minus[N == 1 ? 1 : kPairs], s2[kSums], q2[kSums];
-#pragma unroll
-            for (int k = 0; k < kSums; ++k) s2[k] = q2[k] = 0;
-            const int n = min(kRunSlots, u.p.total - i), valid = min(n * kSlotPasses, u.count - i * kSlotPasses);
-            auto add = [&](const uint4 &raw) __attribute__((always_inline)) {
-                float f[VEC];
-                R::floats(raw, f);
-#pragma unroll
-                for (int k = 0; k < kPairs; ++k) {
-                    const uint64_t d = add2(pair(f[2 * k], f[2 * k + 1]), minus[N == 1 ? 0 : k]);
-                    s2[k % kSums] = add2(s2[k % kSums], d);
-                    q2[k % kSums] = fma2(d, d, q2[k % kSums]);
-                }
-            };
+    uint32_t begin = 0;  // the unit's place in the sequence of loads
+    for (int unit = team; unit < a.units; unit += a.teams) {
+        const int smp = unit / a.slices, g0 = (unit - smp * a.slices) * a.slice_groups;
+        const int gs = min(a.slice_groups, a.G - g0), c0 = g0 * a.cpg, ncols = gs * a.cpg / VEC;
+        const Slots p = slots_of<kSlots>(rows, ncols);
+        const Place at = place_of(0, ncols, rows);
+        const uint32_t stride = p.lanes * ncols * 16;
+        if (threadIdx.x < gs) s.group[threadIdx.x] = Moments{0.f, 0.f, 0.f};
+        Moments mo[N] = {};
+        cur.go(begin);
+        for (int i = 0; i < p.total; i += kRunSlots) {
+            const int n = min(kRunSlots, p.total - i), valid = min(n * kSlotPasses, at.count - i * kSlotPasses);
             cur.wait();
-            {
-                float f[VEC];
-                R::floats(cur.get(0, stride), f);
-#pragma unroll
-                for (int e = 0; e < N; ++e) p[e] = f[e * kPer];
-#pragma unroll
-                for (int k = 0; k < (N == 1 ? 1 : kPairs); ++k)
-                    minus[k] = pair(-p[N == 1 ? 0 : 2 * k / kPer], -p[N == 1 ? 0 : (2 * k + 1) / kPer]);
-            }
+            Run<TI, VEC, N> run(cur.get(0, stride));
 #pragma unroll 1
-            for (int v = 0; v < n; ++v) {
-                if (v > 0) cur.wait();
-                uint4 raw[kSlotPasses];
+            for (int k = 0; k < n; ++k) {
+                if (k > 0) cur.wait();
+                uint4 v[kSlotPasses];
 #pragma unroll
-                for (int w = 0; w < kSlotPasses; ++w) raw[w] = cur.get(w, stride);
-                if (i + v < u.p.total - u.p.held) cur.release();
+                for (int w = 0; w < kSlotPasses; ++w) v[w] = cur.get(w, stride);
+                if (i + k < p.total - p.held) cur.release();
                 cur.next();
-                if ((v + 1) * kSlotPasses <= valid) {
+                if ((k + 1) * kSlotPasses <= valid) {
 #pragma unroll
-                    for (int w = 0; w < kSlotPasses; ++w) add(raw[w]);
+                    for (int w = 0; w < kSlotPasses; ++w) run.add(v[w]);
                 } else {
 #pragma unroll
                     for (int w = 0; w < kSlotPasses; ++w)
-                        if (v * kSlotPasses + w < valid) add(raw[w]);
+                        if (k * kSlotPasses + w < valid) run.add(v[w]);
                 }
             }
-            if (valid > 0) {
-                float sum[N], sq[N];
-#pragma unroll
-                for (int e = 0; e < N; ++e) sum[e] = sq[e] = 0.f;
-#pragma unroll
-                for (int k = 0; k < kSums; ++k) {
-                    const float2 b = floats_of(s2[k]), c = floats_of(q2[k]);
-                    const int e0 = N == 1 ? 0 : 2 * k / kPer, e1 = N == 1 ? 0 : (2 * k + 1) / kPer;
-                    sum[e0] += b.x;
-                    sum[e1] += b.y;
-                    sq[e0] += c.x;
-                    sq[e1] += c.y;
-                }
-                const float cnt = static_cast<float>(valid * kPer), inv = __fdividef(1.f, cnt);
-#pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    Moments run;
-                    run.n = cnt;
-                    run.mean = fmaf(sum[e], inv, p[e]);
-                    run.m2 = fmaxf(fmaf(-sum[e] * inv, sum[e], sq[e]), 0.f * sq[e]);
-                    mo[e] = join(mo[e], run);
-                }
-            }
+            if (valid > 0) run.end(valid, mo);
         }
-        if (sub_lane == 0 && sub < u.gs) group[sub] = Moments();
-#pragma unroll
-        for (int first = 0; first < N; first += kRound) {
-            sync();
-#pragma unroll
-            for (int e = 0; e < kRound; ++e) entry[e][threadIdx.x] = make_float2(mo[first + e].mean, mo[first + e].m2);
-            float n = mo[0].n;
-            entry_n[threadIdx.x] = n;
-            sync();
-            for (int left = u.p.lanes; left > 1;) {
-                const int half = (left + 1) / 2;
-                if (u.rl + half < left) {
-                    const int other = threadIdx.x + half * u.ncols;
-                    const float on = entry_n[other];
-#pragma unroll
-                    for (int e = 0; e < kRound; ++e) {
-                        const float2 o = entry[e][other], m = entry[e][threadIdx.x];
-                        Moments b, c;
-                        b.n = n;
-                        b.mean = m.x;
-                        b.m2 = m.y;
-                        c.n = on;
-                        c.mean = o.x;
-                        c.m2 = o.y;
-                        b = join(b, c);
-                        entry[e][threadIdx.x] = make_float2(b.mean, b.m2);
-                    }
-                    n += on;
-                    entry_n[threadIdx.x] = n;
-                }
-                left = half;
-                sync();
-            }
-            // group `sub`: the moments [sub cpg / kPer, (sub + 1) cpg / kPer) along a row of vectors, those
-            // of this round
-            Moments m;
-            if (sub < u.gs)
-                for (int k = sub * a.cpg / kPer + sub_lane; k < (sub + 1) * a.cpg / kPer; k += a.group_lanes) {
-                    const int e = k % N - first;
-                    if (e >= 0 && e < kRound) {
-                        const float2 o = entry[e][k / N];
-                        Moments c;
-                        c.n = entry_n[0];
-                        c.mean = o.x;
-                        c.m2 = o.y;
-                        m = join(m, c);
-                    }
-                }
-            m = join_lanes(m, a.group_lanes);
-            if (sub_lane == 0 && sub < u.gs) group[sub] = join(group[sub], m);
-        }
+        join_block<VEC, N>(s, mo, at, 0, a.cpg, gs, a.group_lanes, sub, sub_lane, sync);
         sync();
-        join_grid(a, unit, member, group, u.gs, sub, sub_lane, norm, &last, abort, sync);
-    };
+        join_grid(a, unit, member, s.group, gs, sub, sub_lane, norm, &last, abort, sync);
 
-    auto output = [&](const Unit &u) {
         float minus[N], scale[VEC], shift[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const int c = u.col * VEC + e;
-            const float2 mr = norm[min((u.col * VEC + e / kPer * kPer) / a.cpg, u.gs - 1)];
-            const int ch = min(u.g0 * a.cpg + c, a.C - 1);
-            minus[e / kPer] = -mr.x;
-            scale[e] = a.weight ? mr.y * __ldg(a.weight + ch) : mr.y;
-            shift[e] = a.bias ? __ldg(a.bias + ch) : 0.f;
-        }
-        TO *y = static_cast<TO *>(a.y) + u.s * a.y_sample + (r0 + u.rl) * a.y_row + u.g0 * a.cpg + u.col * VEC;
-        const long long y_step = u.p.lanes * a.y_row;
-        const uint32_t stride = u.p.lanes * u.ncols * 16;
-        cur.go(u.begin + u.p.total - u.p.held);
+        affine_of<VEC, N>(a, at.col, c0, norm, minus, scale, shift);
+        TO *y = static_cast<TO *>(a.y) + smp * a.y_sample + (r0 + at.rl) * a.y_row + c0 + at.col * VEC;
+        const long long step = p.lanes * a.y_row;
+        cur.go(begin + p.total - p.held);
         switch (a.act) {
-        case S2_ACT_RELU: write_slots<TI, TO, N, S2_ACT_RELU>(cur, u.p, u.count, stride, y, y_step, minus, scale, shift); break;
-        case S2_ACT_SILU: write_slots<TI, TO, N, S2_ACT_SILU>(cur, u.p, u.count, stride, y, y_step, minus, scale, shift); break;
-        case S2_ACT_GELU: write_slots<TI, TO, N, S2_ACT_GELU>(cur, u.p, u.count, stride, y, y_step, minus, scale, shift); break;
+        case S2_ACT_RELU: write_slots<TI, TO, N, S2_ACT_RELU>(cur, p, at.count, stride, y, step, minus, scale, shift); break;
+        case S2_ACT_SILU: write_slots<TI, TO, N, S2_ACT_SILU>(cur, p, at.count, stride, y, step, minus, scale, shift); break;
+        case S2_ACT_GELU: write_slots<TI, TO, N, S2_ACT_GELU>(cur, p, at.count, stride, y, step, minus, scale, shift); break;
         case S2_ACT_GELU_TANH:
-            write_slots<TI, TO, N, S2_ACT_GELU_TANH>(cur, u.p, u.count, stride, y, y_step, minus, scale, shift);
+            write_slots<TI, TO, N, S2_ACT_GELU_TANH>(cur, p, at.count, stride, y, step, minus, scale, shift);
             break;
-        default: write_slots<TI, TO, N, S2_ACT_NONE>(cur, u.p, u.count, stride, y, y_step, minus, scale, shift);
+        default: write_slots<TI, TO, N, S2_ACT_NONE>(cur, p, at.count, stride, y, step, minus, scale, shift);
         }
-    };
-
-    for (int unit = team; unit < a.units; unit += a.teams) {
-        const Unit u = describe(unit);
-        statistics(unit, u);
-        output(u);
+        begin += 2 * p.total - p.held;
     }
 }
 
-// The units, members and shared memory of a call.
+// ---- host --------------------------------------------------------------------------
+
+constexpr size_t kHold = 22 * kThreads * 16;  // shared memory for rows, two blocks an SM
+
+// The units of a call and the blocks that share them.
 struct Plan {
-    int slices, slice_groups, units, members, teams, join, hold;
+    int slices, slice_groups, units, parts, teams, join;
+    bool ring;
+    long long part_rows;
     size_t smem;
 };
 
@@ -937,13 +846,8 @@ bool is_wide(const s2_group_norm_act_desc &d)
     const size_t ie = elem(d.in_dtype), oe = elem(d.out_dtype), vec = 16 / ie;
     const uintptr_t xb = reinterpret_cast<uintptr_t>(d.x) | d.x_row * ie | (d.samples > 1 ? d.x_sample * ie : 0);
     const uintptr_t yb = reinterpret_cast<uintptr_t>(d.y) | d.y_row * oe | (d.samples > 1 ? d.y_sample * oe : 0);
-    // slices begin at whole groups, so these have to fall on whole vectors too
     return d.channels % vec == 0 && xb % 16 == 0 && yb % (vec * oe) == 0;
 }
-
-constexpr size_t kPiece = kThreads * 16;    // shared memory of one vector a thread
-constexpr size_t kHoldTwo = 22 * kPiece;    // held by each of two blocks an SM
-constexpr size_t kMaxHold = 50 * kPiece;    // by a block alone
 
 Plan plan_of(const s2_group_norm_act_desc &d, int sms)
 {
@@ -954,60 +858,67 @@ Plan plan_of(const s2_group_norm_act_desc &d, int sms)
     int step = 1;
     while (step * cpg % vec != 0) ++step;
     auto slices_of = [&](int sg) { return (d.groups + sg - 1) / sg; };
-    auto bytes_of = [&](int sg) { return d.positions * sg * cpg * size; };  // of a unit
-    auto fit = [&](int sg, int members, size_t hold) { return (bytes_of(sg) + members - 1) / members <= static_cast<long long>(hold * 15 / 16); };
+    auto width = [&](int sg) { return sg * cpg * size; };
+    auto bytes_of = [&](int sg) { return d.positions * width(sg); };  // of a unit
+    auto halve = [&](int sg) { return std::max(step, sg / 2 / step * step); };
+    auto fit = [&](int sg, int members) { return bytes_of(sg) / members <= static_cast<long long>(kHold * 15 / 16); };
     Plan p;
     p.slice_groups = std::max(step, std::min(d.groups, kSliceGroups / step * step));
-    auto halve = [&](int sg) { return std::max(step, sg / 2 / step * step); };
-    auto width = [&](int sg) { return sg * cpg * size; };
-    p.smem = kHoldTwo;
     p.join = kGrid;
+    // Held by a cluster, if need be in narrower slices. Reading 128 bytes of each row at a time costs little,
+    // 32 do once the memory is the limit: 6 x 14400 x 512 took 80 us in slices of 32 bytes and 47 through the
+    // ring, but 3 x 7973 x 96 (9 MB) 12.8 us in slices of 48 and 18.3 on a grid.
+    const int narrow = d.samples * bytes_of(d.groups) <= (32LL << 20) ? 32 : 128;
     for (int sg = p.slice_groups;; sg = halve(sg)) {
-        if (fit(sg, kMaxCluster, kHoldTwo)) {
+        if (fit(sg, kMaxCluster)) {
             p.slice_groups = sg;
             p.join = kCluster;
             break;
         }
-        if (halve(sg) == sg || width(halve(sg)) < 128) break;
+        if (halve(sg) == sg || width(halve(sg)) < narrow) break;
     }
+    // A bulk copy takes the loading warp 60 clocks however short it is: 400 us became 16 ms with rows of 128
+    // bytes apart from one another. Packed rows are copied a slot at a time, others have to be long.
+    const bool rows_fit = d.x_row * size == width(p.slice_groups) || width(p.slice_groups) >= 1024;
+    p.ring = p.join == kGrid && wide && rows_fit && p.slice_groups * cpg / vec <= kThreads;
     if (p.join == kCluster) {
-        p.members = 1;
-        while (!fit(p.slice_groups, p.members, kHoldTwo)) p.members *= 2;
-        auto few = [&] { return 1LL * d.samples * slices_of(p.slice_groups) * p.members < sms; };
-        while (few() && p.members < kMaxCluster && d.positions >= 32 * p.members) p.members *= 2;
-        while (few() && halve(p.slice_groups) < p.slice_groups && width(halve(p.slice_groups)) >= 128) p.slice_groups = halve(p.slice_groups);
-    } else {
-        while (!fit(p.slice_groups, sms, kHoldTwo) && halve(p.slice_groups) < p.slice_groups && width(halve(p.slice_groups)) >= 64)
+        p.parts = 1;
+        while (!fit(p.slice_groups, p.parts)) p.parts *= 2;
+        auto few = [&] { return 1LL * d.samples * slices_of(p.slice_groups) * p.parts < sms; };
+        while (few() && halve(p.slice_groups) < p.slice_groups && width(halve(p.slice_groups)) >= 64)
             p.slice_groups = halve(p.slice_groups);
-        const long long want = (bytes_of(p.slice_groups) + kHoldTwo - 1) / kHoldTwo;
-        p.members = static_cast<int>(std::min<long long>(sms, want));
+        while (few() && p.parts < kMaxCluster && d.positions >= 32 * p.parts) p.parts *= 2;
     }
-    if (const char *e = getenv("GN_SG")) p.slice_groups = atoi(e);
-    if (const char *e = getenv("GN_JOIN")) p.join = atoi(e);
-    if (const char *e = getenv("GN_T")) p.members = atoi(e);
-    if (const char *e = getenv("GN_HOLD")) p.smem = atoi(e) * kPiece;
     p.slices = slices_of(p.slice_groups);
     p.units = d.samples * p.slices;
     p.teams = p.units;
-    if (p.join == kGrid)
-        p.teams = std::max(1, std::min(p.units, (p.smem <= kHoldTwo ? 2 : 1) * sms / p.members));
-    if (p.join == kRing) p.teams = std::max(1, std::min(p.units, 2 * sms / p.members));
-    if (const char *e = getenv("GN_TEAMS")) p.teams = atoi(e);
-    if (p.join == kCluster && p.members == 1) p.join = kAlone;
+    if (p.join == kGrid) {
+        // All units at once up to 8 of them, else three or four in flight, whichever leaves fewer blocks idle in
+        // the last round: while some read, others write. 11 x 57600 x 512 bf16: 387 us with two, 362 / 344 with
+        // three / four, 362 with all; 21 x 921600 x 128: 2.61, 2.34, 2.46 and 2.45 ms. More when a block's share
+        // of a unit would be less than it holds.
+        const int blocks = 2 * sms;
+        auto rounds = [&](int teams) { return static_cast<double>((p.units + teams - 1) / teams) / (blocks / teams); };
+        p.teams = p.units <= 8 ? p.units : (rounds(3) < rounds(4) ? 3 : 4);
+        const long long enough = std::max<long long>(1, (bytes_of(p.slice_groups) + kHold - 1) / static_cast<long long>(kHold));
+        p.teams = static_cast<int>(std::max<long long>(p.teams, std::min<long long>(p.units, blocks / enough)));
+        p.parts = static_cast<int>(std::min<long long>(blocks / p.teams, d.positions));
+    }
+    if (p.join == kCluster && p.parts == 1) p.join = kAlone;
+    p.part_rows = (d.positions + p.parts - 1) / p.parts;
     // no more shared memory than the rows need
-    const long long rows = (d.positions + p.members - 1) / p.members, ncols = p.slice_groups * cpg / vec;
-    const long long lanes = std::max<long long>(1, kThreads / ncols), pieces = (rows + lanes - 1) / lanes;
-    p.smem = std::min<size_t>(p.smem, static_cast<size_t>(pieces) * kThreads * (wide ? 16 : size));
+    const long long lanes = std::max<long long>(1, kThreads * vec / (p.slice_groups * cpg)), pieces = (p.part_rows + lanes - 1) / lanes;
+    p.smem = std::min<size_t>(kHold, static_cast<size_t>(pieces) * kThreads * (wide ? 16 : size));
     return p;
 }
 
 size_t round_up16(size_t v) { return (v + 15) / 16 * 16; }
+size_t counters_of(const Plan &p) { return static_cast<size_t>(p.units) * 8; }
 
 size_t workspace_of(const Plan &p)
 {
-    if (p.join != kGrid && p.join != kRing) return 0;
-    return round_up16(static_cast<size_t>(p.units) * 8) +
-           static_cast<size_t>(p.units) * (p.members + 1) * p.slice_groups * sizeof(float2);
+    if (p.join != kGrid) return 0;
+    return round_up16(counters_of(p)) + static_cast<size_t>(p.units) * (1 + p.parts) * p.slice_groups * sizeof(float2);
 }
 
 int sm_count()
@@ -1018,17 +929,15 @@ int sm_count()
     return sms > 0 ? sms : 148;
 }
 
-template <typename TI, typename TO, int VEC, bool kOne>
-s2_status launch(GnArgs &a, const Plan &p, cudaStream_t st)
+template <typename Kernel>
+s2_status launch(Kernel kernel, std::atomic<uint64_t> &configured, size_t most, size_t smem, int threads, const GnArgs &a,
+                 const Plan &p, cudaStream_t st)
 {
-    auto kernel = group_norm_kernel<TI, TO, VEC, kOne>;
-    static std::atomic<uint64_t> configured{0};
     const s2_status cs = s2::once_per_device(configured, [&] {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxHold);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most));
         return e == cudaSuccess ? S2_OK : s2::set_error(S2_INFERENCE_FAILED, "s2_group_norm_act: %s", cudaGetErrorString(e));
     });
     if (cs != S2_OK) return cs;
-    a.hold = static_cast<int>(p.smem / (kThreads * sizeof(typename Raw<TI, VEC>::type)));
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     if (p.join == kGrid) {
@@ -1036,13 +945,13 @@ s2_status launch(GnArgs &a, const Plan &p, cudaStream_t st)
         attr[0].val.cooperative = 1;
     } else {
         attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = static_cast<unsigned>(p.members);
+        attr[0].val.clusterDim.x = static_cast<unsigned>(p.parts);
         attr[0].val.clusterDim.y = 1;
         attr[0].val.clusterDim.z = 1;
     }
-    cfg.gridDim = dim3(static_cast<unsigned>(p.teams) * p.members);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = p.smem;
+    cfg.gridDim = dim3(static_cast<unsigned>(p.teams) * p.parts);
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
@@ -1050,44 +959,29 @@ s2_status launch(GnArgs &a, const Plan &p, cudaStream_t st)
     return e == cudaSuccess ? S2_OK : s2::set_error(S2_INFERENCE_FAILED, "s2_group_norm_act: launch failed: %s", cudaGetErrorString(e));
 }
 
-template <typename TI, typename TO, int N>
-s2_status launch_ring(const GnArgs &a, const Plan &p, cudaStream_t st)
+template <typename TI, typename TO, int VEC, int N>
+s2_status launch_shape(GnArgs &a, const Plan &p, cudaStream_t st)
 {
-    auto kernel = group_norm_ring_kernel<TI, TO, N>;
-    constexpr int kBytes = static_cast<int>(ring_slots<N>() * kSlotBytes);
-    static std::atomic<uint64_t> configured{0};
-    const s2_status cs = s2::once_per_device(configured, [&] {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
-        return e == cudaSuccess ? S2_OK : s2::set_error(S2_INFERENCE_FAILED, "s2_group_norm_act: %s", cudaGetErrorString(e));
-    });
-    if (cs != S2_OK) return cs;
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeCooperative;
-    attr[0].val.cooperative = 1;
-    cfg.gridDim = dim3(static_cast<unsigned>(p.teams) * p.members);
-    cfg.blockDim = dim3(kRingThreads + 32);
-    cfg.dynamicSmemBytes = kBytes;
-    cfg.stream = st;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
-    return e == cudaSuccess ? S2_OK : s2::set_error(S2_INFERENCE_FAILED, "s2_group_norm_act: launch failed: %s", cudaGetErrorString(e));
+    static std::atomic<uint64_t> held{0};
+    if constexpr (VEC > 1) {
+        static std::atomic<uint64_t> ring{0};
+        constexpr size_t kBytes = ring_slots<N>() * kSlotBytes;
+        if (p.ring) return launch(group_norm_ring_kernel<TI, TO, N>, ring, kBytes, kBytes, kThreads + 32, a, p, st);
+    }
+    a.hold = static_cast<int>(p.smem / (kThreads * sizeof(typename Raw<TI, VEC>::type)));
+    return launch(group_norm_held_kernel<TI, TO, VEC, N>, held, kHold, p.smem, kThreads, a, p, st);
 }
 
 template <typename TI, typename TO>
 s2_status launch_types(GnArgs &a, const Plan &p, bool wide, cudaStream_t st)
 {
     constexpr int kWide = 16 / sizeof(TI);
-    if (p.join == kRing) {
-        if (a.cpg % kWide == 0) return launch_ring<TI, TO, 1>(a, p, st);
-        if (a.cpg % (kWide / 2) == 0) return launch_ring<TI, TO, 2>(a, p, st);
-        if constexpr (kWide == 8)
-            if (a.cpg % 2 == 0) return launch_ring<TI, TO, 4>(a, p, st);
-        return launch_ring<TI, TO, kWide>(a, p, st);
-    }
-    if (!wide) return launch<TI, TO, 1, true>(a, p, st);
-    return a.cpg % kWide == 0 ? launch<TI, TO, kWide, true>(a, p, st) : launch<TI, TO, kWide, false>(a, p, st);
+    if (!wide) return launch_shape<TI, TO, 1, 1>(a, p, st);
+    if (a.cpg % kWide == 0) return launch_shape<TI, TO, kWide, 1>(a, p, st);
+    if (a.cpg % (kWide / 2) == 0) return launch_shape<TI, TO, kWide, 2>(a, p, st);
+    if constexpr (kWide == 8)
+        if (a.cpg % 2 == 0) return launch_shape<TI, TO, kWide, 4>(a, p, st);
+    return launch_shape<TI, TO, kWide, kWide>(a, p, st);
 }
 
 s2_status check(const s2_group_norm_act_desc *d)
@@ -1158,24 +1052,14 @@ extern "C" s2_status s2_group_norm_act(void *stream, const s2_group_norm_act_des
     if (need > 0 && (!d->workspace || d->workspace_bytes < need || reinterpret_cast<uintptr_t>(d->workspace) % 16))
         return s2::set_error(S2_INVALID_ARGUMENT, "s2_group_norm_act: workspace of %zu bytes, 16-byte aligned, needed", need);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    GnArgs a;
+    GnArgs a = {};
     a.x = d->x;
     a.y = d->y;
     a.weight = d->weight;
     a.bias = d->bias;
-    a.part = a.joined = nullptr;
-    a.arrived = a.ready = nullptr;
-    if (p.join == kGrid || p.join == kRing) {
-        a.arrived = static_cast<uint32_t *>(d->workspace);
-        a.ready = a.arrived + p.units;
-        a.joined = reinterpret_cast<float2 *>(static_cast<char *>(d->workspace) + round_up16(static_cast<size_t>(p.units) * 8));
-        a.part = a.joined + static_cast<size_t>(p.units) * p.slice_groups;
-        const cudaError_t e = cudaMemsetAsync(a.arrived, 0, static_cast<size_t>(p.units) * 8, st);
-        if (e != cudaSuccess) return s2::set_error(S2_INFERENCE_FAILED, "s2_group_norm_act: %s", cudaGetErrorString(e));
-    }
     a.err = d->err;
-    a.rows = d->positions / p.members;
-    a.more_rows = static_cast<int>(d->positions % p.members);
+    a.P = d->positions;
+    a.part_rows = p.part_rows;
     a.x_row = d->x_row;
     a.x_sample = d->samples > 1 ? d->x_sample : 0;
     a.y_row = d->y_row;
@@ -1186,13 +1070,21 @@ extern "C" s2_status s2_group_norm_act(void *stream, const s2_group_norm_act_des
     a.slices = p.slices;
     a.slice_groups = p.slice_groups;
     a.units = p.units;
-    a.members = p.members;
+    a.parts = p.parts;
     a.teams = p.teams;
     a.join = p.join;
-    a.group_lanes = 32;
-    while (a.group_lanes * p.slice_groups > (p.join == kRing ? kRingThreads : kThreads)) a.group_lanes /= 2;
     a.act = d->activation;
+    a.group_lanes = 32;
+    while (a.group_lanes * p.slice_groups > kThreads) a.group_lanes /= 2;
     a.eps = d->eps;
+    if (p.join == kGrid) {
+        a.arrived = static_cast<uint32_t *>(d->workspace);
+        a.ready = a.arrived + p.units;
+        a.norm = reinterpret_cast<float2 *>(static_cast<char *>(d->workspace) + round_up16(counters_of(p)));
+        a.part = a.norm + static_cast<size_t>(p.units) * p.slice_groups;
+        const cudaError_t e = cudaMemsetAsync(d->workspace, 0, counters_of(p), st);
+        if (e != cudaSuccess) return s2::set_error(S2_INFERENCE_FAILED, "s2_group_norm_act: %s", cudaGetErrorString(e));
+    }
     const bool wide = is_wide(*d);
     s2_status s;
     if (d->in_dtype == S2_F16)

@@ -958,6 +958,7 @@ def spatial_attention(q, k, v, channels, frames, tokens, out, err, stream=None):
 
 
 # ---- channels-last operators --------------------------------------------------
+# Calls of a few microseconds: what follows is spelled out where a helper's cost would show.
 
 def _fail(what: str):
     raise S2Error(S2_INVALID_ARGUMENT, what)
@@ -976,18 +977,19 @@ def _type_of(t, what: str) -> int:
     return code
 
 
-def _need_vector(t, n: int, device, what: str):
+def _need_vector(t, n: int, index: int, what: str):
     """The address of a contiguous fp32 vector of n values."""
-    if t.device != device or t.dtype != _torch().float32 or t.shape != (n,) or not t.is_contiguous():
-        _fail(f"{what} must be a contiguous fp32 tensor of {n} values on {device}")
+    if (t.get_device() != index or t.dtype != _torch().float32 or t.dim() != 1 or t.numel() != n
+            or not t.is_contiguous()):
+        _fail(f"{what} must be a contiguous fp32 tensor of {n} values on x's device")
     if t.requires_grad:
         _need_no_grad()
     return t.data_ptr()
 
 
-def _need_err(err, device):
-    if err.device != device or err.dtype != _torch().int32 or err.numel() < 1:
-        _fail(f"err must be an int32 tensor on {device}")
+def _need_err(err, index: int):
+    if err.get_device() != index or err.dtype != _torch().int32 or err.numel() < 1:
+        _fail("err must be an int32 tensor on x's device")
     return err.data_ptr()
 
 
@@ -1030,23 +1032,21 @@ def _elsewhere(fn, x, stream, *args):
 
 
 def _run_desc(call, workspace_bytes, desc, x, index: int, what: str):
-    """Calls with a workspace of the current stream's, on the current stream of the current device."""
+    """Calls on the current stream of the current device; a call that is refused for want of a
+    workspace is given one of that stream's."""
+    torch = _torch()
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # a torch.cuda.Stream costs as much as a launch
+    stream = raw(index) if raw is not None else torch.cuda.current_stream(index).cuda_stream
     ref = ctypes.byref(desc)
-    need = workspace_bytes(ref)
-    if need:
-        torch = _torch()
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-        desc.workspace, desc.workspace_bytes = ws.data_ptr(), need
-    status = call(_raw_stream(index), ref, None)
+    status = call(stream, ref, None)
+    if status == S2_INVALID_ARGUMENT:
+        need = workspace_bytes(ref)
+        if need:
+            ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+            desc.workspace, desc.workspace_bytes = ws.data_ptr(), need
+        status = call(stream, ref, None)
     if status != S2_OK:
         _check(status, what)
-
-
-def _raw_stream(index: int) -> int:
-    """The current stream of a device, without the cost of a torch.cuda.Stream object."""
-    torch = _torch()
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return raw(index) if raw is not None else torch.cuda.current_stream(index).cuda_stream
 
 
 def group_norm_act(x, groups: int, weight=None, bias=None, eps: float = 1e-6, activation: str = "none", out=None,
@@ -1057,32 +1057,39 @@ def group_norm_act(x, groups: int, weight=None, bias=None, eps: float = 1e-6, ac
     weight, bias: fp32 [channels] or None. Returns y in out_dtype (x's, or fp16 / bf16 for fp32 x)
     in x's shape; `out` receives it when given (it may be x). err: device int32 error word."""
     torch = _torch()
-    device = x.device
-    index = device.index
-    if stream is not None or not x.is_cuda or index != torch.cuda.current_device():
+    index = x.get_device()
+    if stream is not None or index < 0 or index != torch.cuda.current_device():
         return _elsewhere(group_norm_act, x, stream, groups, weight, bias, eps, activation, out, out_dtype, err)
-    if x.dim() < 2:
+    shape = x.shape
+    if len(shape) < 2:
         _fail("x must be [samples, ..., channels]")
     code = ACTIVATIONS.get(activation)
     if code is None:
         _fail(f"unknown activation {activation!r} (one of {', '.join(ACTIVATIONS)})")
     if x.requires_grad:
         _need_no_grad()
-    shape = x.shape
-    if out is None:
-        out = torch.empty(shape, dtype=out_dtype or x.dtype, device=device)
-    elif out.shape != shape or out.device != device or out_dtype not in (None, out.dtype):
-        _fail("out must have x's shape and device, and out_dtype if both are given")
     samples, channels = shape[0], shape[-1]
     positions, x_row = _pitch(x, 1, "x")
-    _, y_row = _pitch(out, 1, "out")
-    x_sample, y_sample = (x.stride(0), out.stride(0)) if samples > 1 else (0, 0)
-    d = GroupNormActDesc(samples, channels, groups, code, positions, _type_of(x, "x"), _type_of(out, "out"), eps,
-                         x.data_ptr(), x_row, x_sample,
-                         None if weight is None else _need_vector(weight, channels, device, "weight"),
-                         None if bias is None else _need_vector(bias, channels, device, "bias"), out.data_ptr(), y_row,
-                         y_sample, None, 0, None if err is None else _need_err(err, device))
-    L = lib()
+    in_type = out_type = _type_of(x, "x")
+    if out is None:
+        if out_dtype is None or out_dtype == x.dtype:
+            out = x.new_empty(shape)
+        else:
+            out = x.new_empty(shape, dtype=out_dtype)
+            out_type = _type_of(out, "out")
+        y_row, y_sample = channels, positions * channels
+    else:
+        if out.shape != shape or out.get_device() != index or out_dtype not in (None, out.dtype):
+            _fail("out must have x's shape and device, and out_dtype if both are given")
+        y_row = _pitch(out, 1, "out")[1]
+        y_sample = out.stride(0)
+        out_type = _type_of(out, "out")
+    d = GroupNormActDesc(samples, channels, groups, code, positions, in_type, out_type, eps, x.data_ptr(), x_row,
+                         x.stride(0) if samples > 1 else 0,
+                         None if weight is None else _need_vector(weight, channels, index, "weight"),
+                         None if bias is None else _need_vector(bias, channels, index, "bias"), out.data_ptr(), y_row,
+                         y_sample, None, 0, None if err is None else _need_err(err, index))
+    L = _lib or lib()
     _run_desc(L.s2_group_norm_act, L.s2_group_norm_act_workspace_bytes, d, x, index, "s2_group_norm_act")
     return out
 
@@ -1094,11 +1101,11 @@ def linear_act(x, w, bias=None, activation: str = "none", residual=None, out=Non
     output's type or None. Returns y [..., N] in out_dtype (x's, or fp32); `out` receives it when
     given (it may be the residual). err: device int32 error word."""
     torch = _torch()
-    device = x.device
-    index = device.index
-    if stream is not None or not x.is_cuda or index != torch.cuda.current_device():
+    index = x.get_device()
+    if stream is not None or index < 0 or index != torch.cuda.current_device():
         return _elsewhere(linear_act, x, stream, w, bias, activation, residual, out, out_dtype, err)
-    if x.dim() < 1 or w.dim() != 2 or w.shape[1] != x.shape[-1] or w.dtype != x.dtype or w.device != device:
+    shape, dtype = x.shape, x.dtype
+    if len(shape) < 1 or w.dim() != 2 or w.shape[1] != shape[-1] or w.dtype != dtype or w.get_device() != index:
         _fail("x must be [..., K] and w [N, K], of one type on one device")
     code = ACTIVATIONS.get(activation)
     if code is None:
@@ -1106,25 +1113,33 @@ def linear_act(x, w, bias=None, activation: str = "none", residual=None, out=Non
     if x.requires_grad or w.requires_grad:
         _need_no_grad()
     N, K = w.shape
-    shape = x.shape[:-1] + (N,)
-    if out is None:
-        out = torch.empty(shape, dtype=out_dtype or x.dtype, device=device)
-    elif out.shape != shape or out.device != device or out_dtype not in (None, out.dtype):
-        _fail(f"out must be {tuple(shape)} on x's device, and of out_dtype if both are given")
     rows, ldx = _pitch(x, 0, "x")
-    _, ldw = _pitch(w, 0, "w")
-    _, ldy = _pitch(out, 0, "out")
+    ldw = _pitch(w, 0, "w")[1]
+    in_type = out_type = _type_of(x, "x")
+    if out is None:
+        shape = (*shape[:-1], N)
+        if out_dtype is None or out_dtype == dtype:
+            out = x.new_empty(shape)
+        else:
+            out = x.new_empty(shape, dtype=out_dtype)
+            out_type = _type_of(out, "out")
+        ldy = N
+    else:
+        if out.shape != (*shape[:-1], N) or out.get_device() != index or out_dtype not in (None, out.dtype):
+            _fail(f"out must be {(*shape[:-1], N)} on x's device, and of out_dtype if both are given")
+        ldy = _pitch(out, 0, "out")[1]
+        out_type = _type_of(out, "out")
     res, ldr = None, 0
     if residual is not None:
-        if residual.shape != shape or residual.dtype != out.dtype or residual.device != device:
-            _fail(f"residual must be {tuple(shape)} in the output's type on x's device")
+        if residual.shape != out.shape or residual.dtype != out.dtype or residual.get_device() != index:
+            _fail(f"residual must be {tuple(out.shape)} in the output's type on x's device")
         if residual.requires_grad:
             _need_no_grad()
         res, ldr = residual.data_ptr(), _pitch(residual, 0, "residual")[1]
-    d = LinearActDesc(N, K, code, _type_of(x, "x"), _type_of(out, "out"), rows, x.data_ptr(), ldx, w.data_ptr(), ldw,
-                      None if bias is None else _need_vector(bias, N, device, "bias"), res, ldr, out.data_ptr(), ldy,
-                      None, 0, None if err is None else _need_err(err, device))
-    L = lib()
+    d = LinearActDesc(N, K, code, in_type, out_type, rows, x.data_ptr(), ldx, w.data_ptr(), ldw,
+                      None if bias is None else _need_vector(bias, N, index, "bias"), res, ldr, out.data_ptr(), ldy,
+                      None, 0, None if err is None else _need_err(err, index))
+    L = _lib or lib()
     _run_desc(L.s2_linear_act, L.s2_linear_act_workspace_bytes, d, x, index, "s2_linear_act")
     return out
 
