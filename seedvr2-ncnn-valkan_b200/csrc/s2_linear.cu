@@ -21,7 +21,6 @@
 #include <algorithm>
 #include <atomic>
 #include <cstdint>
-#include <type_traits>
 
 #include "s2_act.cuh"
 #include "s2_gemm.h"
@@ -43,6 +42,7 @@ struct LinearArgs {
     uint32_t fmt;     // operand format of the products: 0 fp16, 1 bf16
     int vec;          // residual and y rows start on 16 bytes
     int ks;           // linear_rows_kernel: CTAs that share a tile's K
+    int packed;       // operands come from a pack_rows_kernel right before
     int32_t *err;
 };
 
@@ -141,6 +141,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
 
     if (warp == 0) {
         if (lane == 0) {
+            wait_dependency();
             uint32_t p = 0;
             for (int kc = k_lo; kc < k_hi; ++kc, ++p) {
                 const uint32_t s = p % kStages, u = p / kStages;
@@ -215,22 +216,27 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
         const TO *res = static_cast<const TO *>(a.residual) + (m0 + c0) * a.ldr + n;
         TO *y = static_cast<TO *>(a.y) + (m0 + c0) * a.ldy + n;
         constexpr int kRun = 8;  // rows at a time: their residuals are all asked for first
+        const int last = share - 1;
+#pragma unroll 1
         for (int i = 0; c0 + i < c1; i += kRun) {
             float rv[kRun], v[kRun];
 #pragma unroll
-            for (int k = 0; k < kRun; ++k)
-                rv[k] = a.residual && c0 + i + k < c1 ? to_float<TO>(res[(i + k) * a.ldr]) : 0.f;
+            for (int k = 0; k < kRun; ++k, res += a.ldr) rv[k] = a.residual && c0 + i + k < c1 ? to_float<TO>(*res) : 0.f;
+            const float *q = part + i * kRowsN;
 #pragma unroll
-            for (int k = 0; k < kRun; ++k) v[k] = part[min(i + k, share - 1) * kRowsN];
-            for (int t = 1; t < a.ks; ++t)
+            for (int k = 0; k < kRun; ++k) v[k] = q[(i + k <= last ? k : 0) * kRowsN];
+#pragma unroll 1
+            for (int t = 1; t < a.ks; ++t) {
+                q += share * kRowsN;
 #pragma unroll
-                for (int k = 0; k < kRun; ++k) v[k] += part[(t * share + min(i + k, share - 1)) * kRowsN];
+                for (int k = 0; k < kRun; ++k) v[k] += q[(i + k <= last ? k : 0) * kRowsN];
+            }
 #pragma unroll
             for (int k = 0; k < kRun; ++k) v[k] += bias;
             activate_all<kRun>(v, a.act);
 #pragma unroll
-            for (int k = 0; k < kRun; ++k)
-                if (c0 + i + k < c1) y[(i + k) * a.ldy] = from_float<TO>(v[k] + rv[k]);
+            for (int k = 0; k < kRun; ++k, y += a.ldy)
+                if (c0 + i + k < c1) *y = from_float<TO>(v[k] + rv[k]);
         }
     }
     tc_fence_before();
@@ -241,7 +247,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
     }
 }
 
-// ---- up to four rows ---------------------------------------------------------------
+// ---- one row ---------------------------------------------------------------
 
 constexpr int kVecThreads = 256, kVecWarps = kVecThreads / 32;
 
@@ -287,84 +293,74 @@ struct Raw<1> {
     }
 };
 
-// One to four rows of x: every warp streams two rows of w, a.ks warps (1, 2, 4 or 8) share their K
-// by pieces of 32 vectors. VEC = 8: w and x rows start on 16 bytes; else values one by one.
-template <typename T, typename TO, int MR, int VEC>
-__global__ void __launch_bounds__(kVecThreads)
-    linear_vec_kernel(const T *__restrict__ x, long long ldx, const T *__restrict__ w, long long ldw, const LinearArgs a)
+// One row of x: every warp streams two rows of w, a.ks warps (1, 2, 4 or 8) share their K by pieces of 32
+// vectors, kAhead pieces in flight. VEC = 8: w's rows and x start on 16 bytes; else values one by one.
+template <typename T, typename TO, int VEC, int kAhead>
+__global__ void __launch_bounds__(kVecThreads) linear_vec_kernel(const T *__restrict__ x, const T *__restrict__ w, long long ldw,
+                                                                 const LinearArgs a)
 {
-    constexpr int kPiece = 32 * VEC, kAhead = VEC == 8 ? 4 : 8;
-    __shared__ float sums[kVecWarps][2 * MR];
+    constexpr int kPiece = 32 * VEC;
+    using R = Raw<VEC>;
+    __shared__ float sums[kVecWarps][2];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int group = (static_cast<int>(blockIdx.x) * kVecWarps + warp) / a.ks, part = warp % a.ks;
-    const int n = 2 * group;
-    float acc[2][MR] = {};
+    const int part = warp % a.ks, n = 2 * ((static_cast<int>(blockIdx.x) * kVecWarps + warp) / a.ks);
+    float acc0 = 0.f, acc1 = 0.f;
     if (n < a.N) {
         const T *w0 = w + n * ldw + lane * VEC;
         const T *w1 = w + min(n + 1, a.N - 1) * ldw + lane * VEC;
         const T *xl = x + lane * VEC;
         const int step = kPiece * a.ks, whole = a.K / VEC * VEC - (lane + 1) * VEC;
         for (int k = part * kPiece; k < a.K; k += kAhead * step) {
-            typename Raw<VEC>::type q[2][kAhead];
+            typename R::type q0[kAhead], q1[kAhead];
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
                 const bool in = k + u * step <= whole;
-                q[0][u] = in ? Raw<VEC>::stream(w0 + k + u * step) : Raw<VEC>::zero();
-                q[1][u] = in ? Raw<VEC>::stream(w1 + k + u * step) : Raw<VEC>::zero();
+                q0[u] = in ? R::stream(w0 + k + u * step) : R::zero();
+                q1[u] = in ? R::stream(w1 + k + u * step) : R::zero();
             }
 #pragma unroll
             for (int u = 0; u < kAhead; ++u)
                 if (k + u * step <= whole) {
-                    float f0[VEC], f1[VEC];
-                    Raw<VEC>::template floats<T>(q[0][u], f0);
-                    Raw<VEC>::template floats<T>(q[1][u], f1);
+                    float f0[VEC], f1[VEC], f[VEC];
+                    R::template floats<T>(q0[u], f0);
+                    R::template floats<T>(q1[u], f1);
+                    R::template floats<T>(R::load(xl + k + u * step), f);
 #pragma unroll
-                    for (int m = 0; m < MR; ++m) {
-                        float f[VEC];
-                        Raw<VEC>::template floats<T>(Raw<VEC>::load(xl + min(static_cast<long long>(m), a.M - 1) * ldx + k + u * step), f);
-#pragma unroll
-                        for (int e = 0; e < VEC; ++e) {
-                            acc[0][m] = fmaf(f0[e], f[e], acc[0][m]);
-                            acc[1][m] = fmaf(f1[e], f[e], acc[1][m]);
-                        }
+                    for (int e = 0; e < VEC; ++e) {
+                        acc0 = fmaf(f0[e], f[e], acc0);
+                        acc1 = fmaf(f1[e], f[e], acc1);
                     }
                 }
         }
         // the values past the last whole vector, one a lane
         const int tail = a.K / VEC * VEC + lane;
         if (VEC > 1 && part == 0 && tail < a.K) {
-#pragma unroll
-            for (int m = 0; m < MR; ++m) {
-                const float f = to_float<T>(x[min(static_cast<long long>(m), a.M - 1) * ldx + tail]);
-                acc[0][m] = fmaf(to_float<T>(w[n * ldw + tail]), f, acc[0][m]);
-                acc[1][m] = fmaf(to_float<T>(w[min(n + 1, a.N - 1) * ldw + tail]), f, acc[1][m]);
-            }
+            const float f = to_float<T>(x[tail]);
+            acc0 = fmaf(to_float<T>(w[n * ldw + tail]), f, acc0);
+            acc1 = fmaf(to_float<T>(w[min(n + 1, a.N - 1) * ldw + tail]), f, acc1);
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int m = 0; m < MR; ++m)
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) acc[i][m] += __shfl_xor_sync(0xffffffffu, acc[i][m], o);
+        for (int o = 16; o > 0; o >>= 1) {
+            acc0 += __shfl_xor_sync(0xffffffffu, acc0, o);
+            acc1 += __shfl_xor_sync(0xffffffffu, acc1, o);
+        }
     }
-    if (lane == 0)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int m = 0; m < MR; ++m) sums[warp][i * MR + m] = acc[i][m];
+    if (lane == 0) {
+        sums[warp][0] = acc0;
+        sums[warp][1] = acc1;
+    }
     __syncthreads();
-    // thread (group of the block, i, m): the parts' sums in order, then the epilogue
+    // a thread a column of the block: the parts' sums in order, then the epilogue
     const int groups = kVecWarps / a.ks;
-    if (threadIdx.x < groups * 2 * MR) {
-        const int g = threadIdx.x / (2 * MR), im = threadIdx.x % (2 * MR), m = im % MR;
-        const int col = 2 * (static_cast<int>(blockIdx.x) * groups + g) + im / MR;
-        if (col < a.N && m < a.M) {
-            float v[1] = {sums[g * a.ks][im]};
-            for (int t = 1; t < a.ks; ++t) v[0] += sums[g * a.ks + t][im];
+    if (threadIdx.x < groups * 2) {
+        const int g = threadIdx.x >> 1, i = threadIdx.x & 1, col = 2 * (static_cast<int>(blockIdx.x) * groups + g) + i;
+        if (col < a.N) {
+            float v[1] = {sums[g * a.ks][i]};
+            for (int t = 1; t < a.ks; ++t) v[0] += sums[g * a.ks + t][i];
             if (a.bias) v[0] += __ldg(a.bias + col);
             activate_all<1>(v, a.act);
-            if (a.residual) v[0] += to_float<TO>(static_cast<const TO *>(a.residual)[m * a.ldr + col]);
-            static_cast<TO *>(a.y)[m * a.ldy + col] = from_float<TO>(v[0]);
+            if (a.residual) v[0] += to_float<TO>(static_cast<const TO *>(a.residual)[col]);
+            static_cast<TO *>(a.y)[col] = from_float<TO>(v[0]);
         }
     }
 }
@@ -452,6 +448,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (lane == 0) {
             tma_prefetch_desc(&tmX);
             tma_prefetch_desc(&tmW);
+            wait_dependency();
             uint32_t p = 0;
             bool ok = true;
             for (int t = unit; ok && t < n_tiles; t += n_units) {
@@ -583,11 +580,27 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 } else {
                     if (lane == 0) bulk_wait_group_read<1>();
                     __syncwarp();
-                    if (res)
-                        for (int r = 0; r < 32; ++r)
-                            for (int c = lane; c < kSlab; c += 32)
-                                if (m0 + r < a.M && n + c < a.N)
-                                    slab[(r * 8 + ((c / kE) ^ (r & 7))) * kE + c % kE] = res[(m0 + r) * a.ldr + n + c];
+                    if (res) {
+                        constexpr int kRows = 8;  // rows whose values are asked for together
+#pragma unroll 1
+                        for (int r = 0; r < 32; r += kRows) {
+                            TO t[kRows][kSlab / 32];
+#pragma unroll
+                            for (int k = 0; k < kRows; ++k)
+#pragma unroll
+                                for (int c = 0; c < kSlab / 32; ++c)
+                                    t[k][c] = m0 + r + k < a.M && n + 32 * c + lane < a.N
+                                                  ? res[(m0 + r + k) * a.ldr + n + 32 * c + lane]
+                                                  : from_float<TO>(0.f);
+#pragma unroll
+                            for (int k = 0; k < kRows; ++k)
+#pragma unroll
+                                for (int c = 0; c < kSlab / 32; ++c) {
+                                    const int col = 32 * c + lane;
+                                    slab[((r + k) * 8 + ((col / kE) ^ ((r + k) & 7))) * kE + col % kE] = t[k][c];
+                                }
+                        }
+                    }
                 }
                 __syncwarp();
 #pragma unroll
@@ -681,13 +694,24 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 
 // ---- operands TMA cannot read -----------------------------------------------------
 
-// Rows of K 16-bit values at any pitch -> rows at `ldd`, a multiple of 8 values. A block a row
-// piece; what lies between K and ldd is not written (the tensor map ends at K).
+// Rows of K 16-bit values at any pitch -> rows at `ldd`, a multiple of 8 values: eight a thread, their loads
+// in flight together, one store. Past K zeros. The kernel behind it may start beside it (it waits before it
+// reads).
 __global__ void __launch_bounds__(256) pack_rows_kernel(const uint16_t *__restrict__ src, long long lds, long long rows,
                                                         int K, uint16_t *__restrict__ dst, long long ldd)
 {
-    for (long long r = blockIdx.x; r < rows; r += gridDim.x)
-        for (int k = threadIdx.x; k < K; k += 256) dst[r * ldd + k] = src[r * lds + k];
+    launch_dependents();
+    const long long per = ldd / 8, n = rows * per;
+    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < n; i += 256LL * gridDim.x) {
+        const long long r = i / per;
+        const int k = static_cast<int>(i - r * per) * 8;
+        const uint16_t *p = src + r * lds + k;
+        uint32_t v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = k + e < K ? p[e] : 0u;
+        *reinterpret_cast<uint4 *>(dst + r * ldd + k) =
+            make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+    }
 }
 
 long long round_up8(long long v) { return (v + 7) / 8 * 8; }
@@ -697,32 +721,24 @@ bool tma_ready(const void *p, long long ld, long long rows)
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows == 1 || ld % 8 == 0);
 }
 
-constexpr int kVecRows = 4;
-
 template <typename T, typename TO>
 s2_status launch_vec(LinearArgs a, int sms, const s2_linear_act_desc &d, cudaStream_t st)
 {
     const T *x = static_cast<const T *>(d.x), *w = static_cast<const T *>(d.w);
-    const bool wide = (reinterpret_cast<uintptr_t>(d.x) | reinterpret_cast<uintptr_t>(d.w) |
-                       (d.M > 1 ? d.ldx * 2 : 0) | (d.N > 1 ? d.ldw * 2 : 0)) % 16 == 0;
-    // warps that share a row's K: as many as fill the GPU (32 warps an SM) and have a piece each
+    const bool wide = (reinterpret_cast<uintptr_t>(d.x) | reinterpret_cast<uintptr_t>(d.w) | (d.N > 1 ? d.ldw * 2 : 0)) % 16 == 0;
+    // Warps that share a row's K: as many as fill the GPU (32 warps an SM) and have a piece each. Then two pieces
+    // in flight are enough, else four: 2560 x 2560 (four warps a row) takes 4.6 us with two and 5.5 with four,
+    // 15360 x 2560 (one) 16.7 and 15.9.
     const int pieces = std::max(1, a.K / (wide ? 256 : 32)), pairs = (a.N + 1) / 2;
     a.ks = 1;
     while (a.ks < kVecWarps && a.ks * 2 <= pieces && 1LL * pairs * a.ks < 32LL * sms) a.ks *= 2;
     const unsigned grid = static_cast<unsigned>((1LL * pairs * a.ks + kVecWarps - 1) / kVecWarps);
-    auto go = [&](auto rows) {
-        constexpr int MR = decltype(rows)::value;
-        if (wide)
-            linear_vec_kernel<T, TO, MR, 8><<<grid, kVecThreads, 0, st>>>(x, d.ldx, w, d.ldw, a);
-        else
-            linear_vec_kernel<T, TO, MR, 1><<<grid, kVecThreads, 0, st>>>(x, d.ldx, w, d.ldw, a);
-    };
-    if (a.M == 1)
-        go(std::integral_constant<int, 1>());
-    else if (a.M == 2)
-        go(std::integral_constant<int, 2>());
+    if (!wide)
+        linear_vec_kernel<T, TO, 1, 8><<<grid, kVecThreads, 0, st>>>(x, w, d.ldw, a);
+    else if (a.ks > 1)
+        linear_vec_kernel<T, TO, 8, 2><<<grid, kVecThreads, 0, st>>>(x, w, d.ldw, a);
     else
-        go(std::integral_constant<int, 4>());
+        linear_vec_kernel<T, TO, 8, 4><<<grid, kVecThreads, 0, st>>>(x, w, d.ldw, a);
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? S2_OK : s2::set_error(S2_INFERENCE_FAILED, "s2_linear_act: launch failed: %s", cudaGetErrorString(e));
 }
@@ -743,17 +759,19 @@ s2_status launch_rows(LinearArgs a, int ks, const void *x, long long ldx, const 
     if (cs != S2_OK) return cs;
     a.ks = ks;
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = static_cast<unsigned>(ks);
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3(static_cast<unsigned>((a.N + kRowsN - 1) / kRowsN * ks), static_cast<unsigned>((a.M + MB - 1) / MB));
     cfg.blockDim = dim3(kRowsThreads);
     cfg.dynamicSmemBytes = R::kSmemBytes;
     cfg.stream = st;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = a.packed ? 2 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, linear_rows_kernel<MB, TO>, mw, mx, a);
     return e == cudaSuccess ? S2_OK : s2::set_error(S2_INFERENCE_FAILED, "s2_linear_act: launch failed: %s", cudaGetErrorString(e));
 }
@@ -783,17 +801,19 @@ s2_status launch_tile(const LinearArgs &a, int sms, const void *x, long long ldx
     if (cs != S2_OK) return cs;
     const long long tiles = (a.M + 255) / 256 * ((a.N + kTileN - 1) / kTileN);
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3(static_cast<unsigned>(2 * std::min<long long>(tiles, sms / 2)));
     cfg.blockDim = dim3(kTileThreads);
     cfg.dynamicSmemBytes = Tile::kSmemBytes;
     cfg.stream = st;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = a.packed ? 2 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, linear_tile_kernel<TO>, mx, mw, mr, my, a);
     return e == cudaSuccess ? S2_OK : s2::set_error(S2_INFERENCE_FAILED, "s2_linear_act: launch failed: %s", cudaGetErrorString(e));
 }
@@ -802,16 +822,21 @@ template <typename TO>
 s2_status launch_linear(const LinearArgs &a, int sms, const void *x, long long ldx, const void *w, long long ldw,
                         cudaStream_t st)
 {
-    const long long tiles = (a.M + 255) / 256 * ((a.N + kTileN - 1) / kTileN);
-    if (tiles * 2 > sms && a.M > 128) {
-        if (tiles > (1LL << 30)) return s2::set_error(S2_UNSUPPORTED, "s2_linear_act: too many tiles");
-        return launch_tile<TO>(a, sms, x, ldx, w, ldw, st);
-    }
     const int mb = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;
     const long long ctas = (a.N + kRowsN - 1LL) / kRowsN * ((a.M + mb - 1) / mb);
     const int n_k = (a.K + kBK - 1) / kBK;
+    // CTAs that share a tile's K: as many as two an SM have room for, two slices each at least
     int ks = 8;
     while (ks > 1 && (ctas * ks > 2LL * sms || n_k < 2 * ks)) ks /= 2;
+    // More than 128 rows of x go to the 256 x 256 tiles, unless K is long and these tiles leave so much of the
+    // GPU idle that its split pays: 200 x 2560 x 5120 18.1 us in rows against 30.0 in tiles, 800 26.8 / 31.4,
+    // 800 x 777 x 1000 14.0 / 21.8, but without a split 1237 x 2560 x 5120 41.3 / 31.9, and with a short K
+    // 1237 x 512 x 512 11.1 / 8.5.
+    if (a.M > 128 && (ks == 1 || n_k < 16)) {
+        if ((a.M + 255) / 256 * ((a.N + kTileN - 1) / kTileN) > (1LL << 30))
+            return s2::set_error(S2_UNSUPPORTED, "s2_linear_act: too many tiles");
+        return launch_tile<TO>(a, sms, x, ldx, w, ldw, st);
+    }
     switch (mb) {
     case 16: return launch_rows<16, TO>(a, ks, x, ldx, w, ldw, st);
     case 32: return launch_rows<32, TO>(a, ks, x, ldx, w, ldw, st);
@@ -862,7 +887,7 @@ s2_status check_operands(const s2_linear_act_desc &d)
 extern "C" size_t s2_linear_act_workspace_bytes(const s2_linear_act_desc *d)
 {
     s2::clear_error();
-    if (check(d) != S2_OK || d->M <= kVecRows) return 0;
+    if (check(d) != S2_OK || d->M <= 1) return 0;
     size_t need = 0;
     if (!tma_ready(d->x, d->ldx, d->M)) need += static_cast<size_t>(d->M) * round_up8(d->K) * 2;
     if (!tma_ready(d->w, d->ldw, d->N)) need += static_cast<size_t>(d->N) * round_up8(d->K) * 2;
@@ -896,12 +921,13 @@ extern "C" s2_status s2_linear_act(void *stream, const s2_linear_act_desc *d, in
     a.vec = (reinterpret_cast<uintptr_t>(d->y) | d->ldy * oe | reinterpret_cast<uintptr_t>(d->residual) |
              (d->residual ? d->ldr * oe : 0)) % 16 == 0;
     a.ks = 1;
+    a.packed = 0;
     a.err = d->err;
     int dev = 0, sms = 148;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     int count = 0;
-    if (d->M <= kVecRows) {
+    if (d->M <= 1) {
         const bool f32 = d->out_dtype == S2_F32;
         if (d->dtype == S2_F16)
             s = f32 ? launch_vec<__half, float>(a, sms, *d, st) : launch_vec<__half, __half>(a, sms, *d, st);
@@ -916,7 +942,7 @@ extern "C" s2_status s2_linear_act(void *stream, const s2_linear_act_desc *d, in
             *ldo = rows == 1 ? round_up8(d->K) : ld;
             if (tma_ready(p, ld, rows)) return;
             *ldo = round_up8(d->K);
-            pack_rows_kernel<<<static_cast<unsigned>(std::min<long long>(rows, 65536)), 256, 0, st>>>(
+            pack_rows_kernel<<<static_cast<unsigned>(std::min<long long>((rows * *ldo / 8 + 255) / 256, 1 << 20)), 256, 0, st>>>(
                 static_cast<const uint16_t *>(p), ld, rows, d->K, ws, *ldo);
             *out = ws;
             ws += rows * *ldo;
@@ -926,6 +952,7 @@ extern "C" s2_status s2_linear_act(void *stream, const s2_linear_act_desc *d, in
         long long ldx, ldw;
         operand(d->x, d->ldx, d->M, &x, &ldx);
         operand(d->w, d->ldw, d->N, &w, &ldw);
+        a.packed = count > 0;
         s = d->out_dtype == S2_F32   ? launch_linear<float>(a, sms, x, ldx, w, ldw, st)
             : d->out_dtype == S2_F16 ? launch_linear<__half>(a, sms, x, ldx, w, ldw, st)
                                      : launch_linear<__nv_bfloat16>(a, sms, x, ldx, w, ldw, st);

@@ -121,6 +121,11 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const void *tmap, uint
         : "memory");
 }
 
+// Programmatic dependent launch: the next kernel of the stream may start; wait for the one before to be done
+// (returns at once when this kernel was launched the ordinary way).
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_dependency() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // L2 policies for loads and stores that are told how long their lines matter.
 __device__ __forceinline__ uint64_t l2_evict_first()
 {
