@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 import numpy as np
 
@@ -1031,15 +1032,21 @@ def _elsewhere(fn, x, stream, *args):
         return fn(x, *args)
 
 
-def _run_desc(call, workspace_bytes, desc, x, index: int, what: str):
+# the descriptions' fields as struct.pack takes them (building a ctypes.Structure costs three times as much)
+_NORM_LAYOUT = struct.Struct("@iiiiqiifPqqPPPqqPNP")
+_LINEAR_LAYOUT = struct.Struct("@iiiiiqPqPqPPqPqPNP")
+
+
+def _run_desc(call, workspace_bytes, desc_type, packed: bytes, x, index: int, what: str):
     """Calls on the current stream of the current device; a call that is refused for want of a
     workspace is given one of that stream's."""
     torch = _torch()
     raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # a torch.cuda.Stream costs as much as a launch
     stream = raw(index) if raw is not None else torch.cuda.current_stream(index).cuda_stream
-    ref = ctypes.byref(desc)
-    status = call(stream, ref, None)
+    status = call(stream, packed, None)
     if status == S2_INVALID_ARGUMENT:
+        desc = desc_type.from_buffer_copy(packed)
+        ref = ctypes.byref(desc)
         need = workspace_bytes(ref)
         if need:
             ws = torch.empty(need, dtype=torch.uint8, device=x.device)
@@ -1084,13 +1091,14 @@ def group_norm_act(x, groups: int, weight=None, bias=None, eps: float = 1e-6, ac
         y_row = _pitch(out, 1, "out")[1]
         y_sample = out.stride(0)
         out_type = _type_of(out, "out")
-    d = GroupNormActDesc(samples, channels, groups, code, positions, in_type, out_type, eps, x.data_ptr(), x_row,
-                         x.stride(0) if samples > 1 else 0,
-                         None if weight is None else _need_vector(weight, channels, index, "weight"),
-                         None if bias is None else _need_vector(bias, channels, index, "bias"), out.data_ptr(), y_row,
-                         y_sample, None, 0, None if err is None else _need_err(err, index))
+    d = _NORM_LAYOUT.pack(samples, channels, groups, code, positions, in_type, out_type, eps, x.data_ptr(), x_row,
+                          x.stride(0) if samples > 1 else 0,
+                          0 if weight is None else _need_vector(weight, channels, index, "weight"),
+                          0 if bias is None else _need_vector(bias, channels, index, "bias"), out.data_ptr(), y_row,
+                          y_sample, 0, 0, 0 if err is None else _need_err(err, index))
     L = _lib or lib()
-    _run_desc(L.s2_group_norm_act, L.s2_group_norm_act_workspace_bytes, d, x, index, "s2_group_norm_act")
+    _run_desc(L.s2_group_norm_act, L.s2_group_norm_act_workspace_bytes, GroupNormActDesc, d, x, index,
+              "s2_group_norm_act")
     return out
 
 
@@ -1129,18 +1137,18 @@ def linear_act(x, w, bias=None, activation: str = "none", residual=None, out=Non
             _fail(f"out must be {(*shape[:-1], N)} on x's device, and of out_dtype if both are given")
         ldy = _pitch(out, 0, "out")[1]
         out_type = _type_of(out, "out")
-    res, ldr = None, 0
+    res = ldr = 0
     if residual is not None:
         if residual.shape != out.shape or residual.dtype != out.dtype or residual.get_device() != index:
             _fail(f"residual must be {tuple(out.shape)} in the output's type on x's device")
         if residual.requires_grad:
             _need_no_grad()
         res, ldr = residual.data_ptr(), _pitch(residual, 0, "residual")[1]
-    d = LinearActDesc(N, K, code, in_type, out_type, rows, x.data_ptr(), ldx, w.data_ptr(), ldw,
-                      None if bias is None else _need_vector(bias, N, index, "bias"), res, ldr, out.data_ptr(), ldy,
-                      None, 0, None if err is None else _need_err(err, index))
+    d = _LINEAR_LAYOUT.pack(N, K, code, in_type, out_type, rows, x.data_ptr(), ldx, w.data_ptr(), ldw,
+                            0 if bias is None else _need_vector(bias, N, index, "bias"), res, ldr, out.data_ptr(),
+                            ldy, 0, 0, 0 if err is None else _need_err(err, index))
     L = _lib or lib()
-    _run_desc(L.s2_linear_act, L.s2_linear_act_workspace_bytes, d, x, index, "s2_linear_act")
+    _run_desc(L.s2_linear_act, L.s2_linear_act_workspace_bytes, LinearActDesc, d, x, index, "s2_linear_act")
     return out
 
 

@@ -109,3 +109,12 @@ def test_wrappers_refuse_host_tensors():
         with pytest.raises(s2b200.S2Error) as e:
             call()
         assert e.value.status == INVALID
+
+
+def test_packed_descriptions_match_the_structures():
+    """The wrappers pack their descriptions with struct; the layouts are the structures'."""
+    for layout, cls in ((s2b200._NORM_LAYOUT, s2b200.GroupNormActDesc), (s2b200._LINEAR_LAYOUT, s2b200.LinearActDesc)):
+        assert layout.size == ctypes.sizeof(cls)
+        names = [n for n, _ in cls._fields_]
+        got = cls.from_buffer_copy(layout.pack(*range(1, len(names) + 1)))
+        assert [int(getattr(got, n)) for n in names] == list(range(1, len(names) + 1))
