@@ -647,8 +647,12 @@ struct Cursor {
                      : "memory");
         return v;
     }
+    // The slot's values are used: the next copy may overwrite it. The fence orders this thread's reads before
+    // the copy, which writes through another path of shared memory; without it, and with the arrival before
+    // the values were used, a copy now and then overtook a read of fp32 rows.
     __device__ __forceinline__ void release() const
     {
+        fence_proxy_async_smem();
         __syncwarp();
         if ((threadIdx.x & 31) == 0) mbar_arrive(empty0 + 8 * slot);
     }
@@ -673,8 +677,6 @@ __device__ __forceinline__ void write_slots(Cursor<kSlots> c, const Slots &p, in
         uint4 v[kSlotPasses];
 #pragma unroll
         for (int k = 0; k < kSlotPasses; ++k) v[k] = c.get(k, stride);
-        c.release();
-        c.next();
         if ((i + 1) * kSlotPasses <= count) {
 #pragma unroll
             for (int k = 0; k < kSlotPasses; ++k, py += step) finish<TI, TO, VEC, N, kAct>(v[k], py, minus, scale, shift);
@@ -683,6 +685,8 @@ __device__ __forceinline__ void write_slots(Cursor<kSlots> c, const Slots &p, in
             for (int k = 0; k < kSlotPasses; ++k, py += step)
                 if (i * kSlotPasses + k < count) finish<TI, TO, VEC, N, kAct>(v[k], py, minus, scale, shift);
         }
+        c.release();
+        c.next();
     };
     const long long slot_step = kSlotPasses * step;
     const int first = p.total - p.held;
@@ -791,8 +795,6 @@ __global__ void __launch_bounds__(kThreads + 32, 2) group_norm_ring_kernel(const
                 uint4 v[kSlotPasses];
 #pragma unroll
                 for (int w = 0; w < kSlotPasses; ++w) v[w] = cur.get(w, stride);
-                if (i + k < p.total - p.held) cur.release();
-                cur.next();
                 if ((k + 1) * kSlotPasses <= valid) {
 #pragma unroll
                     for (int w = 0; w < kSlotPasses; ++w) run.add(v[w]);
@@ -801,6 +803,8 @@ __global__ void __launch_bounds__(kThreads + 32, 2) group_norm_ring_kernel(const
                     for (int w = 0; w < kSlotPasses; ++w)
                         if (k * kSlotPasses + w < valid) run.add(v[w]);
                 }
+                if (i + k < p.total - p.held) cur.release();
+                cur.next();
             }
             if (valid > 0) run.end(valid, mo);
         }

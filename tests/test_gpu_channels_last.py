@@ -175,11 +175,18 @@ def test_norm_of_nothing():
         assert y.shape == shape
 
 
-def test_norm_gives_the_same_bits():
-    x = _features((3, 20000, 96), _gen(12), BF16)
-    first = s2b200.group_norm_act(x, 32, activation="silu")
-    for _ in range(5):
-        assert torch.equal(s2b200.group_norm_act(x, 32, activation="silu"), first)
+@pytest.mark.parametrize("dtype", [F16, F32], ids=str)
+@pytest.mark.parametrize("shape", [(3, 20000, 96), (2, 40000, 512), (4, 60000, 128), (2, 1500, 512), (1, 60000, 130)], ids=str)
+def test_norm_gives_the_same_bits(shape, dtype):
+    """Whatever the blocks' order: the joins' and the ring's hand-overs, many times over."""
+    x = _features(shape, _gen(12), dtype)
+    G = 10 if shape[2] == 130 else 32
+    first = s2b200.group_norm_act(x, G, activation="silu")
+    cl.check(first[:1], *cl.norm_exact(x[:1], G, None, None, 1e-6, "silu"))
+    off = torch.zeros((), dtype=torch.int64, device="cuda")
+    for _ in range(100):
+        off += (s2b200.group_norm_act(x, G, activation="silu") != first).sum()
+    assert off.item() == 0
 
 
 @pytest.mark.parametrize("shape", [(1, 600000, 64, 32), (2, 300000, 128, 32), (1, 120000, 512, 32), (1, 2000000, 16, 4)])
@@ -190,6 +197,60 @@ def test_norm_of_large_samples(shape):
     y = s2b200.group_norm_act(x, G, activation="silu")
     for s in range(S):
         cl.check(y[s:s + 1], *cl.norm_exact(x[s:s + 1], G, None, None, 1e-6, "silu"))
+
+
+# channels a group that make 1, 2, 4 and 8 moments of a vector, few and many groups, units that a ring of
+# one pass, of several and of none to spare holds
+@pytest.mark.parametrize("types", NORM_TYPES, ids=lambda t: f"{t[0]}-{t[1]}".replace("torch.", ""))
+@pytest.mark.parametrize("shape", [(2, 40001, 256, 32), (3, 50000, 128, 32), (1, 300017, 64, 32), (9, 30011, 96, 32),
+                                   (2, 60000, 192, 64), (1, 33000, 2048, 1)], ids=str)
+def test_norm_of_large_packed_units(shape, types):
+    S, P, C, G = shape
+    x = _features((S, P, C), _gen(P), types[0])
+    w, b = 1 + 0.1 * _normal((C,), _gen(1)), 0.1 * _normal((C,), _gen(2))
+    act = cl.ACTS[(P + C) % 5]
+    y = s2b200.group_norm_act(x, G, w, b, activation=act, out_dtype=types[1])
+    for s in range(S):
+        cl.check(y[s:s + 1], *cl.norm_exact(x[s:s + 1], G, w, b, 1e-6, act), f"{shape} {act}")
+
+
+@pytest.mark.parametrize("types", NORM_TYPES, ids=lambda t: f"{t[0]}-{t[1]}".replace("torch.", ""))
+@pytest.mark.parametrize("shape,pad", [((2, 40001, 256, 32), 3), ((1, 50000, 130, 10), 0), ((2, 30000, 640, 32), 8),
+                                       ((3, 60000, 64, 16), 8), ((1, 9000, 5120, 2), 0), ((10, 20000, 128, 32), 1)], ids=str)
+def test_norm_of_large_units_in_pitched_rows(shape, pad, types):
+    S, P, C, G = shape
+    x = _features((S, P, C), _gen(P), types[0], pad)
+    y = s2b200.group_norm_act(_padded(x, pad)[1], G, activation="gelu", out_dtype=types[1])
+    for s in range(S):
+        cl.check(y[s:s + 1], *cl.norm_exact(x[s:s + 1], G, None, None, 1e-6, "gelu"), f"{shape}")
+
+
+@pytest.mark.parametrize("shape", [(2, 40000, 512, 32), (1, 400000, 64, 32), (2, 60001, 130, 10)], ids=str)
+@pytest.mark.parametrize("dtype", [F16, F32], ids=str)
+def test_norm_of_large_units_in_place(shape, dtype):
+    S, P, C, G = shape
+    x = _features((S, P, C), _gen(15), dtype)
+    want = s2b200.group_norm_act(x, G, activation="silu")
+    for _ in range(3):
+        got = x.clone()
+        s2b200.group_norm_act(got, G, activation="silu", out=got)
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("shape", [(2, 40000, 512, 32), (1, 60001, 130, 10)], ids=str)
+def test_norm_of_large_units_about_a_large_mean(shape):
+    S, P, C, G = shape
+    x = 300 + 0.5 * _normal((S, P, C), _gen(16))
+    x[0, P // 3, 5] = 1e4
+    y = s2b200.group_norm_act(x, G)
+    for s in range(S):
+        cl.check(y[s:s + 1], *cl.norm_exact(x[s:s + 1], G, None, None, 1e-6, "none"))
+
+
+def test_norm_of_many_samples():
+    x = _features((3000, 33, 48), _gen(17), F16)
+    y = s2b200.group_norm_act(x, 16, activation="silu")
+    cl.check(y, *cl.norm_exact(x, 16, None, None, 1e-6, "silu"))
 
 
 def test_norm_past_2_31_values():
@@ -281,6 +342,16 @@ def test_linear_onto_its_residual(shape):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("shape", [(9000, 512, 512), (20000, 300, 192), (70000, 128, 64)], ids=str)
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=str)
+@pytest.mark.parametrize("out_dtype", [None, F32], ids=str)
+def test_linear_of_short_sums_and_many_rows(shape, dtype, out_dtype):
+    """The VAE's 1 x 1 projections: few products a sum, many rows."""
+    x, w, b, r = _operands(*shape, dtype, 29, out_dtype=out_dtype)
+    y = s2b200.linear_act(x, w, b, "silu", r, out_dtype=out_dtype)
+    cl.check(y, *cl.linear_exact(x, w, b, "silu", r))
+
+
 def test_linear_of_leading_dimensions():
     x, w, b, _ = _operands(60, 48, 64, F16, 25, res=False)
     y = s2b200.linear_act(x.view(3, 4, 5, 64), w, b, "relu")
@@ -306,12 +377,17 @@ def test_linear_bad_rows_stay_alone(shape):
     assert torch.equal(torch.isnan(y[3:4]), torch.isnan(want)) and torch.equal(torch.isinf(y[3:4]), torch.isinf(want))
 
 
-@pytest.mark.parametrize("shape", [(1, 2560, 2560), (58, 2560, 5120), (700, 500, 1024)], ids=str)
-def test_linear_gives_the_same_bits(shape):
-    x, w, b, r = _operands(*shape, F16, 27)
-    first = s2b200.linear_act(x, w, b, "silu", r)
-    for _ in range(5):
-        assert torch.equal(s2b200.linear_act(x, w, b, "silu", r), first)
+@pytest.mark.parametrize("shape", [(1, 2560, 2560), (4, 300, 520), (58, 2560, 5120), (128, 640, 2560), (700, 500, 1024),
+                                   (1237, 777, 1001), (5000, 512, 512), (4300, 2560, 1024)], ids=str)
+@pytest.mark.parametrize("out_dtype", [None, F32], ids=str)
+def test_linear_gives_the_same_bits(shape, out_dtype):
+    """Whatever the blocks' order: the hand-overs of operands, sums, residuals and results, many times over."""
+    x, w, b, r = _operands(*shape, F16, 27, out_dtype=out_dtype)
+    first = s2b200.linear_act(x, w, b, "silu", r, out_dtype=out_dtype)
+    off = torch.zeros((), dtype=torch.int64, device="cuda")
+    for _ in range(60):
+        off += (s2b200.linear_act(x, w, b, "silu", r, out_dtype=out_dtype) != first).sum()
+    assert off.item() == 0
 
 
 def test_linear_past_2_31_values():
@@ -466,6 +542,38 @@ def test_timestep_mlp():
         out = s2b200.linear_act(t, w, b, act)
         cl.check(out, *cl.linear_exact(t, w, b, act, None))
         t = out
+
+
+def test_wrappers_refuse_what_they_cannot_run():
+    x = torch.zeros(4, 64, dtype=F16, device="cuda")
+    w = torch.zeros(32, 64, dtype=F16, device="cuda")
+    v = torch.zeros(64, device="cuda")
+    grad = x.float().half().requires_grad_()
+    calls = [
+        lambda: s2b200.group_norm_act(x, 7), lambda: s2b200.group_norm_act(x[0], 8),
+        lambda: s2b200.group_norm_act(x, 8, activation="swish"), lambda: s2b200.group_norm_act(x, 8, v.half()),
+        lambda: s2b200.group_norm_act(x, 8, v[:32]), lambda: s2b200.group_norm_act(x, 8, v.cpu()),
+        lambda: s2b200.group_norm_act(x, 8, torch.zeros(128, device="cuda")[::2]),
+        lambda: s2b200.group_norm_act(x, 8, out=x.float()), lambda: s2b200.group_norm_act(x, 8, out_dtype=BF16),
+        lambda: s2b200.group_norm_act(x, 8, out=w), lambda: s2b200.group_norm_act(x.t(), 4),
+        lambda: s2b200.group_norm_act(x.double(), 8), lambda: s2b200.group_norm_act(grad, 8),
+        lambda: s2b200.group_norm_act(x[:1].expand(4, 64).view(4, 1, 64), 8, out=x.view(4, 1, 64)),
+        lambda: s2b200.group_norm_act(x.view(1, 4, 64)[:, ::2], 8, out=x.view(1, 4, 64)[:, 1:3]),
+        lambda: s2b200.group_norm_act(x, 8, eps=-1.0), lambda: s2b200.group_norm_act(x, 8, err=v),
+        lambda: s2b200.linear_act(x, w.float()), lambda: s2b200.linear_act(x, w[:, :32]),
+        lambda: s2b200.linear_act(x.float(), w.float()), lambda: s2b200.linear_act(x, w, v),
+        lambda: s2b200.linear_act(x, w, activation=None), lambda: s2b200.linear_act(x, w, residual=x),
+        lambda: s2b200.linear_act(x, w, out=x), lambda: s2b200.linear_act(x, w, out_dtype=BF16),
+        lambda: s2b200.linear_act(x, w.cpu()), lambda: s2b200.linear_act(x, w, residual=x[:, :32].float()),
+        lambda: s2b200.linear_act(x, w, out=x[:, :32]), lambda: s2b200.linear_act(grad, w),
+        lambda: s2b200.linear_act(x.t(), w.t()), lambda: s2b200.linear_act(x, w, err=v),
+    ]
+    for i, call in enumerate(calls):
+        with pytest.raises(s2b200.S2Error) as e:
+            call()
+        assert e.value.status in (s2b200.S2_INVALID_ARGUMENT, s2b200.S2_UNSUPPORTED), i
+    with torch.no_grad():
+        assert torch.equal(s2b200.linear_act(grad, w), s2b200.linear_act(x, w))
 
 
 def test_err_word_stays_zero():
