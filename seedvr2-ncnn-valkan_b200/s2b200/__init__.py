@@ -965,23 +965,28 @@ def _fail(what: str):
     raise S2Error(S2_INVALID_ARGUMENT, what)
 
 
-_DTYPES = {}
+class _Types(dict):
+    """torch dtype -> s2_dtype; -1 for the others."""
+
+    def __missing__(self, dtype):
+        torch = _torch()
+        self.update({torch.float32: S2_F32, torch.float16: S2_F16, torch.bfloat16: S2_BF16})
+        return self.setdefault(dtype, -1)
+
+
+_DTYPES = _Types()
 
 
 def _type_of(t, what: str) -> int:
-    if not _DTYPES:
-        torch = _torch()
-        _DTYPES.update({torch.float32: S2_F32, torch.float16: S2_F16, torch.bfloat16: S2_BF16})
-    code = _DTYPES.get(t.dtype)
-    if code is None:
+    code = _DTYPES[t.dtype]
+    if code < 0:
         _fail(f"{what} must be fp16, bf16 or fp32, not {t.dtype}")
     return code
 
 
 def _need_vector(t, n: int, index: int, what: str):
     """The address of a contiguous fp32 vector of n values."""
-    if (t.get_device() != index or t.dtype != _torch().float32 or t.dim() != 1 or t.numel() != n
-            or not t.is_contiguous()):
+    if t.get_device() != index or _DTYPES[t.dtype] != S2_F32 or t.shape != (n,) or not t.is_contiguous():
         _fail(f"{what} must be a contiguous fp32 tensor of {n} values on x's device")
     if t.requires_grad:
         _need_no_grad()
@@ -1004,6 +1009,9 @@ def _pitch(t, first: int, what: str):
     spaced, over contiguous channels."""
     shape, strides = t.shape, t.stride()
     last = shape[-1]
+    if len(shape) == first + 2 and strides[-1] == 1:
+        size = shape[first]
+        return size, (strides[first] if size != 1 else last)
     if strides[-1] != 1 and last > 1:
         _fail(f"{what}: the last dimension must be contiguous")
     rows, pitch = 1, None
