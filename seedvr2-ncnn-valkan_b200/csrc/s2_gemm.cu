@@ -778,6 +778,21 @@ bool make_map_2d_plain_f32(CUtensorMap *map, const void *ptr, uint64_t inner, ui
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool make_map_3d_plain(CUtensorMap *map, const void *ptr, uint32_t elem, uint64_t inner, uint64_t rows, uint64_t samples,
+                       uint64_t row_bytes, uint64_t sample_bytes, uint32_t box_inner, uint32_t box_rows)
+{
+    auto encode = get_encode();
+    if (!encode) return false;
+    cuuint64_t dims[3] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(samples)};
+    cuuint64_t strides[2] = {static_cast<cuuint64_t>(row_bytes), static_cast<cuuint64_t>(sample_bytes)};
+    cuuint32_t box[3] = {box_inner, box_rows, 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    return encode(map, elem == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                  const_cast<void *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 s2_status gemm_f16(cudaStream_t st, const void *A, const void *B, const GemmArgs &args)
 {
     if (!A || !B || args.M <= 0 || args.N <= 0 || args.K <= 0 || args.K % kBK != 0 || !args.err)

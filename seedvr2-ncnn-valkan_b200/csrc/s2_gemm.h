@@ -21,6 +21,10 @@ bool make_map_2d_plain(CUtensorMap *map, const void *ptr, uint64_t inner, uint64
                        uint32_t box_inner, uint32_t box_rows);
 bool make_map_2d_plain_f32(CUtensorMap *map, const void *ptr, uint64_t inner, uint64_t rows, uint64_t row_bytes,
                            uint32_t box_inner, uint32_t box_rows);
+// 3-D map over [samples][rows][inner] elements of `elem` (2 or 4) bytes, one sample's box_inner x box_rows a box,
+// not swizzled.
+bool make_map_3d_plain(CUtensorMap *map, const void *ptr, uint32_t elem, uint64_t inner, uint64_t rows, uint64_t samples,
+                       uint64_t row_bytes, uint64_t sample_bytes, uint32_t box_inner, uint32_t box_rows);
 
 // Epilogues of D = A B^T (+ bias).
 enum GemmEpilogue : int {

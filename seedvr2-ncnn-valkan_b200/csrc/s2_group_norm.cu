@@ -28,6 +28,7 @@
 #include <cstdint>
 
 #include "s2_act.cuh"
+#include "s2_gemm.h"
 #include "s2_internal.h"
 #include "s2_launch.h"
 #include "s2_overlap.h"
@@ -61,6 +62,7 @@ struct GnArgs {
     long long P, part_rows, x_row, x_sample, y_row, y_sample;
     int C, G, cpg, slices, slice_groups, units, parts, teams, join, hold, act;
     int group_lanes;  // threads that join one group's moments: a power of two up to 32
+    int buffers, boxes, box_rows;  // group_norm_slab_kernel
     float eps;
     // a grid's: (mean, M2) per [unit][part][group], (mean, 1 / sigma) per [unit][group]; counters, zero
     // before: parts whose moments are written, units whose norm is
@@ -83,6 +85,13 @@ __device__ __forceinline__ Moments join(const Moments &a, const Moments &b)
     r.mean = both ? fmaf(d, w, a.mean) : (b.n > 0.f ? b.mean : a.mean);
     r.m2 = both ? fmaf(d * d, a.n * w, a.m2 + b.m2) : a.m2 + b.m2;
     return r;
+}
+
+// The sum over `lanes` neighbouring threads, in all of them.
+__device__ __forceinline__ float sum_lanes(float v, int lanes)
+{
+    for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
 }
 
 // `lanes` neighbouring threads' moments in the first of them.
@@ -328,11 +337,11 @@ struct BlockMoments {
     Moments group[kSliceGroups];
 };
 
-// Joins the threads' moments of the columns at cb to s.group[]. Ends without a barrier.
-// `sync` is the barrier of the kThreads threads.
+// The moments of group `sub` over the block's threads at the columns from cb, in the thread of sub_lane 0. Ends
+// without a barrier. `sync` is the barrier of the kThreads threads.
 template <int VEC, int N, typename Sync>
-__device__ __forceinline__ void join_block(BlockMoments<N> &s, Moments (&mo)[N], const Place &p, int cb, int cpg, int gs,
-                                           int group_lanes, int sub, int sub_lane, Sync sync)
+__device__ __forceinline__ Moments block_moments(BlockMoments<N> &s, Moments (&mo)[N], const Place &p, int cb, int cpg,
+                                                 int gs, int group_lanes, int sub, int sub_lane, Sync sync)
 {
     sync();
 #pragma unroll
@@ -374,7 +383,15 @@ __device__ __forceinline__ void join_block(BlockMoments<N> &s, Moments (&mo)[N],
             m = join(m, t);
         }
     }
-    m = join_lanes(m, group_lanes);
+    return join_lanes(m, group_lanes);
+}
+
+// Joins them to s.group[].
+template <int VEC, int N, typename Sync>
+__device__ __forceinline__ void join_block(BlockMoments<N> &s, Moments (&mo)[N], const Place &p, int cb, int cpg, int gs,
+                                           int group_lanes, int sub, int sub_lane, Sync sync)
+{
+    const Moments m = block_moments<VEC, N>(s, mo, p, cb, cpg, gs, group_lanes, sub, sub_lane, sync);
     if (sub_lane == 0 && sub < gs) s.group[sub] = join(s.group[sub], m);
 }
 
@@ -480,6 +497,20 @@ __device__ __forceinline__ uint32_t ld_acquire(const uint32_t *p)
 // device error codes: the wait for the other parts of a unit, for the ring's loads
 enum : int { E_JOIN = 96, E_RING = 97 };
 
+// Waits until *p is `value`; bounded, and *stop ends it.
+__device__ __forceinline__ bool wait_value(const uint32_t *p, uint32_t value, volatile int *stop, int32_t *err)
+{
+    if (ld_acquire(p) == value) return true;
+    const uint64_t t0 = global_timer_ns();
+    while (ld_acquire(p) != value)
+        if (*stop || global_timer_ns() - t0 > kWaitTimeoutNs) {
+            if (err) atomicCAS(err, 0, E_JOIN);
+            *stop = 1;
+            return false;
+        }
+    return true;
+}
+
 // The parts of a unit on a grid join their moments (group[], gs of them): each writes its own, the last to
 // arrive joins all of them and publishes the unit's mean and 1 / sigma, the others wait for these. `sync` is
 // the barrier of the threads that call this; *stop ends the wait, which is bounded. On return norm[] holds
@@ -512,15 +543,7 @@ __device__ __forceinline__ void join_grid(const GnArgs &a, int unit, int member,
             atomicExch(a.ready + unit, 1u);
         }
     } else {
-        if (threadIdx.x == 0 && ld_acquire(a.ready + unit) == 0) {
-            const uint64_t t0 = global_timer_ns();
-            while (ld_acquire(a.ready + unit) == 0)
-                if (*stop || global_timer_ns() - t0 > kWaitTimeoutNs) {
-                    if (a.err) atomicCAS(a.err, 0, E_JOIN);
-                    *stop = 1;
-                    break;
-                }
-        }
+        if (threadIdx.x == 0) wait_value(a.ready + unit, 1, stop, a.err);
         sync();
         if (threadIdx.x < gs) norm[threadIdx.x] = __ldcg(joined + threadIdx.x);
         sync();
@@ -596,6 +619,14 @@ __global__ void __launch_bounds__(kThreads, 2) group_norm_held_kernel(const GnAr
 constexpr int kSlotPasses = 4;  // rows a thread has in a slot
 constexpr int kRunSlots = kAhead / kSlotPasses;
 constexpr uint32_t kSlotBytes = kSlotPasses * kThreads * 16;
+// 16 bytes written by copies that the compiler does not see, so that the load is spelled out
+__device__ __forceinline__ uint4 ld_shared(uint32_t at)
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+
 // Slots beside the moments, of two blocks an SM.
 template <int N>
 __host__ __device__ constexpr int ring_slots()
@@ -636,17 +667,8 @@ struct Cursor {
     // A wait that runs out raises `abort`, which ends all later ones at once: the block runs on to its end
     // (every thread meets the same barriers) with the error recorded.
     __device__ __forceinline__ void wait() const { mbar_wait(full0 + 8 * slot, phase, abort, err, E_RING); }
-    // the thread's vector of pass k of the slot, `stride` bytes a pass (the ring is written by copies that the
-    // compiler does not see, so its loads are spelled out)
-    __device__ __forceinline__ uint4 get(int k, uint32_t stride) const
-    {
-        uint4 v;
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                     : "r"(mine + slot * kSlotBytes + k * stride)
-                     : "memory");
-        return v;
-    }
+    // the thread's vector of pass k of the slot, `stride` bytes a pass
+    __device__ __forceinline__ uint4 get(int k, uint32_t stride) const { return ld_shared(mine + slot * kSlotBytes + k * stride); }
     // The slot's values are used: the next copy may overwrite it. The fence orders this thread's reads before
     // the copy, which writes through another path of shared memory; without it, and with the arrival before
     // the values were used, a copy now and then overtook a read of fp32 rows.
@@ -830,6 +852,305 @@ __global__ void __launch_bounds__(kThreads + 32, 2) group_norm_ring_kernel(const
     }
 }
 
+// ---- slices held by the whole grid -----------------------------------------------------
+
+constexpr int kMaxBuffers = 8;
+constexpr int kSlabGroups = 16;
+constexpr int kSlabThreads = 128;  // that sum, and as many that write
+constexpr int kPartsLane = 10;     // parts of a unit that a lane joins
+// buffers beside N moments a vector, of two blocks an SM
+constexpr int slab_room(int n) { return 112 * 1024 - n * 2560 - 4096; }
+
+// y of a thread's `count` vectors in shared memory, `stride` bytes apart.
+template <typename TI, typename TO, int N, int kAct>
+__device__ __forceinline__ void write_slab(uint32_t from, int count, uint32_t stride, TO *py, long long step, const float (&minus)[N],
+                                           const float (&scale)[16 / sizeof(TI)], const float (&shift)[16 / sizeof(TI)])
+{
+    constexpr int VEC = 16 / sizeof(TI);
+    int i = 0;
+#pragma unroll 1
+    for (; i + kBatch <= count; i += kBatch) {
+        uint4 v[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) v[k] = ld_shared(from + (i + k) * stride);
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k, py += step) finish<TI, TO, VEC, N, kAct>(v[k], py, minus, scale, shift);
+    }
+#pragma unroll 1
+    for (; i < count; ++i, py += step) finish<TI, TO, VEC, N, kAct>(ld_shared(from + i * stride), py, minus, scale, shift);
+}
+
+// Pairs of floats that are their own flag: all bits set until they are written (a NaN is written as another).
+__device__ __forceinline__ uint64_t ld_pair(const float2 *p)
+{
+    uint64_t v;
+    asm volatile("ld.relaxed.gpu.global.b64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ void st_pair(float2 *p, float2 f)
+{
+    const uint64_t v = pair(f.x != f.x ? __uint_as_float(0x7fffffffu) : f.x, f.y);
+    asm volatile("st.relaxed.gpu.global.b64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
+}
+__device__ __forceinline__ void wait_pair(uint64_t &v, const float2 *p, volatile int *stop, int32_t *err)
+{
+    if (v != ~0ull) return;
+    const uint64_t t0 = global_timer_ns();
+    while ((v = ld_pair(p)) == ~0ull)
+        if (*stop || global_timer_ns() - t0 > kWaitTimeoutNs) {
+            if (err) atomicCAS(err, 0, E_JOIN);
+            *stop = 1;
+            return;
+        }
+}
+// The group's moments of all parts, part lane + 32 k in q[k] (part 0's past the last), when all are written.
+__device__ __forceinline__ void load_parts(uint64_t (&q)[kPartsLane], const float2 *part, int parts, volatile int *stop, int32_t *err)
+{
+    const uint64_t t0 = global_timer_ns();
+    for (;;) {
+        bool all = true;
+#pragma unroll
+        for (int k = 0; k < kPartsLane; ++k) {
+            const int t = (threadIdx.x & 31) + k * 32;
+            q[k] = ld_pair(part + (t < parts ? t : 0));
+        }
+#pragma unroll
+        for (int k = 0; k < kPartsLane; ++k) all = all && q[k] != ~0ull;
+        if (__all_sync(0xffffffffu, all)) return;
+        if (__any_sync(0xffffffffu, *stop || global_timer_ns() - t0 > kWaitTimeoutNs)) {
+            if (err) atomicCAS(err, 0, E_JOIN);
+            *stop = 1;
+            return;
+        }
+    }
+}
+// Until this block has posted its moments of `unit`.
+__device__ __forceinline__ bool wait_posted(const volatile int *posted, int unit, volatile int *stop, int32_t *err)
+{
+    const uint64_t t0 = global_timer_ns();
+    while (*posted <= unit) {
+        __nanosleep(100);
+        if (*stop) return false;
+        if (global_timer_ns() - t0 > kWaitTimeoutNs) {
+            if (err) atomicCAS(err, 0, E_JOIN);
+            *stop = 1;
+            return false;
+        }
+    }
+    return true;
+}
+
+// One team of all blocks takes narrow slices of the channels (64 bytes a row and more), of which each block holds
+// its rows of the last few in shared memory: every value is read once, whatever the sample's size. The work on
+// the units in flight goes on side by side: warps 0-3 sum one and post their block's moments, warps 4-7 write an
+// older one, warp 8 loads the next (and has the one behind it brought to L2), warp 9 joins all blocks' moments of
+// the groups that are its block's turn, warp 10 fetches the results. What bounds it is how long a unit stays in
+// shared memory, about 12 us of which 2.5 for the load, 1.5 for the sums, 5 for the exchange and 2.5 for the
+// output, at 28 MB for the whole GPU. 11 x 57600 x 512 bf16 silu: 265 us, 4.9 TB/s (the ring, which reads
+// twice: 347); 6 x 14400 x 512: 41 us (47). With one role a block after the other the same took 570 us, and 370 while
+// the parts' moments were asked for one after the other.
+template <typename TI, typename TO, int N>
+__global__ void __launch_bounds__(kThreads + 96, 2) group_norm_slab_kernel(const __grid_constant__ CUtensorMap map, const GnArgs a)
+{
+    constexpr int VEC = 16 / sizeof(TI);
+    extern __shared__ uint4 slab_raw[];
+    // the summing threads' (mean, M2), [unit & 1][group][row lane][moment of a row]; their shares of a group's values
+    __shared__ float2 moments[2][kSlabThreads * N];
+    __shared__ float share[kSlabThreads * N];
+    __shared__ float2 norm[kMaxBuffers][kSlabGroups];
+    __shared__ uint64_t bars[3 * kMaxBuffers];
+    __shared__ int abort_flag;
+    __shared__ volatile int posted;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int member = static_cast<int>(blockIdx.x), gs = a.slice_groups, ncols = gs * a.cpg / VEC;
+    const long long r0 = member * a.part_rows, rows = min(a.part_rows, a.P - r0);
+    const uint32_t base = (smem_u32(slab_raw) + 127u) & ~127u, box_bytes = a.box_rows * ncols * 16, buffer_bytes = a.boxes * box_bytes;
+    const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * kMaxBuffers, ready0 = empty0 + 8 * kMaxBuffers;
+    volatile int *abort = &abort_flag;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < a.buffers; ++i) {
+            mbar_init(full0 + 8 * i, 1);
+            mbar_init(empty0 + 8 * i, kSlabThreads / 32);
+            mbar_init(ready0 + 8 * i, 1);
+        }
+        abort_flag = 0;
+        posted = 0;
+        fence_mbar_init();
+    }
+    __syncthreads();
+
+    if (warp == kThreads / 32) {
+        if (lane != 0) return;
+        const uint64_t policy = l2_evict_first();
+        int b = 0, unit = 0;
+        uint32_t phase = 0;
+        for (; unit < a.units; ++unit) {
+            const int smp = unit / a.slices, c0 = (unit - smp * a.slices) * gs * a.cpg;
+            if (!mbar_wait(empty0 + 8 * b, phase ^ 1u, abort, a.err, E_RING)) break;
+            mbar_arrive_expect_tx(full0 + 8 * b, buffer_bytes);
+            for (int i = 0; i < a.boxes; ++i)
+                tma_load_3d(base + b * buffer_bytes + i * box_bytes, &map, full0 + 8 * b, c0, static_cast<int>(r0) + i * a.box_rows, smp,
+                            policy);
+            // the next unit, whose buffer is still in use, to L2: 265 us instead of 273 above
+            const int next = unit + 1;
+            if (next < a.units)
+                for (int i = 0; i < a.boxes; ++i)
+                    tma_prefetch_3d(&map, next % a.slices * gs * a.cpg, static_cast<int>(r0) + i * a.box_rows, next / a.slices);
+            if (++b == a.buffers) {
+                b = 0;
+                phase ^= 1u;
+            }
+        }
+        if (unit < a.units) {
+            // no copy may still be landing when the block ends: wait for the buffers' last loads
+            int dummy = 0;
+            for (int u = max(0, unit - a.buffers); u < unit; ++u)
+                mbar_wait(full0 + 8 * (u % a.buffers), u / a.buffers & 1, &dummy, a.err, E_RING);
+        }
+        return;
+    }
+    if (warp == kThreads / 32 + 1) {
+        // the units' groups go round the blocks
+        const float inv_rows = 1.f / static_cast<float>(a.P), inv_n = inv_rows / a.cpg;
+        float w[kPartsLane];  // the parts' shares of the rows
+#pragma unroll
+        for (int k = 0; k < kPartsLane; ++k) {
+            const int t = lane + k * 32;
+            w[k] = t < a.parts ? static_cast<float>(min(a.part_rows, a.P - t * a.part_rows)) * inv_rows : 0.f;
+        }
+        for (int turn = member; turn < a.units * gs; turn += a.parts) {
+            if (!wait_posted(&posted, turn / gs, abort, a.err)) return;
+            const float2 *part = a.part + static_cast<long long>(turn) * a.parts;
+            uint64_t q[kPartsLane];
+            load_parts(q, part, a.parts, abort, a.err);
+            // sums about the first part's mean
+            float sum = 0.f;
+            const float p0 = __shfl_sync(0xffffffffu, floats_of(q[0]).x, 0);
+#pragma unroll
+            for (int k = 0; k < kPartsLane; ++k) {
+                if (w[k] > 0.f) sum = fmaf(floats_of(q[k]).x - p0, w[k], sum);
+            }
+            const float mean = p0 + sum_lanes(sum, 32);
+            float var = 0.f;
+#pragma unroll
+            for (int k = 0; k < kPartsLane; ++k) {
+                const float d = floats_of(q[k]).x - mean;
+                if (w[k] > 0.f) var += fmaf(d * d, w[k], floats_of(q[k]).y * inv_n);
+            }
+            const Moments m = {1.f, mean, sum_lanes(var, 32)};
+            if (lane == 0) st_pair(a.norm + turn, norm_of(m, a.eps));
+        }
+        return;
+    }
+    if (warp == kThreads / 32 + 2) {
+        int b = 0;
+        for (int unit = 0; unit < a.units; ++unit) {
+            if (!wait_posted(&posted, unit, abort, a.err)) return;
+            if (lane < gs) {
+                uint64_t q = ld_pair(a.norm + unit * gs + lane);
+                wait_pair(q, a.norm + unit * gs + lane, abort, a.err);
+                norm[b][lane] = floats_of(q);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(ready0 + 8 * b);
+            if (++b == a.buffers) b = 0;
+        }
+        return;
+    }
+
+    // one column a thread, every lanes-th row, for the sums and for the output alike. Units are whole slices, so
+    // this is the same for all of them.
+    const int tid = threadIdx.x % kSlabThreads, lanes = kSlabThreads / ncols, rl = tid / ncols, col = tid - rl * ncols;
+    const int count = rl < lanes && rl < rows ? static_cast<int>((rows - rl + lanes - 1) / lanes) : 0;
+    const uint32_t mine = base + tid * 16, stride = lanes * ncols * 16;
+    int b = 0;
+    uint32_t phase = 0;
+    if (warp < kSlabThreads / 32) {
+        const int sub = tid / a.group_lanes, sub_lane = tid % a.group_lanes;
+        // a group's moments of a row lane, of the block
+        const int group_cols = a.cpg / (VEC / N), entries = lanes * group_cols;
+        const float n = static_cast<float>(rows * a.cpg);
+        int to[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int group = (col * N + k) / group_cols, of_row = col * N + k - group * group_cols;
+            to[k] = group * entries + rl * group_cols + of_row;
+            if (rl < lanes && group == 0) share[to[k]] = static_cast<float>(count * (VEC / N)) / n;
+        }
+        for (int unit = 0; unit < a.units; ++unit) {
+            mbar_wait(full0 + 8 * b, phase, abort, a.err, E_RING);
+            Moments mo[N] = {};
+            const uint32_t from = mine + b * buffer_bytes;
+            int i = 0;
+#pragma unroll 1
+            for (; i + kAhead <= count; i += kAhead) {
+                uint4 v[kAhead];
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) v[k] = ld_shared(from + (i + k) * stride);
+                Run<TI, VEC, N> run(v[0]);
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) run.add(v[k]);
+                run.end(kAhead, mo);
+            }
+            if (i < count) {
+                Run<TI, VEC, N> run(ld_shared(from + i * stride));
+#pragma unroll 1
+                for (int k = i; k < count; ++k) run.add(ld_shared(from + k * stride));
+                run.end(count - i, mo);
+            }
+            float2 *entry = moments[unit & 1];
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                if (rl < lanes) entry[to[k]] = make_float2(mo[k].mean, mo[k].m2);
+            named_barrier_sync(1, kSlabThreads);
+            // joined as sums about the first one's mean, then about the mean of all: two short rounds of shuffles
+            const float2 *of = entry + (sub < gs ? sub * entries : 0);
+            const float p0 = of[0].x;
+            float sum = 0.f, m2 = 0.f;
+            for (int k = sub_lane; k < entries; k += a.group_lanes) sum = fmaf(of[k].x - p0, share[k], sum);
+            __syncwarp();
+            const float mean = p0 + sum_lanes(sum, a.group_lanes);
+            for (int k = sub_lane; k < entries; k += a.group_lanes) {
+                const float d = of[k].x - mean;
+                m2 += fmaf(d * d, share[k] * n, of[k].y);
+            }
+            __syncwarp();
+            m2 = sum_lanes(m2, a.group_lanes);
+            if (sub_lane == 0 && sub < gs)
+                st_pair(a.part + (static_cast<long long>(unit) * gs + sub) * a.parts + member, make_float2(mean, m2));
+            if (threadIdx.x == 0) posted = unit + 1;
+            if (++b == a.buffers) {
+                b = 0;
+                phase ^= 1u;
+            }
+        }
+        return;
+    }
+    for (int unit = 0; unit < a.units; ++unit) {
+        const int smp = unit / a.slices, c0 = (unit - smp * a.slices) * gs * a.cpg;
+        mbar_wait(ready0 + 8 * b, phase, abort, a.err, E_RING);
+        float minus[N], scale[VEC], shift[VEC];
+        affine_of<VEC, N>(a, col, c0, norm[b], minus, scale, shift);
+        TO *y = static_cast<TO *>(a.y) + smp * a.y_sample + (r0 + rl) * a.y_row + c0 + col * VEC;
+        const uint32_t from = mine + b * buffer_bytes;
+        const long long step = lanes * a.y_row;
+        switch (a.act) {
+        case S2_ACT_RELU: write_slab<TI, TO, N, S2_ACT_RELU>(from, count, stride, y, step, minus, scale, shift); break;
+        case S2_ACT_SILU: write_slab<TI, TO, N, S2_ACT_SILU>(from, count, stride, y, step, minus, scale, shift); break;
+        case S2_ACT_GELU: write_slab<TI, TO, N, S2_ACT_GELU>(from, count, stride, y, step, minus, scale, shift); break;
+        case S2_ACT_GELU_TANH: write_slab<TI, TO, N, S2_ACT_GELU_TANH>(from, count, stride, y, step, minus, scale, shift); break;
+        default: write_slab<TI, TO, N, S2_ACT_NONE>(from, count, stride, y, step, minus, scale, shift);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty0 + 8 * b);
+        if (++b == a.buffers) {
+            b = 0;
+            phase ^= 1u;
+        }
+    }
+}
+
 // ---- host --------------------------------------------------------------------------
 
 constexpr size_t kHold = 22 * kThreads * 16;  // shared memory for rows, two blocks an SM
@@ -837,12 +1158,21 @@ constexpr size_t kHold = 22 * kThreads * 16;  // shared memory for rows, two blo
 // The units of a call and the blocks that share them.
 struct Plan {
     int slices, slice_groups, units, parts, teams, join;
-    bool ring;
+    bool ring, slab;
+    int buffers, boxes, box_rows;
     long long part_rows;
     size_t smem;
 };
 
 size_t elem(int dtype) { return dtype == S2_F32 ? 4 : 2; }
+
+// Moments a vector of 16 bytes has: one for all the channels that surely share a group.
+int moments_of(int cpg, int vec)
+{
+    int n = 1;
+    while (cpg % (vec / n) != 0) n *= 2;
+    return n;
+}
 
 // Vectors of 16 bytes of x (their y 8 or 16 bytes) need every row to start on one.
 bool is_wide(const s2_group_norm_act_desc &d)
@@ -851,6 +1181,44 @@ bool is_wide(const s2_group_norm_act_desc &d)
     const uintptr_t xb = reinterpret_cast<uintptr_t>(d.x) | d.x_row * ie | (d.samples > 1 ? d.x_sample * ie : 0);
     const uintptr_t yb = reinterpret_cast<uintptr_t>(d.y) | d.y_row * oe | (d.samples > 1 ? d.y_sample * oe : 0);
     return d.channels % vec == 0 && xb % 16 == 0 && yb % (vec * oe) == 0;
+}
+
+// Slices for group_norm_slab_kernel, the widest of which a block holds at least four: 4 x 115200 x 512 bf16 takes
+// 218 us with four (slices of 64 bytes), 243 with two (128) and 256 through the ring. A block's share of a slice
+// below 8 KB does not pay for its exchange: 12 x 6000 x 640 fp16 (6.7 KB) 97 us and 79 through the ring, but
+// 12 x 9000 x 320 (9.9 KB) 54 and 71.
+bool plan_slab(const s2_group_norm_act_desc &d, int sms, Plan &p)
+{
+    const int size = static_cast<int>(elem(d.in_dtype)), vec = 16 / size, cpg = d.channels / d.groups;
+    if (d.x_row * size >= 1LL << 40 || d.x_sample * size >= 1LL << 40) return false;  // a tensor map's strides
+    const long long part_rows = (d.positions + 2 * sms - 1) / (2 * sms), parts = (d.positions + part_rows - 1) / part_rows;
+    if (part_rows * 64 * 4 > slab_room(1) || parts > 32 * kPartsLane) return false;
+    const int boxes = static_cast<int>((part_rows + 255) / 256);
+    for (int sg = std::min(d.groups, kSlabGroups); sg > 0; --sg) {
+        const int channels = sg * cpg, width = channels * size;
+        if (d.groups % sg != 0 || channels % vec != 0 || channels > 256) continue;
+        if (width < 64) break;
+        const int whole = std::max(1, 128 / (width & -width));  // a box is a multiple of 128 bytes
+        const int box_rows = (static_cast<int>((part_rows + boxes - 1) / boxes) + whole - 1) / whole * whole;
+        const long long bytes = 1LL * boxes * box_rows * width;
+        const int buffers = static_cast<int>(std::min<long long>(kMaxBuffers, slab_room(moments_of(cpg, vec)) / bytes));
+        if (buffers < 4) continue;
+        if (bytes < 8192) break;
+        p.slab = true;
+        p.join = kGrid;
+        p.part_rows = part_rows;
+        p.parts = static_cast<int>(parts);
+        p.teams = 1;
+        p.slice_groups = sg;
+        p.slices = d.groups / sg;
+        p.units = d.samples * p.slices;
+        p.boxes = boxes;
+        p.box_rows = box_rows;
+        p.buffers = buffers;
+        p.smem = buffers * bytes + 128;
+        return true;
+    }
+    return false;
 }
 
 Plan plan_of(const s2_group_norm_act_desc &d, int sms)
@@ -866,7 +1234,7 @@ Plan plan_of(const s2_group_norm_act_desc &d, int sms)
     auto bytes_of = [&](int sg) { return d.positions * width(sg); };  // of a unit
     auto halve = [&](int sg) { return std::max(step, sg / 2 / step * step); };
     auto fit = [&](int sg, int members) { return bytes_of(sg) / members <= static_cast<long long>(kHold * 15 / 16); };
-    Plan p;
+    Plan p = {};
     p.slice_groups = std::max(step, std::min(d.groups, kSliceGroups / step * step));
     p.join = kGrid;
     // Held by a cluster, if need be in narrower slices. Reading 128 bytes of each row at a time costs little,
@@ -881,6 +1249,7 @@ Plan plan_of(const s2_group_norm_act_desc &d, int sms)
         }
         if (halve(sg) == sg || width(halve(sg)) < narrow) break;
     }
+    if (p.join == kGrid && wide && plan_slab(d, sms, p)) return p;
     // A bulk copy takes the loading warp 60 clocks however short it is: 400 us became 16 ms with rows of 128
     // bytes apart from one another. Packed rows are copied a slot at a time, others have to be long.
     const bool rows_fit = d.x_row * size == width(p.slice_groups) || width(p.slice_groups) >= 1024;
@@ -917,7 +1286,7 @@ Plan plan_of(const s2_group_norm_act_desc &d, int sms)
 }
 
 size_t round_up16(size_t v) { return (v + 15) / 16 * 16; }
-size_t counters_of(const Plan &p) { return static_cast<size_t>(p.units) * 8; }
+size_t counters_of(const Plan &p) { return p.slab ? 0 : static_cast<size_t>(p.units) * 8; }
 
 size_t workspace_of(const Plan &p)
 {
@@ -933,9 +1302,9 @@ int sm_count()
     return sms > 0 ? sms : 148;
 }
 
-template <typename Kernel>
-s2_status launch(Kernel kernel, std::atomic<uint64_t> &configured, size_t most, size_t smem, int threads, const GnArgs &a,
-                 const Plan &p, cudaStream_t st)
+template <typename... Args>
+s2_status launch(void (*kernel)(Args...), std::atomic<uint64_t> &configured, size_t most, size_t smem, int threads, const Plan &p,
+                 cudaStream_t st, const Args &...args)
 {
     const s2_status cs = s2::once_per_device(configured, [&] {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most));
@@ -959,7 +1328,7 @@ s2_status launch(Kernel kernel, std::atomic<uint64_t> &configured, size_t most, 
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
     return e == cudaSuccess ? S2_OK : s2::set_error(S2_INFERENCE_FAILED, "s2_group_norm_act: launch failed: %s", cudaGetErrorString(e));
 }
 
@@ -970,10 +1339,19 @@ s2_status launch_shape(GnArgs &a, const Plan &p, cudaStream_t st)
     if constexpr (VEC > 1) {
         static std::atomic<uint64_t> ring{0};
         constexpr size_t kBytes = ring_slots<N>() * kSlotBytes;
-        if (p.ring) return launch(group_norm_ring_kernel<TI, TO, N>, ring, kBytes, kBytes, kThreads + 32, a, p, st);
+        if (p.ring) return launch(group_norm_ring_kernel<TI, TO, N>, ring, kBytes, kBytes, kThreads + 32, p, st, a);
+        static std::atomic<uint64_t> slab{0};
+        if (p.slab) {
+            CUtensorMap map;
+            const size_t ie = sizeof(TI);
+            if (!s2::make_map_3d_plain(&map, a.x, ie, a.C, a.P, (a.units / a.slices), a.x_row * ie,
+                                       a.x_sample > 0 ? a.x_sample * ie : a.x_row * ie, a.slice_groups * a.cpg, a.box_rows))
+                return s2::set_error(S2_INFERENCE_FAILED, "s2_group_norm_act: cuTensorMapEncodeTiled failed");
+            return launch(group_norm_slab_kernel<TI, TO, N>, slab, slab_room(N) + 128, p.smem, kThreads + 96, p, st, map, a);
+        }
     }
     a.hold = static_cast<int>(p.smem / (kThreads * sizeof(typename Raw<TI, VEC>::type)));
-    return launch(group_norm_held_kernel<TI, TO, VEC, N>, held, kHold, p.smem, kThreads, a, p, st);
+    return launch(group_norm_held_kernel<TI, TO, VEC, N>, held, kHold, p.smem, kThreads, p, st, a);
 }
 
 template <typename TI, typename TO>
@@ -981,11 +1359,12 @@ s2_status launch_types(GnArgs &a, const Plan &p, bool wide, cudaStream_t st)
 {
     constexpr int kWide = 16 / sizeof(TI);
     if (!wide) return launch_shape<TI, TO, 1, 1>(a, p, st);
-    if (a.cpg % kWide == 0) return launch_shape<TI, TO, kWide, 1>(a, p, st);
-    if (a.cpg % (kWide / 2) == 0) return launch_shape<TI, TO, kWide, 2>(a, p, st);
-    if constexpr (kWide == 8)
-        if (a.cpg % 2 == 0) return launch_shape<TI, TO, kWide, 4>(a, p, st);
-    return launch_shape<TI, TO, kWide, kWide>(a, p, st);
+    switch (moments_of(a.cpg, kWide)) {
+    case 1: return launch_shape<TI, TO, kWide, 1>(a, p, st);
+    case 2: return launch_shape<TI, TO, kWide, 2>(a, p, st);
+    case 4: return launch_shape<TI, TO, kWide, 4>(a, p, st);
+    default: return launch_shape<TI, TO, kWide, kWide>(a, p, st);
+    }
 }
 
 s2_status check(const s2_group_norm_act_desc *d)
@@ -1078,15 +1457,18 @@ extern "C" s2_status s2_group_norm_act(void *stream, const s2_group_norm_act_des
     a.teams = p.teams;
     a.join = p.join;
     a.act = d->activation;
+    a.buffers = p.buffers;
+    a.boxes = p.boxes;
+    a.box_rows = p.box_rows;
     a.group_lanes = 32;
-    while (a.group_lanes * p.slice_groups > kThreads) a.group_lanes /= 2;
+    while (a.group_lanes * p.slice_groups > (p.slab ? kSlabThreads : kThreads)) a.group_lanes /= 2;
     a.eps = d->eps;
     if (p.join == kGrid) {
         a.arrived = static_cast<uint32_t *>(d->workspace);
         a.ready = a.arrived + p.units;
         a.norm = reinterpret_cast<float2 *>(static_cast<char *>(d->workspace) + round_up16(counters_of(p)));
         a.part = a.norm + static_cast<size_t>(p.units) * p.slice_groups;
-        const cudaError_t e = cudaMemsetAsync(d->workspace, 0, counters_of(p), st);
+        const cudaError_t e = p.slab ? cudaMemsetAsync(d->workspace, 0xff, need, st) : cudaMemsetAsync(d->workspace, 0, counters_of(p), st);
         if (e != cudaSuccess) return s2::set_error(S2_INFERENCE_FAILED, "s2_group_norm_act: %s", cudaGetErrorString(e));
     }
     const bool wide = is_wide(*d);

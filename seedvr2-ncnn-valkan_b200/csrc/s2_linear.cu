@@ -2,10 +2,12 @@
 //   y[m][n] = act(sum_k x[m][k] w[n][k] + bias[n]) + residual[m][n],
 // x, w fp16 or bf16, the sum and everything after it in fp32, one rounding at the end.
 //
-// Two kernels on the tensor cores (tcgen05, accumulators in TMEM, operands staged by TMA in
+// One row of x (a time embedding) is a product of a matrix and a vector, linear_vec_kernel. From two rows
+// on, two kernels on the tensor cores (tcgen05, accumulators in TMEM, operands staged by TMA in
 // 64-element K slices, 128-byte swizzle, out-of-range rows and K read as zeros):
 //  * linear_tile_kernel, many rows: a pair of CTAs computes 256 x 256 tiles of y, persistent,
-//    two accumulators, so that a tile's epilogue runs beside the next tile's products.
+//    two accumulators, so that a tile's epilogue runs beside the next tile's products. A 256 x 256 tile
+//    reads 1 byte of operands from L2 for 128 multiplications; smaller ones would be bound by L2.
 //  * linear_rows_kernel, few rows: the operands change sides, 128 rows of w against 16 to 128
 //    rows of x, one tile of y^T a CTA, and K split over the CTAs of a cluster, which join their
 //    sums through distributed shared memory in order. The weights stream through at the rate of
@@ -293,7 +295,10 @@ struct Raw<1> {
     }
 };
 
-// One row of x: every warp streams two rows of w, a.ks warps (1, 2, 4 or 8) share their K by pieces of 32
+// One row of x, bound by the reading of w: 15360 x 2560 (79 MB) takes 15.7 us, 5.0 TB/s with start and end;
+// 2560 x 2560 4.6 us, most of it two trips to memory and the start. The tensor cores would not read faster,
+// and their tiles leave the GPU idle when N is small (2560 x 2560: 8.1 us in linear_rows_kernel).
+// Every warp streams two rows of w, a.ks warps (1, 2, 4 or 8) share their K by pieces of 32
 // vectors, kAhead pieces in flight. VEC = 8: w's rows and x start on 16 bytes; else values one by one.
 template <typename T, typename TO, int VEC, int kAhead>
 __global__ void __launch_bounds__(kVecThreads) linear_vec_kernel(const T *__restrict__ x, const T *__restrict__ w, long long ldw,
