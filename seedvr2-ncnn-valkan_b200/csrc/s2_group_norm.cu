@@ -12,15 +12,18 @@
 // which loses nothing when the mean is far larger than the spread, and an outlier only reaches
 // the run that holds it. What is joined with what depends on the shape alone, never on timing.
 //
-// A unit (a slice of the groups of one sample) is shared by a team of blocks. Two kernels:
-//  * group_norm_held_kernel: the blocks read their rows into shared memory while they sum them, and
-//    write the output from there. Small units are held whole by the blocks of a cluster, which
-//    exchange their moments through distributed shared memory: one read, no workspace. Larger ones
-//    whose rows do not start on 16 bytes take the blocks of a cooperative grid, and rows that are
-//    not held are read twice.
-//  * group_norm_ring_kernel, large units with aligned rows: a loading warp streams the rows through a
-//    ring of slots with bulk copies, so that the memory never waits for the threads that sum and
-//    write; what the ring holds at the end of the statistics is read once.
+// A unit (a slice of the groups of one sample) is shared by a team of blocks. The least to read and write is x
+// and y once (6.5 TB/s); the statistics stand between the two, so what counts is to hold what was read, and to
+// read the next while the last is joined and written. Three kernels:
+//  * group_norm_slab_kernel, aligned rows: teams of blocks hold narrow slices in shared memory, several at a
+//    time, and load, sum, join and write different ones at once. One read, up to 4.9 TB/s.
+//  * group_norm_held_kernel: the blocks read their rows into shared memory while they sum them, and write the
+//    output from there, one step after the other. For units too small to be worth the above: the blocks of a
+//    cluster hold one and exchange their moments through distributed shared memory, without a workspace. And
+//    for rows that do not start on 16 bytes, also on a cooperative grid, where rows not held are read twice.
+//  * group_norm_ring_kernel, aligned units larger than the shared memory of the GPU: a loading warp streams the
+//    rows through a ring of slots with bulk copies, so that the memory never waits for the threads that sum and
+//    write; all but what the ring holds at the end of the statistics is read twice.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -62,7 +65,7 @@ struct GnArgs {
     long long P, part_rows, x_row, x_sample, y_row, y_sample;
     int C, G, cpg, slices, slice_groups, units, parts, teams, join, hold, act;
     int group_lanes;  // threads that join one group's moments: a power of two up to 32
-    int buffers, boxes, box_rows;  // group_norm_slab_kernel
+    int buffers, boxes, box_rows, direct, join_lanes;  // group_norm_slab_kernel
     float eps;
     // a grid's: (mean, M2) per [unit][part][group], (mean, 1 / sigma) per [unit][group]; counters, zero
     // before: parts whose moments are written, units whose norm is
@@ -552,6 +555,8 @@ __device__ __forceinline__ void join_grid(const GnArgs &a, int unit, int member,
 
 // ---- rows held by the blocks ---------------------------------------------------------
 
+// Bound by its steps, one after the other (start, read, exchange, write): 3 x 7973 x 96 fp32 with rows of 101 values,
+// one at a time, 12.6 us; 20 x 500 x 512 bf16 14 us, 2.3 TB/s.
 template <typename TI, typename TO, int VEC, int N>
 __global__ void __launch_bounds__(kThreads, 2) group_norm_held_kernel(const GnArgs a)
 {
@@ -723,7 +728,9 @@ __device__ __forceinline__ void write_slots(Cursor<kSlots> c, const Slots &p, in
     }
 }
 
-// N: moments a vector, 16 / sizeof(TI) / N channels each, which always belong to one group.
+// Bound by the memory: two reads and a write of a unit that L2 does not hold. 21 x 921600 x 128 bf16 silu (236 MB a
+// sample) 2.36 ms, 96 % of these three passes at the copy rate, 6.3 TB/s; reads that the threads issue for
+// themselves took 2.9 ms. N: moments a vector, 16 / sizeof(TI) / N channels each, which always belong to one group.
 template <typename TI, typename TO, int N>
 __global__ void __launch_bounds__(kThreads + 32, 2) group_norm_ring_kernel(const GnArgs a)
 {
@@ -903,15 +910,17 @@ __device__ __forceinline__ void wait_pair(uint64_t &v, const float2 *p, volatile
             return;
         }
 }
-// The group's moments of all parts, part lane + 32 k in q[k] (part 0's past the last), when all are written.
-__device__ __forceinline__ void load_parts(uint64_t (&q)[kPartsLane], const float2 *part, int parts, volatile int *stop, int32_t *err)
+// A group's moments of all parts, by `lanes` neighbouring lanes (`sub` of them): part sub + k lanes in q[k], part 0's
+// past the last; returns when all are written.
+__device__ __forceinline__ void load_parts(uint64_t (&q)[kPartsLane], const float2 *part, int parts, int lanes, int sub,
+                                           volatile int *stop, int32_t *err)
 {
     const uint64_t t0 = global_timer_ns();
     for (;;) {
         bool all = true;
 #pragma unroll
         for (int k = 0; k < kPartsLane; ++k) {
-            const int t = (threadIdx.x & 31) + k * 32;
+            const int t = sub + k * lanes;
             q[k] = ld_pair(part + (t < parts ? t : 0));
         }
 #pragma unroll
@@ -923,6 +932,23 @@ __device__ __forceinline__ void load_parts(uint64_t (&q)[kPartsLane], const floa
             return;
         }
     }
+}
+// Their mean and 1 / sigma; w[k]: the parts' shares of the rows, inv_n: 1 / the group's values.
+__device__ __forceinline__ float2 norm_of_parts(const uint64_t (&q)[kPartsLane], const float (&w)[kPartsLane], int lanes, float inv_n,
+                                                float eps)
+{
+    const float p0 = __shfl_sync(0xffffffffu, floats_of(q[0]).x, 0, lanes);
+    float sum = 0.f, var = 0.f;
+#pragma unroll
+    for (int k = 0; k < kPartsLane; ++k)
+        if (w[k] > 0.f) sum = fmaf(floats_of(q[k]).x - p0, w[k], sum);
+    const float mean = p0 + sum_lanes(sum, lanes);
+#pragma unroll
+    for (int k = 0; k < kPartsLane; ++k) {
+        const float d = floats_of(q[k]).x - mean;
+        if (w[k] > 0.f) var += fmaf(d * d, w[k], floats_of(q[k]).y * inv_n);
+    }
+    return norm_of(Moments{1.f, mean, sum_lanes(var, lanes)}, eps);
 }
 // Until this block has posted its moments of `unit`.
 __device__ __forceinline__ bool wait_posted(const volatile int *posted, int unit, volatile int *stop, int32_t *err)
@@ -940,15 +966,16 @@ __device__ __forceinline__ bool wait_posted(const volatile int *posted, int unit
     return true;
 }
 
-// One team of all blocks takes narrow slices of the channels (64 bytes a row and more), of which each block holds
-// its rows of the last few in shared memory: every value is read once, whatever the sample's size. The work on
-// the units in flight goes on side by side: warps 0-3 sum one and post their block's moments, warps 4-7 write an
-// older one, warp 8 loads the next (and has the one behind it brought to L2), warp 9 joins all blocks' moments of
-// the groups that are its block's turn, warp 10 fetches the results. What bounds it is how long a unit stays in
-// shared memory, about 12 us of which 2.5 for the load, 1.5 for the sums, 5 for the exchange and 2.5 for the
-// output, at 28 MB for the whole GPU. 11 x 57600 x 512 bf16 silu: 265 us, 4.9 TB/s (the ring, which reads
-// twice: 347); 6 x 14400 x 512: 41 us (47). With one role a block after the other the same took 570 us, and 370 while
-// the parts' moments were asked for one after the other.
+// Teams of blocks (one of all of them for large samples) take narrow slices of the channels, 64 bytes a row and
+// more; a block holds its rows of the last few units in shared memory. The work on these goes on side by side:
+// warps 0-3 sum one and post their block's moments, warps 4-7 write an older one, warp 8 loads the next (and has
+// the one behind it brought to L2), warp 9 joins all parts' moments of the groups that are its block's turn,
+// warp 10 fetches the results; where the parts are few, warp 10 joins them all itself. What bounds it is how long a
+// unit stays in shared memory, about 12 us of which 2.5 for the load, 1.5 for the sums, 5 for the exchange and 2.5
+// for the output, at 28 MB for the whole GPU. 11 x 57600 x 512 bf16 silu: 264 us, 4.9 TB/s (347 through the ring,
+// which reads twice); 6 x 14400 x 512: 41 us (47); 40 x 3600 x 512: 73 us (143 held by clusters). With one role
+// after the other in each block the first took 560 us, and 370 while a lane asked for one part's moments after
+// the other.
 template <typename TI, typename TO, int N>
 __global__ void __launch_bounds__(kThreads + 96, 2) group_norm_slab_kernel(const __grid_constant__ CUtensorMap map, const GnArgs a)
 {
@@ -962,7 +989,9 @@ __global__ void __launch_bounds__(kThreads + 96, 2) group_norm_slab_kernel(const
     __shared__ int abort_flag;
     __shared__ volatile int posted;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int member = static_cast<int>(blockIdx.x), gs = a.slice_groups, ncols = gs * a.cpg / VEC;
+    const int team = static_cast<int>(blockIdx.x) / a.parts, member = static_cast<int>(blockIdx.x) - team * a.parts;
+    const int units = (a.units - team + a.teams - 1) / a.teams;  // the team's: team, team + teams, ...
+    const int gs = a.slice_groups, ncols = gs * a.cpg / VEC;
     const long long r0 = member * a.part_rows, rows = min(a.part_rows, a.P - r0);
     const uint32_t base = (smem_u32(slab_raw) + 127u) & ~127u, box_bytes = a.box_rows * ncols * 16, buffer_bytes = a.boxes * box_bytes;
     const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * kMaxBuffers, ready0 = empty0 + 8 * kMaxBuffers;
@@ -982,17 +1011,17 @@ __global__ void __launch_bounds__(kThreads + 96, 2) group_norm_slab_kernel(const
     if (warp == kThreads / 32) {
         if (lane != 0) return;
         const uint64_t policy = l2_evict_first();
-        int b = 0, unit = 0;
+        int b = 0, u = 0;
         uint32_t phase = 0;
-        for (; unit < a.units; ++unit) {
-            const int smp = unit / a.slices, c0 = (unit - smp * a.slices) * gs * a.cpg;
+        for (; u < units; ++u) {
+            const int unit = team + u * a.teams, smp = unit / a.slices, c0 = (unit - smp * a.slices) * gs * a.cpg;
             if (!mbar_wait(empty0 + 8 * b, phase ^ 1u, abort, a.err, E_RING)) break;
             mbar_arrive_expect_tx(full0 + 8 * b, buffer_bytes);
             for (int i = 0; i < a.boxes; ++i)
                 tma_load_3d(base + b * buffer_bytes + i * box_bytes, &map, full0 + 8 * b, c0, static_cast<int>(r0) + i * a.box_rows, smp,
                             policy);
             // the next unit, whose buffer is still in use, to L2: 265 us instead of 273 above
-            const int next = unit + 1;
+            const int next = unit + a.teams;
             if (next < a.units)
                 for (int i = 0; i < a.boxes; ++i)
                     tma_prefetch_3d(&map, next % a.slices * gs * a.cpg, static_cast<int>(r0) + i * a.box_rows, next / a.slices);
@@ -1001,55 +1030,50 @@ __global__ void __launch_bounds__(kThreads + 96, 2) group_norm_slab_kernel(const
                 phase ^= 1u;
             }
         }
-        if (unit < a.units) {
+        if (u < units) {
             // no copy may still be landing when the block ends: wait for the buffers' last loads
             int dummy = 0;
-            for (int u = max(0, unit - a.buffers); u < unit; ++u)
-                mbar_wait(full0 + 8 * (u % a.buffers), u / a.buffers & 1, &dummy, a.err, E_RING);
+            for (int k = max(0, u - a.buffers); k < u; ++k)
+                mbar_wait(full0 + 8 * (k % a.buffers), k / a.buffers & 1, &dummy, a.err, E_RING);
         }
         return;
     }
-    if (warp == kThreads / 32 + 1) {
-        // the units' groups go round the blocks
+    if (warp > kThreads / 32) {
+        const bool joins = warp == kThreads / 32 + 1;
+        if (joins && a.direct) return;
+        // lanes of a group: all, or few for each of a unit's groups at once
+        const int lanes = a.direct ? a.join_lanes : 32, sub = lane % lanes, group = lane / lanes;
         const float inv_rows = 1.f / static_cast<float>(a.P), inv_n = inv_rows / a.cpg;
-        float w[kPartsLane];  // the parts' shares of the rows
+        float w[kPartsLane];
 #pragma unroll
         for (int k = 0; k < kPartsLane; ++k) {
-            const int t = lane + k * 32;
+            const int t = sub + k * lanes;
             w[k] = t < a.parts ? static_cast<float>(min(a.part_rows, a.P - t * a.part_rows)) * inv_rows : 0.f;
         }
-        for (int turn = member; turn < a.units * gs; turn += a.parts) {
-            if (!wait_posted(&posted, turn / gs, abort, a.err)) return;
-            const float2 *part = a.part + static_cast<long long>(turn) * a.parts;
-            uint64_t q[kPartsLane];
-            load_parts(q, part, a.parts, abort, a.err);
-            // sums about the first part's mean
-            float sum = 0.f;
-            const float p0 = __shfl_sync(0xffffffffu, floats_of(q[0]).x, 0);
-#pragma unroll
-            for (int k = 0; k < kPartsLane; ++k) {
-                if (w[k] > 0.f) sum = fmaf(floats_of(q[k]).x - p0, w[k], sum);
+        uint64_t q[kPartsLane];
+        if (joins) {
+            // the units' groups go round the team's blocks
+            for (int turn = member; turn < units * gs; turn += a.parts) {
+                const int u = turn / gs, of = (team + u * a.teams) * gs + turn - u * gs;
+                if (!wait_posted(&posted, u, abort, a.err)) return;
+                load_parts(q, a.part + static_cast<long long>(of) * a.parts, a.parts, lanes, sub, abort, a.err);
+                const float2 r = norm_of_parts(q, w, lanes, inv_n, a.eps);
+                if (lane == 0) st_pair(a.norm + of, r);
             }
-            const float mean = p0 + sum_lanes(sum, 32);
-            float var = 0.f;
-#pragma unroll
-            for (int k = 0; k < kPartsLane; ++k) {
-                const float d = floats_of(q[k]).x - mean;
-                if (w[k] > 0.f) var += fmaf(d * d, w[k], floats_of(q[k]).y * inv_n);
-            }
-            const Moments m = {1.f, mean, sum_lanes(var, 32)};
-            if (lane == 0) st_pair(a.norm + turn, norm_of(m, a.eps));
+            return;
         }
-        return;
-    }
-    if (warp == kThreads / 32 + 2) {
         int b = 0;
-        for (int unit = 0; unit < a.units; ++unit) {
-            if (!wait_posted(&posted, unit, abort, a.err)) return;
-            if (lane < gs) {
-                uint64_t q = ld_pair(a.norm + unit * gs + lane);
-                wait_pair(q, a.norm + unit * gs + lane, abort, a.err);
-                norm[b][lane] = floats_of(q);
+        for (int u = 0; u < units; ++u) {
+            const int of = (team + u * a.teams) * gs;
+            if (!wait_posted(&posted, u, abort, a.err)) return;
+            if (a.direct) {
+                load_parts(q, a.part + static_cast<long long>(of + min(group, gs - 1)) * a.parts, a.parts, lanes, sub, abort, a.err);
+                const float2 r = norm_of_parts(q, w, lanes, inv_n, a.eps);
+                if (sub == 0 && group < gs) norm[b][group] = r;
+            } else if (lane < gs) {
+                uint64_t v = ld_pair(a.norm + of + lane);
+                wait_pair(v, a.norm + of + lane, abort, a.err);
+                norm[b][lane] = floats_of(v);
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(ready0 + 8 * b);
@@ -1077,7 +1101,7 @@ __global__ void __launch_bounds__(kThreads + 96, 2) group_norm_slab_kernel(const
             to[k] = group * entries + rl * group_cols + of_row;
             if (rl < lanes && group == 0) share[to[k]] = static_cast<float>(count * (VEC / N)) / n;
         }
-        for (int unit = 0; unit < a.units; ++unit) {
+        for (int u = 0; u < units; ++u) {
             mbar_wait(full0 + 8 * b, phase, abort, a.err, E_RING);
             Moments mo[N] = {};
             const uint32_t from = mine + b * buffer_bytes;
@@ -1098,7 +1122,7 @@ __global__ void __launch_bounds__(kThreads + 96, 2) group_norm_slab_kernel(const
                 for (int k = i; k < count; ++k) run.add(ld_shared(from + k * stride));
                 run.end(count - i, mo);
             }
-            float2 *entry = moments[unit & 1];
+            float2 *entry = moments[u & 1];
 #pragma unroll
             for (int k = 0; k < N; ++k)
                 if (rl < lanes) entry[to[k]] = make_float2(mo[k].mean, mo[k].m2);
@@ -1117,8 +1141,8 @@ __global__ void __launch_bounds__(kThreads + 96, 2) group_norm_slab_kernel(const
             __syncwarp();
             m2 = sum_lanes(m2, a.group_lanes);
             if (sub_lane == 0 && sub < gs)
-                st_pair(a.part + (static_cast<long long>(unit) * gs + sub) * a.parts + member, make_float2(mean, m2));
-            if (threadIdx.x == 0) posted = unit + 1;
+                st_pair(a.part + (static_cast<long long>(team + u * a.teams) * gs + sub) * a.parts + member, make_float2(mean, m2));
+            if (threadIdx.x == 0) posted = u + 1;
             if (++b == a.buffers) {
                 b = 0;
                 phase ^= 1u;
@@ -1126,7 +1150,7 @@ __global__ void __launch_bounds__(kThreads + 96, 2) group_norm_slab_kernel(const
         }
         return;
     }
-    for (int unit = 0; unit < a.units; ++unit) {
+    for (int unit = team; unit < a.units; unit += a.teams) {
         const int smp = unit / a.slices, c0 = (unit - smp * a.slices) * gs * a.cpg;
         mbar_wait(ready0 + 8 * b, phase, abort, a.err, E_RING);
         float minus[N], scale[VEC], shift[VEC];
@@ -1159,7 +1183,7 @@ constexpr size_t kHold = 22 * kThreads * 16;  // shared memory for rows, two blo
 struct Plan {
     int slices, slice_groups, units, parts, teams, join;
     bool ring, slab;
-    int buffers, boxes, box_rows;
+    int buffers, boxes, box_rows, direct, join_lanes;
     long long part_rows;
     size_t smem;
 };
@@ -1183,39 +1207,45 @@ bool is_wide(const s2_group_norm_act_desc &d)
     return d.channels % vec == 0 && xb % 16 == 0 && yb % (vec * oe) == 0;
 }
 
-// Slices for group_norm_slab_kernel, the widest of which a block holds at least four: 4 x 115200 x 512 bf16 takes
-// 218 us with four (slices of 64 bytes), 243 with two (128) and 256 through the ring. A block's share of a slice
-// below 8 KB does not pay for its exchange: 12 x 6000 x 640 fp16 (6.7 KB) 97 us and 79 through the ring, but
-// 12 x 9000 x 320 (9.9 KB) 54 and 71.
+// Slices for group_norm_slab_kernel: the widest of which as many blocks as there are can hold four. With 4 x 115200
+// x 512 bf16 these are 64 bytes wide and take 218 us; two of 128 took 243, the ring 256. A block's share of a
+// slice below 8 KB does not pay for its exchange: 20 x 9000 x 192 fp16 over the whole grid (5.9 KB) took 70 us
+// and 64 through the ring, but 12 x 9000 x 320 (9.9 KB) 54 and 71. Held by clusters 16 x 5000 x 512 bf16 took 73 us
+// and 47 here, 400 x 256 x 1280 240 and 130, 1 x 1920 x 512 9.5 and 9.2, only 8 x 1000 x 512 11.8 and 12.5.
 bool plan_slab(const s2_group_norm_act_desc &d, int sms, Plan &p)
 {
     const int size = static_cast<int>(elem(d.in_dtype)), vec = 16 / size, cpg = d.channels / d.groups;
     if (d.x_row * size >= 1LL << 40 || d.x_sample * size >= 1LL << 40) return false;  // a tensor map's strides
-    const long long part_rows = (d.positions + 2 * sms - 1) / (2 * sms), parts = (d.positions + part_rows - 1) / part_rows;
-    if (part_rows * 64 * 4 > slab_room(1) || parts > 32 * kPartsLane) return false;
-    const int boxes = static_cast<int>((part_rows + 255) / 256);
+    const long long room = slab_room(moments_of(cpg, vec)) / 4, blocks = 2 * sms;
     for (int sg = std::min(d.groups, kSlabGroups); sg > 0; --sg) {
         const int channels = sg * cpg, width = channels * size;
         if (d.groups % sg != 0 || channels % vec != 0 || channels > 256) continue;
         if (width < 64) break;
         const int whole = std::max(1, 128 / (width & -width));  // a box is a multiple of 128 bytes
-        const int box_rows = (static_cast<int>((part_rows + boxes - 1) / boxes) + whole - 1) / whole * whole;
-        const long long bytes = 1LL * boxes * box_rows * width;
-        const int buffers = static_cast<int>(std::min<long long>(kMaxBuffers, slab_room(moments_of(cpg, vec)) / bytes));
-        if (buffers < 4) continue;
-        if (bytes < 8192) break;
+        const long long most = room / width / whole * whole;    // rows of a quarter of the room
+        const long long units = 1LL * d.samples * (d.groups / sg);
+        if (most == 0 || (d.positions + most - 1) / most > blocks) continue;
+        const long long teams = std::min(units, blocks / ((d.positions + most - 1) / most));
+        const long long part_rows = (d.positions + blocks / teams - 1) / (blocks / teams);
+        const long long boxes = (part_rows + 255) / 256, box_rows = ((part_rows + boxes - 1) / boxes + whole - 1) / whole * whole;
+        const long long bytes = boxes * box_rows * width, parts = (d.positions + part_rows - 1) / part_rows;
+        if (bytes > room || box_rows > 256) continue;
+        if (bytes < 8192 || parts > 32 * kPartsLane) break;
         p.slab = true;
         p.join = kGrid;
         p.part_rows = part_rows;
         p.parts = static_cast<int>(parts);
-        p.teams = 1;
+        p.teams = static_cast<int>(teams);
         p.slice_groups = sg;
         p.slices = d.groups / sg;
-        p.units = d.samples * p.slices;
-        p.boxes = boxes;
-        p.box_rows = box_rows;
-        p.buffers = buffers;
-        p.smem = buffers * bytes + 128;
+        p.units = static_cast<int>(units);
+        p.boxes = static_cast<int>(boxes);
+        p.box_rows = static_cast<int>(box_rows);
+        p.buffers = static_cast<int>(std::min<long long>(kMaxBuffers, 4 * room / bytes));
+        p.join_lanes = 32;
+        while (p.join_lanes * sg > 32) p.join_lanes /= 2;
+        p.direct = parts <= p.join_lanes * kPartsLane;
+        p.smem = p.buffers * bytes + 128;
         return true;
     }
     return false;
@@ -1235,11 +1265,12 @@ Plan plan_of(const s2_group_norm_act_desc &d, int sms)
     auto halve = [&](int sg) { return std::max(step, sg / 2 / step * step); };
     auto fit = [&](int sg, int members) { return bytes_of(sg) / members <= static_cast<long long>(kHold * 15 / 16); };
     Plan p = {};
+    if (wide && plan_slab(d, sms, p)) return p;
     p.slice_groups = std::max(step, std::min(d.groups, kSliceGroups / step * step));
     p.join = kGrid;
     // Held by a cluster, if need be in narrower slices. Reading 128 bytes of each row at a time costs little,
-    // 32 do once the memory is the limit: 6 x 14400 x 512 took 80 us in slices of 32 bytes and 47 through the
-    // ring, but 3 x 7973 x 96 (9 MB) 12.8 us in slices of 48 and 18.3 on a grid.
+    // 32 do once the memory is the limit: 6 x 14400 x 512 took 80 us in slices of 32 bytes and 47 on a grid, but
+    // 3 x 7973 x 96 (9 MB, rows of 101 values) 12.8 us in slices of 48 and 18.3 on a grid.
     const int narrow = d.samples * bytes_of(d.groups) <= (32LL << 20) ? 32 : 128;
     for (int sg = p.slice_groups;; sg = halve(sg)) {
         if (fit(sg, kMaxCluster)) {
@@ -1249,7 +1280,6 @@ Plan plan_of(const s2_group_norm_act_desc &d, int sms)
         }
         if (halve(sg) == sg || width(halve(sg)) < narrow) break;
     }
-    if (p.join == kGrid && wide && plan_slab(d, sms, p)) return p;
     // A bulk copy takes the loading warp 60 clocks however short it is: 400 us became 16 ms with rows of 128
     // bytes apart from one another. Packed rows are copied a slot at a time, others have to be long.
     const bool rows_fit = d.x_row * size == width(p.slice_groups) || width(p.slice_groups) >= 1024;
@@ -1267,9 +1297,9 @@ Plan plan_of(const s2_group_norm_act_desc &d, int sms)
     p.teams = p.units;
     if (p.join == kGrid) {
         // All units at once up to 8 of them, else three or four in flight, whichever leaves fewer blocks idle in
-        // the last round: while some read, others write. 11 x 57600 x 512 bf16: 387 us with two, 362 / 344 with
-        // three / four, 362 with all; 21 x 921600 x 128: 2.61, 2.34, 2.46 and 2.45 ms. More when a block's share
-        // of a unit would be less than it holds.
+        // the last round: while some read, others write. 21 x 921600 x 128 bf16: 2.61 ms with two, 2.34 / 2.46 with
+        // three / four, 2.45 with all; 11 x 57600 x 512: 387, 362 / 344 and 362 us. More when a block's share of a
+        // unit would be less than it holds.
         const int blocks = 2 * sms;
         auto rounds = [&](int teams) { return static_cast<double>((p.units + teams - 1) / teams) / (blocks / teams); };
         p.teams = p.units <= 8 ? p.units : (rounds(3) < rounds(4) ? 3 : 4);
@@ -1459,6 +1489,8 @@ extern "C" s2_status s2_group_norm_act(void *stream, const s2_group_norm_act_des
     a.act = d->activation;
     a.buffers = p.buffers;
     a.boxes = p.boxes;
+    a.direct = p.direct;
+    a.join_lanes = p.join_lanes;
     a.box_rows = p.box_rows;
     a.group_lanes = 32;
     while (a.group_lanes * p.slice_groups > (p.slab ? kSlabThreads : kThreads)) a.group_lanes /= 2;

@@ -105,6 +105,8 @@ struct Rows {
     static_assert(MB * kRowsN * 4 <= kOffBar, "the joined sums reuse the stages");
 };
 
+// Few rows are bound by the reading of w, which every block of x's rows repeats from L2: 58 x 2560 x 5120 takes 10.4 us
+// (26 MB, 4.1 at the copy rate; the rest is the start, a first trip to memory and the join), 200 x 2560 x 5120 18.1 us.
 template <int MB, typename TO>
 __global__ void __launch_bounds__(kRowsThreads, 2)
     linear_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
@@ -408,6 +410,10 @@ __device__ __forceinline__ void tile_of(int t, int m_blocks, int n_blocks, int &
     mb = band * kBand + in - nb * rows;
 }
 
+// Large products run at the rate that the power limit leaves the tensor cores: 57600 x 6912 x 2560 fp16 833 us
+// without an activation, 1.22 PFLOP/s of 1.40 sustained, 882 with gelu, whose arithmetic the epilogue warps do
+// beside the products. With K short the tiles' operands bound it, 2 MB of them from L2 for each 0.5 MB of y at
+// K = 512: 86400 x 512 x 512 with a residual 50 us (40.6 to read and write once).
 template <typename TO>
 __global__ void __launch_bounds__(kTileThreads, 1)
     linear_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,

@@ -176,7 +176,8 @@ def test_norm_of_nothing():
 
 
 @pytest.mark.parametrize("dtype", [F16, F32], ids=str)
-@pytest.mark.parametrize("shape", [(3, 20000, 96), (2, 40000, 512), (4, 60000, 128), (2, 1500, 512), (1, 60000, 130)], ids=str)
+@pytest.mark.parametrize("shape", [(3, 20000, 96), (2, 40000, 512), (4, 60000, 128), (2, 1500, 512), (1, 60000, 130),
+                                   (40, 500, 640), (300, 64, 512), (1, 300000, 64), (2, 140000, 512)], ids=str)
 def test_norm_gives_the_same_bits(shape, dtype):
     """Whatever the blocks' order: the joins' and the ring's hand-overs, many times over."""
     x = _features(shape, _gen(12), dtype)
@@ -203,7 +204,8 @@ def test_norm_of_large_samples(shape):
 # one pass, of several and of none to spare holds
 @pytest.mark.parametrize("types", NORM_TYPES, ids=lambda t: f"{t[0]}-{t[1]}".replace("torch.", ""))
 @pytest.mark.parametrize("shape", [(2, 40001, 256, 32), (3, 50000, 128, 32), (1, 300017, 64, 32), (9, 30011, 96, 32),
-                                   (2, 60000, 192, 64), (1, 33000, 2048, 1)], ids=str)
+                                   (2, 60000, 192, 64), (1, 33000, 2048, 1), (1, 260001, 80, 16), (2, 150001, 512, 32)],
+                         ids=str)
 def test_norm_of_large_packed_units(shape, types):
     S, P, C, G = shape
     x = _features((S, P, C), _gen(P), types[0])
@@ -245,6 +247,100 @@ def test_norm_of_large_units_about_a_large_mean(shape):
     y = s2b200.group_norm_act(x, G)
     for s in range(S):
         cl.check(y[s:s + 1], *cl.norm_exact(x[s:s + 1], G, None, None, 1e-6, "none"))
+
+
+# Slices of the channels that the whole grid, or some of its blocks, hold at once: one block a slice and all of
+# them, moments joined by each block for itself and by one for all, rows in one box and in two, 1 to 8 moments
+# a vector, columns that do not fill the threads, last blocks with fewer rows.
+SLICES = [(2, 1920, 512, 32), (40, 200, 1280, 32), (3, 57601, 512, 32), (1, 100003, 128, 32), (12, 9001, 320, 32),
+          (20, 5003, 120, 24), (300, 64, 512, 32), (2000, 16, 512, 32), (7, 12007, 256, 1), (5, 6001, 640, 32),
+          (9, 30011, 96, 24), (30, 1999, 208, 16)]
+
+
+@pytest.mark.parametrize("types", NORM_TYPES, ids=lambda t: f"{t[0]}-{t[1]}".replace("torch.", ""))
+@pytest.mark.parametrize("pads", [(0, 0), (8, 16)], ids=str)
+@pytest.mark.parametrize("shape", SLICES, ids=str)
+def test_norm_of_slices(shape, pads, types):
+    S, P, C, G = shape
+    gen = _gen(P + C)
+    x = _padded(_features((S, P, C), gen, types[0]), pads[0])[1]
+    buf, out = _padded(torch.zeros(S, P, C, dtype=types[1], device="cuda"), pads[1])
+    w, b = 1 + 0.1 * _normal((C,), gen), 0.1 * _normal((C,), gen)
+    act = cl.ACTS[(P + S + G) % 5]
+    s2b200.group_norm_act(x, G, w, b, activation=act, out=out)
+    for s in {0, S // 2, S - 1}:
+        cl.check(out[s:s + 1], *cl.norm_exact(x[s:s + 1], G, w, b, 1e-6, act), f"{shape} {act}")
+    assert torch.isnan(buf[..., C:]).all() and not torch.isnan(out).any()
+
+
+@pytest.mark.parametrize("shape", SLICES, ids=str)
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
+def test_norm_of_slices_in_place(shape, dtype):
+    S, P, C, G = shape
+    x = _features((S, P, C), _gen(31), dtype)
+    want = s2b200.group_norm_act(x, G, activation="silu")
+    s2b200.group_norm_act(x, G, activation="silu", out=x)
+    assert torch.equal(x, want)
+
+
+@pytest.mark.parametrize("shape", [(2, 1920, 512, 32), (40, 200, 1280, 32), (3, 20001, 512, 32)], ids=str)
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_norm_of_slices_bad_values_and_equal_ones(shape, bad):
+    S, P, C, G = shape
+    x = _features(shape[:3], _gen(32), F16)
+    y0 = s2b200.group_norm_act(x, G, activation="relu")
+    k = C // G
+    for at, g in ((0, 3), (P // 2, G - 1), (P - 1, 0)):
+        z = x.clone()
+        z[S - 1, at, g * k + 1] = bad
+        y = s2b200.group_norm_act(z, G, activation="relu")
+        assert torch.isnan(y[S - 1, :, g * k:(g + 1) * k]).all()
+        y[S - 1, :, g * k:(g + 1) * k] = y0[S - 1, :, g * k:(g + 1) * k]
+        assert torch.equal(y, y0)
+    b = torch.linspace(-1, 1, C, device="cuda")
+    y = s2b200.group_norm_act(torch.full(shape[:3], 3.25, device="cuda", dtype=F16), G, None, b)
+    assert torch.equal(y, b.half().expand_as(y))
+
+
+def test_norm_of_slices_about_a_large_mean():
+    x = 1000 + 0.5 * _normal((2, 20000, 256), _gen(33))
+    x[0, 777, 3] = 3e5
+    y = s2b200.group_norm_act(x, 32)
+    cl.check(y, *cl.norm_exact(x, 32, None, None, 1e-6, "none"))
+
+
+def test_norm_of_slices_on_two_streams_and_replayed():
+    """Two calls that need the whole grid each at the same time, eager and in graphs, on new inputs."""
+    gen = _gen(34)
+    xs = [_features((3, 20001, 512), gen, F16), _features((60, 300, 640), gen, F16)]
+    want = [s2b200.group_norm_act(x, 32, activation="silu") for x in xs]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    off = torch.zeros((), dtype=torch.int64, device="cuda")
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for x, st in zip(xs, streams):
+            with torch.cuda.stream(st):
+                got.append(s2b200.group_norm_act(x, 32, activation="silu"))
+        torch.cuda.synchronize()
+        off += sum((g != w).sum() for g, w in zip(got, want))
+    graphs = []
+    for x in xs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = s2b200.group_norm_act(x, 32, activation="silu")
+        graphs.append((g, y))
+    for x in xs:
+        x.copy_(x.flip(0))
+    want = [s2b200.group_norm_act(x, 32, activation="silu") for x in xs]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for (g, _), st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        off += sum((y != w).sum() for (_, y), w in zip(graphs, want))
+    assert off.item() == 0
 
 
 def test_norm_of_many_samples():
