@@ -420,9 +420,12 @@ typedef enum s2_activation {
  * pivots, joined in order (the same call gives the same bits). x_row, y_row
  * >= channels: elements between positions; x_sample, y_sample: between
  * samples. y may be x itself (same type, pitch and sample stride), and must
- * not overlap it otherwise. samples or positions 0: nothing is done. At most
- * 1024 groups (S2_UNSUPPORTED beyond). err: device int32 error word (may be
- * NULL), set when a bounded wait inside the kernel gives up. */
+ * not overlap it otherwise. The square of a value's distance from the mean
+ * must be finite in fp32; a group with a value that is not gives NaN, and no
+ * other does. samples or positions 0: nothing is done. At most 1024 groups,
+ * 65535 samples and 2^31 positions (S2_UNSUPPORTED beyond). err: device int32
+ * error word (may be NULL), set when a bounded wait inside the kernel gives up
+ * (96 for the other blocks' moments, 97 for a load). */
 typedef struct s2_group_norm_act_desc {
     int samples, channels, groups, activation;
     long long positions;
@@ -449,7 +452,8 @@ S2_API s2_status s2_group_norm_act(void *stream, const s2_group_norm_act_desc *d
  * workspace. Products are summed on the tensor cores in fp32, bias,
  * activation and residual are applied to the fp32 sum, and y is rounded once.
  * y may be residual itself (same pitch) and must not overlap any input
- * otherwise. M 0: nothing is done. err as above. */
+ * otherwise. One row needs no workspace, whatever the alignment. M up to 2^30,
+ * N and K up to 2^21. M 0: nothing is done. err as above (80 to 85). */
 typedef struct s2_linear_act_desc {
     int N, K, activation;
     int dtype, out_dtype; /* s2_dtype */

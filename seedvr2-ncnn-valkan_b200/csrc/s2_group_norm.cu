@@ -65,10 +65,13 @@ struct GnArgs {
     long long P, part_rows, x_row, x_sample, y_row, y_sample;
     int C, G, cpg, slices, slice_groups, units, parts, teams, join, hold, act;
     int group_lanes;  // threads that join one group's moments: a power of two up to 32
-    int buffers, boxes, box_rows, direct, join_lanes;  // group_norm_slab_kernel
+    // group_norm_slab_kernel: units that a block holds, boxes of rows of one; `direct`: every block joins the
+    // parts for itself, join_lanes lanes a group
+    int buffers, boxes, box_rows, direct, join_lanes;
     float eps;
     // a grid's: (mean, M2) per [unit][part][group], (mean, 1 / sigma) per [unit][group]; counters, zero
-    // before: parts whose moments are written, units whose norm is
+    // before: parts whose moments are written, units whose norm is. group_norm_slab_kernel has no counters: its
+    // moments, [unit][group][part], and norms have all bits set until they are written
     float2 *part, *norm;
     uint32_t *arrived, *ready;
 };
@@ -1211,11 +1214,11 @@ bool is_wide(const s2_group_norm_act_desc &d)
 // x 512 bf16 these are 64 bytes wide and take 218 us; two of 128 took 243, the ring 256. A block's share of a
 // slice below 8 KB does not pay for its exchange: 20 x 9000 x 192 fp16 over the whole grid (5.9 KB) took 70 us
 // and 64 through the ring, but 12 x 9000 x 320 (9.9 KB) 54 and 71. Held by clusters 16 x 5000 x 512 bf16 took 73 us
-// and 47 here, 400 x 256 x 1280 240 and 130, 1 x 1920 x 512 9.5 and 9.2, only 8 x 1000 x 512 11.8 and 12.5.
+// and 47 here, 400 x 256 x 1280 240 and 130.
 bool plan_slab(const s2_group_norm_act_desc &d, int sms, Plan &p)
 {
     const int size = static_cast<int>(elem(d.in_dtype)), vec = 16 / size, cpg = d.channels / d.groups;
-    if (d.x_row * size >= 1LL << 40 || d.x_sample * size >= 1LL << 40) return false;  // a tensor map's strides
+    if (d.x_row >= (1LL << 40) / size || d.x_sample >= (1LL << 40) / size) return false;  // a tensor map's strides
     const long long room = slab_room(moments_of(cpg, vec)) / 4, blocks = 2 * sms;
     for (int sg = std::min(d.groups, kSlabGroups); sg > 0; --sg) {
         const int channels = sg * cpg, width = channels * size;
@@ -1265,7 +1268,9 @@ Plan plan_of(const s2_group_norm_act_desc &d, int sms)
     auto halve = [&](int sg) { return std::max(step, sg / 2 / step * step); };
     auto fit = [&](int sg, int members) { return bytes_of(sg) / members <= static_cast<long long>(kHold * 15 / 16); };
     Plan p = {};
-    if (wide && plan_slab(d, sms, p)) return p;
+    // Below 8 MB the slices' GPU time is hardly less, and their workspace, which is cleared first, and cooperative
+    // launch cost the host 5 us: 2 x 1920 x 512 fp16 9.1 us and 16.4 called one by one, 9.2 and 11.5 by clusters.
+    if (wide && d.samples * bytes_of(d.groups) >= (8LL << 20) && plan_slab(d, sms, p)) return p;
     p.slice_groups = std::max(step, std::min(d.groups, kSliceGroups / step * step));
     p.join = kGrid;
     // Held by a cluster, if need be in narrower slices. Reading 128 bytes of each row at a time costs little,
@@ -1280,6 +1285,7 @@ Plan plan_of(const s2_group_norm_act_desc &d, int sms)
         }
         if (halve(sg) == sg || width(halve(sg)) < narrow) break;
     }
+    if (p.join == kGrid && wide && plan_slab(d, sms, p)) return p;
     // A bulk copy takes the loading warp 60 clocks however short it is: 400 us became 16 ms with rows of 128
     // bytes apart from one another. Packed rows are copied a slot at a time, others have to be long.
     const bool rows_fit = d.x_row * size == width(p.slice_groups) || width(p.slice_groups) >= 1024;
@@ -1321,7 +1327,7 @@ size_t counters_of(const Plan &p) { return p.slab ? 0 : static_cast<size_t>(p.un
 size_t workspace_of(const Plan &p)
 {
     if (p.join != kGrid) return 0;
-    return round_up16(counters_of(p)) + static_cast<size_t>(p.units) * (1 + p.parts) * p.slice_groups * sizeof(float2);
+    return round_up16(counters_of(p)) + static_cast<size_t>(p.units) * (!p.direct + p.parts) * p.slice_groups * sizeof(float2);
 }
 
 int sm_count()
@@ -1405,6 +1411,8 @@ s2_status check(const s2_group_norm_act_desc *d)
                              d->samples, d->positions, d->channels, d->groups);
     if (d->groups > kMaxGroups || d->samples > 65535 || d->positions > (1LL << 31))
         return s2::set_error(S2_UNSUPPORTED, "s2_group_norm_act: at most %d groups, 65535 samples and 2^31 positions", kMaxGroups);
+    if (d->positions > (1LL << 44) / d->channels)
+        return s2::set_error(S2_UNSUPPORTED, "s2_group_norm_act: at most 2^44 values a sample");
     const bool types = (d->in_dtype == S2_F32 && (d->out_dtype == S2_F32 || d->out_dtype == S2_F16 || d->out_dtype == S2_BF16)) ||
                        ((d->in_dtype == S2_F16 || d->in_dtype == S2_BF16) && d->out_dtype == d->in_dtype);
     if (!types)
@@ -1453,7 +1461,12 @@ extern "C" s2_status s2_group_norm_act(void *stream, const s2_group_norm_act_des
     if (reinterpret_cast<uintptr_t>(d->x) % ie || reinterpret_cast<uintptr_t>(d->y) % oe ||
         (reinterpret_cast<uintptr_t>(d->weight) | reinterpret_cast<uintptr_t>(d->bias)) % 4)
         return s2::set_error(S2_INVALID_ARGUMENT, "s2_group_norm_act: a pointer is not aligned to its elements");
-    if (d->x_row < d->channels || d->y_row < d->channels || d->x_row > (1LL << 40) || d->y_row > (1LL << 40) ||
+    // (n - 1) strides stay within 2^44 elements, so that no offset below overflows
+    auto far = [](long long n, long long stride) { return n > 1 && stride > (1LL << 44) / (n - 1); };
+    if (d->x_row > (1LL << 40) || d->y_row > (1LL << 40) || far(d->positions, d->x_row) || far(d->positions, d->y_row) ||
+        far(d->samples, d->x_sample) || far(d->samples, d->y_sample))
+        return s2::set_error(S2_INVALID_ARGUMENT, "s2_group_norm_act: a pitch or sample stride beyond any memory");
+    if (d->x_row < d->channels || d->y_row < d->channels ||
         (d->samples > 1 && (d->x_sample < (d->positions - 1) * d->x_row + d->channels ||
                             d->y_sample < (d->positions - 1) * d->y_row + d->channels)))
         return s2::set_error(S2_INVALID_ARGUMENT, "s2_group_norm_act: a pitch is smaller than what it spans");
@@ -1499,7 +1512,7 @@ extern "C" s2_status s2_group_norm_act(void *stream, const s2_group_norm_act_des
         a.arrived = static_cast<uint32_t *>(d->workspace);
         a.ready = a.arrived + p.units;
         a.norm = reinterpret_cast<float2 *>(static_cast<char *>(d->workspace) + round_up16(counters_of(p)));
-        a.part = a.norm + static_cast<size_t>(p.units) * p.slice_groups;
+        a.part = a.norm + (p.direct ? 0 : static_cast<size_t>(p.units) * p.slice_groups);
         const cudaError_t e = p.slab ? cudaMemsetAsync(d->workspace, 0xff, need, st) : cudaMemsetAsync(d->workspace, 0, counters_of(p), st);
         if (e != cudaSuccess) return s2::set_error(S2_INFERENCE_FAILED, "s2_group_norm_act: %s", cudaGetErrorString(e));
     }

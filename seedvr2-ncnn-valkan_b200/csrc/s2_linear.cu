@@ -410,10 +410,11 @@ __device__ __forceinline__ void tile_of(int t, int m_blocks, int n_blocks, int &
     mb = band * kBand + in - nb * rows;
 }
 
-// Large products run at the rate that the power limit leaves the tensor cores: 57600 x 6912 x 2560 fp16 833 us
-// without an activation, 1.22 PFLOP/s of 1.40 sustained, 882 with gelu, whose arithmetic the epilogue warps do
-// beside the products. With K short the tiles' operands bound it, 2 MB of them from L2 for each 0.5 MB of y at
-// K = 512: 86400 x 512 x 512 with a residual 50 us (40.6 to read and write once).
+// Large products run at the rate that the power limit leaves the tensor cores: 21600 x 10240 x 2560 bf16 takes 833 us
+// without an activation, 1.36 PFLOP/s (1.40 measured for a library's plain product kept up for seconds), and 882
+// with gelu, whose arithmetic the epilogue warps do beside the products. With K short the tiles' operands bound
+// it, 0.5 MB of them from L2 for each 128 KB of y at K = 512: 86400 x 512 x 512 fp16 with a residual takes 50 us
+// in a burst (40.6 to read and write once) and 63 under load.
 template <typename TO>
 __global__ void __launch_bounds__(kTileThreads, 1)
     linear_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,

@@ -48,7 +48,9 @@ NORM_REFUSALS = [
     (dict(samples=1 << 20), UNSUPPORTED), (dict(y=BASE + 64), INVALID), (dict(y=BASE, y_row=72, y_sample=7200), INVALID),
     (dict(y=BASE, in_dtype=s2b200.S2_F32), INVALID), (dict(x_row=1 << 50, x_sample=1 << 60), INVALID),
     (dict(x_row=80, y_row=80, x_sample=8000, y_sample=8000, y=BASE + 32), INVALID),
-    (dict(positions=1 << 41), UNSUPPORTED),
+    (dict(positions=1 << 41), UNSUPPORTED), (dict(x_sample=1 << 62), INVALID), (dict(y_sample=1 << 62), INVALID),
+    (dict(positions=1 << 31, x_row=1 << 40), INVALID), (dict(positions=1 << 31, y_row=1 << 40), INVALID),
+    (dict(positions=1 << 31, channels=1 << 30, x_row=1 << 30, y_row=1 << 30), UNSUPPORTED),
 ]
 
 
