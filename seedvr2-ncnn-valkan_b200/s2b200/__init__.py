@@ -1067,7 +1067,7 @@ def _run_desc(call, workspace_bytes, desc_type, packed: bytes, x, index: int, wh
 def group_norm_act(x, groups: int, weight=None, bias=None, eps: float = 1e-6, activation: str = "none", out=None,
                    out_dtype=None, err=None, stream=None):
     """Channels-last group norm with an activation (s2_group_norm_act): x [samples, ..., channels]
-    CUDA tensor (fp16, bf16 or fp32, any even spacing of positions); per sample and group of
+    CUDA tensor (fp16, bf16 or fp32, positions at any one pitch); per sample and group of
     channels / groups consecutive channels, y = act((x - mean) / sqrt(var + eps) * weight + bias).
     weight, bias: fp32 [channels] or None. Returns y in out_dtype (x's, or fp16 / bf16 for fp32 x)
     in x's shape; `out` receives it when given (it may be x). err: device int32 error word."""
@@ -1113,7 +1113,7 @@ def group_norm_act(x, groups: int, weight=None, bias=None, eps: float = 1e-6, ac
 def linear_act(x, w, bias=None, activation: str = "none", residual=None, out=None, out_dtype=None, err=None,
                stream=None):
     """y = act(x w^T + bias) + residual (s2_linear_act): x [..., K] and w [N, K] CUDA tensors of one
-    type (fp16 or bf16, rows of any even pitch), bias fp32 [N] or None, residual [..., N] in the
+    type (fp16 or bf16, rows of any pitch), bias fp32 [N] or None, residual [..., N] in the
     output's type or None. Returns y [..., N] in out_dtype (x's, or fp32); `out` receives it when
     given (it may be the residual). err: device int32 error word."""
     torch = _torch()
