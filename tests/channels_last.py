@@ -72,3 +72,28 @@ def check(got, want, room, what=""):
     bad = ~(off <= limit)
     assert not bad.any(), (f"{what}: {int(bad.sum())} of {bad.numel()} values off, the worst by "
                            f"{(off / limit).nan_to_num(9e9).max().item():.3g} times its bound")
+
+
+def activation_exact(v, act):
+    """(act(v), bound on its error in fp32) for fp32 values v, in 64 bits, every tail relatively exact.
+
+    Roundings, in units of u = 2^-23 (two fp32 half steps, one ulp of the hardware's reciprocal; its 2^x is within
+    2 u): silu, v / (1 + e^-v): 2^x, +, 1 / x, * are 2 + 1 + 1 + 1 with one to spare, and the exponent's product with
+    a rounded log2 e is off by |v| u at most in the exponent. gelu, v h: the fit of h 0.8 u, seven fmas of which the
+    last ones count (2), t 2, products 1.5, 2^x 2: 8, and v^2 / 2 u from the exponent's two products and its constant.
+    gelu_tanh like silu, its exponent w from three roundings and two rounded constants: 2 w u. Above 0 the exponentials
+    weigh at most 0.37 of these last terms; the bound keeps them whole below 0 and drops them above, where 2 u more
+    cover them. Below 2^-119 a result may be 0."""
+    v = v.double()
+    a, u = v.abs(), 2.0 ** -23
+    w = 2 * (2 / torch.pi) ** 0.5 * (a + 0.044715 * a ** 3)
+    if act == "gelu_tanh":
+        y = v * torch.sigmoid(torch.sign(v) * w)
+    elif act == "gelu":
+        y = v * 0.5 * torch.erfc(v * -0.5 ** 0.5)  # special.ndtr is exact absolutely only
+    else:
+        y = activate(v, act)
+    base, slope = {"none": (0, 0 * a), "relu": (0, 0 * a), "silu": (6, a), "gelu": (8, a * a / 2),
+                   "gelu_tanh": (6, 2 * w)}[act]
+    units = torch.where(v < 0, base + slope, (base + 2.0 if base else 0.0) + 0 * a)
+    return y, y.abs() * units * u + (2.0 ** -119 if base else 0.0)

@@ -678,3 +678,37 @@ def test_err_word_stays_zero():
     s2b200.linear_act(x, w, b, err=err)
     s2b200.group_norm_act(x.view(5, 100, 512), 32, err=err)
     assert err.item() == 0
+
+
+# ---- activations -----------------------------------------------------------------------
+
+def _sweep(n):
+    """n values over [-12, 12], and the ones where the activations change their form."""
+    v = torch.linspace(-12, 12, n, device="cuda")
+    v[:8] = torch.tensor([0.0, -0.0, 1e-30, -1e-30, 1e-4, -1e-4, 13.2, -13.3], device="cuda")
+    return v
+
+
+@pytest.mark.parametrize("act", cl.ACTS)
+@pytest.mark.parametrize("out_dtype", [F32, F16, BF16], ids=str)
+@pytest.mark.parametrize("M,N", [(1, 200001), (20, 20001), (300, 5003)])
+def test_activations_of_the_product(M, N, out_dtype, act):
+    """0 x 0 + bias: the activation's own error, relative to its result, in the three kernels' epilogues."""
+    v = _sweep(N)
+    dtype = F16 if out_dtype == F32 else out_dtype
+    y = s2b200.linear_act(torch.zeros(M, 8, device="cuda", dtype=dtype), torch.zeros(N, 8, device="cuda", dtype=dtype), v,
+                          act, out_dtype=out_dtype)
+    want, room = cl.activation_exact(v, act)
+    cl.check(y, want.expand(M, N), room.expand(M, N), act)
+
+
+@pytest.mark.parametrize("act", cl.ACTS)
+@pytest.mark.parametrize("out_dtype", [F32, F16, BF16], ids=str)
+@pytest.mark.parametrize("P,pad", [(3, 0), (3, 1)])
+def test_activations_of_the_norm(P, pad, out_dtype, act):
+    """Equal values: the norm is its bias, exactly."""
+    v = _sweep(1 << 16)
+    x = _padded(torch.full((2, P, 1 << 16), 3.25, device="cuda"), pad)[1]
+    y = s2b200.group_norm_act(x, 1024, None, v, activation=act, out_dtype=out_dtype)
+    want, room = cl.activation_exact(v, act)
+    cl.check(y, want.expand(y.shape), room.expand(y.shape), act)
