@@ -775,7 +775,8 @@ __global__ void __launch_bounds__(kThreads + 32, 2) group_norm_ring_kernel(const
                 const int i = q < p.total ? q : p.total - p.held - 1 - (q - p.total);
                 const long long first = static_cast<long long>(i) * p.rows;
                 const int n = static_cast<int>(min(static_cast<long long>(p.rows), rows - first));
-                ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * slot, phase ^ 1u, abort, a.err, E_RING));
+                // nothing after a time-out: those who gave up release slots that are still being filled
+                ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * slot, phase ^ 1u, abort, a.err, E_RING) && !*abort);
                 if (!ok) break;
                 const uint32_t dst = smem_u32(ring) + slot * kSlotBytes, bar = full0 + 8 * slot;
                 if (lane == 0) mbar_arrive_expect_tx(bar, n * row_bytes);
@@ -953,7 +954,7 @@ __device__ __forceinline__ float2 norm_of_parts(const uint64_t (&q)[kPartsLane],
     }
     return norm_of(Moments{1.f, mean, sum_lanes(var, lanes)}, eps);
 }
-// Until this block has posted its moments of `unit`.
+// Until this block has posted its moments of `unit`: when to begin to ask for the others'. It orders no memory.
 __device__ __forceinline__ bool wait_posted(const volatile int *posted, int unit, volatile int *stop, int32_t *err)
 {
     const uint64_t t0 = global_timer_ns();
@@ -1002,7 +1003,7 @@ __global__ void __launch_bounds__(kThreads + 96, 2) group_norm_slab_kernel(const
     if (threadIdx.x == 0) {
         for (int i = 0; i < a.buffers; ++i) {
             mbar_init(full0 + 8 * i, 1);
-            mbar_init(empty0 + 8 * i, kSlabThreads / 32);
+            mbar_init(empty0 + 8 * i, 2 * kSlabThreads / 32);  // the warps that sum and those that write
             mbar_init(ready0 + 8 * i, 1);
         }
         abort_flag = 0;
@@ -1018,7 +1019,8 @@ __global__ void __launch_bounds__(kThreads + 96, 2) group_norm_slab_kernel(const
         uint32_t phase = 0;
         for (; u < units; ++u) {
             const int unit = team + u * a.teams, smp = unit / a.slices, c0 = (unit - smp * a.slices) * gs * a.cpg;
-            if (!mbar_wait(empty0 + 8 * b, phase ^ 1u, abort, a.err, E_RING)) break;
+            // nothing after a time-out: those who gave up release buffers that are still being filled
+            if (!mbar_wait(empty0 + 8 * b, phase ^ 1u, abort, a.err, E_RING) || *abort) break;
             mbar_arrive_expect_tx(full0 + 8 * b, buffer_bytes);
             for (int i = 0; i < a.boxes; ++i)
                 tma_load_3d(base + b * buffer_bytes + i * box_bytes, &map, full0 + 8 * b, c0, static_cast<int>(r0) + i * a.box_rows, smp,
@@ -1066,8 +1068,11 @@ __global__ void __launch_bounds__(kThreads + 96, 2) group_norm_slab_kernel(const
             return;
         }
         int b = 0;
+        uint32_t phase = 0;
         for (int u = 0; u < units; ++u) {
             const int of = (team + u * a.teams) * gs;
+            // norm[b] is read no more (and will be before the unit is loaded): orders those reads before the writes below
+            if (!mbar_wait(empty0 + 8 * b, phase ^ 1u, abort, a.err, E_RING)) return;
             if (!wait_posted(&posted, u, abort, a.err)) return;
             if (a.direct) {
                 load_parts(q, a.part + static_cast<long long>(of + min(group, gs - 1)) * a.parts, a.parts, lanes, sub, abort, a.err);
@@ -1080,7 +1085,10 @@ __global__ void __launch_bounds__(kThreads + 96, 2) group_norm_slab_kernel(const
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(ready0 + 8 * b);
-            if (++b == a.buffers) b = 0;
+            if (++b == a.buffers) {
+                b = 0;
+                phase ^= 1u;
+            }
         }
         return;
     }
@@ -1146,6 +1154,10 @@ __global__ void __launch_bounds__(kThreads + 96, 2) group_norm_slab_kernel(const
             if (sub_lane == 0 && sub < gs)
                 st_pair(a.part + (static_cast<long long>(team + u * a.teams) * gs + sub) * a.parts + member, make_float2(mean, m2));
             if (threadIdx.x == 0) posted = u + 1;
+            // the buffer is read (see Cursor::release); behind the posting, which others wait for
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty0 + 8 * b);
             if (++b == a.buffers) {
                 b = 0;
                 phase ^= 1u;
@@ -1155,6 +1167,7 @@ __global__ void __launch_bounds__(kThreads + 96, 2) group_norm_slab_kernel(const
     }
     for (int unit = team; unit < a.units; unit += a.teams) {
         const int smp = unit / a.slices, c0 = (unit - smp * a.slices) * gs * a.cpg;
+        mbar_wait(full0 + 8 * b, phase, abort, a.err, E_RING);  // orders the copy before the reads
         mbar_wait(ready0 + 8 * b, phase, abort, a.err, E_RING);
         float minus[N], scale[VEC], shift[VEC];
         affine_of<VEC, N>(a, col, c0, norm[b], minus, scale, shift);

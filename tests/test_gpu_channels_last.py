@@ -712,3 +712,24 @@ def test_activations_of_the_norm(P, pad, out_dtype, act):
     y = s2b200.group_norm_act(x, 1024, None, v, activation=act, out_dtype=out_dtype)
     want, room = cl.activation_exact(v, act)
     cl.check(y, want.expand(y.shape), room.expand(y.shape), act)
+
+
+# Slices whose blocks turn their buffers over many times with few rows in each: one that reads a buffer before
+# its copy has landed, or after the next was begun, meets another unit's rows.
+@pytest.mark.parametrize("dtype,out_dtype", [(F16, F16), (F32, F32), (F32, BF16)], ids=str)
+@pytest.mark.parametrize("shape", [(2000, 80, 128, 8), (260, 160, 512, 32), (24, 20000, 128, 32), (40, 3600, 512, 32)], ids=str)
+def test_norm_of_slices_hands_its_buffers_over(shape, dtype, out_dtype):
+    S, P, C, G = shape
+    x = _features(shape[:3], _gen(51), dtype)
+    x += torch.arange(S, device="cuda", dtype=F32).remainder(17).to(dtype)[:, None, None]
+    want = s2b200.group_norm_act(x, G, activation="gelu", out_dtype=out_dtype)
+    for s in range(0, S, max(1, S // 60)):
+        cl.check(want[s:s + 1], *cl.norm_exact(x[s:s + 1], G, None, None, 1e-6, "gelu"), f"sample {s}")
+    off = torch.zeros((), dtype=torch.int64, device="cuda")
+    for i in range(60):
+        off += (s2b200.group_norm_act(x, G, activation="gelu", out_dtype=out_dtype) != want).sum()
+    if dtype == out_dtype:
+        for i in range(10):
+            y = x.clone()
+            off += (s2b200.group_norm_act(y, G, activation="gelu", out=y) != want).sum()
+    assert off.item() == 0
