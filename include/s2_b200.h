@@ -423,12 +423,13 @@ typedef enum s2_activation {
  * pivots, joined in order (the same call gives the same bits). x_row, y_row
  * >= channels: elements between positions; x_sample, y_sample: between
  * samples. y may be x itself (same type, pitch and sample stride), and must
- * not overlap it otherwise. The square of a value's distance from the mean
- * must be finite in fp32; a group with a value that is not gives NaN, and no
- * other does. samples or positions 0: nothing is done. At most 1024 groups,
- * 65535 samples and 2^31 positions (S2_UNSUPPORTED beyond). err: device int32
- * error word (may be NULL), set when a bounded wait inside the kernel gives up
- * (96 for the other blocks' moments, 97 for a load). */
+ * not overlap it otherwise. With D the largest distance of a value from its
+ * group's mean and n the group's values, max(n, 256) D^2 must be finite in
+ * fp32; a group beyond that, or with a value that is not finite, gives NaN,
+ * and no other does. samples or positions 0: nothing is done. At most 1024
+ * groups, 65535 samples and 2^31 positions (S2_UNSUPPORTED beyond). err:
+ * device int32 error word (may be NULL), set when a bounded wait inside the
+ * kernel gives up (96 for the other blocks' moments, 97 for a load). */
 typedef struct s2_group_norm_act_desc {
     int samples, channels, groups, activation;
     long long positions;

@@ -143,10 +143,12 @@ __device__ __noinline__ Moments join_parts(const float2 *part, int pitch, int pa
     return join_lanes(join(join(chain[0], chain[1]), join(chain[2], chain[3])), group_lanes);
 }
 
-// mean and 1 / sigma of a group
+// mean and 1 / sigma of a group; 1 / sigma is NaN, and with it the group's output, where the squares have
+// overflowed (1 / sqrt(inf) = 0 would make it act(bias))
 __device__ __forceinline__ float2 norm_of(const Moments &m, float eps)
 {
-    return make_float2(m.mean, __frsqrt_rn(__fdiv_rn(m.m2, m.n) + eps));
+    const float v = __fdiv_rn(m.m2, m.n);
+    return make_float2(m.mean, v <= 3.402823466e38f ? __frsqrt_rn(v + eps) : __int_as_float(0x7fffffff));
 }
 
 // VEC elements of T as they are loaded: 16 bytes or one element
@@ -255,7 +257,8 @@ struct Run {
             Moments run;
             run.n = cnt;
             run.mean = fmaf(sum[e], inv, p[e]);
-            // not below 0 by rounding; 0 * sq keeps the NaN of a value that is not finite
+            // not below 0 by rounding; 0 * sq keeps the NaN of a value that is not finite (squares that overflow
+            // leave inf)
             run.m2 = fmaxf(fmaf(-sum[e] * inv, sum[e], sq[e]), 0.f * sq[e]);
             mo[e] = join(mo[e], run);
         }

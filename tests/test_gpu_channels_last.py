@@ -733,3 +733,51 @@ def test_norm_of_slices_hands_its_buffers_over(shape, dtype, out_dtype):
             y = x.clone()
             off += (s2b200.group_norm_act(y, G, activation="gelu", out=y) != want).sum()
     assert off.item() == 0
+
+
+# ---- values near fp32's range ------------------------------------------------------------
+
+# rows held by a block, a cluster and (on 4 bytes) a grid; slices joined by each block and by one; the ring
+RANGE_SHAPES = [(2, 8, 64, 8), (2, 1500, 512, 32), (1, 60000, 130, 10), (40, 3600, 512, 32), (3, 20001, 512, 32),
+                (1, 140000, 512, 32), (1, 300000, 64, 8)]
+
+
+@pytest.mark.parametrize("dtype,out_dtype", [(F32, F32), (BF16, BF16), (F32, F16)], ids=str)
+@pytest.mark.parametrize("how", ["outlier", "first", "spread"])
+@pytest.mark.parametrize("shape", RANGE_SHAPES, ids=str)
+def test_norm_of_squares_that_overflow(shape, how, dtype, out_dtype):
+    """A group whose squares add up beyond fp32 is NaN, all of it; the others do not notice."""
+    S, P, C, G = shape
+    x = _features(shape[:3], _gen(61), dtype)
+    y0 = s2b200.group_norm_act(x, G, activation="relu", out_dtype=out_dtype)
+    g, k = G - 1, C // G
+    if how == "spread":  # n D^2 beyond 3.4e38, each square below
+        x[S - 1, :, g * k:(g + 1) * k] *= 4e18 / x[S - 1, :, g * k:(g + 1) * k].abs().max().item()
+        x[S - 1, 0, g * k] = -8e18
+        x[S - 1, P - 1, g * k] = 8e18
+        x[S - 1, P // 2, g * k:(g + 1) * k] = 1.2e19
+        x[S - 1, P // 3, g * k:(g + 1) * k] = -1.2e19
+    else:
+        x[S - 1, 0 if how == "first" else P // 2 + 1, g * k + k // 2] = 1e20
+    y = s2b200.group_norm_act(x, G, activation="relu", out_dtype=out_dtype)
+    assert torch.isnan(y[S - 1, :, g * k:(g + 1) * k]).all()
+    y[S - 1, :, g * k:(g + 1) * k] = y0[S - 1, :, g * k:(g + 1) * k]
+    assert torch.equal(y, y0)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+@pytest.mark.parametrize("shape", RANGE_SHAPES, ids=str)
+def test_norm_of_large_values_that_do_not(shape, dtype):
+    """max(n, 256) D^2 just within fp32: D = 6 spreads at most.
+
+    The mean of these is about 0, but what its joins round are the means m_i of the parts, by 2^-24 |m_i| each and at
+    most 24 times: weighted with n_i / n that is at most 24 2^-24 mean |x| <= 24 2^-24 sqrt(m^2 + sigma^2), so 24 2^-24
+    of sigma comes on top of norm_exact's room, whose term is 2^-18 |m| alone: in z 24 2^-24 sigma / sigma."""
+    S, P, C, G = shape
+    x = _normal(shape[:3], _gen(62)).clamp(-5.9, 5.9)
+    scale = (3e38 / max(P * C // G, 256)) ** 0.5 / 6
+    x = (x * scale).to(dtype)
+    y = s2b200.group_norm_act(x, G)
+    for s in {0, S - 1}:
+        want, room = cl.norm_exact(x[s:s + 1], G, None, None, 1e-6, "none")
+        cl.check(y[s:s + 1], want, room + 24 * 2.0 ** -24)
