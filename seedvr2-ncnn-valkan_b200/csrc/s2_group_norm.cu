@@ -1150,7 +1150,7 @@ __global__ void __launch_bounds__(kThreads + 96, 2) group_norm_slab_kernel(const
             const float mean = p0 + sum_lanes(sum, a.group_lanes);
             for (int k = sub_lane; k < entries; k += a.group_lanes) {
                 const float d = of[k].x - mean;
-                m2 += fmaf(d * d, share[k] * n, of[k].y);
+                if (share[k] > 0.f) m2 += fmaf(d * d, share[k] * n, of[k].y);  // not 0 * inf for lanes without rows
             }
             __syncwarp();
             m2 = sum_lanes(m2, a.group_lanes);

@@ -781,3 +781,15 @@ def test_norm_of_large_values_that_do_not(shape, dtype):
     for s in {0, S - 1}:
         want, room = cl.norm_exact(x[s:s + 1], G, None, None, 1e-6, "none")
         cl.check(y[s:s + 1], want, room + 24 * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+# the last two: a last part with one row, and lanes without any
+@pytest.mark.parametrize("shape", sorted(set(SLICES + RANGE_SHAPES)) + [(1, 20061, 128, 32), (1, 20061, 512, 32)], ids=str)
+def test_norm_about_a_huge_mean(shape, dtype):
+    """The mean's own square may be beyond fp32: only distances count."""
+    S, P, C, G = shape
+    b = torch.linspace(-1, 1, C, device="cuda")
+    x = torch.full(shape[:3], 1e20, device="cuda", dtype=dtype)
+    y = s2b200.group_norm_act(x, G, None, b)
+    assert torch.equal(y, b.to(dtype).expand_as(y))
