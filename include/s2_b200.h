@@ -816,6 +816,11 @@ S2_API s2_status s2_debug_fail_allocations(int n);
  * device-error query returns S2_INFERENCE_FAILED, its TMEM is freed, and
  * launches after it are unaffected. */
 S2_API s2_status s2_debug_attention_fault(int skip_k_tile, unsigned long long wait_ns);
+/* One shot, for the next s2_group_norm_act launch in the process: its blocks
+ * wait for one another's moments for wait_ns at most (0 = the default 1 s).
+ * With a limit that they cannot keep the launch ends on its own, y wrong, its
+ * error word 96, and launches after it are unaffected. */
+S2_API s2_status s2_debug_norm_wait(unsigned long long wait_ns);
 
 /* ---- misc ---------------------------------------------------------------- */
 

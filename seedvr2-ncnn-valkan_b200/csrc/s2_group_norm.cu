@@ -74,6 +74,7 @@ struct GnArgs {
     // moments, [unit][group][part], and norms have all bits set until they are written
     float2 *part, *norm;
     uint32_t *arrived, *ready;
+    unsigned long long join_ns;  // how long a wait for the other parts may take
 };
 
 struct Moments {
@@ -506,13 +507,13 @@ __device__ __forceinline__ uint32_t ld_acquire(const uint32_t *p)
 // device error codes: the wait for the other parts of a unit, for the ring's loads
 enum : int { E_JOIN = 96, E_RING = 97 };
 
-// Waits until *p is `value`; bounded, and *stop ends it.
-__device__ __forceinline__ bool wait_value(const uint32_t *p, uint32_t value, volatile int *stop, int32_t *err)
+// Waits until *p is `value`; for `most` ns, and *stop ends it.
+__device__ __forceinline__ bool wait_value(const uint32_t *p, uint32_t value, volatile int *stop, int32_t *err, uint64_t most)
 {
     if (ld_acquire(p) == value) return true;
     const uint64_t t0 = global_timer_ns();
     while (ld_acquire(p) != value)
-        if (*stop || global_timer_ns() - t0 > kWaitTimeoutNs) {
+        if (*stop || global_timer_ns() - t0 > most) {
             if (err) atomicCAS(err, 0, E_JOIN);
             *stop = 1;
             return false;
@@ -552,7 +553,7 @@ __device__ __forceinline__ void join_grid(const GnArgs &a, int unit, int member,
             atomicExch(a.ready + unit, 1u);
         }
     } else {
-        if (threadIdx.x == 0) wait_value(a.ready + unit, 1, stop, a.err);
+        if (threadIdx.x == 0) wait_value(a.ready + unit, 1, stop, a.err, a.join_ns);
         sync();
         if (threadIdx.x < gs) norm[threadIdx.x] = __ldcg(joined + threadIdx.x);
         sync();
@@ -797,13 +798,12 @@ __global__ void __launch_bounds__(kThreads + 32, 2) group_norm_ring_kernel(const
                 }
             }
         }
-        if (!ok) {
-            // no copy may still be landing when the block ends: wait for the slots' last loads
-            int dummy = 0;
-            for (uint32_t k = 0; k < kSlots && k < issued; ++k) {
-                const uint32_t q = issued - 1 - k;
-                mbar_wait(full0 + 8 * (q % kSlots), (q / kSlots) & 1u, &dummy, a.err, E_RING);
-            }
+        // No copy may still be landing when the block ends: wait for the slots' last loads. (After a time-out nobody
+        // else may have, also when all were issued before.)
+        int dummy = 0;
+        for (uint32_t k = 0; k < kSlots && k < issued; ++k) {
+            const uint32_t q = issued - 1 - k;
+            mbar_wait(full0 + 8 * (q % kSlots), (q / kSlots) & 1u, &dummy, a.err, E_RING);
         }
         return;
     }
@@ -906,12 +906,12 @@ __device__ __forceinline__ void st_pair(float2 *p, float2 f)
     const uint64_t v = pair(f.x != f.x ? __uint_as_float(0x7fffffffu) : f.x, f.y);
     asm volatile("st.relaxed.gpu.global.b64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
 }
-__device__ __forceinline__ void wait_pair(uint64_t &v, const float2 *p, volatile int *stop, int32_t *err)
+__device__ __forceinline__ void wait_pair(uint64_t &v, const float2 *p, volatile int *stop, int32_t *err, uint64_t most)
 {
     if (v != ~0ull) return;
     const uint64_t t0 = global_timer_ns();
     while ((v = ld_pair(p)) == ~0ull)
-        if (*stop || global_timer_ns() - t0 > kWaitTimeoutNs) {
+        if (*stop || global_timer_ns() - t0 > most) {
             if (err) atomicCAS(err, 0, E_JOIN);
             *stop = 1;
             return;
@@ -920,7 +920,7 @@ __device__ __forceinline__ void wait_pair(uint64_t &v, const float2 *p, volatile
 // A group's moments of all parts, by `lanes` neighbouring lanes (`sub` of them): part sub + k lanes in q[k], part 0's
 // past the last; returns when all are written.
 __device__ __forceinline__ void load_parts(uint64_t (&q)[kPartsLane], const float2 *part, int parts, int lanes, int sub,
-                                           volatile int *stop, int32_t *err)
+                                           volatile int *stop, int32_t *err, uint64_t most)
 {
     const uint64_t t0 = global_timer_ns();
     for (;;) {
@@ -933,7 +933,7 @@ __device__ __forceinline__ void load_parts(uint64_t (&q)[kPartsLane], const floa
 #pragma unroll
         for (int k = 0; k < kPartsLane; ++k) all = all && q[k] != ~0ull;
         if (__all_sync(0xffffffffu, all)) return;
-        if (__any_sync(0xffffffffu, *stop || global_timer_ns() - t0 > kWaitTimeoutNs)) {
+        if (__any_sync(0xffffffffu, *stop || global_timer_ns() - t0 > most)) {
             if (err) atomicCAS(err, 0, E_JOIN);
             *stop = 1;
             return;
@@ -958,13 +958,13 @@ __device__ __forceinline__ float2 norm_of_parts(const uint64_t (&q)[kPartsLane],
     return norm_of(Moments{1.f, mean, sum_lanes(var, lanes)}, eps);
 }
 // Until this block has posted its moments of `unit`: when to begin to ask for the others'. It orders no memory.
-__device__ __forceinline__ bool wait_posted(const volatile int *posted, int unit, volatile int *stop, int32_t *err)
+__device__ __forceinline__ bool wait_posted(const volatile int *posted, int unit, volatile int *stop, int32_t *err, uint64_t most)
 {
     const uint64_t t0 = global_timer_ns();
     while (*posted <= unit) {
         __nanosleep(100);
         if (*stop) return false;
-        if (global_timer_ns() - t0 > kWaitTimeoutNs) {
+        if (global_timer_ns() - t0 > most) {
             if (err) atomicCAS(err, 0, E_JOIN);
             *stop = 1;
             return false;
@@ -1038,12 +1038,10 @@ __global__ void __launch_bounds__(kThreads + 96, 2) group_norm_slab_kernel(const
                 phase ^= 1u;
             }
         }
-        if (u < units) {
-            // no copy may still be landing when the block ends: wait for the buffers' last loads
-            int dummy = 0;
-            for (int k = max(0, u - a.buffers); k < u; ++k)
-                mbar_wait(full0 + 8 * (k % a.buffers), k / a.buffers & 1, &dummy, a.err, E_RING);
-        }
+        // no copy may still be landing when the block ends (see group_norm_ring_kernel): wait for the buffers' last loads
+        int dummy = 0;
+        for (int k = max(0, u - a.buffers); k < u; ++k)
+            mbar_wait(full0 + 8 * (k % a.buffers), k / a.buffers & 1, &dummy, a.err, E_RING);
         return;
     }
     if (warp > kThreads / 32) {
@@ -1063,8 +1061,8 @@ __global__ void __launch_bounds__(kThreads + 96, 2) group_norm_slab_kernel(const
             // the units' groups go round the team's blocks
             for (int turn = member; turn < units * gs; turn += a.parts) {
                 const int u = turn / gs, of = (team + u * a.teams) * gs + turn - u * gs;
-                if (!wait_posted(&posted, u, abort, a.err)) return;
-                load_parts(q, a.part + static_cast<long long>(of) * a.parts, a.parts, lanes, sub, abort, a.err);
+                if (!wait_posted(&posted, u, abort, a.err, a.join_ns)) return;
+                load_parts(q, a.part + static_cast<long long>(of) * a.parts, a.parts, lanes, sub, abort, a.err, a.join_ns);
                 const float2 r = norm_of_parts(q, w, lanes, inv_n, a.eps);
                 if (lane == 0) st_pair(a.norm + of, r);
             }
@@ -1076,14 +1074,14 @@ __global__ void __launch_bounds__(kThreads + 96, 2) group_norm_slab_kernel(const
             const int of = (team + u * a.teams) * gs;
             // norm[b] is read no more (and will be before the unit is loaded): orders those reads before the writes below
             if (!mbar_wait(empty0 + 8 * b, phase ^ 1u, abort, a.err, E_RING)) return;
-            if (!wait_posted(&posted, u, abort, a.err)) return;
+            if (!wait_posted(&posted, u, abort, a.err, a.join_ns)) return;
             if (a.direct) {
-                load_parts(q, a.part + static_cast<long long>(of + min(group, gs - 1)) * a.parts, a.parts, lanes, sub, abort, a.err);
+                load_parts(q, a.part + static_cast<long long>(of + min(group, gs - 1)) * a.parts, a.parts, lanes, sub, abort, a.err, a.join_ns);
                 const float2 r = norm_of_parts(q, w, lanes, inv_n, a.eps);
                 if (sub == 0 && group < gs) norm[b][group] = r;
             } else if (lane < gs) {
                 uint64_t v = ld_pair(a.norm + of + lane);
-                wait_pair(v, a.norm + of + lane, abort, a.err);
+                wait_pair(v, a.norm + of + lane, abort, a.err, a.join_ns);
                 norm[b][lane] = floats_of(v);
             }
             __syncwarp();
@@ -1524,6 +1522,7 @@ extern "C" s2_status s2_group_norm_act(void *stream, const s2_group_norm_act_des
     a.group_lanes = 32;
     while (a.group_lanes * p.slice_groups > (p.slab ? kSlabThreads : kThreads)) a.group_lanes /= 2;
     a.eps = d->eps;
+    a.join_ns = s2::take_norm_wait();
     if (p.join == kGrid) {
         a.arrived = static_cast<uint32_t *>(d->workspace);
         a.ready = a.arrived + p.units;

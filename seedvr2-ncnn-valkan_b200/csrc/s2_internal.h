@@ -39,6 +39,8 @@ s2_status shard_exchange_maps(int T, int H, int W, int wt, int wh, int ww, int t
 // s2_window_attention launch its K tile to leave out (-1: none) and its wait
 // limit, then resets both (one shot).
 void take_attention_fault(int *skip_k, unsigned long long *wait_ns);
+// The same for s2_debug_norm_wait: the wait limit of the next s2_group_norm_act launch.
+unsigned long long take_norm_wait();
 
 // Attention core tiling shared by the planner and the kernel.
 constexpr int kTileM = 128;   // query rows per Q tile (one TMEM lane per row)

@@ -449,6 +449,7 @@ namespace {
 std::atomic<int> g_fail_allocs{0};
 std::atomic<int> g_fault_skip_k{-1};
 std::atomic<unsigned long long> g_fault_wait_ns{0};
+std::atomic<unsigned long long> g_norm_wait_ns{0};
 }  // namespace
 
 namespace s2 {
@@ -466,6 +467,13 @@ void take_attention_fault(int *skip_k, unsigned long long *wait_ns)
     const unsigned long long w = g_fault_wait_ns.exchange(0);
     *wait_ns = w ? w : 1000000000ull;  // the default limit: 1 s
 }
+
+unsigned long long take_norm_wait()
+{
+    // every call comes here: the store only when there is something to take
+    const unsigned long long w = g_norm_wait_ns.load(std::memory_order_relaxed) ? g_norm_wait_ns.exchange(0) : 0;
+    return w ? w : 1000000000ull;
+}
 }  // namespace s2
 
 extern "C" s2_status s2_debug_fail_allocations(int n)
@@ -481,3 +489,8 @@ extern "C" s2_status s2_debug_attention_fault(int skip_k_tile, unsigned long lon
     return S2_OK;
 }
 
+extern "C" s2_status s2_debug_norm_wait(unsigned long long wait_ns)
+{
+    g_norm_wait_ns.store(wait_ns);
+    return S2_OK;
+}

@@ -253,6 +253,7 @@ _SIGS = {
     "s2_linear_act": (ctypes.c_int, [_vp, _vp, _vp]),
     "s2_debug_fail_allocations": (ctypes.c_int, [ctypes.c_int]),
     "s2_debug_attention_fault": (ctypes.c_int, [ctypes.c_int, ctypes.c_ulonglong]),
+    "s2_debug_norm_wait": (ctypes.c_int, [ctypes.c_ulonglong]),
     "s2_last_error": (ctypes.c_char_p, []),
     "s2_device_check": (ctypes.c_int, [ctypes.c_int]),
     "s2_version": (ctypes.c_int, []),

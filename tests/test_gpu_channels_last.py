@@ -793,3 +793,32 @@ def test_norm_about_a_huge_mean(shape, dtype):
     x = torch.full(shape[:3], 1e20, device="cuda", dtype=dtype)
     y = s2b200.group_norm_act(x, G, None, b)
     assert torch.equal(y, b.to(dtype).expand_as(y))
+
+
+# ---- waits that run out --------------------------------------------------------------------
+
+# blocks that wait for one another: slices joined by each block and by one, rows on 4 bytes on a grid, the ring
+WAITING = [((40, 3600, 512, 32), F16, 0), ((3, 20001, 512, 32), F16, 0), ((1, 60000, 130, 10), F32, 1),
+           ((1, 140000, 512, 32), BF16, 0)]
+
+
+@pytest.mark.parametrize("shape,dtype,pad", WAITING, ids=str)
+def test_norm_wait_that_runs_out(shape, dtype, pad):
+    """A limit of 1 ns that no block can keep: the kernel ends, says so, writes y's rows only, and the next call is
+    right."""
+    import time
+    x = _padded(_features(shape[:3], _gen(71), dtype), pad)[1]
+    want = s2b200.group_norm_act(x, shape[3], activation="silu")
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    buf, out = _padded(torch.zeros_like(want), 8)
+    torch.cuda.synchronize()
+    t0 = time.perf_counter()
+    s2b200.lib().s2_debug_norm_wait(1)
+    s2b200.group_norm_act(x, shape[3], activation="silu", out=out, err=err)
+    assert err.item() == 96
+    assert time.perf_counter() - t0 < 0.5
+    assert torch.isnan(buf[..., shape[2]:]).all()
+    err.zero_()
+    for _ in range(3):
+        assert torch.equal(s2b200.group_norm_act(x, shape[3], activation="silu", err=err), want)
+    assert err.item() == 0
