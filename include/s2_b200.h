@@ -398,7 +398,15 @@ S2_API s2_status s2_gemm(void *stream, const s2_gemm_desc *desc, int *extra_laun
  * stream-ordered and capturable, allocate nothing and keep nothing between
  * calls: the caller passes a workspace of at least *_workspace_bytes(desc)
  * bytes, 16-byte aligned (its contents do not matter; calls that may overlap
- * need one each). *launches (may be NULL) receives the kernels launched. */
+ * need one each). *launches (may be NULL) receives the kernels launched.
+ *
+ * A kernel whose blocks wait for one another or for a copy does so for 1 s at
+ * most; then it ends, y is wrong, and the call's error word `err` (device
+ * int32, zeroed by the caller) receives a code. Calls with err NULL share one
+ * word of the device: s2_operator_device_error waits for the current device,
+ * gives that word's code (0 = ok) and clears it, and returns
+ * S2_INFERENCE_FAILED when it was set or the device failed. */
+S2_API s2_status s2_operator_device_error(int *code);
 
 /* Activations: relu max(v, 0); silu v / (1 + e^-v); gelu v (1 + erf(v /
  * sqrt 2)) / 2; gelu_tanh v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) / 2.
@@ -427,9 +435,8 @@ typedef enum s2_activation {
  * group's mean and n the group's values, max(n, 256) D^2 must be finite in
  * fp32; a group beyond that, or with a value that is not finite, gives NaN,
  * and no other does. samples or positions 0: nothing is done. At most 1024
- * groups, 65535 samples and 2^31 positions (S2_UNSUPPORTED beyond). err:
- * device int32 error word (may be NULL), set when a bounded wait inside the
- * kernel gives up (96 for the other blocks' moments, 97 for a load). */
+ * groups, 65535 samples and 2^31 positions (S2_UNSUPPORTED beyond). err's
+ * codes: 96 for a wait for the other blocks' moments, 97 for a load. */
 typedef struct s2_group_norm_act_desc {
     int samples, channels, groups, activation;
     long long positions;
@@ -457,7 +464,7 @@ S2_API s2_status s2_group_norm_act(void *stream, const s2_group_norm_act_desc *d
  * activation and residual are applied to the fp32 sum, and y is rounded once.
  * y may be residual itself (same pitch) and must not overlap any input
  * otherwise. One row needs no workspace, whatever the alignment. M up to 2^30,
- * N and K up to 2^21. M 0: nothing is done. err as above (80 to 85). */
+ * N and K up to 2^21. M 0: nothing is done. err's codes: 80 to 85. */
 typedef struct s2_linear_act_desc {
     int N, K, activation;
     int dtype, out_dtype; /* s2_dtype */

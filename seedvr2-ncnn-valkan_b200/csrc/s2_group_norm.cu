@@ -34,6 +34,7 @@
 #include "s2_gemm.h"
 #include "s2_internal.h"
 #include "s2_launch.h"
+#include "s2_operator_error.h"
 #include "s2_overlap.h"
 #include "s2_sm100.cuh"
 
@@ -1497,7 +1498,7 @@ extern "C" s2_status s2_group_norm_act(void *stream, const s2_group_norm_act_des
     a.y = d->y;
     a.weight = d->weight;
     a.bias = d->bias;
-    a.err = d->err;
+    a.err = d->err ? d->err : s2::operator_error_word();
     a.P = d->positions;
     a.part_rows = p.part_rows;
     a.x_row = d->x_row;

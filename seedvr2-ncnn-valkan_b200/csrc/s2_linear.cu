@@ -28,6 +28,7 @@
 #include "s2_gemm.h"
 #include "s2_internal.h"
 #include "s2_launch.h"
+#include "s2_operator_error.h"
 #include "s2_overlap.h"
 #include "s2_sm100.cuh"
 
@@ -934,7 +935,7 @@ extern "C" s2_status s2_linear_act(void *stream, const s2_linear_act_desc *d, in
              (d->residual ? d->ldr * oe : 0)) % 16 == 0;
     a.ks = 1;
     a.packed = 0;
-    a.err = d->err;
+    a.err = d->err ? d->err : s2::operator_error_word();
     int dev = 0, sms = 148;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);

@@ -251,6 +251,7 @@ _SIGS = {
     "s2_group_norm_act": (ctypes.c_int, [_vp, _vp, _vp]),
     "s2_linear_act_workspace_bytes": (ctypes.c_size_t, [_vp]),
     "s2_linear_act": (ctypes.c_int, [_vp, _vp, _vp]),
+    "s2_operator_device_error": (ctypes.c_int, [_i32p]),
     "s2_debug_fail_allocations": (ctypes.c_int, [ctypes.c_int]),
     "s2_debug_attention_fault": (ctypes.c_int, [ctypes.c_int, ctypes.c_ulonglong]),
     "s2_debug_norm_wait": (ctypes.c_int, [ctypes.c_ulonglong]),
@@ -1071,7 +1072,8 @@ def group_norm_act(x, groups: int, weight=None, bias=None, eps: float = 1e-6, ac
     CUDA tensor (fp16, bf16 or fp32, positions at any one pitch); per sample and group of
     channels / groups consecutive channels, y = act((x - mean) / sqrt(var + eps) * weight + bias).
     weight, bias: fp32 [channels] or None. Returns y in out_dtype (x's, or fp16 / bf16 for fp32 x)
-    in x's shape; `out` receives it when given (it may be x). err: device int32 error word."""
+    in x's shape; `out` receives it when given (it may be x). err: device int32 error word, the
+    device's own (operator_device_error) by default."""
     torch = _torch()
     index = x.get_device()
     if stream is not None or index < 0 or index != torch.cuda.current_device():
@@ -1116,7 +1118,8 @@ def linear_act(x, w, bias=None, activation: str = "none", residual=None, out=Non
     """y = act(x w^T + bias) + residual (s2_linear_act): x [..., K] and w [N, K] CUDA tensors of one
     type (fp16 or bf16, rows of any pitch), bias fp32 [N] or None, residual [..., N] in the
     output's type or None. Returns y [..., N] in out_dtype (x's, or fp32); `out` receives it when
-    given (it may be the residual). err: device int32 error word."""
+    given (it may be the residual). err: device int32 error word, the device's own
+    (operator_device_error) by default."""
     torch = _torch()
     index = x.get_device()
     if stream is not None or index < 0 or index != torch.cuda.current_device():
@@ -1159,6 +1162,19 @@ def linear_act(x, w, bias=None, activation: str = "none", residual=None, out=Non
     L = _lib or lib()
     _run_desc(L.s2_linear_act, L.s2_linear_act_workspace_bytes, LinearActDesc, d, x, index, "s2_linear_act")
     return out
+
+
+def operator_device_error(device=None) -> int:
+    """The code of a wait that gave up in a group_norm_act or linear_act call without `err` on `device`
+    (the current one by default) since the last time this was asked, 0 if none did
+    (s2_operator_device_error). Such a call's result is wrong. Waits for the device."""
+    torch = _torch()
+    code = ctypes.c_int32(0)
+    with torch.cuda.device(device):
+        status = lib().s2_operator_device_error(ctypes.byref(code))
+    if status != S2_OK and code.value == 0:
+        _check(status, "s2_operator_device_error")
+    return code.value
 
 
 VAE_WEIGHT_ORDER = ("norm_bias", "norm_weight", "k_bias", "k_weight", "out_bias", "out_weight", "q_bias", "q_weight",

@@ -120,3 +120,12 @@ def test_packed_descriptions_match_the_structures():
         names = [n for n, _ in cls._fields_]
         got = cls.from_buffer_copy(layout.pack(*range(1, len(names) + 1)))
         assert [int(getattr(got, n)) for n in names] == list(range(1, len(names) + 1))
+
+
+def test_device_error_without_a_device():
+    """Asked where no device can answer: an error, not a code."""
+    if torch.cuda.is_available():
+        pytest.skip("there is a device")
+    code = ctypes.c_int32(7)
+    assert s2b200.lib().s2_operator_device_error(ctypes.byref(code)) == s2b200.S2_INFERENCE_FAILED and code.value == 0
+    assert s2b200.lib().s2_operator_device_error(None) == s2b200.S2_INFERENCE_FAILED

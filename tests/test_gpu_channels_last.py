@@ -822,3 +822,55 @@ def test_norm_wait_that_runs_out(shape, dtype, pad):
     for _ in range(3):
         assert torch.equal(s2b200.group_norm_act(x, shape[3], activation="silu", err=err), want)
     assert err.item() == 0
+
+
+def test_waits_that_run_out_without_a_word_are_asked_for():
+    """A call without `err`: the device's own word says so once, and only for what ran on it."""
+    assert s2b200.operator_device_error() == 0
+    shape, dtype, _ = WAITING[1]
+    x = _features(shape[:3], _gen(72), dtype)
+    want = s2b200.group_norm_act(x, shape[3])
+    torch.cuda.synchronize()
+    s2b200.lib().s2_debug_norm_wait(1)
+    s2b200.group_norm_act(x, shape[3])
+    assert s2b200.operator_device_error("cuda:0") == 96
+    assert s2b200.operator_device_error() == 0
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    s2b200.lib().s2_debug_norm_wait(1)
+    s2b200.group_norm_act(x, shape[3], err=err)
+    assert err.item() == 96 and s2b200.operator_device_error() == 0
+    assert torch.equal(s2b200.group_norm_act(x, shape[3]), want)
+    s2b200.linear_act(x[0, :300, :512], x[1, :512, :512])
+    assert s2b200.operator_device_error() == 0
+
+
+_CAPTURED_FIRST = r"""
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch, s2b200
+x = torch.randn(3, 20001, 512, device="cuda").half()
+w = torch.randn(512, 512, device="cuda").half()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    y = s2b200.group_norm_act(x, 32, activation="silu")
+    z = s2b200.linear_act(y, w)
+    v = s2b200.linear_act(y[0, :1], w)
+    u = s2b200.linear_act(y[0, :40, :511], w[:, :511])
+y.zero_(), z.zero_(), v.zero_(), u.zero_()
+g.replay()
+torch.cuda.synchronize()
+a = s2b200.group_norm_act(x, 32, activation="silu")
+assert torch.equal(a, y) and torch.equal(s2b200.linear_act(a, w), z) and torch.equal(s2b200.linear_act(a[0, :1], w), v)
+assert torch.equal(s2b200.linear_act(a[0, :40, :511], w[:, :511]), u)
+assert s2b200.operator_device_error() == 0
+print("done")
+"""
+
+
+def test_first_calls_of_a_process_inside_a_capture():
+    import os
+    import subprocess
+    import sys
+    r = subprocess.run([sys.executable, "-c", _CAPTURED_FIRST, os.path.dirname(os.path.dirname(s2b200.__file__))],
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "done" in r.stdout, r.stderr
