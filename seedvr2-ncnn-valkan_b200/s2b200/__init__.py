@@ -1014,6 +1014,8 @@ def _pitch(t, first: int, what: str):
     if len(shape) == first + 2 and strides[-1] == 1:
         size = shape[first]
         return size, (strides[first] if size != 1 else last)
+    if 0 in shape[first:-1]:
+        return 0, last  # no rows, whatever the strides of those that could be
     if strides[-1] != 1 and last > 1:
         _fail(f"{what}: the last dimension must be contiguous")
     rows, pitch = 1, None

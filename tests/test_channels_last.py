@@ -129,3 +129,13 @@ def test_device_error_without_a_device():
     code = ctypes.c_int32(7)
     assert s2b200.lib().s2_operator_device_error(ctypes.byref(code)) == s2b200.S2_INFERENCE_FAILED and code.value == 0
     assert s2b200.lib().s2_operator_device_error(None) == s2b200.S2_INFERENCE_FAILED
+
+
+EMPTY = [(0, 64), (3, 0, 64), (0, 3, 64), (2, 3, 0, 64), (2, 0, 3, 64), (2, 0, 0, 64)]
+
+
+@pytest.mark.parametrize("shape", EMPTY, ids=str)
+def test_pitch_of_no_rows(shape):
+    assert s2b200._pitch(torch.empty(shape), 0, "x")[0] == 0
+    assert s2b200._pitch(torch.empty((5,) + shape), 1, "x")[0] == 0
+    assert s2b200._pitch(torch.empty(shape[:-1] + (128,))[..., ::2], 0, "x")[0] == 0

@@ -874,3 +874,14 @@ def test_first_calls_of_a_process_inside_a_capture():
     r = subprocess.run([sys.executable, "-c", _CAPTURED_FIRST, os.path.dirname(os.path.dirname(s2b200.__file__))],
                        capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "done" in r.stdout, r.stderr
+
+
+@pytest.mark.parametrize("shape", [(0, 64), (3, 0, 64), (0, 3, 64), (2, 3, 0, 64), (2, 0, 3, 64)], ids=str)
+def test_no_rows_of_any_shape(shape):
+    x = torch.empty(shape, device="cuda", dtype=F16)
+    w = torch.ones(32, 64, device="cuda", dtype=F16)
+    y = s2b200.linear_act(x, w, residual=torch.empty(shape[:-1] + (32,), device="cuda", dtype=F16))
+    assert y.shape == shape[:-1] + (32,)
+    assert s2b200.linear_act(x, w, out=y) is y
+    assert s2b200.group_norm_act(x, 8).shape == shape
+    assert s2b200.group_norm_act(x[None], 8, out=torch.empty_like(x[None])).shape == (1,) + shape
