@@ -1049,6 +1049,13 @@ _NORM_LAYOUT = struct.Struct("@iiiiqiifPqqPPPqqPNP")
 _LINEAR_LAYOUT = struct.Struct("@iiiiiqPqPqPPqPqPNP")
 
 
+def _pack(layout, *values) -> bytes:
+    try:
+        return layout.pack(*values)
+    except (struct.error, OverflowError) as e:
+        _fail(f"a size or number that the call cannot take: {e}")
+
+
 def _run_desc(call, workspace_bytes, desc_type, packed: bytes, x, index: int, what: str):
     """Calls on the current stream of the current device; a call that is refused for want of a
     workspace is given one of that stream's."""
@@ -1104,11 +1111,11 @@ def group_norm_act(x, groups: int, weight=None, bias=None, eps: float = 1e-6, ac
         y_row = _pitch(out, 1, "out")[1]
         y_sample = out.stride(0)
         out_type = _type_of(out, "out")
-    d = _NORM_LAYOUT.pack(samples, channels, groups, code, positions, in_type, out_type, eps, x.data_ptr(), x_row,
-                          x.stride(0) if samples > 1 else 0,
-                          0 if weight is None else _need_vector(weight, channels, index, "weight"),
-                          0 if bias is None else _need_vector(bias, channels, index, "bias"), out.data_ptr(), y_row,
-                          y_sample, 0, 0, 0 if err is None else _need_err(err, index))
+    d = _pack(_NORM_LAYOUT, samples, channels, groups, code, positions, in_type, out_type, eps, x.data_ptr(), x_row,
+              x.stride(0) if samples > 1 else 0,
+              0 if weight is None else _need_vector(weight, channels, index, "weight"),
+              0 if bias is None else _need_vector(bias, channels, index, "bias"), out.data_ptr(), y_row,
+              y_sample, 0, 0, 0 if err is None else _need_err(err, index))
     L = _lib or lib()
     _run_desc(L.s2_group_norm_act, L.s2_group_norm_act_workspace_bytes, GroupNormActDesc, d, x, index,
               "s2_group_norm_act")
@@ -1158,9 +1165,9 @@ def linear_act(x, w, bias=None, activation: str = "none", residual=None, out=Non
         if residual.requires_grad:
             _need_no_grad()
         res, ldr = residual.data_ptr(), _pitch(residual, 0, "residual")[1]
-    d = _LINEAR_LAYOUT.pack(N, K, code, in_type, out_type, rows, x.data_ptr(), ldx, w.data_ptr(), ldw,
-                            0 if bias is None else _need_vector(bias, N, index, "bias"), res, ldr, out.data_ptr(),
-                            ldy, 0, 0, 0 if err is None else _need_err(err, index))
+    d = _pack(_LINEAR_LAYOUT, N, K, code, in_type, out_type, rows, x.data_ptr(), ldx, w.data_ptr(), ldw,
+              0 if bias is None else _need_vector(bias, N, index, "bias"), res, ldr, out.data_ptr(),
+              ldy, 0, 0, 0 if err is None else _need_err(err, index))
     L = _lib or lib()
     _run_desc(L.s2_linear_act, L.s2_linear_act_workspace_bytes, LinearActDesc, d, x, index, "s2_linear_act")
     return out

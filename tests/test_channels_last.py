@@ -139,3 +139,13 @@ def test_pitch_of_no_rows(shape):
     assert s2b200._pitch(torch.empty(shape), 0, "x")[0] == 0
     assert s2b200._pitch(torch.empty((5,) + shape), 1, "x")[0] == 0
     assert s2b200._pitch(torch.empty(shape[:-1] + (128,))[..., ::2], 0, "x")[0] == 0
+
+
+@pytest.mark.parametrize("at,value", [(2, 1 << 40), (2, 8.0), (0, 1 << 31), (1, -(1 << 40)), (7, None), (7, "1")],
+                         ids=str)
+def test_numbers_that_fit_no_description(at, value):
+    values = [2, 64, 32, 0, 100, 1, 1, 1e-6, BASE, 64, 6400, 0, 0, 2 * BASE, 64, 6400, 0, 0, 0]
+    values[at] = value
+    with pytest.raises(s2b200.S2Error) as e:
+        s2b200._pack(s2b200._NORM_LAYOUT, *values)
+    assert e.value.status == INVALID

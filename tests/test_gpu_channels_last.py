@@ -885,3 +885,11 @@ def test_no_rows_of_any_shape(shape):
     assert s2b200.linear_act(x, w, out=y) is y
     assert s2b200.group_norm_act(x, 8).shape == shape
     assert s2b200.group_norm_act(x[None], 8, out=torch.empty_like(x[None])).shape == (1,) + shape
+
+
+@pytest.mark.parametrize("kw", [dict(groups=1 << 40), dict(groups=8.0), dict(groups=8, eps=None), dict(groups=8, eps=1e39),
+                                dict(groups=-8), dict(groups=8, eps=float("nan"))], ids=str)
+def test_numbers_out_of_range_are_refused_like_others(kw):
+    with pytest.raises(s2b200.S2Error) as e:
+        s2b200.group_norm_act(torch.zeros(2, 5, 64, device="cuda"), **kw)
+    assert e.value.status == s2b200.S2_INVALID_ARGUMENT
