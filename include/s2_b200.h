@@ -397,8 +397,8 @@ S2_API s2_status s2_gemm(void *stream, const s2_gemm_desc *desc, int *extra_laun
  * current device, which must be the one of `stream` and of every pointer, are
  * stream-ordered and capturable, allocate nothing and keep nothing between
  * calls: the caller passes a workspace of at least *_workspace_bytes(desc)
- * bytes, 16-byte aligned (its contents do not matter; calls that may overlap
- * need one each). *launches (may be NULL) receives the kernels launched.
+ * bytes, 16-byte aligned and apart from every operand (its contents do not
+ * matter; calls that may run at the same time need one each). *launches (may be NULL) receives the kernels launched.
  *
  * A kernel whose blocks wait for one another or for a copy does so for 1 s at
  * most; then it ends, y is wrong, and the call's error word `err` (device
@@ -430,11 +430,12 @@ typedef enum s2_activation {
  * the same, or fp32 in and fp16 / bf16 out. Statistics in fp32 about local
  * pivots, joined in order (the same call gives the same bits). x_row, y_row
  * >= channels: elements between positions; x_sample, y_sample: between
- * samples. y may be x itself (same type, pitch and sample stride), and must
- * not overlap it otherwise. With D the largest distance of a value from its
- * group's mean and n the group's values, max(n, 256) D^2 must be finite in
- * fp32; a group beyond that, or with a value that is not finite, gives NaN,
- * and no other does. samples or positions 0: nothing is done. At most 1024
+ * samples, which follow one another (a sample ends before the next begins).
+ * y may be x itself (same type, pitch and sample stride), and must not overlap
+ * it otherwise, nor weight or bias. With D the largest distance of a value
+ * from its group's mean and n the group's values, max(n, 256) D^2 must be
+ * finite in fp32; a group beyond that, or with a value that is not finite,
+ * gives NaN, and no other does. samples or positions 0: nothing is done. At most 1024
  * groups, 65535 samples and 2^31 positions (S2_UNSUPPORTED beyond). err's
  * codes: 96 for a wait for the other blocks' moments, 97 for a load. */
 typedef struct s2_group_norm_act_desc {

@@ -1485,13 +1485,19 @@ extern "C" s2_status s2_group_norm_act(void *stream, const s2_group_norm_act_des
         (d->samples > 1 && (d->x_sample < (d->positions - 1) * d->x_row + d->channels ||
                             d->y_sample < (d->positions - 1) * d->y_row + d->channels)))
         return s2::set_error(S2_INVALID_ARGUMENT, "s2_group_norm_act: a pitch is smaller than what it spans");
-    if (!in_place(*d) && s2::may_overlap(span(d->x, *d, d->x_row, d->x_sample, static_cast<long long>(ie)),
-                                         span(d->y, *d, d->y_row, d->y_sample, static_cast<long long>(oe))))
-        return s2::set_error(S2_INVALID_ARGUMENT, "s2_group_norm_act: y overlaps x");
+    const s2::PitchedSpan xs = span(d->x, *d, d->x_row, d->x_sample, static_cast<long long>(ie));
+    const s2::PitchedSpan ys = span(d->y, *d, d->y_row, d->y_sample, static_cast<long long>(oe));
+    const s2::PitchedSpan ws = s2::bytes_at(d->weight, 4LL * d->channels), bs = s2::bytes_at(d->bias, 4LL * d->channels);
+    if (!in_place(*d) && s2::may_overlap(xs, ys)) return s2::set_error(S2_INVALID_ARGUMENT, "s2_group_norm_act: y overlaps x");
+    if (s2::may_overlap(ws, ys) || s2::may_overlap(bs, ys))
+        return s2::set_error(S2_INVALID_ARGUMENT, "s2_group_norm_act: y overlaps weight or bias");
     const Plan p = plan_of(*d, sm_count());
     const size_t need = workspace_of(p);
     if (need > 0 && (!d->workspace || d->workspace_bytes < need || reinterpret_cast<uintptr_t>(d->workspace) % 16))
         return s2::set_error(S2_INVALID_ARGUMENT, "s2_group_norm_act: workspace of %zu bytes, 16-byte aligned, needed", need);
+    const s2::PitchedSpan work = s2::bytes_at(need > 0 ? d->workspace : nullptr, static_cast<long long>(need));
+    if (s2::may_overlap(work, xs) || s2::may_overlap(work, ys) || s2::may_overlap(work, ws) || s2::may_overlap(work, bs))
+        return s2::set_error(S2_INVALID_ARGUMENT, "s2_group_norm_act: the workspace overlaps an operand");
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     GnArgs a = {};
     a.x = d->x;

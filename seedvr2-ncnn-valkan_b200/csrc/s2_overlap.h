@@ -11,6 +11,8 @@ struct PitchedSpan {
     long long rows, width, pitch;
 };
 
+inline PitchedSpan bytes_at(const void *p, long long n) { return {p, 1, n, n}; }
+
 // True when a and b may share bytes. Equal pitches are told apart by columns (two column
 // ranges of one wider buffer do not overlap); else their whole extents are compared.
 inline bool may_overlap(const PitchedSpan &a, const PitchedSpan &b)

@@ -149,3 +149,18 @@ def test_numbers_that_fit_no_description(at, value):
     with pytest.raises(s2b200.S2Error) as e:
         s2b200._pack(s2b200._NORM_LAYOUT, *values)
     assert e.value.status == INVALID
+
+
+# large enough for a workspace (slices of a grid)
+LARGE = dict(samples=4, channels=512, positions=1 << 14, x_row=512, y_row=512, x_sample=1 << 23, y_sample=1 << 23, x=1 << 32,
+             y=2 << 32, weight=3 << 32, bias=4 << 32, workspace=5 << 32)
+
+
+@pytest.mark.parametrize("kw", [dict(weight=2 << 32), dict(bias=2 << 32), dict(weight=(2 << 32) - 2044),
+                                dict(bias=(2 << 32) + (4 << 24) - 4), dict(workspace=1 << 32), dict(workspace=(2 << 32) + 4096),
+                                dict(workspace=(1 << 32) - 16), dict(workspace=(3 << 32) + 2032), dict(workspace=(4 << 32) - 16)], ids=str)
+def test_norm_refuses_what_would_be_overwritten(kw):
+    d = _norm(**(LARGE | kw))
+    assert s2b200.lib().s2_group_norm_act_workspace_bytes(ctypes.byref(d)) > 0
+    assert _call("s2_group_norm_act", d) == (INVALID, 0)
+    assert "overlaps" in s2b200.last_error()
