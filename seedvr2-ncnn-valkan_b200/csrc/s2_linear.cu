@@ -873,7 +873,16 @@ s2_status check(const s2_linear_act_desc *d)
     return S2_OK;
 }
 
-s2_status check_operands(const s2_linear_act_desc &d)
+size_t workspace_of(const s2_linear_act_desc &d)
+{
+    if (d.M <= 1) return 0;
+    size_t need = 0;
+    if (!tma_ready(d.x, d.ldx, d.M)) need += static_cast<size_t>(d.M) * round_up8(d.K) * 2;
+    if (!tma_ready(d.w, d.ldw, d.N)) need += static_cast<size_t>(d.N) * round_up8(d.K) * 2;
+    return need;
+}
+
+s2_status check_operands(const s2_linear_act_desc &d, size_t workspace)
 {
     const uintptr_t oe = d.out_dtype == S2_F32 ? 4 : 2;
     if (!d.x || !d.w || !d.y) return s2::set_error(S2_INVALID_ARGUMENT, "s2_linear_act: NULL x, w or y");
@@ -886,12 +895,18 @@ s2_status check_operands(const s2_linear_act_desc &d)
         d.ldy > top || d.ldr > top)
         return s2::set_error(S2_INVALID_ARGUMENT, "s2_linear_act: a pitch is smaller than its row");
     const s2::PitchedSpan y{d.y, d.M, static_cast<long long>(d.N * oe), static_cast<long long>(d.ldy * oe)};
+    const s2::PitchedSpan r{d.residual, d.M, static_cast<long long>(d.N * oe), static_cast<long long>(d.ldr * oe)};
+    const s2::PitchedSpan x{d.x, d.M, 2LL * d.K, 2 * d.ldx}, w{d.w, d.N, 2LL * d.K, 2 * d.ldw}, b = s2::bytes_at(d.bias, 4LL * d.N);
     const bool in_place = d.residual == d.y && d.ldr == d.ldy;
-    if (s2::may_overlap(y, {d.x, d.M, 2LL * d.K, 2 * d.ldx}) || s2::may_overlap(y, {d.w, d.N, 2LL * d.K, 2 * d.ldw}) ||
-        s2::may_overlap(y, {d.bias, 1, 4LL * d.N, 4LL * d.N}) ||
-        (!in_place && s2::may_overlap(y, {d.residual, d.M, static_cast<long long>(d.N * oe),
-                                          static_cast<long long>(d.ldr * oe)})))
+    if (s2::may_overlap(y, x) || s2::may_overlap(y, w) || s2::may_overlap(y, b) || (!in_place && s2::may_overlap(y, r)))
         return s2::set_error(S2_INVALID_ARGUMENT, "s2_linear_act: y overlaps an input");
+    if (workspace == 0) return S2_OK;
+    if (!d.workspace || d.workspace_bytes < workspace || reinterpret_cast<uintptr_t>(d.workspace) % 16)
+        return s2::set_error(S2_INVALID_ARGUMENT, "s2_linear_act: workspace of %zu bytes, 16-byte aligned, needed", workspace);
+    const s2::PitchedSpan work = s2::bytes_at(d.workspace, static_cast<long long>(workspace));
+    if (s2::may_overlap(work, x) || s2::may_overlap(work, w) || s2::may_overlap(work, b) || s2::may_overlap(work, r) ||
+        s2::may_overlap(work, y))
+        return s2::set_error(S2_INVALID_ARGUMENT, "s2_linear_act: the workspace overlaps an operand");
     return S2_OK;
 }
 
@@ -900,11 +915,7 @@ s2_status check_operands(const s2_linear_act_desc &d)
 extern "C" size_t s2_linear_act_workspace_bytes(const s2_linear_act_desc *d)
 {
     s2::clear_error();
-    if (check(d) != S2_OK || d->M <= 1) return 0;
-    size_t need = 0;
-    if (!tma_ready(d->x, d->ldx, d->M)) need += static_cast<size_t>(d->M) * round_up8(d->K) * 2;
-    if (!tma_ready(d->w, d->ldw, d->N)) need += static_cast<size_t>(d->N) * round_up8(d->K) * 2;
-    return need;
+    return check(d) == S2_OK ? workspace_of(*d) : 0;
 }
 
 extern "C" s2_status s2_linear_act(void *stream, const s2_linear_act_desc *d, int *launches)
@@ -914,10 +925,7 @@ extern "C" s2_status s2_linear_act(void *stream, const s2_linear_act_desc *d, in
     s2_status s = check(d);
     if (s != S2_OK) return s;
     if (d->M == 0) return S2_OK;
-    if ((s = check_operands(*d)) != S2_OK) return s;
-    const size_t need = s2_linear_act_workspace_bytes(d);
-    if (need > 0 && (!d->workspace || d->workspace_bytes < need || reinterpret_cast<uintptr_t>(d->workspace) % 16))
-        return s2::set_error(S2_INVALID_ARGUMENT, "s2_linear_act: workspace of %zu bytes, 16-byte aligned, needed", need);
+    if ((s = check_operands(*d, workspace_of(*d))) != S2_OK) return s;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     LinearArgs a;
     a.bias = d->bias;

@@ -164,3 +164,12 @@ def test_norm_refuses_what_would_be_overwritten(kw):
     assert s2b200.lib().s2_group_norm_act_workspace_bytes(ctypes.byref(d)) > 0
     assert _call("s2_group_norm_act", d) == (INVALID, 0)
     assert "overlaps" in s2b200.last_error()
+
+
+@pytest.mark.parametrize("at", [BASE, BASE + 2048, 2 * BASE, 3 * BASE, 5 * BASE + 240, 6 * BASE - 2096], ids=str)
+def test_linear_refuses_a_workspace_on_its_operands(at):
+    """x in rows of 129 values is packed into the workspace."""
+    d = _linear(ldx=129, workspace=at, bias=5 * BASE, residual=6 * BASE, ldr=64)
+    assert s2b200.lib().s2_linear_act_workspace_bytes(ctypes.byref(d)) == 10 * 128 * 2
+    assert _call("s2_linear_act", d) == (INVALID, 0)
+    assert "workspace overlaps" in s2b200.last_error()
