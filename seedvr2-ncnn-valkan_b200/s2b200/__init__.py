@@ -1031,7 +1031,8 @@ def _pitch(t, first: int, what: str):
 
 
 def _elsewhere(fn, x, stream, *args):
-    """fn(x, *args, stream=None) with x's device, or `stream`, made current."""
+    """fn(x, *args, stream=None) with x's device, or `stream`, made current. The caller may let go of what it
+    passed while `stream` has yet to read it: its memory is kept from other use until then."""
     torch = _torch()
     if not x.is_cuda:
         _fail(f"x is on {x.device}: the operators run on a CUDA device")
@@ -1041,7 +1042,11 @@ def _elsewhere(fn, x, stream, *args):
     if stream.device != x.device:
         _fail(f"the stream is on {stream.device}, x on {x.device}")
     with torch.cuda.stream(stream):
-        return fn(x, *args)
+        result = fn(x, *args)
+    for t in (x, *args):
+        if isinstance(t, torch.Tensor) and t.is_cuda:
+            t.record_stream(stream)
+    return result
 
 
 # the descriptions' fields as struct.pack takes them (building a ctypes.Structure costs three times as much)

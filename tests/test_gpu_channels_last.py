@@ -893,3 +893,37 @@ def test_numbers_out_of_range_are_refused_like_others(kw):
     with pytest.raises(s2b200.S2Error) as e:
         s2b200.group_norm_act(torch.zeros(2, 5, 64, device="cuda"), **kw)
     assert e.value.status == s2b200.S2_INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("op", ["norm", "linear"])
+def test_tensors_let_go_of_before_another_stream_reads_them(op):
+    """With `stream`, the call's tensors may be dropped at once, though the stream is busy: what is allocated and written
+    next does not take their place."""
+    gen = _gen(81)
+
+    def tensors():
+        if op == "norm":
+            return [_features((3, 20001, 512), gen, F16), 1 + 0.1 * _normal((512,), gen), _normal((512,), gen)]
+        x, w, b, r = _operands(3000, 520, 1000, F16, 82)
+        return [x, w, b, r]
+
+    def call(t, **kw):
+        if op == "norm":
+            return s2b200.group_norm_act(t[0], 32, t[1], t[2], activation="silu", **kw)
+        return s2b200.linear_act(t[0], t[1], t[2], "silu", t[3], **kw)
+
+    held = tensors()
+    want = call(held)
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        dropped = [t.clone() for t in held]
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(100_000_000)
+        got = call(dropped, stream=side)
+        shapes = [(t.shape, t.dtype) for t in dropped]
+        del dropped
+        fresh = [torch.full(s, 7.0, dtype=d, device="cuda") for s, d in shapes for _ in range(2)]
+        side.synchronize()
+        assert torch.equal(got, want)
+        del fresh
