@@ -1113,6 +1113,8 @@ def group_norm_act(x, groups: int, weight=None, bias=None, eps: float = 1e-6, ac
     else:
         if out.shape != shape or out.get_device() != index or out_dtype not in (None, out.dtype):
             _fail("out must have x's shape and device, and out_dtype if both are given")
+        if out.requires_grad:
+            _need_no_grad()
         y_row = _pitch(out, 1, "out")[1]
         y_sample = out.stride(0)
         out_type = _type_of(out, "out")
@@ -1161,6 +1163,8 @@ def linear_act(x, w, bias=None, activation: str = "none", residual=None, out=Non
     else:
         if out.shape != (*shape[:-1], N) or out.get_device() != index or out_dtype not in (None, out.dtype):
             _fail(f"out must be {(*shape[:-1], N)} on x's device, and of out_dtype if both are given")
+        if out.requires_grad:
+            _need_no_grad()
         ldy = _pitch(out, 0, "out")[1]
         out_type = _type_of(out, "out")
     res = ldr = 0

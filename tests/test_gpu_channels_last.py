@@ -927,3 +927,13 @@ def test_tensors_let_go_of_before_another_stream_reads_them(op):
         side.synchronize()
         assert torch.equal(got, want)
         del fresh
+
+
+def test_outputs_that_require_gradients_are_refused():
+    x = torch.zeros(4, 64, dtype=F16, device="cuda")
+    out = torch.zeros(4, 64, dtype=F16, device="cuda", requires_grad=True)
+    for call in (lambda: s2b200.group_norm_act(x, 8, out=out), lambda: s2b200.linear_act(x, torch.zeros_like(x[:1].expand(64, 64)), out=out)):
+        with pytest.raises(s2b200.S2Error):
+            call()
+        with torch.no_grad():
+            assert call() is out
