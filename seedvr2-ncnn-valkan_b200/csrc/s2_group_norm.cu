@@ -584,14 +584,13 @@ __global__ void __launch_bounds__(kThreads, 2) group_norm_held_kernel(const GnAr
         const int gs = min(a.slice_groups, a.G - g0), c0 = g0 * a.cpg, ncols = gs * a.cpg / VEC;
         const TI *x = static_cast<const TI *>(a.x) + smp * a.x_sample + r0 * a.x_row + c0;
         TO *y = static_cast<TO *>(a.y) + smp * a.y_sample + r0 * a.y_row + c0;
-        const int hold = ncols <= kThreads ? a.hold : 0;
         if (threadIdx.x < gs) s.group[threadIdx.x] = Moments{0.f, 0.f, 0.f};
         Place p;
         for (int cb = 0; cb < ncols; cb += kThreads) {
             p = place_of(cb, ncols, rows);
             Moments mo[N] = {};
             read_rows<TI, VEC, N>(x + p.rl * a.x_row + static_cast<long long>(p.col) * VEC, p.lanes * a.x_row, p.count, policy,
-                                  hold, held, mo);
+                                  a.hold, held, mo);
             join_block<VEC, N>(s, mo, p, cb, a.cpg, gs, a.group_lanes, sub, sub_lane, [] { __syncthreads(); });
         }
         __syncthreads();
@@ -621,7 +620,7 @@ __global__ void __launch_bounds__(kThreads, 2) group_norm_held_kernel(const GnAr
             if (ncols > kThreads) p = place_of(cb, ncols, rows);
             if (p.count > 0)
                 write_column<TI, TO, VEC, N>(a, p, c0, norm, x + p.rl * a.x_row + static_cast<long long>(p.col) * VEC,
-                                             y + p.rl * a.y_row + static_cast<long long>(p.col) * VEC, policy, hold, held);
+                                             y + p.rl * a.y_row + static_cast<long long>(p.col) * VEC, policy, a.hold, held);
         }
         __syncthreads();  // the next unit reuses the moments
     }
@@ -1287,6 +1286,11 @@ Plan plan_of(const s2_group_norm_act_desc &d, int sms)
     // launch cost the host 5 us: 2 x 1920 x 512 fp16 9.1 us and 16.4 called one by one, 9.2 and 11.5 by clusters.
     if (wide && d.samples * bytes_of(d.groups) >= (8LL << 20) && plan_slab(d, sms, p)) return p;
     p.slice_groups = std::max(step, std::min(d.groups, kSliceGroups / step * step));
+    // The blocks hold the rows of slices that their threads cover with a column each: 6 x 14400 x 512 fp16 in rows of 515
+    // values takes 117 us in slices of 256 channels, 156 in whole rows, which are read twice. Only where a single group
+    // is wider are columns taken in turns, nothing is held, and the sizes below just choose between cluster and grid.
+    while (p.slice_groups * cpg / vec > kThreads && halve(p.slice_groups) < p.slice_groups) p.slice_groups = halve(p.slice_groups);
+    const bool holds = p.slice_groups * cpg / vec <= kThreads;
     p.join = kGrid;
     // Held by a cluster, if need be in narrower slices. Reading 128 bytes of each row at a time costs little,
     // 32 do once the memory is the limit: 6 x 14400 x 512 took 80 us in slices of 32 bytes and 47 on a grid, but
@@ -1332,7 +1336,7 @@ Plan plan_of(const s2_group_norm_act_desc &d, int sms)
     p.part_rows = (d.positions + p.parts - 1) / p.parts;
     // no more shared memory than the rows need
     const long long lanes = std::max<long long>(1, kThreads * vec / (p.slice_groups * cpg)), pieces = (p.part_rows + lanes - 1) / lanes;
-    p.smem = std::min<size_t>(kHold, static_cast<size_t>(pieces) * kThreads * (wide ? 16 : size));
+    p.smem = holds ? std::min<size_t>(kHold, static_cast<size_t>(pieces) * kThreads * (wide ? 16 : size)) : 0;
     return p;
 }
 

@@ -173,3 +173,15 @@ def test_linear_refuses_a_workspace_on_its_operands(at):
     assert s2b200.lib().s2_linear_act_workspace_bytes(ctypes.byref(d)) == 10 * 128 * 2
     assert _call("s2_linear_act", d) == (INVALID, 0)
     assert "workspace overlaps" in s2b200.last_error()
+
+
+@pytest.mark.parametrize("pad,dtype", [(3, s2b200.S2_F16), (1, s2b200.S2_F32)], ids=str)
+def test_norm_takes_wide_rows_in_slices_that_a_block_holds(pad, dtype):
+    """Rows not on 16 bytes are read value by value, a column a thread: 512 channels are two slices of 256 columns, which
+    blocks hold, like twice as many samples of 256 channels."""
+    def workspace(samples, channels, groups):
+        row = channels + pad
+        d = _norm(samples=samples, channels=channels, groups=groups, positions=14400, x_row=row, y_row=row,
+                  x_sample=14400 * row, y_sample=14400 * row, in_dtype=dtype, out_dtype=dtype, y=1 << 40)
+        return s2b200.lib().s2_group_norm_act_workspace_bytes(ctypes.byref(d))
+    assert workspace(6, 512, 32) == workspace(12, 256, 16) > 0
