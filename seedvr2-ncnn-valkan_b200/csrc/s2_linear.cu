@@ -891,9 +891,10 @@ s2_status check_operands(const s2_linear_act_desc &d, size_t workspace)
         reinterpret_cast<uintptr_t>(d.bias) % 4)
         return s2::set_error(S2_INVALID_ARGUMENT, "s2_linear_act: a pointer is not aligned to its elements");
     const long long top = 1LL << 40;
-    if (d.ldx < d.K || d.ldw < d.K || d.ldy < d.N || (d.residual && d.ldr < d.N) || d.ldx > top || d.ldw > top ||
-        d.ldy > top || d.ldr > top)
+    if (d.ldx < d.K || d.ldw < d.K || d.ldy < d.N || (d.residual && d.ldr < d.N))
         return s2::set_error(S2_INVALID_ARGUMENT, "s2_linear_act: a pitch is smaller than its row");
+    if (d.ldx > top || d.ldw > top || d.ldy > top || (d.residual && d.ldr > top))
+        return s2::set_error(S2_INVALID_ARGUMENT, "s2_linear_act: a pitch beyond any memory");
     const s2::PitchedSpan y{d.y, d.M, static_cast<long long>(d.N * oe), static_cast<long long>(d.ldy * oe)};
     const s2::PitchedSpan r{d.residual, d.M, static_cast<long long>(d.N * oe), static_cast<long long>(d.ldr * oe)};
     const s2::PitchedSpan x{d.x, d.M, 2LL * d.K, 2 * d.ldx}, w{d.w, d.N, 2LL * d.K, 2 * d.ldw}, b = s2::bytes_at(d.bias, 4LL * d.N);

@@ -185,3 +185,12 @@ def test_norm_takes_wide_rows_in_slices_that_a_block_holds(pad, dtype):
                   x_sample=14400 * row, y_sample=14400 * row, in_dtype=dtype, out_dtype=dtype, y=1 << 40)
         return s2b200.lib().s2_group_norm_act_workspace_bytes(ctypes.byref(d))
     assert workspace(6, 512, 32) == workspace(12, 256, 16) > 0
+
+
+def test_linear_looks_at_the_residuals_pitch_only_with_a_residual():
+    """Past the checks of pitches, to the last one: y on its bias."""
+    for ldr in (1 << 50, -1, 0):
+        assert _call("s2_linear_act", _linear(ldr=ldr, bias=3 * BASE)) == (INVALID, 0)
+        assert "y overlaps" in s2b200.last_error()
+    assert _call("s2_linear_act", _linear(ldr=1 << 50, residual=6 * BASE, bias=3 * BASE)) == (INVALID, 0)
+    assert "pitch" in s2b200.last_error()
