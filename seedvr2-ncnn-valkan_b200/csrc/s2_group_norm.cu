@@ -1235,8 +1235,9 @@ bool plan_slab(const s2_group_norm_act_desc &d, int sms, Plan &p)
     if (d.x_row >= (1LL << 40) / size || d.x_sample >= (1LL << 40) / size) return false;  // a tensor map's strides
     const long long room = slab_room(moments_of(cpg, vec)) / 4, blocks = 2 * sms;
     for (int sg = std::min(d.groups, kSlabGroups); sg > 0; --sg) {
-        const int channels = sg * cpg, width = channels * size;
+        const int channels = sg * cpg;
         if (d.groups % sg != 0 || channels % vec != 0 || channels > 256) continue;
+        const int width = channels * size;
         if (width < 64) break;
         const int whole = std::max(1, 128 / (width & -width));  // a box is a multiple of 128 bytes
         const long long most = room / width / whole * whole;    // rows of a quarter of the room

@@ -194,3 +194,15 @@ def test_linear_looks_at_the_residuals_pitch_only_with_a_residual():
         assert "y overlaps" in s2b200.last_error()
     assert _call("s2_linear_act", _linear(ldr=1 << 50, residual=6 * BASE, bias=3 * BASE)) == (INVALID, 0)
     assert "pitch" in s2b200.last_error()
+
+
+@pytest.mark.parametrize("channels,groups", [(1 << 30, 1), ((1 << 31) - 4, 1), ((1 << 31) - 1024, 1024), ((1 << 31) - 1, 1)], ids=str)
+def test_norm_of_as_many_channels_as_an_int_holds(channels, groups):
+    """Planned without overflow: to the last check, y on x."""
+    for dtype in (s2b200.S2_F32, s2b200.S2_BF16):
+        d = _norm(samples=1, positions=1000, channels=channels, groups=groups, x_row=channels, y_row=channels, in_dtype=dtype,
+                  out_dtype=dtype, y=BASE + 64)
+        s2b200.lib().s2_group_norm_act_workspace_bytes(ctypes.byref(d))
+        assert s2b200.last_error() == ""
+        assert _call("s2_group_norm_act", d) == (INVALID, 0)
+        assert "overlaps" in s2b200.last_error()
