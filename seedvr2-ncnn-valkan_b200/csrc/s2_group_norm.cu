@@ -1225,10 +1225,10 @@ bool is_wide(const s2_group_norm_act_desc &d)
 }
 
 // Slices for group_norm_slab_kernel: the widest of which as many blocks as there are can hold four. With 4 x 115200
-// x 512 bf16 these are 64 bytes wide and take 218 us; two of 128 took 243, the ring 256. A block's share of a
-// slice below 8 KB does not pay for its exchange: 20 x 9000 x 192 fp16 over the whole grid (5.9 KB) took 70 us
-// and 64 through the ring, but 12 x 9000 x 320 (9.9 KB) 54 and 71. Held by clusters 16 x 5000 x 512 bf16 took 73 us
-// and 47 here, 400 x 256 x 1280 240 and 130.
+// x 512 bf16 these are 64 bytes wide and take 218 us; two of 128 take 242, the ring 256. However little a block's
+// share of a slice: 1 x 24000 x 32 fp16 (5.2 KB) takes 8.3 us and 16.4 through the ring, 1 x 22000 x 48 (7.2 KB) 12.1
+// and 22.6, 20 x 9000 x 192 44 and 68. Held by clusters 16 x 5000 x 512 bf16 takes 68 us and 47 here, 400 x 256 x 1280
+// 226 and 130.
 bool plan_slab(const s2_group_norm_act_desc &d, int sms, Plan &p)
 {
     const int size = static_cast<int>(elem(d.in_dtype)), vec = 16 / size, cpg = d.channels / d.groups;
@@ -1248,7 +1248,7 @@ bool plan_slab(const s2_group_norm_act_desc &d, int sms, Plan &p)
         const long long boxes = (part_rows + 255) / 256, box_rows = ((part_rows + boxes - 1) / boxes + whole - 1) / whole * whole;
         const long long bytes = boxes * box_rows * width, parts = (d.positions + part_rows - 1) / part_rows;
         if (bytes > room || box_rows > 256) continue;
-        if (bytes < 8192 || parts > 32 * kPartsLane) break;
+        if (parts > 32 * kPartsLane) break;
         p.slab = true;
         p.join = kGrid;
         p.part_rows = part_rows;

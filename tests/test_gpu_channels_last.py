@@ -937,3 +937,17 @@ def test_outputs_that_require_gradients_are_refused():
             call()
         with torch.no_grad():
             assert call() is out
+
+
+@pytest.mark.parametrize("types", NORM_TYPES, ids=lambda t: f"{t[0]}-{t[1]}".replace("torch.", ""))
+@pytest.mark.parametrize("shape", [(1, 24000, 32, 8), (1, 22000, 48, 16), (1, 21500, 32, 1), (2, 25001, 40, 5)], ids=str)
+def test_norm_of_small_shares_of_narrow_slices(shape, types):
+    S, P, C, G = shape
+    x = _features(shape[:3], _gen(91), types[0])
+    for act in ("silu", "none"):
+        y = s2b200.group_norm_act(x, G, activation=act, out_dtype=types[1])
+        cl.check(y, *cl.norm_exact(x, G, None, None, 1e-6, act))
+    off = torch.zeros((), dtype=torch.int64, device="cuda")
+    for _ in range(50):
+        off += (s2b200.group_norm_act(x, G, out_dtype=types[1]) != y).sum()
+    assert off.item() == 0
