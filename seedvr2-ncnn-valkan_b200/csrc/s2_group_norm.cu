@@ -16,14 +16,15 @@
 // and y once (6.5 TB/s); the statistics stand between the two, so what counts is to hold what was read, and to
 // read the next while the last is joined and written. Three kernels:
 //  * group_norm_slab_kernel, aligned rows: teams of blocks hold narrow slices in shared memory, several at a
-//    time, and load, sum, join and write different ones at once. One read, up to 4.9 TB/s.
+//    time, and load, sum, join and write different ones at once. One read, 4 to 4.9 TB/s.
 //  * group_norm_held_kernel: the blocks read their rows into shared memory while they sum them, and write the
 //    output from there, one step after the other. For units too small to be worth the above: the blocks of a
 //    cluster hold one and exchange their moments through distributed shared memory, without a workspace. And
 //    for rows that do not start on 16 bytes, also on a cooperative grid, where rows not held are read twice.
-//  * group_norm_ring_kernel, aligned units larger than the shared memory of the GPU: a loading warp streams the
-//    rows through a ring of slots with bulk copies, so that the memory never waits for the threads that sum and
-//    write; all but what the ring holds at the end of the statistics is read twice.
+//  * group_norm_ring_kernel, aligned rows of samples too large for the first (four slices of 64 bytes a row do not fit
+//    the GPU's shared memory: beyond about 125000 positions, 8 MB a slice): a loading warp streams the rows through a
+//    ring of slots with bulk copies, so that the memory never waits for the threads that sum and write; all but what
+//    the ring holds at the end of the statistics is read twice.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -564,7 +565,7 @@ __device__ __forceinline__ void join_grid(const GnArgs &a, int unit, int member,
 // ---- rows held by the blocks ---------------------------------------------------------
 
 // Bound by its steps, one after the other (start, read, exchange, write): 3 x 7973 x 96 fp32 with rows of 101 values,
-// one at a time, 12.6 us; 20 x 500 x 512 bf16 14 us, 2.3 TB/s.
+// one at a time, 15.6 us from memory (13.3 when L2 has x); 2 x 1920 x 512 fp16 on clusters 9.3 us.
 template <typename TI, typename TO, int VEC, int N>
 __global__ void __launch_bounds__(kThreads, 2) group_norm_held_kernel(const GnArgs a)
 {
@@ -736,7 +737,7 @@ __device__ __forceinline__ void write_slots(Cursor<kSlots> c, const Slots &p, in
 }
 
 // Bound by the memory: two reads and a write of a unit that L2 does not hold. 21 x 921600 x 128 bf16 silu (236 MB a
-// sample) 2.36 ms, 96 % of these three passes at the copy rate, 6.3 TB/s; reads that the threads issue for
+// sample) 2.37 ms, 96 % of these three passes at the copy rate, 6.3 TB/s; reads that the threads issue for
 // themselves took 2.9 ms. N: moments a vector, 16 / sizeof(TI) / N channels each, which always belong to one group.
 template <typename TI, typename TO, int N>
 __global__ void __launch_bounds__(kThreads + 32, 2) group_norm_ring_kernel(const GnArgs a)
@@ -979,10 +980,10 @@ __device__ __forceinline__ bool wait_posted(const volatile int *posted, int unit
 // the one behind it brought to L2), warp 9 joins all parts' moments of the groups that are its block's turn,
 // warp 10 fetches the results; where the parts are few, warp 10 joins them all itself. What bounds it is how long a
 // unit stays in shared memory, about 12 us of which 2.5 for the load, 1.5 for the sums, 5 for the exchange and 2.5
-// for the output, at 28 MB for the whole GPU. 11 x 57600 x 512 bf16 silu: 264 us, 4.9 TB/s (347 through the ring,
-// which reads twice); 6 x 14400 x 512: 41 us (47); 40 x 3600 x 512: 73 us (143 held by clusters). With one role
-// after the other in each block the first took 560 us, and 370 while a lane asked for one part's moments after
-// the other.
+// for the output, at 28 MB for the whole GPU. 11 x 57600 x 512 bf16 silu: 270 us, 4.8 TB/s (346 through the ring,
+// which reads twice; 264 without an activation, 286 with gelu_tanh, 373 with gelu, which the writing warps do not
+// hide); 6 x 14400 x 512: 42 us (48); 40 x 3600 x 512: 73 us (136 held by clusters). With one role after the other
+// in each block the first took 560 us, and 370 while a lane asked for one part's moments after the other.
 template <typename TI, typename TO, int N>
 __global__ void __launch_bounds__(kThreads + 96, 2) group_norm_slab_kernel(const __grid_constant__ CUtensorMap map, const GnArgs a)
 {
@@ -1028,7 +1029,7 @@ __global__ void __launch_bounds__(kThreads + 96, 2) group_norm_slab_kernel(const
             for (int i = 0; i < a.boxes; ++i)
                 tma_load_3d(base + b * buffer_bytes + i * box_bytes, &map, full0 + 8 * b, c0, static_cast<int>(r0) + i * a.box_rows, smp,
                             policy);
-            // the next unit, whose buffer is still in use, to L2: 265 us instead of 273 above
+            // the next unit, whose buffer is still in use, to L2: 11 x 57600 x 512 3 % faster
             const int next = unit + a.teams;
             if (next < a.units)
                 for (int i = 0; i < a.boxes; ++i)
@@ -1283,8 +1284,8 @@ Plan plan_of(const s2_group_norm_act_desc &d, int sms)
     auto halve = [&](int sg) { return std::max(step, sg / 2 / step * step); };
     auto fit = [&](int sg, int members) { return bytes_of(sg) / members <= static_cast<long long>(kHold * 15 / 16); };
     Plan p = {};
-    // Below 8 MB the slices' GPU time is hardly less, and their workspace, which is cleared first, and cooperative
-    // launch cost the host 5 us: 2 x 1920 x 512 fp16 9.1 us and 16.4 called one by one, 9.2 and 11.5 by clusters.
+    // Below 8 MB the slices' GPU time is no less, and their workspace, which is cleared first, and cooperative
+    // launch cost the host 5 us: 2 x 1920 x 512 fp16 10.9 us and 17.2 called one by one, 9.5 and 11.3 by clusters.
     if (wide && d.samples * bytes_of(d.groups) >= (8LL << 20) && plan_slab(d, sms, p)) return p;
     p.slice_groups = std::max(step, std::min(d.groups, kSliceGroups / step * step));
     // The blocks hold the rows of slices that their threads cover with a column each: 6 x 14400 x 512 fp16 in rows of 515
@@ -1294,8 +1295,8 @@ Plan plan_of(const s2_group_norm_act_desc &d, int sms)
     const bool holds = p.slice_groups * cpg / vec <= kThreads;
     p.join = kGrid;
     // Held by a cluster, if need be in narrower slices. Reading 128 bytes of each row at a time costs little,
-    // 32 do once the memory is the limit: 6 x 14400 x 512 took 80 us in slices of 32 bytes and 47 on a grid, but
-    // 3 x 7973 x 96 (9 MB, rows of 101 values) 12.8 us in slices of 48 and 18.3 on a grid.
+    // 32 do once the memory is the limit: 6 x 14400 x 512 takes 87 us in slices of 32 bytes and 47 on a grid, but
+    // 3 x 7973 x 96 (9 MB, rows of 101 values) 15.6 us in slices of 48 and 21.5 on a grid.
     const int narrow = d.samples * bytes_of(d.groups) <= (32LL << 20) ? 32 : 128;
     for (int sg = p.slice_groups;; sg = halve(sg)) {
         if (fit(sg, kMaxCluster)) {
@@ -1323,9 +1324,9 @@ Plan plan_of(const s2_group_norm_act_desc &d, int sms)
     p.teams = p.units;
     if (p.join == kGrid) {
         // All units at once up to 8 of them, else three or four in flight, whichever leaves fewer blocks idle in
-        // the last round: while some read, others write. 21 x 921600 x 128 bf16: 2.61 ms with two, 2.34 / 2.46 with
-        // three / four, 2.45 with all; 11 x 57600 x 512: 387, 362 / 344 and 362 us. More when a block's share of a
-        // unit would be less than it holds.
+        // the last round: while some read, others write. 21 x 921600 x 128 bf16: 2.43 ms with two, 2.36 / 2.46 with
+        // three / four, 2.47 with all; 11 x 57600 x 512 through the ring: 380, 359 / 348 and 350 us. More when a block's
+        // share of a unit would be less than it holds.
         const int blocks = 2 * sms;
         auto rounds = [&](int teams) { return static_cast<double>((p.units + teams - 1) / teams) / (blocks / teams); };
         p.teams = p.units <= 8 ? p.units : (rounds(3) < rounds(4) ? 3 : 4);

@@ -106,8 +106,8 @@ struct Rows {
     static_assert(MB * kRowsN * 4 <= kOffBar, "the joined sums reuse the stages");
 };
 
-// Few rows are bound by the reading of w, which every block of x's rows repeats from L2: 58 x 2560 x 5120 takes 10.4 us
-// (26 MB, 4.1 at the copy rate; the rest is the start, a first trip to memory and the join), 200 x 2560 x 5120 18.1 us.
+// Few rows are bound by the reading of w, which every block of x's rows repeats from L2: 58 x 2560 x 5120 takes 12.4 us
+// (26 MB, 4.1 at the copy rate; the rest is the start, a first trip to memory and the join), 200 x 2560 x 5120 17.6 us.
 template <int MB, typename TO>
 __global__ void __launch_bounds__(kRowsThreads, 2)
     linear_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
@@ -298,9 +298,9 @@ struct Raw<1> {
     }
 };
 
-// One row of x, bound by the reading of w: 15360 x 2560 (79 MB) takes 15.7 us, 5.0 TB/s with start and end;
-// 2560 x 2560 4.6 us, most of it two trips to memory and the start. The tensor cores would not read faster,
-// and their tiles leave the GPU idle when N is small (2560 x 2560: 8.1 us in linear_rows_kernel).
+// One row of x, bound by the reading of w: 15360 x 2560 (79 MB) takes 16.4 us, 4.8 TB/s with start and end;
+// 2560 x 2560 5.6 us, most of it two trips to memory and the start. The tensor cores would not read faster,
+// and their tiles leave the GPU idle when N is small (2560 x 2560: 7.3 us in linear_rows_kernel).
 // Every warp streams two rows of w, a.ks warps (1, 2, 4 or 8) share their K by pieces of 32
 // vectors, kAhead pieces in flight. VEC = 8: w's rows and x start on 16 bytes; else values one by one.
 template <typename T, typename TO, int VEC, int kAhead>
@@ -411,11 +411,11 @@ __device__ __forceinline__ void tile_of(int t, int m_blocks, int n_blocks, int &
     mb = band * kBand + in - nb * rows;
 }
 
-// Large products run at the rate that the power limit leaves the tensor cores: 21600 x 10240 x 2560 bf16 takes 833 us
-// without an activation, 1.36 PFLOP/s (1.40 measured for a library's plain product kept up for seconds), and 882
-// with gelu, whose arithmetic the epilogue warps do beside the products. With K short the tiles' operands bound
-// it, 0.5 MB of them from L2 for each 128 KB of y at K = 512: 86400 x 512 x 512 fp16 with a residual takes 50 us
-// in a burst (40.6 to read and write once) and 63 under load.
+// Large products run at the rate that the power limit leaves the tensor cores: 21600 x 10240 x 2560 bf16 takes 772 us
+// without an activation, 1.47 PFLOP/s (1.40 measured for a library's plain product kept up for seconds), and 754 (cool)
+// to 850 with gelu, whose arithmetic the epilogue warps do beside the products. With K short the tiles' operands bound
+// it, 0.5 MB of them from L2 for each 128 KB of y at K = 512: 86400 x 512 x 512 fp16 takes 51 us
+// with a residual (40.6 to read and write once), 43.5 without, and about 65 at the clocks of a long run.
 template <typename TO>
 __global__ void __launch_bounds__(kTileThreads, 1)
     linear_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
@@ -740,8 +740,8 @@ s2_status launch_vec(LinearArgs a, int sms, const s2_linear_act_desc &d, cudaStr
     const T *x = static_cast<const T *>(d.x), *w = static_cast<const T *>(d.w);
     const bool wide = (reinterpret_cast<uintptr_t>(d.x) | reinterpret_cast<uintptr_t>(d.w) | (d.N > 1 ? d.ldw * 2 : 0)) % 16 == 0;
     // Warps that share a row's K: as many as fill the GPU (32 warps an SM) and have a piece each. Then two pieces
-    // in flight are enough, else four: 2560 x 2560 (four warps a row) takes 4.6 us with two and 5.5 with four,
-    // 15360 x 2560 (one) 16.7 and 15.9.
+    // in flight are enough, else four: 2560 x 2560 (four warps a row) takes 5.3 us with two and 6.4 with four,
+    // 15360 x 2560 (one) 16.6 and 16.2.
     const int pieces = std::max(1, a.K / (wide ? 256 : 32)), pairs = (a.N + 1) / 2;
     a.ks = 1;
     while (a.ks < kVecWarps && a.ks * 2 <= pieces && 1LL * pairs * a.ks < 32LL * sms) a.ks *= 2;
@@ -842,9 +842,10 @@ s2_status launch_linear(const LinearArgs &a, int sms, const void *x, long long l
     int ks = 8;
     while (ks > 1 && (ctas * ks > 2LL * sms || n_k < 2 * ks)) ks /= 2;
     // More than 128 rows of x go to the 256 x 256 tiles, unless K is long and these tiles leave so much of the
-    // GPU idle that its split pays: 200 x 2560 x 5120 18.1 us in rows against 30.0 in tiles, 800 26.8 / 31.4,
-    // 800 x 777 x 1000 14.0 / 21.8, but without a split 1237 x 2560 x 5120 41.3 / 31.9, and with a short K
-    // 1237 x 512 x 512 11.1 / 8.5.
+    // GPU idle that its split pays: 200 x 2560 x 5120 17.6 us in rows against 30.4 in tiles, 800 26.5 / 31.1,
+    // 800 x 777 x 1000 13.6 / 21.8, but without a split 1237 x 2560 x 5120 41.0 / 31.7, and with a short K
+    // 1237 x 512 x 512 10.8 / 8.6. (Near the border either may win by a tenth: 1000 x 512 x 896 9.7 / 10.8, 1000 x 512 x
+    // 1024 12.9 / 11.5.)
     if (a.M > 128 && (ks == 1 || n_k < 16)) {
         if ((a.M + 255) / 256 * ((a.N + kTileN - 1) / kTileN) > (1LL << 30))
             return s2::set_error(S2_UNSUPPORTED, "s2_linear_act: too many tiles");
