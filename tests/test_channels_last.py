@@ -206,3 +206,15 @@ def test_norm_of_as_many_channels_as_an_int_holds(channels, groups):
         assert s2b200.last_error() == ""
         assert _call("s2_group_norm_act", d) == (INVALID, 0)
         assert "overlaps" in s2b200.last_error()
+
+
+def test_operands_between_the_rows_of_y():
+    """Weights in the gaps of y's pitched rows overlap nothing; a byte further they do. (The calls end at the missing
+    workspace.)"""
+    row = 512 + 2048
+    d = LARGE | dict(y_row=row, y_sample=(1 << 14) * row, workspace=None)
+    for at, what in ((1024, "workspace of"), (7 * 2 * row + 1024, "workspace of"), (7 * 2 * row + 2 * row - 2048, "workspace of"),
+                     (1020, "overlaps"), (7 * 2 * row + 2 * row - 2044, "overlaps")):
+        for name in ("weight", "bias"):
+            assert _call("s2_group_norm_act", _norm(**(d | {name: d["y"] + at}))) == (INVALID, 0)
+            assert what in s2b200.last_error(), (at, name)
