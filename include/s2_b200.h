@@ -398,21 +398,24 @@ S2_API s2_status s2_gemm(void *stream, const s2_gemm_desc *desc, int *extra_laun
  * stream-ordered and capturable, allocate nothing and keep nothing between
  * calls: the caller passes a workspace of at least *_workspace_bytes(desc)
  * bytes, 16-byte aligned and apart from every operand (its contents do not
- * matter; calls that may run at the same time need one each). *launches (may be NULL) receives the kernels launched.
+ * matter; calls that may run at the same time need one each). *launches (may
+ * be NULL) receives the kernels launched.
  *
  * A kernel whose blocks wait for one another or for a copy does so for 1 s at
  * most; then it ends, y is wrong, and the call's error word `err` (device
  * int32, zeroed by the caller) receives a code. Calls with err NULL share one
  * word of the device: s2_operator_device_error waits for the current device,
  * gives that word's code (0 = ok) and clears it, and returns
- * S2_INFERENCE_FAILED when it was set or the device failed. */
+ * S2_INFERENCE_FAILED when it was set or the device failed. Not to be asked
+ * during a stream capture. */
 S2_API s2_status s2_operator_device_error(int *code);
 
 /* Activations: relu max(v, 0); silu v / (1 + e^-v); gelu v (1 + erf(v /
  * sqrt 2)) / 2; gelu_tanh v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) / 2.
  * Evaluated in fp32 to within 10 2^-23 of the result, below 0 also e 2^-23
  * of it, where e is |v| for silu, v^2 / 2 for gelu and 4 sqrt(2 / pi) (|v| +
- * 0.044715 |v|^3) for gelu_tanh (as rounding v would); results below 2^-119 may be 0. */
+ * 0.044715 |v|^3) for gelu_tanh (as rounding v would); results below 2^-119
+ * may be 0. */
 typedef enum s2_activation {
     S2_ACT_NONE = 0,
     S2_ACT_RELU = 1,
@@ -433,11 +436,13 @@ typedef enum s2_activation {
  * samples, which follow one another (a sample ends before the next begins).
  * y may be x itself (same type, pitch and sample stride), and must not overlap
  * it otherwise, nor weight or bias. With D the largest distance of a value
- * from its group's mean and n the group's values, max(n, 256) D^2 must be
- * finite in fp32; a group beyond that, or with a value that is not finite,
- * gives NaN, and no other does. samples or positions 0: nothing is done. At most 1024
- * groups, 65535 samples and 2^31 positions (S2_UNSUPPORTED beyond). err's
- * codes: 96 for a wait for the other blocks' moments, 97 for a load. */
+ * from its group's mean and n the group's values, max(n, 256) D^2 should be
+ * finite in fp32 (and with eps 0 the variance a normal number): a group beyond
+ * that may be NaN, one with a value that is not finite is, all of it, and no
+ * other is. samples or positions 0: nothing is
+ * done. At most 1024 groups, 65535 samples and 2^31 positions (S2_UNSUPPORTED
+ * beyond). err's codes: 96 for a wait for the other blocks' moments, 97 for a
+ * load. */
 typedef struct s2_group_norm_act_desc {
     int samples, channels, groups, activation;
     long long positions;

@@ -46,8 +46,9 @@ extern "C" s2_status s2_operator_device_error(int *code)
     if (code) *code = 0;
     int32_t *word = s2::operator_error_word();
     int32_t h = 0;
+    // cleared before this returns: what the caller runs next may report again
     if (!word || cudaDeviceSynchronize() != cudaSuccess || cudaMemcpy(&h, word, 4, cudaMemcpyDeviceToHost) != cudaSuccess ||
-        (h != 0 && cudaMemset(word, 0, 4) != cudaSuccess))
+        (h != 0 && (cudaMemset(word, 0, 4) != cudaSuccess || cudaDeviceSynchronize() != cudaSuccess)))
         return s2::set_error(S2_INFERENCE_FAILED, "s2_operator_device_error: device failure: %s",
                              cudaGetErrorString(cudaGetLastError()));
     if (code) *code = h;

@@ -951,3 +951,30 @@ def test_norm_of_small_shares_of_narrow_slices(shape, types):
     for _ in range(50):
         off += (s2b200.group_norm_act(x, G, out_dtype=types[1]) != y).sum()
     assert off.item() == 0
+
+
+def test_captured_on_the_stream_that_is_passed():
+    """`stream` may be the one that is being captured; what the calls hand on may be dropped inside the capture."""
+    gen = _gen(95)
+    x = _features((3, 20001, 512), gen, F16)
+    w, b = (_normal((512, 512), gen) * 0.05).half(), _normal((512,), gen)
+    side = torch.cuda.Stream()
+
+    def run(**kw):
+        h = s2b200.group_norm_act(x, 32, activation="silu", **kw)
+        a = s2b200.linear_act(h, w, b, **kw)
+        del h
+        h = s2b200.linear_act(a, w, b, "gelu", x, **kw)
+        del a
+        return s2b200.group_norm_act(h, 16, b, **kw)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        y = run(stream=side)
+    for seed in (96, 97):
+        x.copy_(_features((3, 20001, 512), _gen(seed), F16))
+        want = run()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+    assert s2b200.operator_device_error() == 0
